@@ -1,6 +1,7 @@
 """Build steps for the native parts of hayai_b200 (called by __graft_entry__.build()).
 
-* ``gen_tables``  -- IQ codebook header from the reference sources (build time only).
+* ``gen_tables``  -- IQ codebook header from the reference sources, or else by gguf-py's decoder
+  (build time only).
 * ``build_cuda``  -- libhayai_cuda.so: every .cu under csrc/, sm_100a, static cudart.
 * ``build_oracle`` -- the CPU parity oracle (test infrastructure, oracle/_build/).
 
@@ -9,6 +10,7 @@ Builds are incremental: a target is rebuilt when any of its inputs is newer.
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -57,7 +59,8 @@ def _run(cmd: list[str]) -> None:
 
 
 def gen_tables(force: bool = False) -> str:
-    """Generate the IQ codebook header from the reference (needs the reference tree)."""
+    """Generate the IQ codebook header: from the reference's sources where they are, or else
+    by decoding with gguf-py.  A header that is there already is kept when neither is."""
     script = os.path.join(CSRC, "gen_iq_tables.py")
     srcs = [os.path.join(REFERENCE, "crates/hayai-model/src/iq2.rs"),
             os.path.join(REFERENCE, "crates/hayai-model/src/iq3.rs"),
@@ -66,12 +69,16 @@ def gen_tables(force: bool = False) -> str:
         if force or _newer(TABLES, srcs + [script]):
             _run([sys.executable, script, REFERENCE, TABLES])
     elif not os.path.exists(TABLES):
+        if importlib.util.find_spec("gguf") is not None:
+            _run([sys.executable, script, "-", TABLES])
+            return TABLES
         missing = [s for s in srcs if not os.path.exists(s)]
         raise RuntimeError(
             "cannot build: the IQ2/IQ3/IQ4 codebooks (GGUF format constants) are generated at build time from "
             f"the reference's sources, and these are missing: {', '.join(missing)}.  Check out aitups/hayai "
-            f"v0.2.3 beside this repository (expected at {REFERENCE}) or set HAYAI_REFERENCE to its path; "
-            f"the generated header ({TABLES}) is not kept in the repository")
+            f"v0.2.3 beside this repository (expected at {REFERENCE}), set HAYAI_REFERENCE to its path, or "
+            f"install gguf-py, whose decoder gives the same values; the generated header ({TABLES}) is not "
+            "kept in the repository")
     return TABLES
 
 

@@ -18,7 +18,11 @@ The sign table ``KSIGNS_IQ2XS`` (iq2.rs:18) is not extracted: entry ``i`` is
 ``i`` with bit 7 set to the parity of ``i`` (so every sign byte has an even
 number of set bits); both the kernels and the oracle compute it from that rule.
 
-Usage: python gen_iq_tables.py <reference_root> <out_header>
+Where the reference checkout is not there, ``-`` in its place derives the same tables from
+gguf-py's public decoder: one block per run of codebook entries is decoded with scale 1 and no
+signs, so that every decoded value is its grid value times a known constant.
+
+Usage: python gen_iq_tables.py <reference_root | -> <out_header>
 """
 from __future__ import annotations
 
@@ -64,13 +68,60 @@ def extract_i8(src: str, name: str, n: int) -> list[int]:
     return vals
 
 
+def from_decoder() -> dict[str, list[int]]:
+    """The tables by C name, from gguf.quants.dequantize over blocks that hold each entry once."""
+    import numpy as np
+    from gguf import GGMLQuantizationType as Q
+    from gguf.quants import dequantize
+
+    def blocks(entries: int, per: int, size: int):
+        """Zeroed blocks with f16 d = 1, and the entry numbers that each block holds."""
+        b = np.zeros((entries // per, size), np.uint8)
+        b[:, 0:2] = np.frombuffer(np.float16(1.0).tobytes(), np.uint8)
+        return b, np.arange(entries).reshape(-1, per)
+
+    def packed(b, qtype, factor: float, per_entry: int) -> list[int]:
+        """Little-endian words of per_entry unsigned bytes: decoded value x factor."""
+        v = dequantize(b, qtype).reshape(-1, per_entry) * np.float32(factor)
+        u = np.rint(v)
+        if not (np.array_equal(u, v) and u.min() >= 0 and u.max() <= 255):
+            raise SystemExit(f"gen_iq_tables: {qtype} does not decode to grid bytes")
+        return [int.from_bytes(row.astype(np.uint8).tobytes(), "little") for row in u]
+
+    out = {}
+    b, at = blocks(256, 32, 66)  # IQ2_XXS: per 32 weights 4 index bytes, then signs | scale: (0.5 + 0) / 4
+    b[:, 2:].reshape(-1, 8, 8)[:, :, :4] = at.reshape(-1, 8, 4)
+    out["hc_iq2xxs_grid"] = packed(b, Q.IQ2_XXS, 8, 8)
+    b, at = blocks(512, 32, 74)  # IQ2_XS: 9-bit index | 7 sign bits; scale (0.5 + 0) / 4
+    b[:, 2:66] = at.astype("<u2").view(np.uint8)
+    out["hc_iq2xs_grid"] = packed(b, Q.IQ2_XS, 8, 8)
+    b, at = blocks(1024, 32, 82)  # IQ2_S: low index bytes, signs, two high bits per index
+    b[:, 2:34] = at & 255
+    hi = (at >> 8).reshape(-1, 8, 4)
+    b[:, 66:74] = hi[..., 0] | hi[..., 1] << 2 | hi[..., 2] << 4 | hi[..., 3] << 6
+    out["hc_iq2s_grid"] = packed(b, Q.IQ2_S, 8, 8)
+    b, at = blocks(256, 64, 98)  # IQ3_XXS: index bytes, then signs | scale words: (0.5 + 0) / 2
+    b[:, 2:66] = at
+    out["hc_iq3xxs_grid"] = packed(b, Q.IQ3_XXS, 4, 4)
+    b, at = blocks(512, 64, 110)  # IQ3_S: low index bytes, one high bit per index; scale 1 + 2 x 0
+    b[:, 2:66] = at & 255
+    b[:, 66:74] = np.packbits((at >> 8).astype(np.uint8).reshape(-1, 8, 8), axis=-1, bitorder="little")[..., 0]
+    out["hc_iq3s_grid"] = packed(b, Q.IQ3_S, 1, 4)
+    b = np.zeros((1, 18), np.uint8)  # IQ4_NL: low nibbles are the first 16 weights
+    b[0, 0:2] = np.frombuffer(np.float16(1.0).tobytes(), np.uint8)
+    b[0, 2:] = np.arange(16)
+    out["hc_iq4nl_values"] = [int(v) for v in dequantize(b, Q.IQ4_NL).reshape(-1)[:16]]
+    return out
+
+
 def main(argv: list[str]) -> int:
     if len(argv) != 3:
         print(__doc__)
         return 2
     ref, out = argv[1], argv[2]
+    decoded = from_decoder() if ref == "-" else None
     lines = [
-        "/* Generated at build time by gen_iq_tables.py from the reference's IQ codebooks. */",
+        "/* Generated at build time by gen_iq_tables.py: the IQ codebooks of the GGUF formats. */",
         "#pragma once",
         "#include <stdint.h>",
         "/* Storage qualifier: plain static const for host code; CUDA code defines",
@@ -81,12 +132,18 @@ def main(argv: list[str]) -> int:
         "",
     ]
     cache: dict[str, str] = {}
-    for path, rname, cname, ctype, n in TABLES:
-        full = os.path.join(ref, path)
+
+    def source(full: str) -> str:
         if full not in cache:
             with open(full, encoding="utf-8") as f:
                 cache[full] = f.read()
-        vals = extract(cache[full], rname, n)
+        return cache[full]
+
+    for path, rname, cname, ctype, n in TABLES:
+        if decoded is not None:
+            vals = decoded[cname]
+        else:
+            vals = extract(source(os.path.join(ref, path)), rname, n)
         width = 16 if ctype == "uint64_t" else 8
         suffix = "ull" if ctype == "uint64_t" else "u"
         lines.append(f"#define {cname.upper()}_LEN {n}")
@@ -98,11 +155,10 @@ def main(argv: list[str]) -> int:
         lines.append("};")
         lines.append("")
     for path, rname, cname, n in SIGNED:
-        full = os.path.join(ref, path)
-        if full not in cache:
-            with open(full, encoding="utf-8") as f:
-                cache[full] = f.read()
-        vals = extract_i8(cache[full], rname, n)
+        if decoded is not None:
+            vals = decoded[cname]
+        else:
+            vals = extract_i8(source(os.path.join(ref, path)), rname, n)
         lines.append(f"HC_IQ_QUAL int8_t {cname}[{n}] = {{{', '.join(str(v) for v in vals)}}};")
         lines.append("")
     os.makedirs(os.path.dirname(os.path.abspath(out)), exist_ok=True)
