@@ -72,6 +72,9 @@ SIGNATURES: dict[str, list] = {
     "hc_moe_ffn_ep_dev": [_P, _P, _S, _S, _I, _F, _P, _P, _P, _S, _S, _P, _S, _P, _P, _P],
     "hc_moe_stack_dev": [_P, _S, _P, _S, _S, _I, _F, _P, _P, _P, _P, _S],
     "hc_moe_stack_ep_dev": [_P, _S, _P, _S, _S, _I, _F, _P, _P, _P, _S, _S, _P, _S],
+    "hc_kv_append_dev": [_P, _P, _P, _I, _P, _S, _P, _S],
+    "hc_kv_read_dev": [_P, _P, _P, _I, _P, _S, _P, _S],
+    "hc_attn_paged_dev": [_P, _P, _P, _I, _S, _P, _S, _P, _S, _P, _F, _I, _I, _I],
     "hc_synth_normal_dev": [_P, ctypes.c_uint64, _S, _F, _F, _P],
     "hc_quantize_dev": [_P, _I, _P, _S, _P],
 }

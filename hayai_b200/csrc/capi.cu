@@ -333,6 +333,8 @@ static int flag_error(hc_engine* e, int flag) {
             return hc_set_error(HC_ERR_RANGE,
                                 "an activation magnitude reached 65504 (outside the f16 range of the tensor-core split)");
         if (flag & 2) return hc_set_error(HC_ERR_TIMEOUT, "a bounded device wait expired");
+        if (flag & 4)
+            return hc_set_error(HC_ERR_INVALID, "kv batch: a page number, length or offset on the device is out of range");
         return hc_set_error(HC_ERR_CUDA, "device error flag 0x%x", flag);
     }
     return HC_OK;

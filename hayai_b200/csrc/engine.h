@@ -44,7 +44,7 @@ struct hc_engine {
     int smem_optin = 0;
     cudaStream_t stream = nullptr;      // stream all work is enqueued on
     cudaStream_t own_stream = nullptr;  // the engine's own stream
-    int* d_err = nullptr;               // device error flags (bit 0: f16 range, bit 1: wait timeout)
+    int* d_err = nullptr;               // device error flags (bit 0: f16 range, bit 1: wait timeout, bit 2: kv batch)
     int* h_err = nullptr;               // pinned host copy of d_err, read back with a call's results
     bool use_graphs = true;
     // grow-on-demand workspaces (the reference's GemvSyncWorkspace, compute.rs:10-17)

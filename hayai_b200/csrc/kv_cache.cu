@@ -1,0 +1,165 @@
+// kv_cache.cu -- writing the step's key and value rows into the paged cache, and reading rows of
+// it back.
+//
+// One row is one token's head_dim values of one head.  An 8-bit cache holds
+//     scale = max|x| * r, r = f32(1/127),   code = x / scale rounded to nearest (ties to even)
+// with the product and the quotient rounded to f32 as IEEE rounds them and codes held to [-127,
+// 127], so that they do not depend on the kernel; a row of zeros has scale 0 and codes 0, and a row that is not finite has scale NaN, so
+// that it reads back as NaN and is not hidden.  The scale stays in f32: 4 bytes beside 64 to 128.
+// Reading back gives code * scale, rounded once to the type of the rows.
+#include "kv_launch.h"
+
+namespace hc {
+
+// Where the batch's token t lives: its page's and row's offset in the cache (64-byte units, of
+// head 0) and in the scales, or false where it has no place.
+template <int GL>
+__device__ __forceinline__ bool kv_slot(const KvDev& c, const KvBatchDev& b, int t, uint32_t& at, long long& sat) {
+    const int s = kv_find_seq<GL>(b, t);
+    if (s < 0) return false;
+    const int len = __ldg(b.kv_len + s), pos = len - __ldg(b.q_start + s + 1) + t;
+    if (pos < 0) return false;
+    const int p = pos / c.page_size, r = pos - p * c.page_size;
+    const int page = p < b.max_pages ? __ldg(b.table + s * b.table_stride + p) : -1;
+    if ((unsigned)page >= (unsigned)c.n_pages) {
+        atomicOr(b.err, kErrKvRange);
+        return false;
+    }
+    at = (uint32_t)page * c.page + (uint32_t)r * c.row;
+    sat = page * c.spage + r;
+    return true;
+}
+
+template <class C>
+__device__ __forceinline__ C* kv_elem(uint8_t* base, uint32_t units) {
+    return reinterpret_cast<C*>(base + (unsigned long long)units * 64);
+}
+
+// One group of D / 8 lanes per (token, U heads): each lane holds 8 values of each row, k and v.
+// Bound by memory: every value is read once and written once.
+template <class T, class C, int D, int U>
+__global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, KvRows r) {
+    constexpr int GL = D / 8;
+    const int chunks = (c.n_heads + U - 1) / U;
+    const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL;
+    const int l = threadIdx.x & (GL - 1);
+    const int t = (int)min(g / chunks, (long long)b.n_tok - 1), h0 = (int)(g % chunks) * U;
+    const bool real = g < (long long)b.n_tok * chunks;
+    const T* src[2] = {(const T*)r.k + t * r.ldk + l * 8, (const T*)r.v + t * r.ldv + l * 8};
+    float x[2][U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) Elem<T>::load8(src[w] + min(h0 + u, c.n_heads - 1) * D, x[w][u]);
+    uint32_t at = 0;
+    long long sat = 0;
+    const bool has = kv_slot<GL>(c, b, t, at, sat) && real;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int h = h0 + u;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            C* dst = kv_elem<C>(w ? c.v : c.k, at + (uint32_t)h * c.head) + l * 8;
+            if constexpr (sizeof(C) == 1) {
+                float m = 0.f;
+                bool fin = true;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    m = fmaxf(m, fabsf(x[w][u][i]));
+                    fin = fin && fabsf(x[w][u][i]) <= 3.402823466e38f;
+                }
+#pragma unroll
+                for (int o = GL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const uint32_t all = __ballot_sync(0xffffffffu, fin), mine = (GL == 8 ? 0xffu : 0xffffu) << (lane_id() & ~(GL - 1));
+                fin = (all & mine) == mine;
+                const float scale = fin ? m * (1.f / 127.f) : __int_as_float(0x7fffffff);
+                uint32_t q[2] = {0, 0};
+                if (scale > 0.f) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float v = fminf(fmaxf(rintf(__fdiv_rn(x[w][u][i], scale)), -127.f), 127.f);
+                        q[i >> 2] |= ((uint32_t)(int)v & 255u) << (8 * (i & 3));
+                    }
+                }
+                if (has && h < c.n_heads) {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+                    if (l == 0) (w ? c.vs : c.ks)[sat + (long long)h * c.page_size] = scale;
+                }
+            } else {
+                if (has && h < c.n_heads) Elem<C>::store8(dst, x[w][u]);
+            }
+        }
+    }
+}
+
+template <class T, class C, int D, int U>
+__global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvRows r) {
+    constexpr int GL = D / 8;
+    const int chunks = (c.n_heads + U - 1) / U;
+    const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL;
+    const int l = threadIdx.x & (GL - 1);
+    const int t = (int)min(g / chunks, (long long)b.n_tok - 1), h0 = (int)(g % chunks) * U;
+    uint32_t at = 0;
+    long long sat = 0;
+    if (!kv_slot<GL>(c, b, t, at, sat) || g >= (long long)b.n_tok * chunks) return;
+    float x[2][U][8], sc[2][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int h = min(h0 + u, c.n_heads - 1);
+            Elem<C>::load8(kv_elem<C>(w ? c.v : c.k, at + (uint32_t)h * c.head) + l * 8, x[w][u]);
+            if constexpr (sizeof(C) == 1) sc[w][u] = __ldg((w ? c.vs : c.ks) + sat + (long long)h * c.page_size);
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            if (h0 + u >= c.n_heads) continue;
+            if constexpr (sizeof(C) == 1)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[w][u][i] *= sc[w][u];
+            Elem<T>::store8((T*)(w ? r.v : r.k) + t * (w ? r.ldv : r.ldk) + (h0 + u) * D + l * 8, x[w][u]);
+        }
+}
+
+namespace {
+
+template <class T, class C, int D>
+cudaError_t launch(bool write, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
+    constexpr int U = 2;
+    const long long groups = (long long)b.n_tok * ((c.n_heads + U - 1) / U);
+    const unsigned grid = (unsigned)((groups * (D / 8) + 255) / 256);
+    if (write)
+        kv_append_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r);
+    else
+        kv_read_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r);
+    return cudaGetLastError();
+}
+
+template <class T, int D>
+cudaError_t by_cache(bool write, int ct, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
+    if (ct == T_F16) return launch<T, __half, D>(write, c, b, r, s);
+    if (ct == T_BF16) return launch<T, __nv_bfloat16, D>(write, c, b, r, s);
+    return launch<T, int8_t, D>(write, c, b, r, s);
+}
+
+template <int D>
+cudaError_t by_type(bool write, int ct, int dt, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
+    if (dt == T_F32) return by_cache<float, D>(write, ct, c, b, r, s);
+    if (dt == T_F16) return by_cache<__half, D>(write, ct, c, b, r, s);
+    return by_cache<__nv_bfloat16, D>(write, ct, c, b, r, s);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(int ct, int dt, int head_dim, const KvDev& c, const KvBatchDev& b, const KvRows& r,
+                             cudaStream_t s) {
+    return head_dim == 64 ? by_type<64>(true, ct, dt, c, b, r, s) : by_type<128>(true, ct, dt, c, b, r, s);
+}
+cudaError_t launch_kv_read(int ct, int dt, int head_dim, const KvDev& c, const KvBatchDev& b, const KvRows& r,
+                           cudaStream_t s) {
+    return head_dim == 64 ? by_type<64>(false, ct, dt, c, b, r, s) : by_type<128>(false, ct, dt, c, b, r, s);
+}
+
+}  // namespace hc

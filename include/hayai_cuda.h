@@ -262,6 +262,60 @@ int hc_moe_stack_ep_dev(hc_engine* eng, size_t n_layers, const float* const* rou
                         const hc_weights* const* up, const hc_weights* const* down, size_t expert_lo, size_t n_local,
                         float* x, size_t n_tok);
 
+/* ---- paged key/value cache and attention over it ------------------------------------
+ * Counterpart of the reference's KV cache and decode attention (crates/hayai-cpu/src/
+ * kv_cache.rs, attention.rs; device form crates/hayai-opencl/src/attn.rs), over pages that
+ * sequences of a batch share out of one pool.  All pointers are device memory of the engine's
+ * GPU; the calls enqueue on the engine's stream.
+ *
+ * hc_kv_cache: one layer's pool.  k and v hold n_pages x n_heads x page_size rows of head_dim
+ * (64 or 128) elements: F16, BF16, or 8-bit codes (type 24, GGUF's I8) with one f32 scale per row,
+ * value = code * scale.  Row (page, head, r) starts at page * page_stride + head * head_stride +
+ * r * row_stride elements; strides are whole multiples of 64 bytes.  Scale (page, head, r) is at
+ * page * scale_page_stride + head * page_size + r.
+ *
+ * hc_kv_batch: n_seq sequences.  Sequence s has kv_len[s] tokens, at positions 0.. of the pages
+ * page_table[s * table_stride + position / page_size]; its last q_start[s+1] - q_start[s] tokens
+ * are the step's new ones, rows [q_start[s], q_start[s+1]) of the packed row arrays of n_tok rows
+ * (q_start ascends; rows that no sequence has are left alone, as are tokens before position 0).
+ * max_new is the host's bound on any sequence's new tokens (0: n_tok); a sequence with more is
+ * still computed, at lower speed.  Page numbers, lengths or offsets out of range touch no
+ * memory out of the pool: they are cut to it, and hc_sync reports HC_ERR_INVALID. */
+#define HC_KV_MAX_SEQ 4096
+typedef struct hc_kv_cache {
+    int type, n_pages, n_heads, page_size, head_dim;
+    void *k, *v;
+    float *k_scale, *v_scale; /* 8-bit codes only */
+    size_t page_stride, head_stride, row_stride, scale_page_stride;
+} hc_kv_cache;
+typedef struct hc_kv_batch {
+    int n_seq, n_tok, max_new, max_pages;
+    const int32_t* page_table;
+    size_t table_stride;
+    const int32_t *q_start, *kv_len;
+} hc_kv_batch;
+
+/* Store the new tokens' rows k, v [n_tok][n_heads * head_dim] (leading dimensions ldk, ldv; dtype
+ * F32, F16 or BF16) in the cache.  8-bit: scale = max|x| * f32(1/127) and code = x / scale to
+ * nearest even, both in f32; a row that is not finite reads back as NaN. */
+int hc_kv_append_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, int dtype, const void* k,
+                     size_t ldk, const void* v, size_t ldv);
+
+/* Gather the same rows back out of the cache, as the values they stand for (with kv_len[s] new
+ * tokens for a sequence: all of it). */
+int hc_kv_read_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, int dtype, void* k, size_t ldk,
+                   void* v, size_t ldv);
+
+/* out_i = sum_j softmax_j(scale q_i . k_j) v_j for the new tokens' n_heads query heads (q, out
+ * [n_tok][n_heads * head_dim], leading dimensions ldq, ldo, of one dtype), n_heads a multiple of
+ * the cache's (query head h reads kv head h / (n_heads / cache heads)).  causal: a token sees the
+ * positions up to its own, of which window > 0 leaves the last `window` and the first `sink`; else
+ * all kv_len.  lse (NULL or [n_tok][n_heads]) receives log sum_j exp(scale q_i . k_j).  A token
+ * that sees nothing gets out 0 and lse -inf. */
+int hc_attn_paged_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, int dtype, size_t n_heads,
+                      const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale, int causal, int window,
+                      int sink);
+
 /* ---- synthetic data ----------------------------------------------------------------
  * Seeded N(mean, std^2) floats on the device (splitmix64 at a position + Box-Muller in
  * double; the same stream as the test oracle's generator up to last-bit differences of

@@ -15,6 +15,35 @@ pub struct hc_pending {
     _p: [u8; 0],
 }
 
+#[repr(C)]
+pub struct hc_kv_cache {
+    pub ggml_type: c_int,
+    pub n_pages: c_int,
+    pub n_heads: c_int,
+    pub page_size: c_int,
+    pub head_dim: c_int,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub page_stride: usize,
+    pub head_stride: usize,
+    pub row_stride: usize,
+    pub scale_page_stride: usize,
+}
+#[repr(C)]
+pub struct hc_kv_batch {
+    pub n_seq: c_int,
+    pub n_tok: c_int,
+    pub max_new: c_int,
+    pub max_pages: c_int,
+    pub page_table: *const i32,
+    pub table_stride: usize,
+    pub q_start: *const i32,
+    pub kv_len: *const i32,
+}
+
+pub const HC_KV_MAX_SEQ: c_int = 4096;
 pub const HC_OK: c_int = 0;
 pub const HC_ERR_INVALID: c_int = 1;
 pub const HC_ERR_UNSUPPORTED: c_int = 2;
@@ -106,6 +135,13 @@ extern "C" {
                                gate: *const *const hc_weights, up: *const *const hc_weights,
                                down: *const *const hc_weights, expert_lo: usize, n_local: usize, x: *mut f32,
                                n_tok: usize) -> c_int;
+    pub fn hc_kv_append_dev(eng: *mut hc_engine, cache: *const hc_kv_cache, batch: *const hc_kv_batch, dtype: c_int,
+                            k: *const c_void, ldk: usize, v: *const c_void, ldv: usize) -> c_int;
+    pub fn hc_kv_read_dev(eng: *mut hc_engine, cache: *const hc_kv_cache, batch: *const hc_kv_batch, dtype: c_int,
+                          k: *mut c_void, ldk: usize, v: *mut c_void, ldv: usize) -> c_int;
+    pub fn hc_attn_paged_dev(eng: *mut hc_engine, cache: *const hc_kv_cache, batch: *const hc_kv_batch, dtype: c_int,
+                             n_heads: usize, q: *const c_void, ldq: usize, out: *mut c_void, ldo: usize,
+                             lse: *mut f32, scale: f32, causal: c_int, window: c_int, sink: c_int) -> c_int;
     pub fn hc_synth_normal_dev(eng: *mut hc_engine, seed: u64, n: usize, mean: f32, stdv: f32, out: *mut f32) -> c_int;
     pub fn hc_quantize_dev(eng: *mut hc_engine, ggml_type: c_int, x: *const f32, n: usize, out: *mut u8) -> c_int;
 }

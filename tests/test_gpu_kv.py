@@ -1,0 +1,463 @@
+"""GPU tests of the paged key/value cache (kv_append_dev, kv_read_dev) and of the attention over it
+(attn_paged_dev) against their definitions in 64 bits.
+
+Tolerances, from the number formats alone (u = half a unit in the last place, A_i = sum_j p_ij |v_j|,
+which every rounding of a weight p_ij or of a product is relative to):
+  * cache: codes and scales exactly; values read back exactly (one rounding of code * scale);
+  * attention in 16 bits: the weights are rounded to at most 8 significant bits (u = 2^-9), the
+    result to its type (2^-9 or 2^-12): |err| <= 2^-8 (A + |out|); where both the cache and the rows
+    are float16 the weights keep 11 bits: 2^-10 (A + |out|);
+  * attention in 32 bits: weights of at least 16 bits (2^-17), scores of 22 bits or more with f32
+    sums of up to 128 products (128 * 2^-24 of sum |q k| scale, about 16 here): 2^-13 (A + |out|)
+    holds elementwise at worst, 1e-5 in the 2-norm, where errors of random sign average out;
+  * lse: the scores' error, 128 * 2^-24 * 16 < 2^-12, and f32's own of |lse|.
+"""
+import math
+
+import pytest
+import torch
+
+import hayai_b200 as hb
+from hayai_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+T = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i8": torch.int8}
+
+
+@pytest.fixture(autouse=True)
+def _stream(engine):
+    engine.set_stream(torch.cuda.current_stream())
+    yield
+    engine.sync()
+    engine.set_stream(None)
+
+
+def quantised(x):
+    scale = x.abs().amax(-1) / 127.0
+    codes = torch.where(scale[..., None] > 0, (x / scale[..., None]).round().clamp(-127, 127), torch.zeros_like(x))
+    return codes.to(torch.int8), scale
+
+
+class Setup:
+    """A pool with shuffled pages, of which the slots that no token has hold NaN (16-bit) or NaN scales."""
+
+    def __init__(self, lens, kv_heads, dim, page, cache, seed=1, order="phrd", extra=2, spread=1.0):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.new, self.kv = [a for a, _ in lens], [b for _, b in lens]
+        self.page, self.kv_heads, self.dim, self.type = page, kv_heads, dim, cache
+        need = [-(-max(k, 0) // page) for k in self.kv]
+        self.n_pages = sum(need) + extra
+        perm = torch.randperm(self.n_pages, generator=g, device=DEV, dtype=torch.int32)
+        self.table = torch.full((len(lens), max(need + [1])), -7, dtype=torch.int32, device=DEV)
+        used = torch.zeros(self.n_pages, page, dtype=torch.bool, device=DEV)
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = perm[at:at + n]
+            pos = torch.arange(max(self.kv[i], 0), device=DEV)
+            used[self.table[i].long()[pos // page], pos % page] = True
+            at += n
+        shape = (self.n_pages, kv_heads, page, dim)
+        self.pool, self.scale = [], []
+        for w in range(2):
+            x = torch.randn(shape, generator=g, device=DEV) * spread
+            if cache == "i8":
+                c, s = quantised(x)
+                s[~used[:, None].expand(s.shape)] = math.nan
+            else:
+                c, s = x.to(T[cache]), None
+                c[~used[:, None, :, None].expand(c.shape)] = math.nan
+            if order == "prhd":  # rows of all heads together
+                c = c.transpose(1, 2).contiguous().transpose(1, 2)
+            elif order == "both":  # k and v of a page side by side, in a pool of three layers
+                big = torch.zeros((self.n_pages, 3, 2) + shape[1:], dtype=c.dtype, device=DEV)
+                big[:, 1, w] = c
+                c = big[:, 1, w]
+            self.pool.append(c)
+            self.scale.append(s)
+        self.q_start = torch.tensor([0] + self.new, device=DEV).cumsum(0).to(torch.int32)
+        self.kv_len = torch.tensor(self.kv, dtype=torch.int32, device=DEV)
+        self.rows = sum(self.new)
+        self.g = g
+        self.cache = hb.KvCache(*self.pool, *self.scale)
+        self.batch = hb.KvBatch(self.table, self.q_start, self.kv_len, self.rows, max(self.new + [0]))
+
+    def q(self, heads, dtype, scale=1.0):
+        return (torch.randn(self.rows, heads, self.dim, generator=self.g, device=DEV) * scale).to(T[dtype])
+
+    def values(self, w, i, lo, hi):
+        pos = torch.arange(lo, hi, device=DEV)
+        p, r = self.table[i].long()[pos // self.page], pos % self.page
+        x = self.pool[w][p, :, r].double()
+        return x if self.scale[w] is None else x * self.scale[w][p, :, r].double()[..., None]
+
+    def attention(self, q, scale=None, causal=True, window=0, sink=0):
+        """(out, lse, A) in 64 bits."""
+        scale = self.dim ** -0.5 if scale is None else scale
+        heads = q.shape[1]
+        group = heads // self.kv_heads
+        out = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+        amp = torch.zeros_like(out)
+        lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device=DEV)
+        done = 0
+        for i, (n, k) in enumerate(zip(self.new, self.kv)):
+            if n and k > 0:
+                K, V = self.values(0, i, 0, k), self.values(1, i, 0, k)
+                ip = torch.arange(k - n, k, device=DEV).view(n, 1)
+                jp = torch.arange(k, device=DEV).view(1, k)
+                see = (jp <= ip) if causal else torch.ones(n, k, dtype=torch.bool, device=DEV)
+                if window:
+                    see = see & ((ip - jp < window) | (jp < sink))
+                for h in range(heads):
+                    s = (q[done:done + n, h].double() @ K[:, h // group].T) * scale
+                    s = torch.where(see, s, -math.inf)
+                    m = s.amax(-1, keepdim=True)
+                    m = torch.where(m == -math.inf, torch.zeros_like(m), m)
+                    p = torch.where(see, (s - m).exp(), torch.zeros_like(s))
+                    tot = p.sum(-1, keepdim=True)
+                    w = torch.where(tot > 0, p / tot, torch.zeros_like(p))
+                    vis = see.any(0)  # a value that no row sees is not looked at
+                    v = torch.where(vis[:, None], V[:, h // group], torch.zeros_like(V[:, 0]))
+                    out[done:done + n, h] = w @ v
+                    amp[done:done + n, h] = w @ v.abs()
+                    lse[done:done + n, h] = (m + tot.log()).squeeze(-1)
+            done += n
+        return out, lse, amp
+
+
+def check(engine, s, heads, dtype, q=None, **kw):
+    q = s.q(heads, dtype) if q is None else q
+    out = torch.full_like(q, math.nan)
+    lse = torch.full(q.shape[:2], math.nan, device=DEV)
+    engine.attn_paged_dev(s.cache, s.batch, q, out, lse=lse, **kw)
+    engine.sync()
+    ref, ref_lse, amp = s.attention(q, **kw)
+    got = out.double()
+    c = 2.0 ** -13 if dtype == "f32" else 2.0 ** -10 if dtype == s.type == "f16" else 2.0 ** -8
+    assert torch.isfinite(got).all()
+    worst = ((got - ref).abs() - c * (amp + ref.abs())).max().item() if got.numel() else 0.0
+    assert worst <= 1e-30, f"off by {worst} more than its bound"
+    if dtype == "f32" and got.numel():
+        rel = ((got - ref).norm() / ref.norm().clamp_min(1e-300)).item()
+        assert rel <= 1e-5, rel
+    none = ref_lse == -math.inf
+    assert torch.equal(lse == -math.inf, none) and (got[none] == 0).all()
+    off = (lse.double() - ref_lse)[~none].abs() - 2.0 ** -12 - ref_lse[~none].abs() * 2.0 ** -20
+    assert not off.numel() or off.max().item() <= 0, off.max().item()
+    return out, lse
+
+
+# ------------------------------------------------------------------ the cache
+LENS = [(1, 1), (3, 3), (0, 0), (1, 40), (17, 100), (0, 9), (5, 5)]
+
+
+@pytest.mark.parametrize("cache", ["i8", "f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,kv_heads,page,order", [(64, 3, 16, "phrd"), (128, 8, 24, "prhd"), (128, 1, 1, "phrd"),
+                                                     (64, 5, 100, "both")])
+def test_append_then_read(engine, cache, dtype, dim, kv_heads, page, order):
+    s = Setup(LENS, kv_heads, dim, page, cache, order=order)
+    before = [p.clone() for p in s.pool]
+    x = [(torch.randn(s.rows, kv_heads, dim, generator=s.g, device=DEV) * 10 ** w).to(T[dtype]) for w in (0, 1)]
+    x[0][2] = 0  # a row of zeros
+    if dtype == "f32":
+        x[1][4, 0] = 1e-44  # a scale that is not a normal number
+    engine.kv_append_dev(s.cache, s.batch, *x)
+    back = [torch.full_like(t, math.nan) for t in x]
+    engine.kv_read_dev(s.cache, s.batch, *back)
+    engine.sync()
+    written = torch.zeros(s.n_pages, page, dtype=torch.bool, device=DEV)
+    done = 0
+    for i, (n, k) in enumerate(zip(s.new, s.kv)):
+        pos = torch.arange(k - n, k, device=DEV)
+        p, r = s.table[i].long()[pos // page], pos % page
+        written[p, r] = True
+        for w in range(2):
+            v = x[w][done:done + n].float()
+            if cache == "i8":
+                codes, scale = quantised(v)
+                assert torch.equal(s.pool[w][p, :, r], codes) and torch.equal(s.scale[w][p, :, r], scale)
+                v = codes.float() * scale[..., None]
+            else:
+                v = v.to(T[cache])
+                assert torch.equal(s.pool[w][p, :, r], v)
+            assert torch.equal(back[w][done:done + n], v.float().to(T[dtype]))
+        done += n
+    for w in range(2):  # nothing else is touched
+        rest = ~written[:, None, :, None].expand(before[w].shape)
+        a, b = s.pool[w][rest].float(), before[w][rest].float()
+        assert torch.equal(a.nan_to_num(7e4), b.nan_to_num(7e4))
+
+
+def test_rows_that_are_not_finite_read_back_as_nan(engine):
+    s = Setup([(4, 4)], 2, 64, 16, "i8")
+    x = s.q(2, "f32")
+    x[1, 0, 3], x[2, 1, 9] = math.nan, -math.inf
+    engine.kv_append_dev(s.cache, s.batch, x, x)
+    back = [torch.zeros_like(x) for _ in range(2)]
+    engine.kv_read_dev(s.cache, s.batch, *back)
+    engine.sync()
+    bad = torch.zeros(4, 2, dtype=torch.bool, device=DEV)
+    bad[1, 0] = bad[2, 1] = True
+    for b in back:
+        assert b[bad].isnan().all() and b[~bad].isfinite().all()
+
+
+def test_packed_projection_rows(engine):
+    """q, k and v as slices of one projection's rows [n_tok][(heads + 2 kv_heads) * dim]."""
+    s = Setup([(5, 70), (2, 2)], 2, 64, 16, "i8", extra=3)
+    qkv = torch.randn(s.rows, 8, 64, generator=s.g, device=DEV)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    engine.kv_append_dev(s.cache, s.batch, k, v)
+    wide = torch.full((s.rows, 6, 64), math.nan, device=DEV)
+    ref, _, amp = s.attention(q)
+    engine.attn_paged_dev(s.cache, s.batch, q, wide[:, 1:5])
+    engine.sync()
+    assert ((wide[:, 1:5].double() - ref).abs() <= 2.0 ** -13 * (amp + ref.abs()) + 1e-30).all()
+    assert wide[:, 0].isnan().all() and wide[:, 5].isnan().all()
+
+
+# ------------------------------------------------------------------ attention
+ODD = [(1, n) for n in (1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 257, 1000)] + [(0, 0), (0, 5)]
+
+
+@pytest.mark.parametrize("cache", ["i8", "f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(9, 3, 64, 16), (32, 8, 128, 16), (16, 2, 128, 64), (5, 1, 128, 1),
+                                                     (2, 2, 64, 100), (40, 2, 64, 24)])
+def test_single_tokens(engine, cache, dtype, heads, kv_heads, dim, page):
+    check(engine, Setup(ODD, kv_heads, dim, page, cache), heads, dtype)
+
+
+CHUNKS = {"one": [(130, 130)], "tail": [(64, 500), (1, 300), (0, 0), (257, 1000)], "few": [(2, 40), (5, 600), (9, 9), (3, 129)],
+          "mixed": [(1, 77), (300, 300), (1, 1), (33, 2000), (1, 700), (128, 128), (129, 385)]}
+
+
+@pytest.mark.parametrize("cache", ["i8", "f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", list(CHUNKS))
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 1, 128, 16), (6, 2, 64, 24), (8, 8, 128, 64)])
+def test_chunks(engine, cache, dtype, lens, heads, kv_heads, dim, page):
+    check(engine, Setup(CHUNKS[lens], kv_heads, dim, page, cache), heads, dtype)
+
+
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("window,sink", [(1, 0), (16, 4), (100, 1), (128, 130), (5000, 3), (37, 10000)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_and_first_tokens(engine, cache, dtype, window, sink, dim):
+    check(engine, Setup(CHUNKS["mixed"] + [(1, 1500), (4, 260)], 2, dim, 16, cache), 8, dtype, window=window, sink=sink)
+
+
+@pytest.mark.parametrize("cache,dtype", [("i8", "f16"), ("f16", "f32"), ("bf16", "bf16")])
+def test_every_position_seen(engine, cache, dtype):
+    check(engine, Setup(CHUNKS["mixed"], 2, 128, 32, cache), 4, dtype, causal=False)
+
+
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "f32"), ("f16", "f16"), ("i8", "bf16")])
+def test_tokens_before_the_first_position_see_nothing(engine, cache, dtype):
+    """More new tokens than the sequence holds: the first ones have no position, and rows 0 / -inf."""
+    out, lse = check(engine, Setup([(6, 2), (140, 10), (3, 0), (1, 5)], 2, 64, 16, cache), 4, dtype)
+    assert (lse[:4] == -math.inf).all() and (out[:4] == 0).all()
+
+
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("i8", "bf16")])
+@pytest.mark.parametrize("lens", [[(1, 20000)], [(40, 9001)], [(1, 5), (1, 30011), (1, 64)]])
+def test_long_and_split(engine, cache, dtype, lens):
+    s = Setup(lens, 2, 128, 64, cache)
+    q = s.q(8, dtype)
+    a = check(engine, s, 8, dtype, q=q)
+    b = check(engine, s, 8, dtype, q=q)  # the same bits again
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("lens", [[(1, 3000)], [(200, 3000)]])
+def test_scores_that_rise_and_fall(engine, lens):
+    """Scores over hundreds, the largest late: the running maximum moves often, weights underflow."""
+    for cache, dtype in (("i8", "f32"), ("f16", "f16"), ("bf16", "bf16")):
+        s = Setup(lens, 1, 64, 16, cache)
+        ramp = torch.linspace(0.01, 6.0, 3000, device=DEV)
+        pos = torch.arange(3000, device=DEV)
+        p, r = s.table[0].long()[pos // 16], pos % 16
+        if cache == "i8":
+            s.scale[0][p, :, r] *= ramp[:, None]
+        else:
+            s.pool[0][p, :, r] = (s.pool[0][p, :, r].float() * ramp[:, None, None]).to(T[cache])
+        q = s.q(4, dtype)
+        out = torch.empty_like(q)
+        engine.attn_paged_dev(s.cache, s.batch, q, out, scale=2.0)
+        ref, _, amp = s.attention(q, scale=2.0)
+        # scores up to 800: 128 * 2^-24 * sum |q k| scale is up to 2^-17 * 2500 in a weight's exponent;
+        # weights under f32's smallest normal (and so results made of them alone) may be flushed
+        c = 2.0 ** -8 + 2500 * 2.0 ** -17
+        assert ((out.double() - ref).abs() <= c * (amp + ref.abs()) + 1e-30).all(), cache
+
+
+@pytest.mark.parametrize("small", [1e-6, 1e6])
+def test_values_of_any_size(engine, small):
+    """8-bit values whose scales differ by many orders between tokens."""
+    for lens, dtype in (([(1, 700)], "f32"), ([(1, 700)], "bf16"), ([(150, 700)], "bf16"), ([(150, 700)], "f32")):
+        s = Setup(lens, 2, 128, 16, "i8")
+        pos = torch.arange(0, 700, 2, device=DEV)
+        s.scale[1][s.table[0].long()[pos // 16], :, pos % 16] *= small
+        check(engine, s, 4, dtype)
+
+
+@pytest.mark.parametrize("lens", [[(5, 100)], [(130, 300)]])
+@pytest.mark.parametrize("cache,dtype", [("f16", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("i8", "bf16")])
+def test_not_finite_where_masked(engine, lens, cache, dtype):
+    """A later new token's key and value are not finite: the tokens before it do not see them, and
+    those from it on get NaN."""
+    s = Setup(lens, 2, 128, 16, cache)
+    n, k = lens[0]
+    at = k - 3
+    p, r = int(s.table[0, at // 16]), at % 16
+    clean = s.attention(s.q(4, dtype))  # advances the generator alike
+    s.g.manual_seed(5)
+    q = s.q(4, dtype)
+    ref, _, amp = s.attention(q)
+    for w, bad in ((0, math.nan), (1, math.inf)):
+        if cache == "i8":
+            s.scale[w][p, :, r] = bad
+        else:
+            s.pool[w][p, :, r, ::3] = bad
+    out = torch.empty_like(q)
+    engine.attn_paged_dev(s.cache, s.batch, q, out)
+    engine.sync()
+    assert clean is not None and torch.isfinite(out[:n - 3]).all()
+    assert ((out.double() - ref).abs()[:n - 3] <= (2.0 ** -8 * (amp + ref.abs()))[:n - 3]).all()
+    assert out[n - 3:].isnan().any(-1).all()
+
+
+@pytest.mark.parametrize("order", ["prhd", "both"])
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "bf16")])
+def test_orders_of_the_pool(engine, order, cache, dtype):
+    check(engine, Setup(CHUNKS["mixed"], 2, 64, 16, cache, order=order), 4, dtype)
+
+
+def test_offsets_past_32_bits(engine):
+    """A pool of 6 GiB codes: the sequence's pages lie past 4 GiB."""
+    n_pages, page = 6 << 30 >> 13, 64
+    k = torch.zeros(n_pages, 1, page, 128, dtype=torch.int8, device=DEV)
+    sc = torch.zeros(n_pages, 1, page, device=DEV)
+    table = torch.arange(n_pages - 9, n_pages, dtype=torch.int32, device=DEV).flip(0)[None]
+    q_start = torch.tensor([0, 550], dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor([550], dtype=torch.int32, device=DEV)
+    cache, batch = hb.KvCache(k, k, sc, sc), hb.KvBatch(table, q_start, kv_len, 550, 550)
+    x = torch.randn(550, 1, 128, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))
+    engine.kv_append_dev(cache, batch, x, x)
+    back = [torch.empty_like(x) for _ in range(2)]
+    engine.kv_read_dev(cache, batch, *back)
+    codes, scale = quantised(x)
+    v = codes.float() * scale[..., None]
+    assert torch.equal(back[0], v) and torch.equal(back[1], v)
+    for lo in (0, 549):
+        b = hb.KvBatch(table, torch.tensor([0, 550 - lo], dtype=torch.int32, device=DEV), kv_len, 550 - lo)
+        q, out = x[lo:], torch.empty_like(x[lo:])
+        engine.attn_paged_dev(cache, b, q, out)
+        s = (q[:, 0].double() @ v[:, 0].double().T) * 128 ** -0.5
+        s = s.masked_fill(torch.arange(550, device=DEV)[None] > torch.arange(lo, 550, device=DEV)[:, None], -math.inf)
+        ref = s.softmax(-1) @ v[:, 0].double()
+        assert ((out[:, 0].double() - ref).norm() / ref.norm()).item() <= 1e-5
+
+
+def test_another_stream_and_a_captured_graph(engine):
+    """The calls run on the engine's stream, and a captured graph follows lengths changed in place."""
+    s = Setup([(1, 600), (1, 90)], 2, 128, 16, "i8")
+    q, out = s.q(8, "bf16"), torch.empty(2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    engine.attn_paged_dev(s.cache, s.batch, q, out)  # workspaces exist before the capture
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    engine.set_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        engine.attn_paged_dev(s.cache, s.batch, q, out)
+    for kv in ([600, 90], [1, 33], [599, 0]):
+        s.kv_len.copy_(torch.tensor(kv, dtype=torch.int32))
+        s.kv = kv
+        ref, _, amp = s.attention(q)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert ((out.double() - ref).abs() <= 2.0 ** -8 * (amp + ref.abs())).all()
+
+
+@pytest.mark.parametrize("what", ["page", "len", "q_start"])
+@pytest.mark.parametrize("new", [1, 150])
+def test_device_values_out_of_range_are_reported(engine, what, new):
+    s = Setup([(new, 200), (new, 250)], 2, 64, 16, "i8")
+    {"page": s.table, "len": s.kv_len, "q_start": s.q_start}[what].view(-1)[1] = {"page": 1 << 20, "len": 100000,
+                                                                                 "q_start": 1 << 20}[what]
+    q = s.q(4, "f16")
+    with pytest.raises(hb.CudaError) as e:
+        engine.attn_paged_dev(s.cache, s.batch, q, torch.empty_like(q))
+        engine.sync()
+    assert e.value.code == _lib.HC_ERR_INVALID
+    engine.sync()  # reported once
+
+
+def test_empty_batches(engine):
+    s = Setup([(0, 4), (0, 0)], 1, 64, 16, "f16")
+    q = s.q(2, "f16")
+    engine.attn_paged_dev(s.cache, s.batch, q, q)
+    engine.kv_append_dev(s.cache, s.batch, q[:, :1], q[:, :1])
+    none = hb.KvBatch(s.table[:0], s.q_start[:1], s.kv_len[:0], 0)
+    engine.attn_paged_dev(s.cache, none, q, q)
+
+
+def test_rows_of_no_sequence_are_left_alone(engine):
+    s = Setup([(2, 50), (3, 80)], 1, 64, 16, "f16")
+    batch = hb.KvBatch(s.table, s.q_start + 1, s.kv_len, 8, 3)
+    q = torch.randn(8, 4, 64, device=DEV).half()
+    out = torch.full_like(q, 7.0)
+    engine.attn_paged_dev(s.cache, batch, q, out)
+    ref, _, amp = s.attention(q[1:6])
+    assert (out[0] == 7).all() and (out[6:] == 7).all()
+    assert ((out[1:6].double() - ref).abs() <= 2.0 ** -10 * (amp + ref.abs())).all()
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals(engine):
+    s = Setup([(2, 50)], 2, 64, 16, "i8")
+    q, out, kv = s.q(4, "f16"), torch.empty(2, 4, 64, dtype=torch.float16, device=DEV), s.q(2, "f16")
+    k, ks = s.pool[0], s.scale[0]
+    bad = [
+        lambda: hb.KvCache(k.float(), k.float()), lambda: hb.KvCache(k, k), lambda: hb.KvCache(k.half(), k.half(), ks, ks),
+        lambda: hb.KvCache(k.cpu(), k.cpu(), ks, ks), lambda: hb.KvCache(k[0], k[0], ks[0], ks[0]),
+        lambda: hb.KvCache(k.transpose(2, 3), k.transpose(2, 3), ks, ks),
+        lambda: hb.KvBatch(s.table.long(), s.q_start, s.kv_len, 2), lambda: hb.KvBatch(s.table, s.q_start[:1], s.kv_len, 2),
+        lambda: hb.KvBatch(s.table, s.q_start, s.kv_len, -1),
+        lambda: engine.attn_paged_dev(s.cache, s.batch, q[:1], out[:1]),
+        lambda: engine.attn_paged_dev(s.cache, s.batch, q, out.float()),
+        lambda: engine.attn_paged_dev(s.cache, s.batch, q.double(), out.double()),
+        lambda: engine.attn_paged_dev(s.cache, s.batch, q.cpu(), out),
+        lambda: engine.attn_paged_dev(s.cache, s.batch, q, out, lse=torch.empty(2, 3, device=DEV)),
+        lambda: engine.attn_paged_dev(s.cache, s.batch, q.transpose(1, 2).contiguous().transpose(1, 2), out),
+        lambda: engine.kv_append_dev(s.cache, s.batch, q, q), lambda: engine.kv_read_dev(s.cache, s.batch, kv, kv.float()),
+    ]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+    odd = s.q(3, "f16")
+    native = [
+        (lambda: engine.attn_paged_dev(s.cache, s.batch, odd, torch.empty_like(odd)), _lib.HC_ERR_INVALID),
+        (lambda: engine.attn_paged_dev(s.cache, s.batch, q, out, window=-1), _lib.HC_ERR_INVALID),
+        (lambda: engine.attn_paged_dev(s.cache, s.batch, q, out, window=8, causal=False), _lib.HC_ERR_INVALID),
+        (lambda: engine.attn_paged_dev(s.cache, s.batch, q, out, scale=math.inf), _lib.HC_ERR_INVALID),
+    ]
+    for dim in (32, 96, 256):
+        x = torch.zeros(3, 2, 16, dim, dtype=torch.float16, device=DEV)
+        c, y = hb.KvCache(x, x), torch.zeros(2, 2, dim, dtype=torch.float16, device=DEV)
+        native.append((lambda c=c, y=y: engine.attn_paged_dev(c, s.batch, y, y), _lib.HC_ERR_UNSUPPORTED))
+    flat = torch.zeros(1 << 16, dtype=torch.float16, device=DEV)
+    c = hb.KvCache(*[flat.as_strided((3, 2, 16, 64), (4096, 2048, 72, 1))] * 2)  # rows 144 bytes apart
+    native.append((lambda: engine.kv_append_dev(c, s.batch, kv, kv), _lib.HC_ERR_INVALID))
+    many = hb.KvBatch(torch.zeros(5000, 1, dtype=torch.int32, device=DEV), torch.zeros(5001, dtype=torch.int32, device=DEV),
+                      torch.zeros(5000, dtype=torch.int32, device=DEV), 2)
+    native.append((lambda: engine.kv_append_dev(s.cache, many, kv, kv), _lib.HC_ERR_INVALID))
+    skew = torch.zeros(2 * 4 * 64 + 1, dtype=torch.float16, device=DEV)[1:].view(2, 4, 64)
+    native.append((lambda: engine.attn_paged_dev(s.cache, s.batch, skew, out), _lib.HC_ERR_INVALID))
+    for f, code in native:
+        with pytest.raises(hb.CudaError) as e:
+            f()
+        assert e.value.code == code, str(e.value)
+    engine.sync()
