@@ -1,0 +1,734 @@
+// attn_few.cu -- attention over the paged cache for sequences with few rows per kv head (single
+// tokens, short drafts): bound by reading the cache.
+//
+//     out_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(c q_i . k_j - m_i),   c = scale log2 e
+// in one pass with the running maximum m_i and sum of every row, lse_i = (m_i + log2 sum) ln 2.
+// m_i need not be the maximum itself, only near it: it moves when a score passes it by 8 (weights
+// up to 2^8), so after the first units a unit's maximum costs one vote.
+//
+// Both products run on the tensor cores transposed, S^T = K Q^T and O^T = V^T P^T with
+// mma.m16n8k16: the cache's rows fill the 16 rows of the first operand, and the 8 query rows of a
+// group of heads the 8 columns, where the plain orientation would leave half or more of 16 query
+// rows empty.  The order of k inside a product is free as long as both operands agree, so every
+// lane takes 16 adjacent bytes of a cache row (8-bit: four k steps; 16-bit: two), and V^T's pairs
+// of tokens come from two rows by PRMT, with no transposed copy.  S^T's accumulators become P^T's
+// operand with one MOVMATRIX per 8 tokens.
+//
+// Formats.  8-bit K codes are exact in f16, 8-bit V codes in bf16 (|code| <= 127); a token's K scale
+// multiplies its score and its V scale its weights, whose range bf16 holds.  Query rows are scaled
+// by a power of two to have their largest element in [1, 2) and rounded to the products' type: f16
+// and bf16 rows are exact or keep 11 bits in f16; f32 rows are split into 2 f16 terms (22 bits) or 3
+// bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11 bits of 16).  Weights are rounded to one
+// f16 or bf16 term (relative error 2^-11 or 2^-9, of the order of the 16-bit results' own rounding),
+// for f32 results to two (2^-16 at worst, or 2^-25 absolute).  All sums are f32; for f32 results a
+// unit's products are added to zero and then to the running sum in FADD, as the tensor cores' own
+// chained additions truncate.
+//
+// One block of 8 warps per SM walks its share of the line of units (attn_rows.cuh); its warps take
+// the units of a tile in turn, each with its own ring of 16-byte asynchronous copies (no block
+// barrier inside a tile; 2 to 3 stages of 8 KB a warp, ~128 KB in flight per SM), whose issue runs
+// ahead over tile boundaries.  At a tile's end the warps' (m, l, O) are joined in shared memory.
+#include <math.h>
+
+#include "attn_rows.cuh"
+
+namespace hc {
+
+constexpr int kFewWarps = 8, kFewThreads = 32 * kFewWarps;
+
+template <class C, int D, int NT>
+struct FewCfg {
+    static constexpr int ES = sizeof(C), CPR = D * ES / 16;  // 16-byte chunks of a row
+    static constexpr int ST = CPR == 16 ? 16 : 32;           // tokens of a unit
+    static constexpr int KB = ST * CPR * 16;                 // bytes of a unit's keys (or values)
+    static constexpr int SB = 2 * KB + (ES == 1 ? 8 * ST : 0);
+    static constexpr int NS = CPR == 4 ? 4 : NT == 1 ? 3 : 2;  // stages of a warp's ring
+    static constexpr int RS = D + 4;                           // row stride of the joining buffer, floats
+};
+
+template <class T, class C>
+struct FewTerms {
+    static constexpr bool kBf = sizeof(C) == 2 && !(__is_same(C, __half));  // bf16 products for the scores
+    static constexpr int Q = sizeof(T) == 4 ? (kBf ? 3 : 2) : (kBf && __is_same(T, __half)) ? 2 : 1;
+    static constexpr int P = sizeof(T) == 4 ? 2 : 1;
+    static constexpr bool pBf = !__is_same(C, __half);  // bf16 weights
+};
+
+// D (+)= A B, 16 x 8 x 16 (mma16816's bf16 twin).
+__device__ __forceinline__ void mma16816_bf(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool BF>
+__device__ __forceinline__ void mma_any(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        mma16816_bf(c, a[0], a[1], a[2], a[3], b0, b1);
+    else
+        mma16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+// The next term of a pair's expansion: (lo, hi) rounded to the products' type, and what is left.
+template <bool BF>
+__device__ __forceinline__ uint32_t split_pair(float& x, float& y) {
+    if constexpr (BF) {
+        const uint32_t u = pack_b2(x, y);
+        x -= __uint_as_float(u << 16);
+        y -= __uint_as_float(u & 0xffff0000u);
+        return u;
+    } else {
+        const uint32_t u = pack_h2(x, y);
+        const float2 f = __half22float2(u32_as_h2(u));
+        x -= f.x;
+        y -= f.y;
+        return u;
+    }
+}
+
+// Copy 16 bytes (or with ok false: 16 zero bytes) to shared memory.
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4_or_zero(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ float lds32f(uint32_t a) {
+    float r;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a));
+    return r;
+}
+
+// Places of 16-byte chunks in a stage, permuted so that the 8 lanes of a load's phase (two rows by
+// four chunks of K, four rows by two chunks of V) touch all banks once.
+template <int CPR>
+__device__ __forceinline__ uint32_t few_k_at(int r, int c) {
+    return (r * CPR + (CPR == 4 ? c : c ^ ((r & 1) << 2))) * 16;
+}
+template <int CPR>
+__device__ __forceinline__ uint32_t few_v_at(int r, int c) {
+    if constexpr (CPR == 4) {
+        const int rr = (r & ~3) | ((r & 1) << 1) | ((r >> 1) & 1);
+        return (rr * 4 + (c ^ (((r >> 2) & 1) << 1))) * 16;
+    } else {
+        return (r * CPR + (c ^ (((r >> 1) & 3) << 1))) * 16;
+    }
+}
+
+// A warp's walk over its units: unit `st` of the item's [0, hi).
+struct FewWalk {
+    AttnIter it;
+    int st, hi, u1;
+    bool live;
+    __device__ __forceinline__ void segment(int u0, int w) {
+        st = max(u0 - it.u_item, 0) + w;
+        hi = min(u1 - it.u_item, it.t.units);
+    }
+    // Skip segments that have no unit for this warp.
+    __device__ __forceinline__ void settle(const AttnArgs& a, int w, int rows, int unit) {
+        while (st >= hi) {
+            if (it.u_item + it.t.units >= u1) {
+                live = false;
+                return;
+            }
+            it.next(a, rows, unit);
+            segment(0, w);
+        }
+    }
+};
+
+template <class T, class C, int D, int NT>
+__global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_constant__ AttnArgs a) {
+    using F = FewCfg<C, D, NT>;
+    using X = FewTerms<T, C>;
+    constexpr int ST = F::ST, CPR = F::CPR, MT = ST / 16, KS = D / 16, ROWS = 8 * NT, I8 = F::ES == 1;
+    constexpr int QB = KS * NT * X::Q * 256;  // the query tile as B operands
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int w = threadIdx.x >> 5, ln = lane_id(), g = ln >> 2, t4 = ln & 3;
+    const uint32_t ring = smem_addr(smem) + w * F::NS * F::SB;
+    uint8_t* const qf = smem + kFewWarps * F::NS * F::SB;
+    float* const red = reinterpret_cast<float*>(qf + QB);  // [4][ROWS][RS]; the schedule's prefix before
+    float* const ml = red + 4 * ROWS * F::RS;              // [8][ROWS][2]
+    float* const rscale = ml + kFewWarps * ROWS * 2;       // [ROWS]
+    __shared__ int last_s;
+
+    int* const pre = reinterpret_cast<int*>(red);
+    const int U = attn_schedule<kFewThreads>(a, ROWS, ST, pre);
+    const int G = min((int)gridDim.x, max(1, U / kFewWarps)), c = blockIdx.x;
+    if (U <= 0 || c >= G) return;
+    const int u0 = attn_begin(c, U, G), u1 = attn_begin(c + 1, U, G);
+    AttnIter it;  // the block's place
+    it.seek(a, pre, u0, ROWS, ST);
+    __syncthreads();  // `pre` is read
+
+    // ---- the copies' walk: units are issued NS - 1 ahead
+    FewWalk pw;
+    pw.it = it;
+    pw.u1 = u1;
+    pw.live = true;
+    pw.segment(u0, w);
+    pw.settle(a, w, ROWS, ST);
+    int pg = -1, pr = 0;  // page and row of this lane's token of the unit to be issued
+    auto look_up = [&]() {
+        pg = -1;
+        if (!pw.live) return;
+        const int v = pw.st * ST + ln;
+        if (ln < ST && v < pw.it.t.nvis) {
+            const int j = v < pw.it.t.n1 ? v : v - pw.it.t.n1 + pw.it.t.lo;
+            const int p = j / a.c.page_size;
+            pr = j - p * a.c.page_size;
+            pg = __ldg(a.b.table + pw.it.s * a.b.table_stride + p);
+            if ((unsigned)pg >= (unsigned)a.c.n_pages) {
+                atomicOr(a.b.err, kErrKvRange);
+                pg = -1;
+            }
+        }
+    };
+    int islot = 0;
+    auto issue = [&]() {
+        if (pw.live) {
+            const uint32_t base = ring + islot * F::SB;
+            const bool ok = pg >= 0;
+            const uint32_t off = ok ? (uint32_t)pg * a.c.page + (uint32_t)pr * a.c.row + (uint32_t)pw.it.hk * a.c.head
+                                    : 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < ST * CPR / 32; ++i) {
+                const int r = (i * 32 + ln) / CPR, ch = ln % CPR;
+                const uint32_t o = __shfl_sync(0xffffffffu, off, r);
+                const bool have = o != 0xffffffffu;
+                const unsigned long long at = have ? (unsigned long long)o * 64 + ch * 16 : 0;
+                cp16_or_zero(base + few_k_at<CPR>(r, ch), a.c.k + at, have);
+                cp16_or_zero(base + F::KB + few_v_at<CPR>(r, ch), a.c.v + at, have);
+            }
+            if constexpr (I8) {
+                const long long so = ok ? pg * a.c.spage + (long long)pw.it.hk * a.c.page_size + pr : 0;
+                cp4_or_zero(base + 2 * F::KB + ln * 4, a.c.ks + so, ok);
+                cp4_or_zero(base + 2 * F::KB + ST * 4 + ln * 4, a.c.vs + so, ok);
+            }
+            islot = islot + 1 == F::NS ? 0 : islot + 1;
+            pw.st += kFewWarps;
+            pw.settle(a, w, ROWS, ST);
+            look_up();
+        }
+        cp_async_commit();
+    };
+    look_up();
+#pragma unroll
+    for (int i = 0; i < F::NS - 1; ++i) issue();
+
+    int cslot = 0;
+    for (;;) {  // the block's tiles
+        const AttnTile& tl = it.t;
+        const int lo = max(u0 - it.u_item, 0), hi = min(u1 - it.u_item, tl.units);
+        // ---- the query tile as B operands
+        for (int r = w; r < ROWS; r += kFewWarps) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (r < tl.nr && ln < D / 4) {
+                const int row = tl.r0 + r, tok = it.q.q0 + row / a.group, h = it.hk * a.group + row % a.group;
+                const T* q = (const T*)a.q + (long long)tok * a.ldq + h * D + 4 * ln;
+                if constexpr (sizeof(T) == 4) {
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(q));
+                    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+                } else {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(q));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint16_t b = (uint16_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
+                        if constexpr (__is_same(T, __half))
+                            x[i] = h2f(b);
+                        else
+                            x[i] = __uint_as_float((uint32_t)b << 16);
+                    }
+                }
+            }
+            float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            // the power of two of m, taken out of the row (none for 0, infinity and the smallest)
+            const uint32_t e = __float_as_uint(m) >> 23;
+            const bool norm = e >= 2 && e <= 252;
+            const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
+            const float up = norm ? __uint_as_float(e << 23) : 1.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] *= down;
+            if (ln == 0) rscale[r] = up * a.scale * 1.44269504f;
+            if (ln < D / 4) {
+                // d = 4 ln + i: 16-byte chunk of the cache row, its k step and the lane that holds it
+                const int ch = I8 ? ln >> 2 : ln >> 1, j = I8 ? 4 * (ch >> 2) + (ln & 3) : 2 * (ch >> 2) + (ln & 1);
+                uint8_t* dst = qf + (j * NT + (r >> 3)) * X::Q * 256 + ((r & 7) * 4 + (ch & 3)) * 8;
+#pragma unroll
+                for (int s = 0; s < X::Q; ++s)
+                    *reinterpret_cast<uint2*>(dst + s * 256) =
+                        make_uint2(split_pair<X::kBf>(x[0], x[1]), split_pair<X::kBf>(x[2], x[3]));
+            }
+        }
+        __syncthreads();
+        float m[NT][2], l[NT][2], o[KS][NT][4], rs[NT][2];
+        int lim[NT][2], wlo[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = n * 8 + 2 * t4 + e;
+                m[n][e] = -INFINITY;
+                l[n][e] = 0.f;
+                rs[n][e] = rscale[r];
+                const int pos = it.q.len - (it.q.q1 - it.q.q0) + (tl.r0 + r) / a.group;
+                lim[n][e] = r >= tl.nr ? -1 : a.causal ? pos : it.q.len - 1;
+                wlo[n][e] = a.window ? pos - a.window + 1 : 0;
+            }
+#pragma unroll
+        for (int d = 0; d < KS; ++d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d][n][e] = 0.f;
+
+        for (int st = lo + w; st < hi; st += kFewWarps) {
+            issue();
+            cp_async_wait(F::NS - 1);
+            __syncwarp();
+            const uint32_t kb = ring + cslot * F::SB, vb = kb + F::KB, sb = kb + 2 * F::KB;
+            cslot = cslot + 1 == F::NS ? 0 : cslot + 1;
+            // ---- S^T = K Q^T
+            float s[MT][NT][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+#pragma unroll
+            for (int cg = 0; cg < CPR / 4; ++cg) {
+                uint4 ka[MT], kc[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    ka[i] = lds128(kb + few_k_at<CPR>(16 * i + g, t4 + 4 * cg));
+                    kc[i] = lds128(kb + few_k_at<CPR>(16 * i + g + 8, t4 + 4 * cg));
+                }
+#pragma unroll
+                for (int jj = 0; jj < (I8 ? 4 : 2); ++jj) {
+                    uint32_t A[MT][4];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const uint32_t wa[4] = {ka[i].x, ka[i].y, ka[i].z, ka[i].w};
+                        const uint32_t wc[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
+                        if constexpr (I8) {  // code + 1152 by PRMT, minus 1152: exact
+                            const uint32_t fa = wa[jj] ^ 0x80808080u, fc = wc[jj] ^ 0x80808080u;
+                            A[i][0] = hsub2_u32(prmt(fa, 0x64646464u, 0x4140u), 0x64806480u);
+                            A[i][1] = hsub2_u32(prmt(fc, 0x64646464u, 0x4140u), 0x64806480u);
+                            A[i][2] = hsub2_u32(prmt(fa, 0x64646464u, 0x4342u), 0x64806480u);
+                            A[i][3] = hsub2_u32(prmt(fc, 0x64646464u, 0x4342u), 0x64806480u);
+                        } else {
+                            A[i][0] = wa[2 * jj];
+                            A[i][1] = wc[2 * jj];
+                            A[i][2] = wa[2 * jj + 1];
+                            A[i][3] = wc[2 * jj + 1];
+                        }
+                    }
+                    const int j = (I8 ? 4 : 2) * cg + jj;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int q = 0; q < X::Q; ++q) {
+                            const uint2 b = *reinterpret_cast<const uint2*>(qf + ((j * NT + n) * X::Q + q) * 256 + ln * 8);
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) mma_any<X::kBf>(s[i][n], A[i], b.x, b.y);
+                        }
+                }
+            }
+            // ---- scores in units of log 2, masked
+            const int v0 = st * ST, v1 = v0 + ST;
+            const int j0 = v0 < tl.n1 ? v0 : v0 - tl.n1 + tl.lo, j1 = v1 - tl.n1 + tl.lo - 1;
+            const bool full = v1 <= tl.nvis &&
+                              (tl.p_lo == tl.p_hi || !a.causal ||
+                               (j1 <= tl.p_lo && (!a.window || v1 <= tl.n1 || (v0 >= tl.n1 && j0 > tl.p_hi - a.window))));
+            float vsc[MT][2];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float ksc[2] = {1.f, 1.f};
+                vsc[i][0] = vsc[i][1] = 1.f;
+                if constexpr (I8) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        ksc[h] = lds32f(sb + (16 * i + 8 * h + g) * 4);
+                        vsc[i][h] = lds32f(sb + ST * 4 + (16 * i + 8 * h + g) * 4);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[i][n][e] *= I8 ? rs[n][e & 1] * ksc[e >> 1] : rs[n][e & 1];
+                        if (!full) {
+                            const int v = v0 + 16 * i + 8 * (e >> 1) + g;
+                            const int j = v < tl.n1 ? v : v - tl.n1 + tl.lo;
+                            const bool see = v < tl.nvis && j <= lim[n][e & 1] && (j >= wlo[n][e & 1] || j < a.sink);
+                            if (!see) s[i][n][e] = -INFINITY;
+                        }
+                    }
+            }
+            // ---- move the maxima where a score passes them by 8
+            bool up = false;
+            float mx[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    mx[n][e] = fmaxf(s[0][n][e], s[0][n][e + 2]);
+                    if constexpr (MT == 2) mx[n][e] = fmaxf(mx[n][e], fmaxf(s[MT - 1][n][e], s[MT - 1][n][e + 2]));
+                    up |= mx[n][e] > m[n][e] + 8.f;
+                }
+            if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = mx[n][e];
+#pragma unroll
+                        for (int q = 4; q < 32; q <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, q));
+                        x = fmaxf(x, m[n][e]);
+                        const float f = x == -INFINITY ? 1.f : ex2(m[n][e] - x);
+                        m[n][e] = x;
+                        l[n][e] *= f;
+#pragma unroll
+                        for (int d = 0; d < KS; ++d) {
+                            o[d][n][e] *= f;
+                            o[d][n][e + 2] *= f;
+                        }
+                    }
+            }
+            // ---- weights, and P^T as B operands
+            uint32_t pb[MT][NT][X::P][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = ex2(s[i][n][e] - (e & 1 ? m1 : m0));
+                        l[n][e & 1] += p[e];
+                        if constexpr (I8) {
+                            p[e] *= vsc[i][e >> 1];
+                            if (!full && s[i][n][e] == -INFINITY) p[e] = 0.f;  // whatever the scale of a masked token
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < X::P; ++q)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            pb[i][n][q][h] = movmatrix(split_pair<X::pBf>(p[2 * h], p[2 * h + 1]));
+                }
+            }
+            // ---- O^T += V^T P^T
+            bool odd = false;  // a value that is not finite in a unit that some row does not see whole
+            if constexpr (!I8) {
+                if (!full) {
+                    constexpr uint32_t E = X::pBf ? 0x7f80u : 0x7c00u;
+#pragma unroll 4
+                    for (int i = 0; i < F::KB / 512; ++i) {
+                        const uint4 x = lds128(vb + i * 512 + ln * 16);
+                        const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) odd |= (y[k] & E) == E || ((y[k] >> 16) & E) == E;
+                    }
+                    odd = __any_sync(0xffffffffu, odd);
+                }
+            }
+            if (odd) {  // rare: 0 * infinity must not reach a row that is masked there, so no products
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll 1
+                    for (int k = 0; k < 16; ++k) {
+                        uint32_t word[KS];
+#pragma unroll
+                        for (int d = 0; d < KS; ++d) {
+                            const uint4 x = lds128(vb + few_v_at<CPR>(16 * i + k, g + 8 * (d >> 2)));
+                            word[d] = (d & 3) == 0 ? x.x : (d & 3) == 1 ? x.y : (d & 3) == 2 ? x.z : x.w;
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float sv = k < 8 ? s[i][n][e] : s[i][n][e + 2];
+                                const float sc = __shfl_sync(0xffffffffu, sv, 4 * (k & 7) + t4);
+                                if (sc == -INFINITY) continue;
+                                const float p = ex2(sc - (m[n][e] == -INFINITY ? 0.f : m[n][e]));
+#pragma unroll
+                                for (int d = 0; d < KS; ++d) {
+                                    const uint32_t lo16 = word[d] & 0xffffu, hi16 = word[d] >> 16;
+                                    o[d][n][e] += p * (X::pBf ? __uint_as_float(lo16 << 16) : h2f((uint16_t)lo16));
+                                    o[d][n][e + 2] += p * (X::pBf ? __uint_as_float(hi16 << 16) : h2f((uint16_t)hi16));
+                                }
+                            }
+                    }
+            } else {
+                constexpr bool EXACT = X::P == 2;
+                if constexpr (I8) {
+                    uint4 vw[MT][4];  // 16 (D = 128) or 8 (D = 64) adjacent values of four tokens
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = 16 * i + 2 * t4 + (k & 1) + 8 * (k >> 1);
+                            if constexpr (D == 128) {
+                                vw[i][k] = lds128(vb + few_v_at<CPR>(r, g));
+                            } else {
+                                const uint2 x = lds64(vb + few_v_at<CPR>(r, g >> 1) + 8 * (g & 1));
+                                vw[i][k] = make_uint4(x.x, x.y, 0, 0);
+                            }
+                        }
+#pragma unroll
+                    for (int d = 0; d < KS; ++d) {
+                        float z[NT][4];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[n][e] = EXACT ? 0.f : o[d][n][e];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t A[4];
+                            const int wi = d >> 1;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {  // e & 1: value 2 d or 2 d + 1; e >> 1: token pair
+                                const uint4 &x = vw[i][2 * (e >> 1)], &y = vw[i][2 * (e >> 1) + 1];
+                                const uint32_t xa = wi == 0 ? x.x : wi == 1 ? x.y : wi == 2 ? x.z : x.w;
+                                const uint32_t ya = wi == 0 ? y.x : wi == 1 ? y.y : wi == 2 ? y.z : y.w;
+                                const uint32_t b = 2 * (d & 1) + (e & 1);
+                                const uint32_t u = prmt(xa, ya, b | (b << 4) | ((4 + b) << 8) | ((4 + b) << 12));
+                                // code = (128 + low 7 bits) - (128 + 128 * sign bit), exact in bf16
+                                const uint32_t lo7 = lop3_and_or(u, 0x007f007fu, 0x43004300u);
+                                const uint32_t sg = lop3_and_or(u, 0x00800080u, 0x43004300u);
+                                const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo7),
+                                                                 *reinterpret_cast<const __nv_bfloat162*>(&sg));
+                                A[e] = *reinterpret_cast<const uint32_t*>(&v);
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int q = 0; q < X::P; ++q) mma_any<true>(z[n], A, pb[i][n][q][0], pb[i][n][q][1]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[d][n][e] = EXACT ? o[d][n][e] + z[n][e] : z[n][e];
+                    }
+                } else {
+#pragma unroll
+                    for (int cg = 0; cg < CPR / 8; ++cg) {
+                        uint4 vw[MT][4];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                vw[i][k] = lds128(vb + few_v_at<CPR>(16 * i + 2 * t4 + (k & 1) + 8 * (k >> 1), g + 8 * cg));
+#pragma unroll
+                        for (int dd = 0; dd < 4; ++dd) {
+                            const int d = 4 * cg + dd;
+                            float z[NT][4];
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) z[n][e] = EXACT ? 0.f : o[d][n][e];
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) {
+                                uint32_t A[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint4 &x = vw[i][2 * (e >> 1)], &y = vw[i][2 * (e >> 1) + 1];
+                                    const uint32_t xa = dd == 0 ? x.x : dd == 1 ? x.y : dd == 2 ? x.z : x.w;
+                                    const uint32_t ya = dd == 0 ? y.x : dd == 1 ? y.y : dd == 2 ? y.z : y.w;
+                                    A[e] = prmt(xa, ya, e & 1 ? 0x7632u : 0x5410u);
+                                }
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int q = 0; q < X::P; ++q)
+                                        mma_any<X::pBf>(z[n], A, pb[i][n][q][0], pb[i][n][q][1]);
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[d][n][e] = EXACT ? o[d][n][e] + z[n][e] : z[n][e];
+                        }
+                    }
+                }
+            }
+            __syncwarp();  // the slot is free for the next issue
+        }
+
+        // ---- the warps' results joined: rows' maxima and sums, then the scaled O in two halves
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int q = 4; q < 32; q <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], q);
+                if (g == 0) {
+                    float* x = ml + (w * ROWS + n * 8 + 2 * t4 + e) * 2;
+                    x[0] = m[n][e];
+                    x[1] = l[n][e];
+                }
+            }
+        __syncthreads();
+        float f[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < kFewWarps; ++q) top = fmaxf(top, ml[(q * ROWS + n * 8 + 2 * t4 + e) * 2]);
+                f[n][e] = m[n][e] == -INFINITY ? (l[n][e] == 0.f ? 0.f : 1.f) : ex2(m[n][e] - top);
+            }
+        // lane (g, t4) holds values 16-bit: 64 cg + 8 g + x, 8-bit: (D / 8) g + x, of rows 2 t4 + e
+        auto put = [&](bool add) {
+            float* buf = red + (w & 3) * ROWS * F::RS;
+#pragma unroll
+            for (int d = 0; d < KS; ++d)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int col = I8 ? (D / 8) * g + 2 * d : 64 * (d >> 2) + 8 * g + 2 * (d & 3);
+                        float2* x = reinterpret_cast<float2*>(buf + (n * 8 + 2 * t4 + e) * F::RS + col);
+                        float2 y = make_float2(f[n][e] == 0.f ? 0.f : o[d][n][e] * f[n][e],
+                                               f[n][e] == 0.f ? 0.f : o[d][n][e + 2] * f[n][e]);
+                        if (add) {
+                            const float2 z = *x;
+                            y.x += z.x;
+                            y.y += z.y;
+                        }
+                        *x = y;
+                    }
+        };
+        if (w >= 4) put(false);
+        __syncthreads();
+        if (w < 4) put(true);
+        __syncthreads();
+        const bool whole = lo == 0 && hi == tl.units;
+        const int first = whole ? c : attn_owner(it.u_item, U, G);
+        const int pieces = whole ? 1 : attn_owner(it.u_item + tl.units - 1, U, G) - first + 1;
+        constexpr int PS = ROWS * (D + 2);  // floats of a partial result: rows of D values, then (m, l) of each
+        float* const part = a.part + (size_t)(2 * c + (lo == 0)) * PS;
+        for (int x = threadIdx.x; x < tl.nr * (D / 4); x += kFewThreads) {
+            const int r = x / (D / 4), d = x % (D / 4) * 4;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 z = *reinterpret_cast<const float4*>(red + (q * ROWS + r) * F::RS + d);
+                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+            }
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < kFewWarps; ++q) top = fmaxf(top, ml[(q * ROWS + r) * 2]);
+#pragma unroll
+            for (int q = 0; q < kFewWarps; ++q) {
+                const float mq = ml[(q * ROWS + r) * 2], lq = ml[(q * ROWS + r) * 2 + 1];
+                sum += mq == -INFINITY ? lq : lq * ex2(mq - top);
+            }
+            if (whole) {
+                attn_store<T, D>(a, it, r, d, y, top, sum);
+            } else {
+                *reinterpret_cast<float4*>(part + r * D + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(top, sum);
+            }
+        }
+        if (!whole) {  // the last of the tile's blocks joins its partial results in block order
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                last_s = atomicAdd(a.count + first, 1) == pieces - 1;
+                if (last_s) a.count[first] = 0;
+            }
+            __syncthreads();
+            if (last_s) {
+                __threadfence();
+                for (int x = threadIdx.x; x < tl.nr * (D / 4); x += kFewThreads) {
+                    const int r = x / (D / 4), d = x % (D / 4) * 4;
+                    // the first block's piece is its last (slot 1), the others' their first (slot 0)
+                    auto slot = [&](int q) { return a.part + (size_t)(2 * (first + q) + (q == 0)) * PS; };
+                    float top = -INFINITY, sum = 0.f;
+                    for (int q = 0; q < pieces; ++q) top = fmaxf(top, __ldcg(slot(q) + ROWS * D + 2 * r));
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int q = 0; q < pieces; ++q) {
+                        const float2 s2 = __ldcg(reinterpret_cast<const float2*>(slot(q) + ROWS * D + 2 * r));
+                        const float4 z = __ldcg(reinterpret_cast<const float4*>(slot(q) + r * D + d));
+                        if (s2.x == -INFINITY && s2.y == 0.f) continue;  // saw nothing
+                        const float k = s2.x == -INFINITY ? 1.f : ex2(s2.x - top);
+                        sum += s2.y * k;
+                        y.x += z.x * k, y.y += z.y * k, y.z += z.z * k, y.w += z.w * k;
+                    }
+                    attn_store<T, D>(a, it, r, d, y, top, sum);
+                }
+            }
+        }
+        if (it.u_item + tl.units >= u1) break;
+        it.next(a, ROWS, ST);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+namespace {
+
+template <class T, class C, int D, int NT>
+cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
+    using F = FewCfg<C, D, NT>;
+    constexpr int ROWS = 8 * NT;
+    constexpr int head = kFewWarps * F::NS * F::SB + D / 16 * NT * FewTerms<T, C>::Q * 256;
+    constexpr int red = 4 * ROWS * F::RS * 4;
+    constexpr int most = head + (red > 4 * HC_KV_SEQS ? red : 4 * HC_KV_SEQS) + kFewWarps * ROWS * 8 + ROWS * 4;
+    static_assert(most <= 227 * 1024 - 64, "shared memory of a block");
+    static_assert(red >= 4 * HC_KV_SEQS, "the schedule's prefix lies in the joining buffer");
+    const cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return e;
+    attn_few_kernel<T, C, D, NT><<<blocks, kFewThreads, most, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <class T, class C, int D>
+cudaError_t by_rows(const AttnArgs& a, int blocks, cudaStream_t s) {
+    const int rows = attn_few_tile(a.max_rows);
+    if (rows == 8) return launch<T, C, D, 1>(a, blocks, s);
+    if (rows == 16) return launch<T, C, D, 2>(a, blocks, s);
+    return launch<T, C, D, 4>(a, blocks, s);
+}
+
+template <class T>
+cudaError_t by_cache(int ct, int D, const AttnArgs& a, int blocks, cudaStream_t s) {
+    if (D == 64) {
+        if (ct == T_F16) return by_rows<T, __half, 64>(a, blocks, s);
+        if (ct == T_BF16) return by_rows<T, __nv_bfloat16, 64>(a, blocks, s);
+        return by_rows<T, int8_t, 64>(a, blocks, s);
+    }
+    if (ct == T_F16) return by_rows<T, __half, 128>(a, blocks, s);
+    if (ct == T_BF16) return by_rows<T, __nv_bfloat16, 128>(a, blocks, s);
+    return by_rows<T, int8_t, 128>(a, blocks, s);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_few(int ct, int dt, int D, const AttnArgs& a, int blocks, cudaStream_t s) {
+    if (dt == T_F32) return by_cache<float>(ct, D, a, blocks, s);
+    if (dt == T_F16) return by_cache<__half>(ct, D, a, blocks, s);
+    return by_cache<__nv_bfloat16>(ct, D, a, blocks, s);
+}
+
+}  // namespace hc

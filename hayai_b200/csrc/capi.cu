@@ -230,6 +230,8 @@ extern "C" int hc_engine_free(hc_engine* e) {
     e->sk_cnt.release();
     e->stack_bar.release();
     e->ws_tc.release();
+    e->attn_part.release();
+    e->attn_cnt.release();
     hc_peer_release(e);
     for (auto& kv : e->ptr_tables) cudaFree(kv.second);
     e->ptr_tables.clear();

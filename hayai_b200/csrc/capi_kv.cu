@@ -8,6 +8,8 @@
 
 using namespace hc;
 
+static_assert(HC_KV_MAX_SEQ == HC_KV_SEQS, "one limit");
+
 static bool half_type(int t) { return t == T_F16 || t == T_BF16; }
 
 static int check_cache(const hc_kv_cache* c, KvDev* d) {
@@ -119,6 +121,25 @@ extern "C" int hc_kv_read_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_ba
     return kv_rows(e, c, b, dtype, k, ldk, v, ldv, false);
 }
 
+// The split tiles' partial results and counters: as much as any call of any kernel takes, so that
+// they never move under a captured graph.
+static int attn_workspace(hc_engine* e, AttnArgs* a) {
+    const size_t part = attn_few_part_bytes(32, 128, e->num_sms);
+    if (part > e->attn_part.cap) {
+        const int rc = e->attn_part.ensure(part);
+        if (rc) return rc;
+    }
+    const size_t cnt = (size_t)e->num_sms * sizeof(int);
+    if (cnt > e->attn_cnt.cap) {
+        const int rc = e->attn_cnt.ensure(cnt);
+        if (rc) return rc;
+        HC_CUDA(cudaMemsetAsync(e->attn_cnt.p, 0, cnt, e->stream));
+    }
+    a->part = (float*)e->attn_part.p;
+    a->count = (int*)e->attn_cnt.p;
+    return HC_OK;
+}
+
 extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_batch* b, int dtype, size_t n_heads,
                                  const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale, int causal,
                                  int window, int sink) {
@@ -127,6 +148,8 @@ extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv
     if (!rc) rc = check_cache(c, &a.c);
     if (!rc) rc = check_batch(e, c, b, &a.b);
     if (rc) return rc;
+    if ((unsigned long long)b->n_tok * n_heads > INT32_MAX)
+        return hc_set_error(HC_ERR_INVALID, "attn_paged: %d tokens of %zu heads are past 2^31 rows", b->n_tok, n_heads);
     if (n_heads == 0 || n_heads % (size_t)c->n_heads || n_heads > 65535)
         return hc_set_error(HC_ERR_INVALID, "attn_paged: %zu query heads on %d kv heads", n_heads, c->n_heads);
     if (window < 0 || sink < 0 || (window && !causal))
@@ -149,6 +172,12 @@ extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv
     a.window = window;
     a.sink = window ? sink : 0;
     a.scale = scale;
-    const cudaError_t ce = launch_attn_paged(c->type, dtype, c->head_dim, a, e->stream);
+    const long long rows = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
+    a.max_rows = (int)(rows < INT32_MAX ? rows : INT32_MAX);
+    a.row_min = 1;
+    a.row_max = INT32_MAX;
+    rc = attn_workspace(e, &a);
+    if (rc) return rc;
+    const cudaError_t ce = launch_attn_few(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_paged launch");
 }

@@ -54,6 +54,7 @@ struct hc_engine {
     DevBuf stack_bar;             // grid-barrier counter of the persistent FFN-stack kernel
     DevBuf ws_tc;                 // batched Q8_0 tensor-core GEMM: canonical activations + partials
     DevBuf ws_tp;                 // tensor parallelism at batch > 1: this rank's down partial
+    DevBuf attn_part, attn_cnt;   // paged attention: partial results of split tiles, and their counters
     bool use_stack_kernel = true; // batch-1 stacks run as one persistent kernel when they fit
     bool use_tc = true;           // batches of 8+ rows of Q8_0/Q4_K/Q6_K on the tcgen05 GEMM
     HostBuf hs_out;

@@ -281,7 +281,7 @@ int hc_moe_stack_ep_dev(hc_engine* eng, size_t n_layers, const float* const* rou
  * max_new is the host's bound on any sequence's new tokens (0: n_tok); a sequence with more is
  * still computed, at lower speed.  Page numbers, lengths or offsets out of range touch no
  * memory out of the pool: they are cut to it, and hc_sync reports HC_ERR_INVALID. */
-#define HC_KV_MAX_SEQ 4096
+#define HC_KV_MAX_SEQ 2048
 typedef struct hc_kv_cache {
     int type, n_pages, n_heads, page_size, head_dim;
     void *k, *v;

@@ -43,7 +43,7 @@ pub struct hc_kv_batch {
     pub kv_len: *const i32,
 }
 
-pub const HC_KV_MAX_SEQ: c_int = 4096;
+pub const HC_KV_MAX_SEQ: c_int = 2048;
 pub const HC_OK: c_int = 0;
 pub const HC_ERR_INVALID: c_int = 1;
 pub const HC_ERR_UNSUPPORTED: c_int = 2;
