@@ -14,44 +14,55 @@
 // of tokens come from two rows by PRMT, with no transposed copy.  S^T's accumulators become P^T's
 // operand with one MOVMATRIX per 8 tokens.
 //
-// Formats.  8-bit K codes are exact in f16, 8-bit V codes in bf16 (|code| <= 127); a token's K scale
-// multiplies its score and its V scale its weights, whose range bf16 holds.  Query rows are scaled
-// by a power of two to have their largest element in [1, 2) and rounded to the products' type: f16
-// and bf16 rows are exact or keep 11 bits in f16; f32 rows are split into 2 f16 terms (22 bits) or 3
-// bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11 bits of 16).  Weights are rounded to one
-// f16 or bf16 term (relative error 2^-11 or 2^-9, of the order of the 16-bit results' own rounding),
-// for f32 results to two (2^-16 at worst, or 2^-25 absolute).  All sums are f32; for f32 results a
-// unit's products are added to zero and then to the running sum in FADD, as the tensor cores' own
-// chained additions truncate.
+// Formats.  8-bit codes are exact in f16 and in bf16.  For 16-bit results they go in as f16 1152 +
+// code (one PRMT and no subtraction: bits 0x6400 + code + 128), and the product's accumulator starts
+// at -1152 sum q or -1152 sum p of the operand as rounded, so that the codes' own product is left
+// (the larger sums cost about 2^-24 * 1152 / 40 of a result's size).  A token's K scale multiplies
+// its score and its V scale its weights; a unit's weights of a row are then brought to at most 1 by a
+// power of two, which multiplies the unit's product, so that f16 holds them whatever the scales are
+// (what is under 2^-25 of the unit's largest is lost).  For f32 results the codes are taken as they
+// are, and the weights times scales as bf16 terms, whose range needs no such care.  Query rows are
+// scaled by a power of two to have their largest element in [1, 2) and rounded to the products'
+// type: f16 and bf16 rows are exact or keep 11 bits in f16; f32 rows are split into 2 f16 terms (22
+// bits) or 3 bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11 bits of 16).  Weights are
+// rounded to one term of the cache's type, of the order of the 16-bit results' own rounding (f16
+// results on a bf16 cache: two), for f32 results to two f16 or three bf16 terms.  All sums are f32;
+// for f32 results a unit's products are added to zero and then to the running sum in FADD, as the
+// tensor cores' own chained additions truncate.
 //
-// One block of 8 warps per SM walks its share of the line of units (attn_rows.cuh); its warps take
-// the units of a tile in turn, each with its own ring of 16-byte asynchronous copies (no block
-// barrier inside a tile; 2 to 3 stages of 8 KB a warp, ~128 KB in flight per SM), whose issue runs
-// ahead over tile boundaries.  At a tile's end the warps' (m, l, O) are joined in shared memory.
+// The workers of the line (attn_rows.cuh) are warps, one block of 8 or 12 of them per SM.  A warp
+// streams its units through a ring of 16-byte asynchronous copies of its own, whose issue runs ahead
+// over tile boundaries, and meets the others only once: a tile that it has whole it writes itself;
+// of its first and last tile's pieces the partial (m, l, O) go to the workspace, where after one
+// block barrier the block joins its warps' pieces, and the last block of a tile the blocks'.
+// (Tiles shared by all warps of a block, with a barrier and a joining at each tile's end, took
+// 160 us where this takes 9x us: 64 sequences of 300 to 12000 tokens, 64 heads on 8.)
 #include <math.h>
 
 #include "attn_rows.cuh"
 
 namespace hc {
 
-constexpr int kFewWarps = 8, kFewThreads = 32 * kFewWarps;
+template <class T, class C>
+struct FewTerms {
+    static constexpr bool kBf = sizeof(C) == 2 && !(__is_same(C, __half));  // bf16 products for the scores
+    static constexpr int Q = sizeof(T) == 4 ? (kBf ? 3 : 2) : (kBf && __is_same(T, __half)) ? 2 : 1;
+    static constexpr bool pBf = kBf || (sizeof(C) == 1 && sizeof(T) == 4);       // bf16 products for the result
+    static constexpr int P = sizeof(T) == 4 ? (pBf ? 3 : 2) : (pBf && __is_same(T, __half)) ? 2 : 1;
+    static constexpr bool kBias = sizeof(C) == 1 && sizeof(T) == 2;  // codes as 1152 + code
+};
 
-template <class C, int D, int NT>
+template <class T, class C, int D, int NT>
 struct FewCfg {
     static constexpr int ES = sizeof(C), CPR = D * ES / 16;  // 16-byte chunks of a row
     static constexpr int ST = CPR == 16 ? 16 : 32;           // tokens of a unit
     static constexpr int KB = ST * CPR * 16;                 // bytes of a unit's keys (or values)
     static constexpr int SB = 2 * KB + (ES == 1 ? 8 * ST : 0);
-    static constexpr int NS = CPR == 4 ? 4 : NT == 1 ? 3 : 2;  // stages of a warp's ring
-    static constexpr int RS = D + 4;                           // row stride of the joining buffer, floats
-};
-
-template <class T, class C>
-struct FewTerms {
-    static constexpr bool kBf = sizeof(C) == 2 && !(__is_same(C, __half));  // bf16 products for the scores
-    static constexpr int Q = sizeof(T) == 4 ? (kBf ? 3 : 2) : (kBf && __is_same(T, __half)) ? 2 : 1;
-    static constexpr int P = sizeof(T) == 4 ? 2 : 1;
-    static constexpr bool pBf = !__is_same(C, __half);  // bf16 weights
+    static constexpr int W = NT == 1 && FewTerms<T, C>::Q == 1 ? 12 : 8;  // warps of a block
+    static constexpr int NS = CPR == 4 ? 4 : 2;                   // stages of a warp's ring
+    static constexpr int QB = D / 16 * NT * FewTerms<T, C>::Q * 256;  // a query tile as B operands
+    static constexpr int WB = NS * SB + QB + 64 * NT;  // bytes of a warp: ring, queries, rows' scales and biases
+    static constexpr int PS = 8 * NT * (D + 2);  // floats of a partial result: rows of D values, then (m, l) of each
 };
 
 // D (+)= A B, 16 x 8 x 16 (mma16816's bf16 twin).
@@ -68,6 +79,21 @@ __device__ __forceinline__ void mma_any(float (&c)[4], const uint32_t (&a)[4], u
         mma16816_bf(c, a[0], a[1], a[2], a[3], b0, b1);
     else
         mma16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+// D = A B + (c0, c1, c0, c1).
+template <bool BF>
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                         float c1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%11,%10,%11};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%11,%10,%11};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
     uint32_t d;
@@ -133,56 +159,61 @@ __device__ __forceinline__ uint32_t few_v_at(int r, int c) {
 // A warp's walk over its units: unit `st` of the item's [0, hi).
 struct FewWalk {
     AttnIter it;
-    int st, hi, u1;
+    int st, hi, b0, b1;
     bool live;
-    __device__ __forceinline__ void segment(int u0, int w) {
-        st = max(u0 - it.u_item, 0) + w;
-        hi = min(u1 - it.u_item, it.t.units);
+    __device__ __forceinline__ void enter() {
+        st = max(b0 - it.u_item, 0);
+        hi = min(b1 - it.u_item, it.t.units);
     }
-    // Skip segments that have no unit for this warp.
-    __device__ __forceinline__ void settle(const AttnArgs& a, int w, int rows, int unit) {
+    // On to the next item with a unit of this warp, if there is one.
+    __device__ __forceinline__ void settle(const AttnArgs& a, int rows, int unit) {
         while (st >= hi) {
-            if (it.u_item + it.t.units >= u1) {
+            if (it.u_item + it.t.span >= b1) {
                 live = false;
                 return;
             }
             it.next(a, rows, unit);
-            segment(0, w);
+            enter();
         }
     }
 };
 
+// A tile that several warps share, for the joining.
+struct FewShared {
+    int valid, q0, hk, r0, nr, u_item, units;
+};
+
 template <class T, class C, int D, int NT>
-__global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_constant__ AttnArgs a) {
-    using F = FewCfg<C, D, NT>;
+__global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kernel(const __grid_constant__ AttnArgs a) {
+    using F = FewCfg<T, C, D, NT>;
     using X = FewTerms<T, C>;
-    constexpr int ST = F::ST, CPR = F::CPR, MT = ST / 16, KS = D / 16, ROWS = 8 * NT, I8 = F::ES == 1;
-    constexpr int QB = KS * NT * X::Q * 256;  // the query tile as B operands
+    constexpr int W = F::W, THREADS = 32 * W, ST = F::ST, CPR = F::CPR, MT = ST / 16, KS = D / 16, ROWS = 8 * NT, I8 = F::ES == 1;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ FewShared shared_s[W + 1];  // tiles that start in warp w and go on past it; the block's first
+    __shared__ int last_s[2];
     const int w = threadIdx.x >> 5, ln = lane_id(), g = ln >> 2, t4 = ln & 3;
-    const uint32_t ring = smem_addr(smem) + w * F::NS * F::SB;
-    uint8_t* const qf = smem + kFewWarps * F::NS * F::SB;
-    float* const red = reinterpret_cast<float*>(qf + QB);  // [4][ROWS][RS]; the schedule's prefix before
-    float* const ml = red + 4 * ROWS * F::RS;              // [8][ROWS][2]
-    float* const rscale = ml + kFewWarps * ROWS * 2;       // [ROWS]
-    __shared__ int last_s;
+    const uint32_t ring = smem_addr(smem) + w * F::WB;
+    uint8_t* const qf = smem + w * F::WB + F::NS * F::SB;
+    float* const rscale = reinterpret_cast<float*>(qf + F::QB);  // [ROWS], and [ROWS] of -1152 sum q
 
-    int* const pre = reinterpret_cast<int*>(red);
-    const int U = attn_schedule<kFewThreads>(a, ROWS, ST, pre);
-    const int G = min((int)gridDim.x, max(1, U / kFewWarps)), c = blockIdx.x;
+    int* const pre = reinterpret_cast<int*>(smem);
+    const int U = attn_schedule<THREADS>(a, ROWS, ST, pre);
+    const int G = min((int)gridDim.x, max(1, U / W)), c = blockIdx.x;
     if (U <= 0 || c >= G) return;
-    const int u0 = attn_begin(c, U, G), u1 = attn_begin(c + 1, U, G);
-    AttnIter it;  // the block's place
-    it.seek(a, pre, u0, ROWS, ST);
+    FewWalk pw;  // the copies' walk: units are issued NS - 1 ahead
+    const AttnShares share(U, G * W);
+    pw.b0 = share.begin(c * W + w);
+    pw.b1 = share.begin(c * W + w + 1);
+    pw.live = pw.b0 < pw.b1;
+    if (pw.live) {
+        pw.it.seek(a, pre, pw.b0, ROWS, ST);
+        pw.enter();
+    }
+    if (threadIdx.x <= W) shared_s[threadIdx.x].valid = 0;
     __syncthreads();  // `pre` is read
-
-    // ---- the copies' walk: units are issued NS - 1 ahead
-    FewWalk pw;
-    pw.it = it;
-    pw.u1 = u1;
-    pw.live = true;
-    pw.segment(u0, w);
-    pw.settle(a, w, ROWS, ST);
+    AttnIter it = pw.it;
+    const int b0 = pw.b0, b1 = pw.b1;
+    if (pw.live) pw.settle(a, ROWS, ST);
     int pg = -1, pr = 0;  // page and row of this lane's token of the unit to be issued
     auto look_up = [&]() {
         pg = -1;
@@ -190,7 +221,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
         const int v = pw.st * ST + ln;
         if (ln < ST && v < pw.it.t.nvis) {
             const int j = v < pw.it.t.n1 ? v : v - pw.it.t.n1 + pw.it.t.lo;
-            const int p = j / a.c.page_size;
+            const int p = a.by_page(j);
             pr = j - p * a.c.page_size;
             pg = __ldg(a.b.table + pw.it.s * a.b.table_stride + p);
             if ((unsigned)pg >= (unsigned)a.c.n_pages) {
@@ -221,8 +252,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                 cp4_or_zero(base + 2 * F::KB + ST * 4 + ln * 4, a.c.vs + so, ok);
             }
             islot = islot + 1 == F::NS ? 0 : islot + 1;
-            pw.st += kFewWarps;
-            pw.settle(a, w, ROWS, ST);
+            if (++pw.st >= pw.hi) pw.settle(a, ROWS, ST);
             look_up();
         }
         cp_async_commit();
@@ -232,14 +262,28 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
     for (int i = 0; i < F::NS - 1; ++i) issue();
 
     int cslot = 0;
-    for (;;) {  // the block's tiles
+    while (b0 < b1) {  // the warp's tiles
         const AttnTile& tl = it.t;
-        const int lo = max(u0 - it.u_item, 0), hi = min(u1 - it.u_item, tl.units);
+        const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
+        if (lo >= hi) {
+            if (it.u_item + tl.span >= b1) break;
+            it.next(a, ROWS, ST);
+            continue;
+        }
         // ---- the query tile as B operands
-        for (int r = w; r < ROWS; r += kFewWarps) {
+#pragma unroll 4
+        for (int r = 0; r < ROWS; ++r) {
+            if (r >= tl.nr) {  // no row: zeros, so that what is there before does not move the maxima
+                if (ln == 0) rscale[r] = rscale[ROWS + r] = 0.f;
+#pragma unroll
+                for (int i = ln; i < KS * X::Q * 4; i += 32)
+                    *reinterpret_cast<uint2*>(qf + (((i >> 2) / X::Q * NT + (r >> 3)) * X::Q + (i >> 2) % X::Q) * 256 +
+                                              ((r & 7) * 4 + (i & 3)) * 8) = make_uint2(0, 0);
+                continue;
+            }
             float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if (r < tl.nr && ln < D / 4) {
-                const int row = tl.r0 + r, tok = it.q.q0 + row / a.group, h = it.hk * a.group + row % a.group;
+            if (ln < D / 4) {
+                const int row = tl.r0 + r, tr = a.by_group(row), tok = it.q.q0 + tr, h = it.hk * a.group + row - tr * a.group;
                 const T* q = (const T*)a.q + (long long)tok * a.ldq + h * D + 4 * ln;
                 if constexpr (sizeof(T) == 4) {
                     const float4 f = __ldg(reinterpret_cast<const float4*>(q));
@@ -267,6 +311,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] *= down;
             if (ln == 0) rscale[r] = up * a.scale * 1.44269504f;
+            if constexpr (X::kBias) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += __half2float(__float2half_rn(x[i]));
+                sum = warp_sum(sum);
+                if (ln == 0) rscale[ROWS + r] = -1152.f * sum;
+            }
             if (ln < D / 4) {
                 // d = 4 ln + i: 16-byte chunk of the cache row, its k step and the lane that holds it
                 const int ch = I8 ? ln >> 2 : ln >> 1, j = I8 ? 4 * (ch >> 2) + (ln & 3) : 2 * (ch >> 2) + (ln & 1);
@@ -277,8 +328,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                         make_uint2(split_pair<X::kBf>(x[0], x[1]), split_pair<X::kBf>(x[2], x[3]));
             }
         }
-        __syncthreads();
-        float m[NT][2], l[NT][2], o[KS][NT][4], rs[NT][2];
+        __syncwarp();
+        float m[NT][2], l[NT][2], o[KS][NT][4], rs[NT][2], qb[NT][2];
         int lim[NT][2], wlo[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -288,7 +339,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                 m[n][e] = -INFINITY;
                 l[n][e] = 0.f;
                 rs[n][e] = rscale[r];
-                const int pos = it.q.len - (it.q.q1 - it.q.q0) + (tl.r0 + r) / a.group;
+                qb[n][e] = X::kBias ? rscale[ROWS + r] : 0.f;
+                const int pos = it.q.len - (it.q.q1 - it.q.q0) + a.by_group(tl.r0 + r);
                 lim[n][e] = r >= tl.nr ? -1 : a.causal ? pos : it.q.len - 1;
                 wlo[n][e] = a.window ? pos - a.window + 1 : 0;
             }
@@ -299,7 +351,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[d][n][e] = 0.f;
 
-        for (int st = lo + w; st < hi; st += kFewWarps) {
+        for (int st = lo; st < hi; ++st) {
             issue();
             cp_async_wait(F::NS - 1);
             __syncwarp();
@@ -307,12 +359,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
             cslot = cslot + 1 == F::NS ? 0 : cslot + 1;
             // ---- S^T = K Q^T
             float s[MT][NT][4];
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
 #pragma unroll
             for (int cg = 0; cg < CPR / 4; ++cg) {
                 uint4 ka[MT], kc[MT];
@@ -328,12 +374,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                     for (int i = 0; i < MT; ++i) {
                         const uint32_t wa[4] = {ka[i].x, ka[i].y, ka[i].z, ka[i].w};
                         const uint32_t wc[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
-                        if constexpr (I8) {  // code + 1152 by PRMT, minus 1152: exact
+                        if constexpr (I8) {
                             const uint32_t fa = wa[jj] ^ 0x80808080u, fc = wc[jj] ^ 0x80808080u;
-                            A[i][0] = hsub2_u32(prmt(fa, 0x64646464u, 0x4140u), 0x64806480u);
-                            A[i][1] = hsub2_u32(prmt(fc, 0x64646464u, 0x4140u), 0x64806480u);
-                            A[i][2] = hsub2_u32(prmt(fa, 0x64646464u, 0x4342u), 0x64806480u);
-                            A[i][3] = hsub2_u32(prmt(fc, 0x64646464u, 0x4342u), 0x64806480u);
+                            A[i][0] = prmt(fa, 0x64646464u, 0x4140u);
+                            A[i][1] = prmt(fc, 0x64646464u, 0x4140u);
+                            A[i][2] = prmt(fa, 0x64646464u, 0x4342u);
+                            A[i][3] = prmt(fc, 0x64646464u, 0x4342u);
+                            if constexpr (!X::kBias)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) A[i][e] = hsub2_u32(A[i][e], 0x64806480u);
                         } else {
                             A[i][0] = wa[2 * jj];
                             A[i][1] = wc[2 * jj];
@@ -348,7 +397,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                         for (int q = 0; q < X::Q; ++q) {
                             const uint2 b = *reinterpret_cast<const uint2*>(qf + ((j * NT + n) * X::Q + q) * 256 + ln * 8);
 #pragma unroll
-                            for (int i = 0; i < MT; ++i) mma_any<X::kBf>(s[i][n], A[i], b.x, b.y);
+                            for (int i = 0; i < MT; ++i) {
+                                if (j == 0 && q == 0)
+                                    mma_from<X::kBf>(s[i][n], A[i], b.x, b.y, qb[n][0], qb[n][1]);
+                                else
+                                    mma_any<X::kBf>(s[i][n], A[i], b.x, b.y);
+                            }
                         }
                 }
             }
@@ -415,27 +469,47 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
             }
             // ---- weights, and P^T as B operands
             uint32_t pb[MT][NT][X::P][2];
+            float unit[NT][2];  // 8-bit: what the unit's weights of a row are divided by
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+                float p[MT][4];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    float p[4];
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[e] = ex2(s[i][n][e] - (e & 1 ? m1 : m0));
-                        l[n][e & 1] += p[e];
+                        p[i][e] = ex2(s[i][n][e] - (e & 1 ? m1 : m0));
+                        l[n][e & 1] += p[i][e];
                         if constexpr (I8) {
-                            p[e] *= vsc[i][e >> 1];
-                            if (!full && s[i][n][e] == -INFINITY) p[e] = 0.f;  // whatever the scale of a masked token
+                            p[i][e] *= vsc[i][e >> 1];
+                            if (!full && s[i][n][e] == -INFINITY) p[i][e] = 0.f;  // whatever a masked token's scale is
                         }
                     }
+                unit[n][0] = unit[n][1] = 1.f;
+                if constexpr (X::kBias) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(fmaxf(fabsf(p[0][e]), fabsf(p[0][e + 2])),
+                                        fmaxf(fabsf(p[MT - 1][e]), fabsf(p[MT - 1][e + 2])));
+#pragma unroll
+                        for (int q = 4; q < 32; q <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, q));
+                        const uint32_t b = min(max(__float_as_uint(x) & 0x7f800000u, 0x01000000u), 0x7e000000u);
+                        unit[n][e] = __uint_as_float(b + 0x00800000u);
+                        const float inv = __uint_as_float(0x7e800000u - b);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            p[i][e] *= inv;
+                            p[i][e + 2] *= inv;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int q = 0; q < X::P; ++q)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
-                            pb[i][n][q][h] = movmatrix(split_pair<X::pBf>(p[2 * h], p[2 * h + 1]));
-                }
+                            pb[i][n][q][h] = movmatrix(split_pair<X::pBf>(p[i][2 * h], p[i][2 * h + 1]));
             }
             // ---- O^T += V^T P^T
             bool odd = false;  // a value that is not finite in a unit that some row does not see whole
@@ -480,7 +554,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                             }
                     }
             } else {
-                constexpr bool EXACT = X::P == 2;
+                constexpr bool EXACT = sizeof(T) == 4;
                 if constexpr (I8) {
                     uint4 vw[MT][4];  // 16 (D = 128) or 8 (D = 64) adjacent values of four tokens
 #pragma unroll
@@ -494,14 +568,27 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                                 const uint2 x = lds64(vb + few_v_at<CPR>(r, g >> 1) + 8 * (g & 1));
                                 vw[i][k] = make_uint4(x.x, x.y, 0, 0);
                             }
+                            if constexpr (X::kBias) {
+                                vw[i][k].x ^= 0x80808080u, vw[i][k].y ^= 0x80808080u;
+                                vw[i][k].z ^= 0x80808080u, vw[i][k].w ^= 0x80808080u;
+                            }
                         }
+                    float pbias[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        pbias[n][0] = pbias[n][1] = 0.f;
+                        if constexpr (X::kBias) {  // -1152 sum p, by a product with ones
+                            const uint32_t one[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                            float z[4];
+                            mma_from<false>(z, one, pb[0][n][0][0], pb[0][n][0][1], 0.f, 0.f);
+                            if constexpr (MT == 2) mma_any<false>(z, one, pb[MT - 1][n][0][0], pb[MT - 1][n][0][1]);
+                            pbias[n][0] = -1152.f * z[0];
+                            pbias[n][1] = -1152.f * z[1];
+                        }
+                    }
 #pragma unroll
                     for (int d = 0; d < KS; ++d) {
                         float z[NT][4];
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) z[n][e] = EXACT ? 0.f : o[d][n][e];
 #pragma unroll
                         for (int i = 0; i < MT; ++i) {
                             uint32_t A[4];
@@ -513,22 +600,30 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
                                 const uint32_t ya = wi == 0 ? y.x : wi == 1 ? y.y : wi == 2 ? y.z : y.w;
                                 const uint32_t b = 2 * (d & 1) + (e & 1);
                                 const uint32_t u = prmt(xa, ya, b | (b << 4) | ((4 + b) << 8) | ((4 + b) << 12));
-                                // code = (128 + low 7 bits) - (128 + 128 * sign bit), exact in bf16
-                                const uint32_t lo7 = lop3_and_or(u, 0x007f007fu, 0x43004300u);
-                                const uint32_t sg = lop3_and_or(u, 0x00800080u, 0x43004300u);
-                                const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo7),
-                                                                 *reinterpret_cast<const __nv_bfloat162*>(&sg));
-                                A[e] = *reinterpret_cast<const uint32_t*>(&v);
+                                if constexpr (X::kBias) {
+                                    A[e] = lop3_and_or(u, 0x00ff00ffu, 0x64006400u);  // 1152 + code (words flipped)
+                                } else {  // code = (128 + low 7 bits) - (128 + 128 * sign bit), exact in bf16
+                                    const uint32_t lo7 = lop3_and_or(u, 0x007f007fu, 0x43004300u);
+                                    const uint32_t sg = lop3_and_or(u, 0x00800080u, 0x43004300u);
+                                    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo7),
+                                                                     *reinterpret_cast<const __nv_bfloat162*>(&sg));
+                                    A[e] = *reinterpret_cast<const uint32_t*>(&v);
+                                }
                             }
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int q = 0; q < X::P; ++q) mma_any<true>(z[n], A, pb[i][n][q][0], pb[i][n][q][1]);
+                                for (int q = 0; q < X::P; ++q) {
+                                    if (i == 0 && q == 0)
+                                        mma_from<X::pBf>(z[n], A, pb[i][n][q][0], pb[i][n][q][1], pbias[n][0], pbias[n][1]);
+                                    else
+                                        mma_any<X::pBf>(z[n], A, pb[i][n][q][0], pb[i][n][q][1]);
+                                }
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[d][n][e] = EXACT ? o[d][n][e] + z[n][e] : z[n][e];
+                            for (int e = 0; e < 4; ++e) o[d][n][e] = fmaf(z[n][e], unit[n][e & 1], o[d][n][e]);
                     }
                 } else {
 #pragma unroll
@@ -574,141 +669,126 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_few_kernel(const __grid_c
             __syncwarp();  // the slot is free for the next issue
         }
 
-        // ---- the warps' results joined: rows' maxima and sums, then the scaled O in two halves
+        // ---- the tile's end: lane (g, t4) holds values 64 cg + 8 g + x (8-bit: (D / 8) g + x) of rows 2 t4 + e
+        const bool whole = lo == 0 && hi == tl.units;
+        float* const part = a.part + (size_t)(2 * (c * W + w) + (lo == 0)) * F::PS;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int q = 4; q < 32; q <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], q);
+                const int r = n * 8 + 2 * t4 + e;
+                if (r >= tl.nr) continue;
+#pragma unroll
+                for (int d = 0; d < KS; d += 2) {
+                    const int col = I8 ? (D / 8) * g + 2 * d : 64 * (d >> 2) + 8 * g + 2 * (d & 3);
+                    const float y[4] = {o[d][n][e], o[d][n][e + 2], o[d + 1][n][e], o[d + 1][n][e + 2]};
+                    if (whole)
+                        attn_store<T, 4>(a, it.q.q0, it.hk, tl.r0 + r, D, col, y, l[n][e]);
+                    else
+                        *reinterpret_cast<float4*>(part + r * D + col) = make_float4(y[0], y[1], y[2], y[3]);
+                }
                 if (g == 0) {
-                    float* x = ml + (w * ROWS + n * 8 + 2 * t4 + e) * 2;
-                    x[0] = m[n][e];
-                    x[1] = l[n][e];
+                    if (whole)
+                        attn_store_lse(a, it.q.q0, it.hk, tl.r0 + r, m[n][e], l[n][e]);
+                    else
+                        *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m[n][e], l[n][e]);
                 }
             }
-        __syncthreads();
-        float f[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int q = 0; q < kFewWarps; ++q) top = fmaxf(top, ml[(q * ROWS + n * 8 + 2 * t4 + e) * 2]);
-                f[n][e] = m[n][e] == -INFINITY ? (l[n][e] == 0.f ? 0.f : 1.f) : ex2(m[n][e] - top);
-            }
-        // lane (g, t4) holds values 16-bit: 64 cg + 8 g + x, 8-bit: (D / 8) g + x, of rows 2 t4 + e
-        auto put = [&](bool add) {
-            float* buf = red + (w & 3) * ROWS * F::RS;
-#pragma unroll
-            for (int d = 0; d < KS; ++d)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int col = I8 ? (D / 8) * g + 2 * d : 64 * (d >> 2) + 8 * g + 2 * (d & 3);
-                        float2* x = reinterpret_cast<float2*>(buf + (n * 8 + 2 * t4 + e) * F::RS + col);
-                        float2 y = make_float2(f[n][e] == 0.f ? 0.f : o[d][n][e] * f[n][e],
-                                               f[n][e] == 0.f ? 0.f : o[d][n][e + 2] * f[n][e]);
-                        if (add) {
-                            const float2 z = *x;
-                            y.x += z.x;
-                            y.y += z.y;
-                        }
-                        *x = y;
-                    }
-        };
-        if (w >= 4) put(false);
-        __syncthreads();
-        if (w < 4) put(true);
-        __syncthreads();
-        const bool whole = lo == 0 && hi == tl.units;
-        const int first = whole ? c : attn_owner(it.u_item, U, G);
-        const int pieces = whole ? 1 : attn_owner(it.u_item + tl.units - 1, U, G) - first + 1;
-        constexpr int PS = ROWS * (D + 2);  // floats of a partial result: rows of D values, then (m, l) of each
-        float* const part = a.part + (size_t)(2 * c + (lo == 0)) * PS;
-        for (int x = threadIdx.x; x < tl.nr * (D / 4); x += kFewThreads) {
-            const int r = x / (D / 4), d = x % (D / 4) * 4;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 z = *reinterpret_cast<const float4*>(red + (q * ROWS + r) * F::RS + d);
-                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-            }
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < kFewWarps; ++q) top = fmaxf(top, ml[(q * ROWS + r) * 2]);
-#pragma unroll
-            for (int q = 0; q < kFewWarps; ++q) {
-                const float mq = ml[(q * ROWS + r) * 2], lq = ml[(q * ROWS + r) * 2 + 1];
-                sum += mq == -INFINITY ? lq : lq * ex2(mq - top);
-            }
-            if (whole) {
-                attn_store<T, D>(a, it, r, d, y, top, sum);
-            } else {
-                *reinterpret_cast<float4*>(part + r * D + d) = y;
-                if (d == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(top, sum);
-            }
-        }
-        if (!whole) {  // the last of the tile's blocks joins its partial results in block order
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                last_s = atomicAdd(a.count + first, 1) == pieces - 1;
-                if (last_s) a.count[first] = 0;
-            }
-            __syncthreads();
-            if (last_s) {
-                __threadfence();
-                for (int x = threadIdx.x; x < tl.nr * (D / 4); x += kFewThreads) {
-                    const int r = x / (D / 4), d = x % (D / 4) * 4;
-                    // the first block's piece is its last (slot 1), the others' their first (slot 0)
-                    auto slot = [&](int q) { return a.part + (size_t)(2 * (first + q) + (q == 0)) * PS; };
-                    float top = -INFINITY, sum = 0.f;
-                    for (int q = 0; q < pieces; ++q) top = fmaxf(top, __ldcg(slot(q) + ROWS * D + 2 * r));
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int q = 0; q < pieces; ++q) {
-                        const float2 s2 = __ldcg(reinterpret_cast<const float2*>(slot(q) + ROWS * D + 2 * r));
-                        const float4 z = __ldcg(reinterpret_cast<const float4*>(slot(q) + r * D + d));
-                        if (s2.x == -INFINITY && s2.y == 0.f) continue;  // saw nothing
-                        const float k = s2.x == -INFINITY ? 1.f : ex2(s2.x - top);
-                        sum += s2.y * k;
-                        y.x += z.x * k, y.y += z.y * k, y.z += z.z * k, y.w += z.w * k;
-                    }
-                    attn_store<T, D>(a, it, r, d, y, top, sum);
-                }
-            }
-        }
-        if (it.u_item + tl.units >= u1) break;
+        if (!whole && ln == 0 && (lo == 0 || w == 0))
+            shared_s[lo == 0 ? w : W] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units};
+        if (it.u_item + tl.span >= b1) break;
         it.next(a, ROWS, ST);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+
+    // ---- the block's tiles of several warps: a row per warp at a time, its D values over D / 4 lanes
+    float* const bpart = a.part + (size_t)2 * gridDim.x * W * F::PS;  // the blocks' partial results, two each
+    int crossing = 0, turn = 0;
+    for (int x = 0; x <= W; ++x) {
+        const FewShared sh = shared_s[x];
+        if (!sh.valid) continue;
+        const int wf = share.owner(sh.u_item), wl = share.owner(sh.u_item + sh.units - 1);
+        const bool cross = wf / W != c || wl / W != c;
+        crossing |= cross ? 1 << (x == W ? 0 : 1) : 0;
+        for (int r = 0; r < sh.nr; ++r) {
+            if (turn++ % W != w) continue;
+            // of fewer places than warps some warps have none, and no piece
+            const int q0 = max(wf, c * W), q1 = min(wl, c * W + W - 1);
+            AttnJoin j;
+            j.join(q1 - q0 + 1, ln < D / 4,
+                   [&](int i) -> const float* {
+                       const int q = q0 + i;
+                       if (share.q == 0 && q >= share.rem) return nullptr;
+                       return a.part + (size_t)(2 * q + (q == wf)) * F::PS + ROWS * D + 2 * r;
+                   },
+                   [&](int i) { return a.part + (size_t)(2 * (q0 + i) + (q0 + i == wf)) * F::PS + r * D; });
+            if (ln >= D / 4) continue;
+            if (cross) {
+                float* p = bpart + (size_t)(2 * c + (wf / W == c)) * F::PS;
+                *reinterpret_cast<float4*>(p + r * D + 4 * ln) = make_float4(j.y[0], j.y[1], j.y[2], j.y[3]);
+                if (ln == 0) *reinterpret_cast<float2*>(p + ROWS * D + 2 * r) = make_float2(j.m, j.l);
+            } else {
+                attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
+                if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
+            }
+        }
+    }
+    if (!crossing) return;
+    // ---- tiles of several blocks: the last of them joins
+    __threadfence();
+    __syncthreads();
+    for (int x = 0; x <= W; ++x) {
+        const FewShared sh = shared_s[x];
+        if (!sh.valid) continue;
+        const int bf = share.owner(sh.u_item) / W, bl = share.owner(sh.u_item + sh.units - 1) / W;
+        if (bf == bl) continue;
+        if (threadIdx.x == 0) {
+            last_s[0] = atomicAdd(a.count + bf, 1) == bl - bf;
+            if (last_s[0]) a.count[bf] = 0;
+            __threadfence();
+        }
+        __syncthreads();
+        if (last_s[0]) {
+            for (int r = w; r < sh.nr; r += W) {
+                AttnJoin j;
+                auto piece = [&](int i) { return bpart + (size_t)(2 * (bf + i) + (i == 0)) * F::PS; };
+                j.join(bl - bf + 1, ln < D / 4, [&](int i) -> const float* { return piece(i) + ROWS * D + 2 * r; },
+                       [&](int i) { return piece(i) + r * D; });
+                if (ln >= D / 4) continue;
+                attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
+                if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
+            }
+        }
+        __syncthreads();
+    }
 }
 
 namespace {
 
 template <class T, class C, int D, int NT>
 cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
-    using F = FewCfg<C, D, NT>;
-    constexpr int ROWS = 8 * NT;
-    constexpr int head = kFewWarps * F::NS * F::SB + D / 16 * NT * FewTerms<T, C>::Q * 256;
-    constexpr int red = 4 * ROWS * F::RS * 4;
-    constexpr int most = head + (red > 4 * HC_KV_SEQS ? red : 4 * HC_KV_SEQS) + kFewWarps * ROWS * 8 + ROWS * 4;
-    static_assert(most <= 227 * 1024 - 64, "shared memory of a block");
-    static_assert(red >= 4 * HC_KV_SEQS, "the schedule's prefix lies in the joining buffer");
+    using F = FewCfg<T, C, D, NT>;
+    constexpr int most = F::W * F::WB;
+    static_assert(most <= 227 * 1024 - 1024, "shared memory of a block");
+    static_assert(most >= 4 * HC_KV_SEQS, "the schedule's prefix lies in the rings");
+    static_assert((size_t)F::PS * 4 * 2 * (F::W + 1) <= kFewPartBytes, "the workspace of a block");
     const cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
-    attn_few_kernel<T, C, D, NT><<<blocks, kFewThreads, most, s>>>(a);
+    attn_few_kernel<T, C, D, NT><<<blocks, 32 * F::W, most, s>>>(a);
     return cudaGetLastError();
 }
 
+// Tiles of 8, 16 or 32 rows, by the batch's largest sequence; of more terms (f32 rows) at most 16,
+// whose operands fill the shared memory.
 template <class T, class C, int D>
 cudaError_t by_rows(const AttnArgs& a, int blocks, cudaStream_t s) {
-    const int rows = attn_few_tile(a.max_rows);
-    if (rows == 8) return launch<T, C, D, 1>(a, blocks, s);
-    if (rows == 16) return launch<T, C, D, 2>(a, blocks, s);
-    return launch<T, C, D, 4>(a, blocks, s);
+    if (a.max_rows <= 8) return launch<T, C, D, 1>(a, blocks, s);
+    if constexpr (FewTerms<T, C>::Q == 1)
+        if (a.max_rows > 16) return launch<T, C, D, 4>(a, blocks, s);
+    return launch<T, C, D, 2>(a, blocks, s);
 }
 
 template <class T>

@@ -7,10 +7,10 @@
 // window the first n1 = min(sink, lo) and then [lo, end).  They are counted through as v = 0 ..
 // nvis - 1, position j = v < n1 ? v : v - n1 + lo, and cut into units of `unit` of them.
 //
-// All units of a call, in the order (sequence, kv head, tile, unit), are one line of U units; block
-// c of G works on [c U / G, (c + 1) U / G), so that blocks differ by one unit at most whatever the
-// lengths are.  A tile whose units fall to several blocks is joined from their partial results by
-// the block that finishes last, in block order (the same bits every time).
+// All units of a call, in the order (sequence, kv head, tile, unit), are one line; after a tile's
+// units come `kOver` places that stand for what starting and finishing a tile costs.  Of the U
+// places the workers take equal shares, whatever the lengths are.  A tile whose units fall to several workers is joined from their partial results,
+// in the workers' order (the same bits every time).
 #pragma once
 
 #include <math.h>
@@ -19,11 +19,13 @@
 
 namespace hc {
 
+constexpr int kOver = 2;  // measured with units of 32 tokens: a tile costs about what two of them do
+
 struct AttnTile {
     int r0, nr;        // first row and number of rows
     int p_lo, p_hi;    // positions of the first and last row
     int lo, n1, nvis;  // visible positions (see above)
-    int units;
+    int units, span;   // span: units + kOver
 };
 
 __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q, int tile, int rows, int unit) {
@@ -31,13 +33,14 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
     const int n = q.q1 - q.q0;
     t.r0 = tile * rows;
     t.nr = min(rows, n * a.group - t.r0);
-    t.p_lo = q.len - n + t.r0 / a.group;
-    t.p_hi = q.len - n + (t.r0 + t.nr - 1) / a.group;
+    t.p_lo = q.len - n + a.by_group(t.r0);
+    t.p_hi = q.len - n + a.by_group(t.r0 + t.nr - 1);
     const int end = a.causal ? max(min(q.len, t.p_hi + 1), 0) : q.len;
     t.lo = a.window ? min(max(t.p_lo - a.window + 1, 0), end) : 0;
     t.n1 = min(a.sink, t.lo);
     t.nvis = t.n1 + end - t.lo;
     t.units = max(1, (t.nvis + unit - 1) / unit);  // a tile that sees nothing still has to write zeros
+    t.span = t.units + kOver;
     return t;
 }
 
@@ -46,7 +49,7 @@ __device__ __forceinline__ int attn_tiles(const AttnArgs& a, const KvSeq& q, int
     return r >= a.row_min && r <= a.row_max ? (r + rows - 1) / rows : 0;
 }
 
-// Units of every sequence, as an inclusive prefix sum in `pre` (n_seq ints of shared memory);
+// Places of every sequence, as an inclusive prefix sum in `pre` (n_seq ints of shared memory);
 // returns U, or -1 (and the error flag) if they do not fit 31 bits.  The whole block calls it.
 template <int THREADS>
 __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int unit, int* pre) {
@@ -59,7 +62,7 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
             const KvSeq q = kv_seq(a.b, cap, s);
             const int n = attn_tiles(a, q, rows);
             long long w = 0;
-            for (int t = ln; t < n; t += 32) w += attn_tile(a, q, t, rows, unit).units;
+            for (int t = ln; t < n; t += 32) w += attn_tile(a, q, t, rows, unit).span;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
             if (ln == 0) pre[s] = (int)min(w * a.c.n_heads, 0x7fffffffll);
@@ -69,7 +72,7 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
             const KvSeq q = kv_seq(a.b, cap, s);
             const int n = attn_tiles(a, q, rows);
             long long w = 0;
-            for (int t = 0; t < n; ++t) w += attn_tile(a, q, t, rows, unit).units;
+            for (int t = 0; t < n; ++t) w += attn_tile(a, q, t, rows, unit).span;
             pre[s] = (int)min(w * a.c.n_heads, 0x7fffffffll);
         }
     }
@@ -101,7 +104,7 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
     return (int)carry_s;
 }
 
-// A place in the line of units: the item (sequence, kv head, tile) and its first unit.
+// An item of the line, (sequence, kv head, tile), and its first place.
 struct AttnIter {
     int s, hk, tile, n_tiles, u_item;
     KvSeq q;
@@ -112,7 +115,7 @@ struct AttnIter {
         n_tiles = attn_tiles(a, q, rows);
         hk = tile = 0;
     }
-    // The item that holds unit u (0 <= u < U).
+    // The item that holds place u (0 <= u < U).
     __device__ __forceinline__ void seek(const AttnArgs& a, const int* pre, int u, int rows, int unit) {
         int lo = 0, hi = a.b.n_seq - 1;  // first sequence whose prefix is past u
         while (lo < hi) {
@@ -126,14 +129,14 @@ struct AttnIter {
         hk = (u - before) / w;
         u_item = before + hk * w;
         t = attn_tile(a, q, 0, rows, unit);
-        while (u_item + t.units <= u) {
-            u_item += t.units;
+        while (u_item + t.span <= u) {
+            u_item += t.span;
             t = attn_tile(a, q, ++tile, rows, unit);
         }
     }
     // The next item (there has to be one).
     __device__ __forceinline__ void next(const AttnArgs& a, int rows, int unit) {
-        u_item += t.units;
+        u_item += t.span;
         if (++tile == n_tiles) {
             tile = 0;
             if (++hk == a.c.n_heads) {
@@ -147,9 +150,17 @@ struct AttnIter {
     }
 };
 
-__device__ __forceinline__ int attn_begin(int c, int U, int G) { return (int)((long long)c * U / G); }
-// The block of G whose range holds unit u.
-__device__ __forceinline__ int attn_owner(int u, int U, int G) { return (int)(((long long)(u + 1) * G - 1) / U); }
+// The workers' shares of U places: U / G each, and one more for the first U % G.
+struct AttnShares {
+    int q, rem;
+    __device__ __forceinline__ AttnShares(int U, int G) : q(U / G), rem(U - q * G) {}
+    __device__ __forceinline__ int begin(int c) const { return c * q + min(c, rem); }
+    // The worker whose share holds place u.
+    __device__ __forceinline__ int owner(int u) const {
+        const int big = rem * (q + 1);
+        return u < big ? u / (q + 1) : rem + (u - big) / q;
+    }
+};
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -157,22 +168,79 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Four values (y, the weighted sum) of row r of the item's tile, and at d = 0 its lse.
-template <class T, int D>
-__device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnIter& it, int r, int d, float4 y, float m, float l) {
-    const int row = it.t.r0 + r, h = it.hk * a.group + row % a.group;
-    const long long tok = it.q.q0 + row / a.group;
+// N (4 or 2) adjacent values of the weighted sum of row `row` of an item's kv head, over l.
+template <class T, int N>
+__device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[N],
+                                           float l) {
     const bool none = l == 0.f;  // saw nothing (a sum that is not a number is kept)
     const float k = none ? 0.f : 1.f / l;
-    if (none) y = make_float4(0.f, 0.f, 0.f, 0.f);
-    T* out = (T*)a.out + tok * a.ldo + h * D + d;
-    if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4*>(out) = make_float4(y.x * k, y.y * k, y.z * k, y.w * k);
-    else if constexpr (__is_same(T, __half))
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2(y.x * k, y.y * k), pack_h2(y.z * k, y.w * k));
-    else
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack_b2(y.x * k, y.y * k), pack_b2(y.z * k, y.w * k));
-    if (d == 0 && a.lse) a.lse[tok * a.heads + h] = none ? -INFINITY : (m + log2f(l)) * 0.693147181f;
+    const int t = a.by_group(row);
+    T* out = (T*)a.out + (long long)(q0 + t) * a.ldo + (hk * a.group + row - t * a.group) * D + d;
+    float z[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = none ? 0.f : y[i] * k;
+    uint32_t u[N / 2];
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (N == 4) *reinterpret_cast<float4*>(out) = make_float4(z[0], z[1], z[2], z[3]);
+        else *reinterpret_cast<float2*>(out) = make_float2(z[0], z[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+            u[i] = __is_same(T, __half) ? pack_h2(z[2 * i], z[2 * i + 1]) : pack_b2(z[2 * i], z[2 * i + 1]);
+        if constexpr (N == 4) *reinterpret_cast<uint2*>(out) = make_uint2(u[0], u[1]);
+        else *reinterpret_cast<uint32_t*>(out) = u[0];
+    }
 }
+__device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l) {
+    const int t = a.by_group(row);
+    if (a.lse)
+        a.lse[(long long)(q0 + t) * a.heads + hk * a.group + row - t * a.group] =
+            l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
+}
+
+// One row of n partial results joined by a warp: piece i has (m, l) at ml(i) (or none) and D values at y(i),
+// of which the lane gets 4 (4 lane ..).  All (m, l) are loaded together and the values eight pieces
+// at a time: with one piece after the other the trips to L2 took 8 to 15 us of a call.
+struct AttnJoin {
+    float m = -INFINITY, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    template <class ML, class Y>
+    __device__ __forceinline__ void join(int n, bool mine, ML ml, Y at) {
+        const int ln = lane_id();
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int cnt = min(32, n - i0);
+            float2 v = make_float2(-INFINITY, 0.f);
+            if (ln < cnt) {
+                const float* p = ml(i0 + ln);
+                if (p) v = __ldcg(reinterpret_cast<const float2*>(p));
+            }
+            float top = v.x;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m);
+            // a piece that saw nothing has m = -inf and l = 0; one of scores that are not numbers has m = -inf only
+            const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : ex2(v.x - top);
+            const float old = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - top);
+            l = l * old + warp_sum(v.y * f);
+            m = top;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = old == 0.f ? 0.f : y[k] * old;
+            for (int i = 0; i < cnt; i += 8) {
+                float4 x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (mine && i + k < cnt) x[k] = __ldcg(reinterpret_cast<const float4*>(at(i0 + i + k)) + ln);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float g = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+                    if (i + k >= cnt || g == 0.f) continue;
+                    y[0] = fmaf(x[k].x, g, y[0]), y[1] = fmaf(x[k].y, g, y[1]);
+                    y[2] = fmaf(x[k].z, g, y[2]), y[3] = fmaf(x[k].w, g, y[3]);
+                }
+            }
+        }
+    }
+};
 
 }  // namespace hc

@@ -124,7 +124,7 @@ extern "C" int hc_kv_read_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_ba
 // The split tiles' partial results and counters: as much as any call of any kernel takes, so that
 // they never move under a captured graph.
 static int attn_workspace(hc_engine* e, AttnArgs* a) {
-    const size_t part = attn_few_part_bytes(32, 128, e->num_sms);
+    const size_t part = kFewPartBytes * e->num_sms;
     if (part > e->attn_part.cap) {
         const int rc = e->attn_part.ensure(part);
         if (rc) return rc;
@@ -168,6 +168,8 @@ extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv
     a.ldo = (long long)ldo;
     a.heads = (int)n_heads;
     a.group = (int)(n_heads / c->n_heads);
+    a.by_group = FastDiv((uint32_t)a.group);
+    a.by_page = FastDiv((uint32_t)c->page_size);
     a.causal = causal != 0;
     a.window = window;
     a.sink = window ? sink : 0;

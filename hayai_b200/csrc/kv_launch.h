@@ -19,6 +19,20 @@ cudaError_t launch_kv_append(int cache_type, int dtype, int head_dim, const KvDe
 cudaError_t launch_kv_read(int cache_type, int dtype, int head_dim, const KvDev& c, const KvBatchDev& b,
                            const KvRows& r, cudaStream_t s);
 
+// Division of 0 <= n < 2^31 by d >= 1 as a multiplication: with 2^k >= d and m = ceil(2^(31+k) / d),
+// floor(n m / 2^(31+k)) = floor(n / d), as m d - 2^(31+k) < d <= 2^k.
+struct FastDiv {
+    uint32_t d, m, k;
+    explicit FastDiv(uint32_t div = 1) : d(div) {
+        k = 0;
+        while (k < 31 && (1u << k) < div) ++k;
+        m = (uint32_t)(((1ull << (31 + k)) + div - 1) / div);
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return (int)(((unsigned long long)(uint32_t)n * m) >> (31 + k));
+    }
+};
+
 struct AttnArgs {
     KvDev c;
     KvBatchDev b;
@@ -27,6 +41,7 @@ struct AttnArgs {
     float* lse;
     long long ldq, ldo;
     int heads, group;  // query heads, and query heads per kv head
+    FastDiv by_group, by_page;
     int causal, window, sink;
     float scale;
     int max_rows;          // the host's bound on a sequence's rows of one kv head (new tokens x group)
@@ -35,11 +50,8 @@ struct AttnArgs {
     int* count;            // one counter per block, zero between calls
 };
 
-// Rows per tile of the kernel for few rows, by the batch's largest sequence.
-inline int attn_few_tile(int max_rows) { return max_rows <= 8 ? 8 : max_rows <= 16 ? 16 : 32; }
-inline size_t attn_few_part_bytes(int rows, int head_dim, int blocks) {
-    return (size_t)blocks * 2 * rows * (head_dim + 2) * sizeof(float);
-}
+// Partial results of the kernel for few rows: bytes for each block.
+constexpr size_t kFewPartBytes = 2 * 9 * 32 * (128 + 2) * 4;
 cudaError_t launch_attn_few(int cache_type, int dtype, int head_dim, const AttnArgs& a, int blocks, cudaStream_t s);
 
 }  // namespace hc
