@@ -178,26 +178,22 @@ struct FewWalk {
     }
 };
 
-// A tile that several warps share, for the joining.
-struct FewShared {
-    int valid, q0, hk, r0, nr, u_item, units;
-};
-
 template <class T, class C, int D, int NT>
 __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kernel(const __grid_constant__ AttnArgs a) {
     using F = FewCfg<T, C, D, NT>;
     using X = FewTerms<T, C>;
     constexpr int W = F::W, THREADS = 32 * W, ST = F::ST, CPR = F::CPR, MT = ST / 16, KS = D / 16, ROWS = 8 * NT, I8 = F::ES == 1;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ FewShared shared_s[W + 1];  // tiles that start in warp w and go on past it; the block's first
+    __shared__ AttnShared shared_s[W + 1];  // tiles that start in warp w and go on past it; the block's first
     __shared__ int last_s[2];
+    __shared__ __align__(8) int scratch[32];
     const int w = threadIdx.x >> 5, ln = lane_id(), g = ln >> 2, t4 = ln & 3;
     const uint32_t ring = smem_addr(smem) + w * F::WB;
     uint8_t* const qf = smem + w * F::WB + F::NS * F::SB;
     float* const rscale = reinterpret_cast<float*>(qf + F::QB);  // [ROWS], and [ROWS] of -1152 sum q
 
     int* const pre = reinterpret_cast<int*>(smem);
-    const int U = attn_schedule<THREADS>(a, ROWS, ST, pre);
+    const int U = attn_schedule<THREADS>(a, ROWS, ST, pre, scratch);
     const int G = min((int)gridDim.x, max(1, U / W)), c = blockIdx.x;
     if (U <= 0 || c >= G) return;
     FewWalk pw;  // the copies' walk: units are issued NS - 1 ahead
@@ -708,7 +704,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
     float* const bpart = a.part + (size_t)2 * gridDim.x * W * F::PS;  // the blocks' partial results, two each
     int crossing = 0, turn = 0;
     for (int x = 0; x <= W; ++x) {
-        const FewShared sh = shared_s[x];
+        const AttnShared sh = shared_s[x];
         if (!sh.valid) continue;
         const int wf = share.owner(sh.u_item), wl = share.owner(sh.u_item + sh.units - 1);
         const bool cross = wf / W != c || wl / W != c;
@@ -741,7 +737,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
     __threadfence();
     __syncthreads();
     for (int x = 0; x <= W; ++x) {
-        const FewShared sh = shared_s[x];
+        const AttnShared sh = shared_s[x];
         if (!sh.valid) continue;
         const int bf = share.owner(sh.u_item) / W, bl = share.owner(sh.u_item + sh.units - 1) / W;
         if (bf == bl) continue;
@@ -805,7 +801,9 @@ cudaError_t by_cache(int ct, int D, const AttnArgs& a, int blocks, cudaStream_t 
 
 }  // namespace
 
-cudaError_t launch_attn_few(int ct, int dt, int D, const AttnArgs& a, int blocks, cudaStream_t s) {
+cudaError_t launch_attn_few(int ct, int dt, int D, const AttnArgs& args, int blocks, cudaStream_t s) {
+    AttnArgs a = args;
+    a.over = 2;  // a tile's start and end cost about what two of its units do
     if (dt == T_F32) return by_cache<float>(ct, D, a, blocks, s);
     if (dt == T_F16) return by_cache<__half>(ct, D, a, blocks, s);
     return by_cache<__nv_bfloat16>(ct, D, a, blocks, s);

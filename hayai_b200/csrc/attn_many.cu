@@ -1,0 +1,719 @@
+// attn_many.cu -- attention over the paged cache for sequences with many rows per kv head (prompts,
+// chunks of prompts), on the 5th-generation tensor cores.
+//
+// The mathematics is attn_few.cu's: one pass with a running maximum m and sum per row, m moved only
+// when a score passes it by 8 (in log 2).  Work comes in tiles of 256 rows (attn_rows.cuh), two
+// halves of 128 with their own accumulators, and units of 128 positions; one block of 16 warps per SM
+// takes an equal share of the line of units.
+//
+//   warps 0-3, 4-7   one thread per row of half 0 and 1: S from TMEM, weights P = 2^(s - m) back into
+//                    the same TMEM columns in 16 bits, m and the sum in registers; the row's O in TMEM
+//                    is rescaled by its thread in the rare units where m moves;
+//   warps 8-11       bring keys and values in: 16-byte asynchronous copies (8-bit pages: by way of a
+//                    staging ring, from which each thread converts what it copied itself) into
+//                    128-byte-swizzled operand tiles, a ring of 4 or 5 of 32 KB;
+//   warp 12          issues S = Q K^T and O += P V (P from TMEM, V as it lies: its tile is read with
+//                    the transposed, d-major view), one half's products while the other half's
+//                    weights are made.
+//
+// Per unit and half the tensor cores take 2 x 512 cycles (D = 128) and the 16384 exponentials 1024 of
+// the special function unit: the two pipes are equally loaded, and the rest of the softmax has to fit
+// under them.
+//
+// Formats: products of f16 (f16 and 8-bit caches) or bf16.  8-bit codes are exact in f16; a K scale
+// multiplies its column of S, a V scale its column of P, and m follows the largest score + log2 of the
+// unit's largest V scale, so that P times scale stays under 2^8 whatever the scales are.  Rows of
+// bf16 on f16 products are scaled by a power of two to have their largest element in [1, 2).
+#include <math.h>
+
+#include "attn_rows.cuh"
+#include "tc5.cuh"
+
+namespace hc {
+
+constexpr int kManyRows = 256, kManyUnit = 128, kManyThreads = 512, kManyRegs = 176, kManyRegsLow = 80;
+
+template <class C, int D>
+struct ManyCfg {
+    static constexpr int ES = sizeof(C);
+    static constexpr bool I8 = ES == 1, BF = ES == 2 && !__is_same(C, __half);
+    static constexpr int TILE = 128 * D * 2;                 // an operand tile: 128 rows of D 16-bit values
+    static constexpr int NB = D == 64 ? 6 : I8 ? 4 : 5;      // ring of key and value tiles
+    static constexpr int CPR = D * ES / 16;                  // 16-byte chunks of a cache row
+    static constexpr int STG = I8 ? 64 * D : 0, NSTG = I8 ? 3 : 0;  // staging: 64 rows of codes
+    static constexpr int oQ = 0, oKV = 2 * TILE, oSTG = oKV + NB * TILE, oSC = oSTG + NSTG * STG;
+    static constexpr int oBAR = oSC + (I8 ? 3 * 1024 : 0);   // scales: ring of 3 units, K then V
+    static constexpr int oMISC = oBAR + 256, BYTES = oMISC + 512;
+};
+
+// One thread's wait with a limit; false once any wait of the thread has run out.
+__device__ __forceinline__ bool many_wait(uint32_t bar, uint32_t parity, bool& ok) {
+    if (ok && !mbar_wait(bar, parity)) ok = false;
+    return ok;
+}
+
+// V tile as B operand, N = d: 64 values of d to a 128-byte row, rows = positions (K of the product),
+// halves of d one tile half apart (leading byte offset), 8 positions 1024 bytes apart (stride).
+__device__ __forceinline__ uint64_t many_v_desc(uint32_t saddr, uint32_t half_bytes) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(half_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The wait for loads still in flight, tied to their registers so that no use moves before it.
+__device__ __forceinline__ void tc_wait_ld32(float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t tc_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r)
+                 : "r"(taddr)
+                 : "memory");
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+        "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// The range of a row's visible positions in the tile's count v: v < c and (v >= b or v < a).
+struct ManyRow {
+    int a, b, c;
+};
+__device__ __forceinline__ ManyRow many_row(const AttnArgs& ar, const KvSeq& q, const AttnTile& t, int row, bool real) {
+    ManyRow r;
+    const int pos = q.len - (q.q1 - q.q0) + ar.by_group(row);
+    const int lim = ar.causal ? min(pos + 1, q.len) : q.len;  // positions j < lim
+    r.c = lim <= t.n1 ? lim : lim < t.lo ? t.n1 : lim - t.lo + t.n1;
+    if (!real) r.c = 0;
+    r.b = ar.window ? max(pos - ar.window + 1, t.lo) - t.lo + t.n1 : 0;
+    r.a = ar.sink <= t.lo ? t.n1 : ar.sink - t.lo + t.n1;
+    return r;
+}
+
+// O += P V of one unit by the rows' threads, leaving out weights of zero.
+template <bool BF, int D>
+__device__ __noinline__ void many_product(uint32_t tO, uint32_t tP, const uint8_t* v, bool fresh) {
+#pragma unroll 1
+    for (int k = 0; k < D / 32; ++k) {
+        float o[32];
+        tc_ld32(tO + 32 * k, o);
+        tc_wait_ld32(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = fresh ? 0.f : o[i];
+#pragma unroll 1
+        for (int t = 0; t < 128; ++t) {
+            const uint32_t two = tc_ld1(tP + (t >> 1)), w = t & 1 ? two >> 16 : two & 0xffffu;
+            const float p = BF ? __uint_as_float(w << 16) : h2f((uint16_t)w);
+            if (p != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int d = 32 * k + i;
+                    const uint16_t x = *reinterpret_cast<const uint16_t*>(v + (d >> 6) * (128 * 128) + t * 128 +
+                                                                         ((((d & 63) >> 3) ^ (t & 7)) << 4) + (d & 7) * 2);
+                    o[i] += p * (BF ? __uint_as_float((uint32_t)x << 16) : h2f(x));
+                }
+            }
+            __syncwarp();
+        }
+        tc_st32(tO + 32 * k, o);
+    }
+    tc_wait_st();
+}
+
+template <class T, class C, int D>
+__global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid_constant__ AttnArgs a) {
+    using F = ManyCfg<C, D>;
+    constexpr bool I8 = F::I8, BF = F::BF;
+    constexpr int ROWS = kManyRows, UNIT = kManyUnit, NB = F::NB, TILE = F::TILE, HALF = 128 * 128;
+    constexpr int PS = ROWS * (D + 2);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sb = smem_addr(smem), bars = sb + F::oBAR;
+    // barriers: full[NB], empty[NB], s[2] (S or the last O ready), p[2] (P ready), q[2] (queries ready)
+    const uint32_t b_full = bars, b_empty = bars + 8 * NB, b_s = bars + 16 * NB, b_p = b_s + 16, b_q = b_s + 32;
+    int* const misc = reinterpret_cast<int*>(smem + F::oMISC);  // [0] TMEM base, [1] last; [8..] the schedule's sums
+    AttnShared* const shared_s = reinterpret_cast<AttnShared*>(misc + 64);  // the block's first and last tile, where shared
+    const int warp = threadIdx.x >> 5, ln = lane_id(), c = blockIdx.x;
+
+    int* const pre = reinterpret_cast<int*>(smem);
+    const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre, misc + 8);
+    const int G = min((int)gridDim.x, U);
+    if (U <= 0 || c >= G) return;
+    const AttnShares share(U, G);
+    const int b0 = share.begin(c), b1 = share.begin(c + 1);
+    AttnIter it;
+    it.seek(a, pre, b0, ROWS, UNIT);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NB; ++i) {
+            mbar_init(b_full + 8 * i, 4);
+            mbar_init(b_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b_s + 8 * i, 1);
+            mbar_init(b_p + 8 * i, 4);
+            mbar_init(b_q + 8 * i, 4);
+            shared_s[i].valid = 0;
+        }
+        mbar_fence_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(misc)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t*)misc;
+    bool ok = true;
+
+    if (warp < 8) {
+        // ================================================================ softmax, a thread per row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
+        const int half = warp >> 2, rt = threadIdx.x & 127;  // half of the tile, row of the half
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t tS = tmem + lanes + half * 128, tO = tmem + lanes + 256 + half * 128;
+        uint8_t* const qs = smem + half * TILE;
+        uint32_t ph_s = 0;
+        int unit = 0;   // units of the block so far, for the scales' ring
+        int kvt = 0;    // key and value tiles so far
+        for (;;) {
+            const AttnTile& tl = it.t;
+            const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
+            if (lo < hi && half * 128 < tl.nr) {
+                const int r = half * 128 + rt, row = tl.r0 + r;
+                const bool real = r < tl.nr;
+                float rs = fabsf(a.scale) * 1.44269504f;
+                // ---- the row's queries as the A operand
+                {
+                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the scale's sign goes into the queries
+                    const int tr = a.by_group(real ? row : tl.r0);
+                    const T* q = (const T*)a.q + (long long)(it.q.q0 + tr) * a.ldq +
+                                 (it.hk * a.group + (real ? row : tl.r0) - tr * a.group) * D;
+                    uint4 x[D / 8];
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        x[i] = real ? __ldg(reinterpret_cast<const uint4*>(q) + i) : make_uint4(0, 0, 0, 0);
+                    if constexpr (!__is_same(T, __half) && !BF) {  // bf16 rows into f16
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i) {
+                            const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                m = max(m, max(y[k] & 0x7fffu, (y[k] >> 16) & 0x7fffu));
+                        }
+                        const uint32_t e = m >> 7;
+                        const bool norm = e >= 2 && e <= 252;
+                        const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
+                        if (norm) rs *= __uint_as_float(e << 23);
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i) {
+                            uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                y[k] = pack_h2(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down);
+                            x[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        *reinterpret_cast<uint4*>(qs + (i >> 3) * HALF + rt * 128 + (((i & 7) ^ (rt & 7)) << 4)) =
+                            make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (ln == 0) mbar_arrive(b_q + 8 * half);
+                rs = fmaxf(rs, 1e-30f);
+                const ManyRow vis = many_row(a, it.q, tl, row, real);
+                // a unit is whole for this half's rows if it ends before every row's limit and starts past
+                // every row's window (or lies in the first tokens that all see)
+                const int h0 = min(half * 128, tl.nr - 1), h1 = min(half * 128 + 127, tl.nr - 1);
+                const ManyRow first = many_row(a, it.q, tl, tl.r0 + h0, true), lastr = many_row(a, it.q, tl, tl.r0 + h1, true);
+                const int cmin = min(first.c, lastr.c), bmax = lastr.b, amin = first.a;
+
+                float m = -INFINITY;
+                float2 l2 = make_float2(0.f, 0.f);
+                for (int st = lo; st < hi; ++st, ++unit) {
+                    if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
+                    ph_s ^= 1;
+                    tc_fence_after();
+                    float ev = 0.f;
+                    const float4 *ksc = nullptr, *vsc = nullptr;
+                    if constexpr (I8) {
+                        // the scales come with the tiles: both are in (or soon), and the waits make them visible
+                        const int kt = kvt + 2 * (st - lo);
+                        if (!many_wait(b_full + 8 * (kt % NB), (kt / NB) & 1, ok)) break;
+                        if (!many_wait(b_full + 8 * ((kt + 1) % NB), ((kt + 1) / NB) & 1, ok)) break;
+                        const uint8_t* sc = smem + F::oSC + (unit % 3) * 1024;
+                        ksc = reinterpret_cast<const float4*>(sc);
+                        vsc = reinterpret_cast<const float4*>(sc + 512);
+                        const float4 v = vsc[ln];
+                        auto size = [](float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; };  // what is not finite has none
+                        float top = fmaxf(fmaxf(size(v.x), size(v.y)), fmaxf(size(v.z), size(v.w)));
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        ev = (float)((int)(__float_as_uint(top) >> 23) - 126);  // log2 of a power of two over it
+                    }
+                    const int v0 = st * UNIT;
+                    const bool full = v0 + UNIT <= cmin && (v0 >= bmax || v0 + UNIT <= amin);
+                    const int vc = vis.c - v0, vb = vis.b - v0, va = vis.a - v0;
+                    // 32 scores from TMEM: times their K scales, masked
+                    auto scores = [&](int k, float* s) {
+                        if constexpr (I8) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 f = ksc[8 * k + i];
+                                const float2 x = mul2(make_float2(s[4 * i], s[4 * i + 1]), make_float2(f.x, f.y));
+                                const float2 y = mul2(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(f.z, f.w));
+                                s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = y.x, s[4 * i + 3] = y.y;
+                            }
+                        }
+                        if (!full) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const int v = 32 * k + i;
+                                if (!(v < vc && (v >= vb || v < va))) s[i] = -INFINITY;
+                            }
+                        }
+                    };
+                    // two passes over S, 32 columns at a time with the next 32 on their way: all 128 in
+                    // registers would take more than a thread has
+                    float sa[2][32];
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tc_ld32(tS, sa[0]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float* s = sa[k & 1];
+                        tc_wait_ld32(s);
+                        tc_ld32(tS + (k < 3 ? 32 * (k + 1) : 0), sa[(k + 1) & 1]);  // last: the second pass's first
+                        scores(k, s);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
+                    }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const float cand = top == -INFINITY ? top : top * rs + ev;
+                    tc_wait_ld32(sa[0]);  // before other loads and waits
+                    if (__any_sync(0xffffffffu, cand > m + 8.f)) {
+                        const float mn = fmaxf(m, cand), f = mn == -INFINITY ? 1.f : ex2(m - mn);
+                        m = mn;
+                        l2.x *= f;
+                        l2.y *= f;
+                        if (st != lo) {  // the unit's S came after the last P V: O is complete
+#pragma unroll 1
+                            for (int k = 0; k < D / 32; ++k) {
+                                float o[32];
+                                tc_ld32(tO + 32 * k, o);
+                                tc_wait_ld32(o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] *= f;
+                                tc_st32(tO + 32 * k, o);
+                            }
+                        }
+                    }
+                    const float mm = m == -INFINITY ? 0.f : m;
+                    const float2 rs2 = make_float2(rs, rs), nm2 = make_float2(-mm, -mm);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float* s = sa[k & 1];
+                        if (k > 0) tc_wait_ld32(s);
+                        if (k < 3) tc_ld32(tS + 32 * (k + 1), sa[(k + 1) & 1]);
+                        scores(k, s);
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int e = 2 * i;
+                            const float2 x = fma2(make_float2(s[e], s[e + 1]), rs2, nm2);
+                            float2 p = make_float2(ex2(x.x), ex2(x.y));
+                            l2 = add2(l2, p);
+                            if constexpr (I8) {
+                                const float2 f = reinterpret_cast<const float2*>(vsc)[16 * k + i];
+                                p = mul2(p, f);
+                                if (!full) {  // whatever a masked position's scale is
+                                    if (s[e] == -INFINITY) p.x = 0.f;
+                                    if (s[e + 1] == -INFINITY) p.y = 0.f;
+                                }
+                            }
+                            pk[i] = BF ? pack_b2(p.x, p.y) : pack_h2(p.x, p.y);
+                        }
+                        tc_st16(tS + 16 * k, pk);
+                    }
+                    tc_wait_st();
+                    if constexpr (!I8) {
+                        // a value that is not finite, in a unit that some row does not see whole: 0 * infinity must
+                        // not reach a masked row, so that the unit's product is done here (rare)
+                        if (!full) {
+                            const int vt = kvt + 2 * (st - lo) + 1;
+                            if (!many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok)) break;
+                            const uint8_t* vtile = smem + F::oKV + (vt % NB) * TILE;
+                            constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+                            uint32_t odd = 0;
+#pragma unroll 4
+                            for (int i = 0; i < D / 8; ++i) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(vtile + (i >> 3) * HALF + rt * 128 +
+                                                                                (((i + rt) & 7) << 4));
+                                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) odd |= (y[k] & E) == E || ((y[k] >> 16) & E) == E;
+                            }
+                            asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %0, 0;\nbarrier.cta.red.or.pred q, %1, 128, p;\n"
+                                         "selp.u32 %0, 1, 0, q;\n}"
+                                         : "+r"(odd)
+                                         : "r"(2 + half)
+                                         : "memory");
+                            if (rt == 0) misc[2 + half] = (int)odd;  // read by the products' thread after the arrivals
+                            if (odd) many_product<BF, D>(tO, tS, vtile, st == lo);
+                        } else if (rt == 0) {
+                            misc[2 + half] = 0;
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (ln == 0) mbar_arrive(b_p + 8 * half);
+                }
+                // ---- the tile's end: O out
+                many_wait(b_s + 8 * half, ph_s, ok);
+                ph_s ^= 1;
+                tc_fence_after();
+                const float l = l2.x + l2.y;
+                const bool whole = lo == 0 && hi == tl.units;
+                const float k1 = l == 0.f ? 0.f : 1.f / l;
+                const int tr = a.by_group(row);
+                T* const out = (T*)a.out + (long long)(it.q.q0 + tr) * a.ldo + (it.hk * a.group + row - tr * a.group) * D;
+                float* const part = a.part + (size_t)(2 * c + (lo == 0)) * PS;
+#pragma unroll 1
+                for (int k = 0; k < D / 32; ++k) {
+                    float o[32];
+                    tc_ld32(tO + 32 * k, o);
+                    tc_wait_ld32(o);
+                    if (!real || !ok) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : o[8 * i + e] * k1;
+                            Elem<T>::store8(out + 32 * k + 8 * i, y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(part + r * D + 32 * k + 4 * i) =
+                                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+                tc_fence_before();
+                if (real && ok) {
+                    if (whole)
+                        attn_store_lse(a, it.q.q0, it.hk, row, m, l);
+                    else
+                        *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m, l);
+                }
+                if (!whole && rt == 0 && half == 0)
+                    shared_s[lo == 0] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units};
+            } else if (lo < hi) {
+                unit += hi - lo;
+            }
+            if (lo < hi) kvt += 2 * (hi - lo);
+            if (!ok || it.u_item + tl.span >= b1) break;
+            it.next(a, ROWS, UNIT);
+        }
+        // ---- tiles that several blocks share: the last of them joins
+        __threadfence();
+        named_bar_sync(1, 256);
+        for (int x = 0; x < 2; ++x) {
+            const AttnShared sh = shared_s[x];
+            if (!sh.valid) continue;
+            const int bf = share.owner(sh.u_item), bl = share.owner(sh.u_item + sh.units - 1);
+            if (threadIdx.x == 0) {
+                misc[1] = atomicAdd(a.count + bf, 1) == bl - bf;
+                if (misc[1]) a.count[bf] = 0;
+                __threadfence();
+            }
+            named_bar_sync(1, 256);
+            if (misc[1]) {
+                for (int r = warp; r < sh.nr; r += 8) {
+                    AttnJoin j;
+                    auto piece = [&](int i) { return a.part + (size_t)(2 * (bf + i) + (i == 0)) * PS; };
+                    j.join(bl - bf + 1, ln < D / 4, [&](int i) -> const float* { return piece(i) + ROWS * D + 2 * r; },
+                           [&](int i) { return piece(i) + r * D; });
+                    if (ln >= D / 4) continue;
+                    attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
+                    if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
+                }
+            }
+            named_bar_sync(1, 256);
+        }
+    } else if (warp < 12) {
+        // ================================================================ keys and values in
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsLow));
+        // each warp copies RPW rows of 16-byte chunks at a time; lane i owns the address of row(i)
+        constexpr int CPR = F::CPR, RPW = 32 / CPR, IT = CPR;
+        const int pw = warp - 8;
+        const int own = (ln / RPW) * 4 * RPW + pw * RPW + ln % RPW;  // this lane's row of the 128
+        const int sub = pw * RPW + ln / CPR, ch = ln % CPR;          // its row (of 4 RPW) and chunk of a copy
+        int t_issue = 0, t_done = 0;  // tiles issued and completed (16-bit), or converted (8-bit)
+        int stg = 0, unit = 0;
+        auto publish = [&](int t) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (ln == 0) mbar_arrive(b_full + 8 * (t % NB));
+        };
+        for (;;) {
+            const AttnTile& tl = it.t;
+            const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
+            for (int st = lo; st < hi && ok; ++st, ++unit) {
+                const int v = st * UNIT + own;
+                uint32_t off = 0xffffffffu;
+                float ksc = 0.f, vsc = 0.f;
+                if (v < tl.nvis) {
+                    const int j = v < tl.n1 ? v : v - tl.n1 + tl.lo;
+                    const int p = a.by_page(j), r = j - p * a.c.page_size;
+                    const int pg = __ldg(a.b.table + it.s * a.b.table_stride + p);
+                    if ((unsigned)pg >= (unsigned)a.c.n_pages) {
+                        atomicOr(a.b.err, kErrKvRange);
+                    } else {
+                        off = (uint32_t)pg * a.c.page + (uint32_t)r * a.c.row + (uint32_t)it.hk * a.c.head;
+                        if constexpr (I8) {
+                            const long long so = pg * a.c.spage + (long long)it.hk * a.c.page_size + r;
+                            ksc = __ldg(a.c.ks + so);
+                            vsc = __ldg(a.c.vs + so);
+                        }
+                    }
+                }
+                if constexpr (!I8) {
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int t = t_issue++, buf = t % NB;
+                        if (t >= NB && !many_wait(b_empty + 8 * buf, ((t / NB) - 1) & 1, ok)) break;
+                        const uint32_t dst = sb + F::oKV + buf * TILE;
+                        const uint8_t* src = kv ? a.c.v : a.c.k;
+#pragma unroll
+                        for (int i = 0; i < IT; ++i) {
+                            const uint32_t o = __shfl_sync(0xffffffffu, off, i * RPW + ln / CPR);
+                            const int r = i * 4 * RPW + sub;
+                            const bool have = o != 0xffffffffu;
+                            const unsigned long long at = have ? (unsigned long long)o * 64 + ch * 16 : 0;
+                            const uint32_t d = dst + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src + at),
+                                         "r"(have ? 16 : 0)
+                                         : "memory");
+                        }
+                        cp_async_commit();
+                        if (t_issue - t_done > 2) {
+                            cp_async_wait(2);
+                            publish(t_done++);
+                        }
+                    }
+                } else {
+                    // scales of the unit: its ring slot's last readers are done once the tiles' buffers are free
+                    uint8_t* const sc = smem + F::oSC + (unit % 3) * 1024;
+                    (void)stg;
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int t = t_issue++, buf = t % NB;
+                        if (t >= NB && !many_wait(b_empty + 8 * buf, ((t / NB) - 1) & 1, ok)) break;
+                        reinterpret_cast<float*>(sc + kv * 512)[own] = kv ? vsc : ksc;
+                        uint8_t* const dst = smem + F::oKV + buf * TILE;
+                        const uint8_t* src = kv ? a.c.v : a.c.k;
+                        uint4 x[IT];
+#pragma unroll
+                        for (int i = 0; i < IT; ++i) {
+                            const uint32_t o = __shfl_sync(0xffffffffu, off, i * RPW + ln / CPR);
+                            x[i] = make_uint4(0, 0, 0, 0);
+                            if (o != 0xffffffffu)
+                                x[i] = ldg_stream128(src + (unsigned long long)o * 64 + ch * 16);
+                        }
+#pragma unroll
+                        for (int i = 0; i < IT; ++i) {
+                            const int r = i * 4 * RPW + sub;
+                            const uint32_t y[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u,
+                                                   x[i].w ^ 0x80808080u};
+                            uint32_t h[8];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                h[2 * k] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4140u), 0x64806480u);
+                                h[2 * k + 1] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4342u), 0x64806480u);
+                            }
+                            // chunk ch holds d = 16 ch ..: two 16-byte places of the tile's row
+                            uint8_t* const row = dst + (ch >> 2) * HALF + r * 128;
+                            const int p = 2 * (ch & 3);
+                            *reinterpret_cast<uint4*>(row + ((p ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4*>(row + (((p + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                        }
+                        publish(t);
+                    }
+                }
+            }
+            if (!ok || it.u_item + tl.span >= b1) break;
+            it.next(a, ROWS, UNIT);
+        }
+        if constexpr (!I8) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            while (t_done < t_issue && ok) publish(t_done++);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsLow));
+        if (warp == 12 && ln == 0) {
+            // ============================================================ the products
+            constexpr uint32_t fmt = BF ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t idS = (1u << 4) | fmt | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t idO = (1u << 4) | fmt | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+            uint32_t ph_p[2] = {0, 0}, ph_q[2] = {0, 0};
+            int t = 0;  // key and value tiles so far
+            for (;;) {
+                const AttnTile& tl = it.t;
+                const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
+                if (lo < hi) {
+                    const int halves = tl.nr > 128 ? 2 : 1, n = hi - lo;
+                    auto scores = [&](int h, int kt) {  // S_h = Q_h K^T
+                        const uint32_t q = sb + h * TILE, k = sb + F::oKV + (kt % NB) * TILE;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i)
+                            tc_mma(tmem + h * 128, tc_desc(q + (i >> 2) * HALF + (i & 3) * 32),
+                                   tc_desc(k + (i >> 2) * HALF + (i & 3) * 32), idS, i ? 1u : 0u);
+                    };
+                    for (int h = 0; h < halves; ++h) {
+                        many_wait(b_q + 8 * h, ph_q[h], ok);
+                        ph_q[h] ^= 1;
+                    }
+                    many_wait(b_full + 8 * (t % NB), (t / NB) & 1, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (int h = 0; h < halves; ++h) {
+                        scores(h, t);
+                        tc_commit(b_s + 8 * h);
+                    }
+                    tc_commit(b_empty + 8 * (t % NB));
+                    for (int u = 0; u < n && ok; ++u, t += 2) {
+                        const int vt = t + 1, kn = t + 2;
+                        many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok);
+                        if (u + 1 < n) many_wait(b_full + 8 * (kn % NB), (kn / NB) & 1, ok);
+                        for (int h = 0; h < halves; ++h) {
+                            if (!many_wait(b_p + 8 * h, ph_p[h], ok)) break;
+                            ph_p[h] ^= 1;
+                            tc_fence_after();
+                            const uint32_t v = sb + F::oKV + (vt % NB) * TILE;
+                            if (I8 || !*(volatile int*)&misc[2 + h])
+#pragma unroll
+                            for (int i = 0; i < UNIT / 16; ++i)  // O_h += P_h V
+                                tc_mma_ta(tmem + 256 + h * 128, tmem + h * 128 + 8 * i, many_v_desc(v + i * 2048, HALF), idO,
+                                          u || i ? 1u : 0u);
+                            if (u + 1 < n) scores(h, kn);
+                            tc_commit(b_s + 8 * h);  // the next S, or the last O
+                        }
+                        tc_commit(b_empty + 8 * (vt % NB));
+                        if (u + 1 < n) tc_commit(b_empty + 8 * (kn % NB));
+                    }
+                }
+                if (!ok || it.u_item + tl.span >= b1) break;
+                it.next(a, ROWS, UNIT);
+            }
+        }
+    }
+    if (!ok) atomicOr(a.b.err, 2);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+namespace {
+
+template <class T, class C, int D>
+cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
+    constexpr int bytes = ManyCfg<C, D>::BYTES;
+    static_assert(bytes <= 227 * 1024, "shared memory of a block");
+    static_assert(sizeof(float) * 2 * kManyRows * (D + 2) <= kManyPartBytes, "the workspace of a block");
+    const cudaError_t e = cudaFuncSetAttribute(attn_many_kernel<T, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    AttnArgs b = a;
+    b.over = 2;  // a tile's start and end cost about what two of its units do
+    attn_many_kernel<T, C, D><<<blocks, kManyThreads, bytes, s>>>(b);
+    return cudaGetLastError();
+}
+
+template <class T, int D>
+cudaError_t by_cache(int ct, const AttnArgs& a, int blocks, cudaStream_t s) {
+    if (ct == T_F16) return launch<T, __half, D>(a, blocks, s);
+    return launch<T, int8_t, D>(a, blocks, s);
+}
+
+}  // namespace
+
+bool attn_many_supported(int ct, int dt) { return (dt == T_F16 && ct != T_BF16) || dt == T_BF16; }
+
+cudaError_t launch_attn_many(int ct, int dt, int D, const AttnArgs& a, int blocks, cudaStream_t s) {
+    if (ct == T_BF16)
+        return D == 64 ? launch<__nv_bfloat16, __nv_bfloat16, 64>(a, blocks, s)
+                       : launch<__nv_bfloat16, __nv_bfloat16, 128>(a, blocks, s);
+    if (dt == T_F16) return D == 64 ? by_cache<__half, 64>(ct, a, blocks, s) : by_cache<__half, 128>(ct, a, blocks, s);
+    return D == 64 ? by_cache<__nv_bfloat16, 64>(ct, a, blocks, s) : by_cache<__nv_bfloat16, 128>(ct, a, blocks, s);
+}
+
+}  // namespace hc

@@ -8,7 +8,7 @@
 // nvis - 1, position j = v < n1 ? v : v - n1 + lo, and cut into units of `unit` of them.
 //
 // All units of a call, in the order (sequence, kv head, tile, unit), are one line; after a tile's
-// units come `kOver` places that stand for what starting and finishing a tile costs.  Of the U
+// units come `over` places that stand for what starting and finishing a tile costs.  Of the U
 // places the workers take equal shares, whatever the lengths are.  A tile whose units fall to several workers is joined from their partial results,
 // in the workers' order (the same bits every time).
 #pragma once
@@ -19,13 +19,11 @@
 
 namespace hc {
 
-constexpr int kOver = 2;  // measured with units of 32 tokens: a tile costs about what two of them do
-
 struct AttnTile {
     int r0, nr;        // first row and number of rows
     int p_lo, p_hi;    // positions of the first and last row
     int lo, n1, nvis;  // visible positions (see above)
-    int units, span;   // span: units + kOver
+    int units, span;   // span: units + a.over
 };
 
 __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q, int tile, int rows, int unit) {
@@ -40,7 +38,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
     t.n1 = min(a.sink, t.lo);
     t.nvis = t.n1 + end - t.lo;
     t.units = max(1, (t.nvis + unit - 1) / unit);  // a tile that sees nothing still has to write zeros
-    t.span = t.units + kOver;
+    t.span = t.units + a.over;
     return t;
 }
 
@@ -50,11 +48,13 @@ __device__ __forceinline__ int attn_tiles(const AttnArgs& a, const KvSeq& q, int
 }
 
 // Places of every sequence, as an inclusive prefix sum in `pre` (n_seq ints of shared memory);
-// returns U, or -1 (and the error flag) if they do not fit 31 bits.  The whole block calls it.
+// returns U, or -1 (and the error flag) if they do not fit 31 bits.  The whole block calls it, with 32
+// words of shared memory as scratch.
 template <int THREADS>
-__device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int unit, int* pre) {
-    __shared__ long long carry_s;
-    __shared__ int wsum[THREADS / 32];
+__device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int unit, int* pre, int* scratch) {
+    static_assert(THREADS <= 32 * 16, "scratch");
+    long long& carry_s = *reinterpret_cast<long long*>(scratch);
+    int* const wsum = scratch + 2;
     const int cap = a.b.max_pages * a.c.page_size, tid = threadIdx.x, wid = tid >> 5, ln = tid & 31;
     const bool by_warp = a.max_rows > 8 * rows;  // many tiles in a sequence: its tiles over a warp's lanes
     if (by_warp) {
@@ -103,6 +103,11 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
     }
     return (int)carry_s;
 }
+
+// A tile that several workers share, for the joining.
+struct AttnShared {
+    int valid, q0, hk, r0, nr, u_item, units;
+};
 
 // An item of the line, (sequence, kv head, tile), and its first place.
 struct AttnIter {

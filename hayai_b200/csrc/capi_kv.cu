@@ -124,7 +124,7 @@ extern "C" int hc_kv_read_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_ba
 // The split tiles' partial results and counters: as much as any call of any kernel takes, so that
 // they never move under a captured graph.
 static int attn_workspace(hc_engine* e, AttnArgs* a) {
-    const size_t part = kFewPartBytes * e->num_sms;
+    const size_t part = kAttnPartBytes * e->num_sms;
     if (part > e->attn_part.cap) {
         const int rc = e->attn_part.ensure(part);
         if (rc) return rc;
@@ -176,10 +176,23 @@ extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv
     a.scale = scale;
     const long long rows = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
     a.max_rows = (int)(rows < INT32_MAX ? rows : INT32_MAX);
-    a.row_min = 1;
-    a.row_max = INT32_MAX;
     rc = attn_workspace(e, &a);
     if (rc) return rc;
-    const cudaError_t ce = launch_attn_few(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
+    // Sequences of up to kFewRows rows per kv head go to the kernel for few rows, longer ones to the
+    // other, which has tiles of 256: both are launched where the batch may have both.
+    constexpr int kFewRows = 32;
+    const bool many = attn_many_supported(c->type, dtype) && a.max_rows > kFewRows;
+    cudaError_t ce = cudaSuccess;
+    if (many) {
+        a.row_min = b->n_seq > 1 ? kFewRows + 1 : 1;
+        a.row_max = INT32_MAX;
+        ce = launch_attn_many(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
+    }
+    if (ce == cudaSuccess && (!many || b->n_seq > 1)) {
+        a.row_min = 1;
+        a.row_max = many ? kFewRows : INT32_MAX;
+        if (many) a.max_rows = kFewRows;
+        ce = launch_attn_few(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
+    }
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_paged launch");
 }

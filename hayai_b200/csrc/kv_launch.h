@@ -46,12 +46,20 @@ struct AttnArgs {
     float scale;
     int max_rows;          // the host's bound on a sequence's rows of one kv head (new tokens x group)
     int row_min, row_max;  // sequences with fewer or more rows are left to another kernel
+    int over;              // places of the line that stand for a tile's start and end
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
     int* count;            // one counter per block, zero between calls
 };
 
 // Partial results of the kernel for few rows: bytes for each block.
 constexpr size_t kFewPartBytes = 2 * 9 * 32 * (128 + 2) * 4;
+constexpr size_t kManyPartBytes = 2 * 256 * (128 + 2) * 4;
+constexpr size_t kAttnPartBytes = kFewPartBytes > kManyPartBytes ? kFewPartBytes : kManyPartBytes;
+
+// Sequences with few rows of a kv head, on mma.sync; any types.
 cudaError_t launch_attn_few(int cache_type, int dtype, int head_dim, const AttnArgs& a, int blocks, cudaStream_t s);
+// Sequences with many rows of a kv head, on tcgen05; 16-bit rows.
+bool attn_many_supported(int cache_type, int dtype);
+cudaError_t launch_attn_many(int cache_type, int dtype, int head_dim, const AttnArgs& a, int blocks, cudaStream_t s);
 
 }  // namespace hc
