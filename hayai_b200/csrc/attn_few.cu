@@ -117,10 +117,6 @@ __device__ __forceinline__ uint32_t split_pair(float& x, float& y) {
     }
 }
 
-// Copy 16 bytes (or with ok false: 16 zero bytes) to shared memory.
-__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp4_or_zero(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }

@@ -11,10 +11,12 @@
 //                    is rescaled by its thread in the rare units where m moves;
 //   warps 8-11       bring keys and values in: 16-byte asynchronous copies (8-bit pages: by way of a
 //                    staging ring, from which each thread converts what it copied itself) into
-//                    128-byte-swizzled operand tiles, a ring of 4 or 5 of 32 KB;
+//                    128-byte-swizzled operand tiles, a ring of 3 (8-bit) or 5 of 32 KB;
 //   warp 12          issues S = Q K^T and O += P V (P from TMEM, V as it lies: its tile is read with
 //                    the transposed, d-major view), one half's products while the other half's
-//                    weights are made.
+//                    weights are made;
+//   warp 13          walks the block's tiles and hands them to the others as segments (ring of 4);
+//   warps 14-15      bring the queries in, the next segment's while the last unit's weights are made.
 //
 // Per unit and half the tensor cores take 2 x 512 cycles (D = 128) and the 16384 exponentials 1024 of
 // the special function unit: the two pipes are equally loaded, and the rest of the softmax has to fit
@@ -31,19 +33,20 @@
 
 namespace hc {
 
-constexpr int kManyRows = 256, kManyUnit = 128, kManyThreads = 512, kManyRegs = 176, kManyRegsLow = 80;
+constexpr int kManyRows = 256, kManyUnit = 128, kManyThreads = 512, kManyRegs = 192, kManyRegsLow = 64;
 
 template <class C, int D>
 struct ManyCfg {
     static constexpr int ES = sizeof(C);
     static constexpr bool I8 = ES == 1, BF = ES == 2 && !__is_same(C, __half);
     static constexpr int TILE = 128 * D * 2;                 // an operand tile: 128 rows of D 16-bit values
-    static constexpr int NB = D == 64 ? 6 : I8 ? 4 : 5;      // ring of key and value tiles
+    static constexpr int NB = I8 ? 3 : D == 64 ? 6 : 5;      // ring of key and value tiles
     static constexpr int CPR = D * ES / 16;                  // 16-byte chunks of a cache row
-    static constexpr int STG = I8 ? 64 * D : 0, NSTG = I8 ? 3 : 0;  // staging: 64 rows of codes
+    static constexpr int STG = I8 ? 128 * D : 0, NSTG = I8 ? 3 : 0;  // staging ring of tiles of codes
     static constexpr int oQ = 0, oKV = 2 * TILE, oSTG = oKV + NB * TILE, oSC = oSTG + NSTG * STG;
-    static constexpr int oBAR = oSC + (I8 ? 3 * 1024 : 0);   // scales: ring of 3 units, K then V
-    static constexpr int oMISC = oBAR + 256, BYTES = oMISC + 512;
+    static constexpr int oRS = oSC + (I8 ? 4 * 1024 : 0);    // scales: ring of 4 units, K then V
+    static constexpr int oBAR = oRS + 2048;                  // the rows' score factors, of two segments
+    static constexpr int oSEG = oBAR + 256, oMISC = oSEG + 256, BYTES = oMISC + 512;
 };
 
 // One thread's wait with a limit; false once any wait of the thread has run out.
@@ -57,6 +60,28 @@ __device__ __forceinline__ bool many_wait(uint32_t bar, uint32_t parity, bool& o
 __device__ __forceinline__ uint64_t many_v_desc(uint32_t saddr, uint32_t half_bytes) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(half_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
+}
+
+// The products' instructions as a whole warp issues them, by the lane that elect picks: control and
+// operands are then uniform for the compiler, which halves what an issue costs (70 against 55 cycles
+// and less per product of 128 x 64 x 16; one of 128 x 128 x 16 runs 64).
+__device__ __forceinline__ void many_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void many_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void many_commit(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
@@ -139,6 +164,16 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// A run of one tile's units, as the block's roles get it.
+struct ManySeg {
+    int lo, hi;               // units [lo, hi); lo = hi: there are no more
+    int nr, r0;               // rows of the tile, its first
+    int q0, q1, len, s, hk;   // the sequence and kv head
+    int vlo, n1, nvis;        // its visible positions (AttnTile)
+    int whole, slot;          // the whole tile; else the block's slot of partial results
+    int pad[2];
+};
+
 // The range of a row's visible positions in the tile's count v: v < c and (v >= b or v < a).
 struct ManyRow {
     int a, b, c;
@@ -192,20 +227,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     constexpr int PS = ROWS * (D + 2);
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sb = smem_addr(smem), bars = sb + F::oBAR;
-    // barriers: full[NB], empty[NB], s[2] (S or the last O ready), p[2] (P ready), q[2] (queries ready)
-    const uint32_t b_full = bars, b_empty = bars + 8 * NB, b_s = bars + 16 * NB, b_p = b_s + 16, b_q = b_s + 32;
-    int* const misc = reinterpret_cast<int*>(smem + F::oMISC);  // [0] TMEM base, [1] last; [8..] the schedule's sums
+    // barriers: key and value tiles full and empty; S ready, P ready, O ready, queries in, queries free
+    // (of each half); segments full and empty
+    const uint32_t b_full = bars, b_empty = bars + 8 * NB, b_s = bars + 16 * NB, b_p = b_s + 16, b_o = b_s + 32,
+                   b_q = b_s + 48, b_qf = b_s + 64, b_seg = b_s + 80, b_sege = b_seg + 32;
+    float* const rsc = reinterpret_cast<float*>(smem + F::oRS);
+    ManySeg* const segs = reinterpret_cast<ManySeg*>(smem + F::oSEG);
+    int* const misc = reinterpret_cast<int*>(smem + F::oMISC);  // TMEM base, last, [2..3] a product done by hand; [8..] scratch
     AttnShared* const shared_s = reinterpret_cast<AttnShared*>(misc + 64);  // the block's first and last tile, where shared
-    const int warp = threadIdx.x >> 5, ln = lane_id(), c = blockIdx.x;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
 
-    int* const pre = reinterpret_cast<int*>(smem);
-    const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre, misc + 8);
+    // the schedule's prefix sums lie in the last key and value tile until warp 13 has its place
+    int* const pre_s = reinterpret_cast<int*>(smem + F::oKV + (NB - 1) * TILE);
+    const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 8);
     const int G = min((int)gridDim.x, U);
     if (U <= 0 || c >= G) return;
     const AttnShares share(U, G);
-    const int b0 = share.begin(c), b1 = share.begin(c + 1);
-    AttnIter it;
-    it.seek(a, pre, b0, ROWS, UNIT);
     if (threadIdx.x == 0) {
         for (int i = 0; i < NB; ++i) {
             mbar_init(b_full + 8 * i, 4);
@@ -214,8 +251,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
         for (int i = 0; i < 2; ++i) {
             mbar_init(b_s + 8 * i, 1);
             mbar_init(b_p + 8 * i, 4);
-            mbar_init(b_q + 8 * i, 4);
+            mbar_init(b_o + 8 * i, 1);
+            mbar_init(b_q + 8 * i, 2);
+            mbar_init(b_qf + 8 * i, 1);
             shared_s[i].valid = 0;
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(b_seg + 8 * i, 1);
+            mbar_init(b_sege + 8 * i, 15);  // 8 softmax, 4 copying and 2 query warps, and the products' thread
         }
         mbar_fence_init();
     }
@@ -227,8 +270,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *(volatile uint32_t*)misc;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *(volatile uint32_t*)misc, 0);
     bool ok = true;
+    // The n-th segment, once it is there; a role's warp gives it back when it needs it no more.
+    auto segment = [&](int n) {
+        many_wait(b_seg + 8 * (n & 3), (n >> 2) & 1, ok);
+        return segs + (n & 3);
+    };
+    auto give_back = [&](int n) {
+        __syncwarp();
+        if (ln == 0) mbar_arrive(b_sege + 8 * (n & 3));
+    };
 
     if (warp < 8) {
         // ================================================================ softmax, a thread per row
@@ -236,79 +288,44 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
         const int half = warp >> 2, rt = threadIdx.x & 127;  // half of the tile, row of the half
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + lanes + half * 128, tO = tmem + lanes + 256 + half * 128;
-        uint8_t* const qs = smem + half * TILE;
-        uint32_t ph_s = 0;
+        uint32_t ph_s = 0, ph_o = 0, ph_q = 0;
         int unit = 0;   // units of the block so far, for the scales' ring
-        int kvt = 0;    // key and value tiles so far
-        for (;;) {
-            const AttnTile& tl = it.t;
-            const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
-            if (lo < hi && half * 128 < tl.nr) {
-                const int r = half * 128 + rt, row = tl.r0 + r;
-                const bool real = r < tl.nr;
-                float rs = fabsf(a.scale) * 1.44269504f;
-                // ---- the row's queries as the A operand
-                {
-                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the scale's sign goes into the queries
-                    const int tr = a.by_group(real ? row : tl.r0);
-                    const T* q = (const T*)a.q + (long long)(it.q.q0 + tr) * a.ldq +
-                                 (it.hk * a.group + (real ? row : tl.r0) - tr * a.group) * D;
-                    uint4 x[D / 8];
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        x[i] = real ? __ldg(reinterpret_cast<const uint4*>(q) + i) : make_uint4(0, 0, 0, 0);
-                    if constexpr (!__is_same(T, __half) && !BF) {  // bf16 rows into f16
-                        uint32_t m = 0;
-#pragma unroll
-                        for (int i = 0; i < D / 8; ++i) {
-                            const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                m = max(m, max(y[k] & 0x7fffu, (y[k] >> 16) & 0x7fffu));
-                        }
-                        const uint32_t e = m >> 7;
-                        const bool norm = e >= 2 && e <= 252;
-                        const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
-                        if (norm) rs *= __uint_as_float(e << 23);
-#pragma unroll
-                        for (int i = 0; i < D / 8; ++i) {
-                            uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                y[k] = pack_h2(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down);
-                            x[i] = make_uint4(y[0], y[1], y[2], y[3]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<uint4*>(qs + (i >> 3) * HALF + rt * 128 + (((i & 7) ^ (rt & 7)) << 4)) =
-                            make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (ln == 0) mbar_arrive(b_q + 8 * half);
-                rs = fmaxf(rs, 1e-30f);
-                const ManyRow vis = many_row(a, it.q, tl, row, real);
+        for (int n = 0;; ++n) {
+            const ManySeg* const sg = segment(n);
+            const int lo = sg->lo, hi = sg->hi, nr = sg->nr;
+            if (!ok || lo == hi) break;
+            const int kvt = 2 * unit;  // key and value tiles before this segment's
+            unit += hi - lo;
+            if (half * 128 < nr) {
+                const int r = half * 128 + rt, row = sg->r0 + r;
+                const bool real = r < nr;
+                const KvSeq q{sg->q0, sg->q1, sg->len};
+                AttnTile tl;
+                tl.lo = sg->vlo, tl.n1 = sg->n1;
+                const ManyRow vis = many_row(a, q, tl, row, real);
                 // a unit is whole for this half's rows if it ends before every row's limit and starts past
                 // every row's window (or lies in the first tokens that all see)
-                const int h0 = min(half * 128, tl.nr - 1), h1 = min(half * 128 + 127, tl.nr - 1);
-                const ManyRow first = many_row(a, it.q, tl, tl.r0 + h0, true), lastr = many_row(a, it.q, tl, tl.r0 + h1, true);
+                const ManyRow first = many_row(a, q, tl, sg->r0 + half * 128, true),
+                              lastr = many_row(a, q, tl, sg->r0 + min(half * 128 + 127, nr - 1), true);
                 const int cmin = min(first.c, lastr.c), bmax = lastr.b, amin = first.a;
 
+                if (!many_wait(b_q + 8 * half, ph_q, ok)) break;
+                ph_q ^= 1;
+                const float rs = rsc[(n & 1) * 256 + r];
                 float m = -INFINITY;
                 float2 l2 = make_float2(0.f, 0.f);
-                for (int st = lo; st < hi; ++st, ++unit) {
+                for (int st = lo; st < hi; ++st) {
                     if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
                     ph_s ^= 1;
                     tc_fence_after();
                     float ev = 0.f;
                     const float4 *ksc = nullptr, *vsc = nullptr;
                     if constexpr (I8) {
-                        // the scales come with the tiles: both are in (or soon), and the waits make them visible
-                        const int kt = kvt + 2 * (st - lo);
-                        if (!many_wait(b_full + 8 * (kt % NB), (kt / NB) & 1, ok)) break;
-                        if (!many_wait(b_full + 8 * ((kt + 1) % NB), ((kt + 1) / NB) & 1, ok)) break;
-                        const uint8_t* sc = smem + F::oSC + (unit % 3) * 1024;
+                        // V's tile is not given back before this unit's weights, so its barrier is at its phase (K's
+                        // may be one further); K's scales were written before it by the same threads
+                        const int vt = kvt + 2 * (st - lo) + 1;
+                        if (!many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok)) break;
+                        const uint8_t* sc = smem + F::oSC + ((kvt / 2 + st - lo) & 3) * 1024;
                         ksc = reinterpret_cast<const float4*>(sc);
                         vsc = reinterpret_cast<const float4*>(sc + 512);
                         const float4 v = vsc[ln];
@@ -340,23 +357,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                             }
                         }
                     };
-                    // two passes over S, 32 columns at a time with the next 32 on their way: all 128 in
-                    // registers would take more than a thread has
-                    float sa[2][32];
+                    float sa[4][32];
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    tc_ld32(tS, sa[0]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_ld32(tS + 32 * k, sa[k]);
+                    tc_wait_ld32(sa[0]);
+                    tc_wait_ld32(sa[1]);
+                    tc_wait_ld32(sa[2]);
+                    tc_wait_ld32(sa[3]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        float* s = sa[k & 1];
-                        tc_wait_ld32(s);
-                        tc_ld32(tS + (k < 3 ? 32 * (k + 1) : 0), sa[(k + 1) & 1]);  // last: the second pass's first
+                        float* s = sa[k];
                         scores(k, s);
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
                     }
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     const float cand = top == -INFINITY ? top : top * rs + ev;
-                    tc_wait_ld32(sa[0]);  // before other loads and waits
                     if (__any_sync(0xffffffffu, cand > m + 8.f)) {
                         const float mn = fmaxf(m, cand), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                         m = mn;
@@ -378,10 +395,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     const float2 rs2 = make_float2(rs, rs), nm2 = make_float2(-mm, -mm);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        float* s = sa[k & 1];
-                        if (k > 0) tc_wait_ld32(s);
-                        if (k < 3) tc_ld32(tS + 32 * (k + 1), sa[(k + 1) & 1]);
-                        scores(k, s);
+                        const float* s = sa[k];
                         uint32_t pk[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
@@ -435,15 +449,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     if (ln == 0) mbar_arrive(b_p + 8 * half);
                 }
                 // ---- the tile's end: O out
-                many_wait(b_s + 8 * half, ph_s, ok);
-                ph_s ^= 1;
+                many_wait(b_o + 8 * half, ph_o, ok);
+                ph_o ^= 1;
                 tc_fence_after();
                 const float l = l2.x + l2.y;
-                const bool whole = lo == 0 && hi == tl.units;
+                const bool whole = sg->whole;
                 const float k1 = l == 0.f ? 0.f : 1.f / l;
                 const int tr = a.by_group(row);
-                T* const out = (T*)a.out + (long long)(it.q.q0 + tr) * a.ldo + (it.hk * a.group + row - tr * a.group) * D;
-                float* const part = a.part + (size_t)(2 * c + (lo == 0)) * PS;
+                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + (sg->hk * a.group + row - tr * a.group) * D;
+                float* const part = a.part + (size_t)(2 * c + sg->slot) * PS;
 #pragma unroll 1
                 for (int k = 0; k < D / 32; ++k) {
                     float o[32];
@@ -468,18 +482,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 tc_fence_before();
                 if (real && ok) {
                     if (whole)
-                        attn_store_lse(a, it.q.q0, it.hk, row, m, l);
+                        attn_store_lse(a, q.q0, sg->hk, row, m, l);
                     else
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m, l);
                 }
-                if (!whole && rt == 0 && half == 0)
-                    shared_s[lo == 0] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units};
-            } else if (lo < hi) {
-                unit += hi - lo;
             }
-            if (lo < hi) kvt += 2 * (hi - lo);
-            if (!ok || it.u_item + tl.span >= b1) break;
-            it.next(a, ROWS, UNIT);
+            if (!ok) break;
+            give_back(n);
         }
         // ---- tiles that several blocks share: the last of them joins
         __threadfence();
@@ -515,162 +524,265 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
         const int pw = warp - 8;
         const int own = (ln / RPW) * 4 * RPW + pw * RPW + ln % RPW;  // this lane's row of the 128
         const int sub = pw * RPW + ln / CPR, ch = ln % CPR;          // its row (of 4 RPW) and chunk of a copy
-        int t_issue = 0, t_done = 0;  // tiles issued and completed (16-bit), or converted (8-bit)
-        int stg = 0, unit = 0;
-        auto publish = [&](int t) {
+        constexpr int AHEAD = 2;      // tiles on their way behind the one that is waited for
+        int t_issue = 0, t_done = 0;  // tiles whose copies are issued; tiles handed on
+        // A tile has arrived: 16-bit tiles are operands already, codes are converted by the threads that copied them.
+        auto hand_on = [&]() {
+            const int t = t_done++, buf = t % NB;
+            if constexpr (I8) {
+                if (t >= NB && !many_wait(b_empty + 8 * buf, ((t / NB) - 1) & 1, ok)) return;
+                const uint32_t stg = sb + F::oSTG + (t % F::NSTG) * F::STG;
+                const uint32_t dst = sb + F::oKV + buf * TILE;
+#pragma unroll
+                for (int i = 0; i < IT; ++i) {
+                    const int r = i * 4 * RPW + sub;
+                    uint4 x;
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                 : "r"(stg + r * D + ch * 16));
+                    const uint32_t y[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+                    uint32_t h[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        h[2 * k] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4140u), 0x64806480u);
+                        h[2 * k + 1] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4342u), 0x64806480u);
+                    }
+                    // chunk ch holds d = 16 ch ..: two 16-byte places of the tile's row
+                    const uint32_t row = dst + (ch >> 2) * HALF + r * 128;
+                    const int p = 2 * (ch & 3);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((p ^ (r & 7)) << 4)), "r"(h[0]),
+                                 "r"(h[1]), "r"(h[2]), "r"(h[3])
+                                 : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((p + 1) ^ (r & 7)) << 4)), "r"(h[4]),
+                                 "r"(h[5]), "r"(h[6]), "r"(h[7])
+                                 : "memory");
+                }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (ln == 0) mbar_arrive(b_full + 8 * (t % NB));
+            if (ln == 0) mbar_arrive(b_full + 8 * buf);
         };
-        for (;;) {
-            const AttnTile& tl = it.t;
-            const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
-            for (int st = lo; st < hi && ok; ++st, ++unit) {
+        for (int n = 0;; ++n) {
+            const ManySeg* const sg = segment(n);
+            const int lo = sg->lo, hi = sg->hi;
+            if (!ok || lo == hi) break;
+            const int nvis = sg->nvis, n1 = sg->n1, vlo = sg->vlo, hk = sg->hk;
+            const int* const table = a.b.table + sg->s * a.b.table_stride;
+            give_back(n);
+            auto page_of = [&](int st, int& r) {  // page and row of this lane's position of unit st, -1 if it has none
                 const int v = st * UNIT + own;
+                if (v >= nvis || st >= hi) return -1;
+                const int j = v < n1 ? v : v - n1 + vlo, p = a.by_page(j);
+                r = j - p * a.c.page_size;
+                return __ldg(table + p);
+            };
+            int r = 0, pg = page_of(lo, r);
+            for (int st = lo; st < hi && ok; ++st) {
                 uint32_t off = 0xffffffffu;
-                float ksc = 0.f, vsc = 0.f;
-                if (v < tl.nvis) {
-                    const int j = v < tl.n1 ? v : v - tl.n1 + tl.lo;
-                    const int p = a.by_page(j), r = j - p * a.c.page_size;
-                    const int pg = __ldg(a.b.table + it.s * a.b.table_stride + p);
-                    if ((unsigned)pg >= (unsigned)a.c.n_pages) {
-                        atomicOr(a.b.err, kErrKvRange);
-                    } else {
-                        off = (uint32_t)pg * a.c.page + (uint32_t)r * a.c.row + (uint32_t)it.hk * a.c.head;
-                        if constexpr (I8) {
-                            const long long so = pg * a.c.spage + (long long)it.hk * a.c.page_size + r;
-                            ksc = __ldg(a.c.ks + so);
-                            vsc = __ldg(a.c.vs + so);
-                        }
+                float sc[2] = {0.f, 0.f};
+                if ((unsigned)pg < (unsigned)a.c.n_pages) {
+                    off = (uint32_t)pg * a.c.page + (uint32_t)r * a.c.row + (uint32_t)hk * a.c.head;
+                    if constexpr (I8) {
+                        const long long so = pg * a.c.spage + (long long)hk * a.c.page_size + r;
+                        sc[0] = __ldg(a.c.ks + so);
+                        sc[1] = __ldg(a.c.vs + so);
                     }
+                } else if (pg != -1) {
+                    atomicOr(a.b.err, kErrKvRange);
                 }
-                if constexpr (!I8) {
+                pg = page_of(st + 1, r);
 #pragma unroll 1
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const int t = t_issue++, buf = t % NB;
-                        if (t >= NB && !many_wait(b_empty + 8 * buf, ((t / NB) - 1) & 1, ok)) break;
-                        const uint32_t dst = sb + F::oKV + buf * TILE;
-                        const uint8_t* src = kv ? a.c.v : a.c.k;
-#pragma unroll
-                        for (int i = 0; i < IT; ++i) {
-                            const uint32_t o = __shfl_sync(0xffffffffu, off, i * RPW + ln / CPR);
-                            const int r = i * 4 * RPW + sub;
-                            const bool have = o != 0xffffffffu;
-                            const unsigned long long at = have ? (unsigned long long)o * 64 + ch * 16 : 0;
-                            const uint32_t d = dst + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src + at),
-                                         "r"(have ? 16 : 0)
-                                         : "memory");
-                        }
-                        cp_async_commit();
-                        if (t_issue - t_done > 2) {
-                            cp_async_wait(2);
-                            publish(t_done++);
-                        }
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int t = t_issue++;
+                    if constexpr (!I8) {
+                        if (t >= NB && !many_wait(b_empty + 8 * (t % NB), ((t / NB) - 1) & 1, ok)) break;
+                    } else {
+                        // the slot's last readers, of four units before, were done before the tile that was handed
+                        // on last could be (its buffer held the keys of three units before)
+                        reinterpret_cast<float*>(smem + F::oSC + ((t >> 1) & 3) * 1024 + kv * 512)[own] = kv ? sc[1] : sc[0];
                     }
-                } else {
-                    // scales of the unit: its ring slot's last readers are done once the tiles' buffers are free
-                    uint8_t* const sc = smem + F::oSC + (unit % 3) * 1024;
-                    (void)stg;
-#pragma unroll 1
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const int t = t_issue++, buf = t % NB;
-                        if (t >= NB && !many_wait(b_empty + 8 * buf, ((t / NB) - 1) & 1, ok)) break;
-                        reinterpret_cast<float*>(sc + kv * 512)[own] = kv ? vsc : ksc;
-                        uint8_t* const dst = smem + F::oKV + buf * TILE;
-                        const uint8_t* src = kv ? a.c.v : a.c.k;
-                        uint4 x[IT];
+                    const uint32_t dst = I8 ? sb + F::oSTG + (t % max(F::NSTG, 1)) * F::STG : sb + F::oKV + (t % NB) * TILE;
+                    const uint8_t* src = kv ? a.c.v : a.c.k;
 #pragma unroll
-                        for (int i = 0; i < IT; ++i) {
-                            const uint32_t o = __shfl_sync(0xffffffffu, off, i * RPW + ln / CPR);
-                            x[i] = make_uint4(0, 0, 0, 0);
-                            if (o != 0xffffffffu)
-                                x[i] = ldg_stream128(src + (unsigned long long)o * 64 + ch * 16);
-                        }
-#pragma unroll
-                        for (int i = 0; i < IT; ++i) {
-                            const int r = i * 4 * RPW + sub;
-                            const uint32_t y[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u,
-                                                   x[i].w ^ 0x80808080u};
-                            uint32_t h[8];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                h[2 * k] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4140u), 0x64806480u);
-                                h[2 * k + 1] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4342u), 0x64806480u);
-                            }
-                            // chunk ch holds d = 16 ch ..: two 16-byte places of the tile's row
-                            uint8_t* const row = dst + (ch >> 2) * HALF + r * 128;
-                            const int p = 2 * (ch & 3);
-                            *reinterpret_cast<uint4*>(row + ((p ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                            *reinterpret_cast<uint4*>(row + (((p + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-                        }
-                        publish(t);
+                    for (int i = 0; i < IT; ++i) {
+                        const uint32_t o = __shfl_sync(0xffffffffu, off, i * RPW + ln / CPR);
+                        const int rr = i * 4 * RPW + sub;
+                        const bool have = o != 0xffffffffu;
+                        const unsigned long long at = have ? (unsigned long long)o * 64 + ch * 16 : 0;
+                        const uint32_t d = I8 ? dst + rr * D + ch * 16
+                                              : dst + (ch >> 3) * HALF + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+                        cp16_or_zero(d, src + at, have);
+                    }
+                    cp_async_commit();
+                    if (t_issue - t_done > AHEAD) {
+                        cp_async_wait(AHEAD);
+                        hand_on();
                     }
                 }
             }
-            if (!ok || it.u_item + tl.span >= b1) break;
-            it.next(a, ROWS, UNIT);
         }
-        if constexpr (!I8) {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            while (t_done < t_issue && ok) publish(t_done++);
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        while (t_done < t_issue && ok) hand_on();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsLow));
-        if (warp == 12 && ln == 0) {
+        if (warp == 12) {
             // ============================================================ the products
             constexpr uint32_t fmt = BF ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t idS = (1u << 4) | fmt | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             constexpr uint32_t idO = (1u << 4) | fmt | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
             uint32_t ph_p[2] = {0, 0}, ph_q[2] = {0, 0};
             int t = 0;  // key and value tiles so far
-            for (;;) {
-                const AttnTile& tl = it.t;
-                const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, tl.units);
-                if (lo < hi) {
-                    const int halves = tl.nr > 128 ? 2 : 1, n = hi - lo;
-                    auto scores = [&](int h, int kt) {  // S_h = Q_h K^T
-                        const uint32_t q = sb + h * TILE, k = sb + F::oKV + (kt % NB) * TILE;
+            for (int n = 0;; ++n) {
+                const ManySeg* const sg = segment(n);
+                const int nu = sg->hi - sg->lo, halves = sg->nr > 128 ? 2 : 1;
+                if (!ok || nu == 0) break;
+                give_back(n);
+                auto scores = [&](int h, int kt, bool last) {  // S_h = Q_h K^T
+                    const uint32_t q = sb + h * TILE, k = sb + F::oKV + (kt % NB) * TILE;
 #pragma unroll
-                        for (int i = 0; i < D / 16; ++i)
-                            tc_mma(tmem + h * 128, tc_desc(q + (i >> 2) * HALF + (i & 3) * 32),
-                                   tc_desc(k + (i >> 2) * HALF + (i & 3) * 32), idS, i ? 1u : 0u);
-                    };
-                    for (int h = 0; h < halves; ++h) {
-                        many_wait(b_q + 8 * h, ph_q[h], ok);
-                        ph_q[h] ^= 1;
-                    }
-                    many_wait(b_full + 8 * (t % NB), (t / NB) & 1, ok);
-                    if (!ok) break;
+                    for (int i = 0; i < D / 16; ++i)
+                        many_mma(tmem + h * 128, tc_desc(q + (i >> 2) * HALF + (i & 3) * 32),
+                               tc_desc(k + (i >> 2) * HALF + (i & 3) * 32), idS, i ? 1u : 0u);
+                    many_commit(b_s + 8 * h);
+                    if (last) many_commit(b_qf + 8 * h);
+                };
+                many_wait(b_full + 8 * (t % NB), (t / NB) & 1, ok);
+                for (int h = 0; h < halves; ++h) {
+                    if (!many_wait(b_q + 8 * h, ph_q[h], ok)) break;
+                    ph_q[h] ^= 1;
                     tc_fence_after();
+                    scores(h, t, nu == 1);
+                }
+                if (!ok) break;
+                many_commit(b_empty + 8 * (t % NB));
+                for (int u = 0; u < nu && ok; ++u, t += 2) {
+                    const int vt = t + 1, kn = t + 2;
+                    many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok);
+                    if (u + 1 < nu) many_wait(b_full + 8 * (kn % NB), (kn / NB) & 1, ok);
                     for (int h = 0; h < halves; ++h) {
-                        scores(h, t);
-                        tc_commit(b_s + 8 * h);
-                    }
-                    tc_commit(b_empty + 8 * (t % NB));
-                    for (int u = 0; u < n && ok; ++u, t += 2) {
-                        const int vt = t + 1, kn = t + 2;
-                        many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok);
-                        if (u + 1 < n) many_wait(b_full + 8 * (kn % NB), (kn / NB) & 1, ok);
-                        for (int h = 0; h < halves; ++h) {
-                            if (!many_wait(b_p + 8 * h, ph_p[h], ok)) break;
-                            ph_p[h] ^= 1;
-                            tc_fence_after();
-                            const uint32_t v = sb + F::oKV + (vt % NB) * TILE;
-                            if (I8 || !*(volatile int*)&misc[2 + h])
+                        if (!many_wait(b_p + 8 * h, ph_p[h], ok)) break;
+                        ph_p[h] ^= 1;
+                        tc_fence_after();
+                        const uint32_t v = sb + F::oKV + (vt % NB) * TILE;
+                        if (I8 || !*(volatile int*)&misc[2 + h]) {
 #pragma unroll
                             for (int i = 0; i < UNIT / 16; ++i)  // O_h += P_h V
-                                tc_mma_ta(tmem + 256 + h * 128, tmem + h * 128 + 8 * i, many_v_desc(v + i * 2048, HALF), idO,
+                                many_mma_ta(tmem + 256 + h * 128, tmem + h * 128 + 8 * i, many_v_desc(v + i * 2048, HALF), idO,
                                           u || i ? 1u : 0u);
-                            if (u + 1 < n) scores(h, kn);
-                            tc_commit(b_s + 8 * h);  // the next S, or the last O
                         }
-                        tc_commit(b_empty + 8 * (vt % NB));
-                        if (u + 1 < n) tc_commit(b_empty + 8 * (kn % NB));
+                        if (u + 1 < nu) scores(h, kn, u + 2 == nu);
+                        else many_commit(b_o + 8 * h);
                     }
+                    many_commit(b_empty + 8 * (vt % NB));
+                    if (u + 1 < nu) many_commit(b_empty + 8 * (kn % NB));
                 }
-                if (!ok || it.u_item + tl.span >= b1) break;
+            }
+        } else if (warp == 13) {
+            // ============================================================ the segments
+            const int b0 = share.begin(c), b1 = share.begin(c + 1);
+            AttnIter it;
+            it.seek(a, pre_s, b0, ROWS, UNIT);
+            int n = 0;
+            for (;;) {
+                const int lo = max(b0 - it.u_item, 0), hi = min(b1 - it.u_item, it.t.units);
+                if (lo < hi) {
+                    if (n >= 4 && !many_wait(b_sege + 8 * (n & 3), ((n >> 2) - 1) & 1, ok)) break;
+                    if (ln == 0) {
+                        const bool whole = lo == 0 && hi == it.t.units;
+                        segs[n & 3] = {lo, hi, it.t.nr, it.t.r0, it.q.q0, it.q.q1, it.q.len, it.s, it.hk, it.t.lo, it.t.n1,
+                                       it.t.nvis, whole, lo == 0, {0, 0}};
+                        if (!whole) shared_s[lo == 0] = {1, it.q.q0, it.hk, it.t.r0, it.t.nr, it.u_item, it.t.units};
+                        mbar_arrive(b_seg + 8 * (n & 3));
+                    }
+                    ++n;
+                }
+                if (it.u_item + it.t.span >= b1) break;
                 it.next(a, ROWS, UNIT);
+            }
+            if (n < 4 || many_wait(b_sege + 8 * (n & 3), ((n >> 2) - 1) & 1, ok))
+                if (ln == 0) {
+                    segs[n & 3].lo = segs[n & 3].hi = 0;
+                    mbar_arrive(b_seg + 8 * (n & 3));
+                }
+        } else if (warp > 13) {
+            // ============================================================ queries in, and the rows' factors
+            constexpr int CH = D / 8, RP = 32 / CH;  // 16-byte chunks of a row; rows a warp takes at a time
+            constexpr bool CONV = !__is_same(T, __half) && !BF;  // bf16 rows into f16
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // the scale's sign goes into the queries
+            uint32_t ph_qf[2] = {1, 1};  // a half's first queries find it free
+            for (int n = 0;; ++n) {
+                const ManySeg* const sg = segment(n);
+                const int lo = sg->lo, hi = sg->hi, nr = sg->nr, r0 = sg->r0, q0 = sg->q0, hk = sg->hk;
+                if (!ok || lo == hi) break;
+                give_back(n);
+                // the rows come to L2 while the half's place is still in use
+                for (int r = (warp - 14) * 32 + ln; r < nr; r += 64) {
+                    const int tr = a.by_group(r0 + r);
+                    const T* const q = (const T*)a.q + (long long)(q0 + tr) * a.ldq + (hk * a.group + r0 + r - tr * a.group) * D;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+                    if constexpr (D == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64));
+                }
+                for (int h = 0; h < 2 && h * 128 < nr; ++h) {
+                    if (!many_wait(b_qf + 8 * h, ph_qf[h], ok)) break;
+                    ph_qf[h] ^= 1;
+                    const uint32_t qs = sb + h * TILE;
+                    const int ch = ln % CH;
+                    auto row_of = [&](int i) { return (warp - 14) * 64 + i * RP + ln / CH; };
+                    auto source = [&](int r) {
+                        const int row = r0 + h * 128 + r, tr = a.by_group(row);
+                        return (const T*)a.q + (long long)(q0 + tr) * a.ldq + (hk * a.group + row - tr * a.group) * D + 8 * ch;
+                    };
+                    auto place = [&](int r) { return qs + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+                    const float rs0 = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-30f);  // not 0: 0 * -inf
+                    if (!CONV && !flip) {
+#pragma unroll 4
+                        for (int i = 0; i < 64 / RP; ++i) {
+                            const int r = row_of(i);
+                            cp16_or_zero(place(r), h * 128 + r < nr ? source(r) : a.q, h * 128 + r < nr);
+                            if (ch == 0) rsc[(n & 1) * 256 + h * 128 + r] = rs0;
+                        }
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                    } else {
+#pragma unroll 1
+                        for (int i0 = 0; i0 < 64 / RP; i0 += 8) {  // 8 loads on their way
+                            uint4 x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int r = row_of(i0 + i);
+                                x[i] = make_uint4(0, 0, 0, 0);
+                                if (h * 128 + r < nr) x[i] = __ldg(reinterpret_cast<const uint4*>(source(r)));
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int r = row_of(i0 + i);
+                                float rs = rs0;
+                                uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                                if constexpr (CONV) {
+                                    uint32_t m = 0;
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) m = max(m, max(y[k] & 0x7fffu, (y[k] >> 16) & 0x7fffu));
+#pragma unroll
+                                    for (int o = CH / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                                    const uint32_t e = m >> 7;
+                                    const bool norm = e >= 2 && e <= 252;
+                                    const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
+                                    if (norm) rs = fmaxf(rs * __uint_as_float(e << 23), 1e-30f);
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k)
+                                        y[k] = pack_h2(__uint_as_float(y[k] << 16) * down,
+                                                       __uint_as_float(y[k] & 0xffff0000u) * down);
+                                }
+                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(place(r)), "r"(y[0] ^ flip),
+                                             "r"(y[1] ^ flip), "r"(y[2] ^ flip), "r"(y[3] ^ flip)
+                                             : "memory");
+                                if (ch == 0) rsc[(n & 1) * 256 + h * 128 + r] = rs;
+                            }
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (ln == 0) mbar_arrive(b_q + 8 * h);
+                }
             }
         }
     }

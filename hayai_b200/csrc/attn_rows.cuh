@@ -173,6 +173,11 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Copy 16 bytes (or with ok false: 16 zero bytes) to shared memory.
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
 // N (4 or 2) adjacent values of the weighted sum of row `row` of an item's kv head, over l.
 template <class T, int N>
 __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[N],
