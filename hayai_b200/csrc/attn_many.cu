@@ -228,18 +228,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sb = smem_addr(smem), bars = sb + F::oBAR;
     // barriers: key and value tiles full and empty; S ready, P ready, O ready, queries in, queries free
-    // (of each half); segments full and empty
+    // (of each half); segments full and empty; a unit checked (of each half)
     const uint32_t b_full = bars, b_empty = bars + 8 * NB, b_s = bars + 16 * NB, b_p = b_s + 16, b_o = b_s + 32,
-                   b_q = b_s + 48, b_qf = b_s + 64, b_seg = b_s + 80, b_sege = b_seg + 32;
+                   b_q = b_s + 48, b_qf = b_s + 64, b_seg = b_s + 80, b_sege = b_seg + 32, b_chk = b_sege + 32;
     float* const rsc = reinterpret_cast<float*>(smem + F::oRS);
     ManySeg* const segs = reinterpret_cast<ManySeg*>(smem + F::oSEG);
-    int* const misc = reinterpret_cast<int*>(smem + F::oMISC);  // TMEM base, last, [2..3] a product done by hand; [8..] scratch
+    int* const misc = reinterpret_cast<int*>(smem + F::oMISC);  // TMEM base, last, [2..3] a product done by hand, [4..9] checks; [16..] scratch
     AttnShared* const shared_s = reinterpret_cast<AttnShared*>(misc + 64);  // the block's first and last tile, where shared
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
 
     // the schedule's prefix sums lie in the last key and value tile until warp 13 has its place
     int* const pre_s = reinterpret_cast<int*>(smem + F::oKV + (NB - 1) * TILE);
-    const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 8);
+    const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 16);
     const int G = min((int)gridDim.x, U);
     if (U <= 0 || c >= G) return;
     const AttnShares share(U, G);
@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             mbar_init(b_o + 8 * i, 1);
             mbar_init(b_q + 8 * i, 2);
             mbar_init(b_qf + 8 * i, 1);
-            shared_s[i].valid = 0;
+            mbar_init(b_chk + 8 * i, 4);
+            misc[4 + 3 * i] = misc[5 + 3 * i] = misc[6 + 3 * i] = 0;
+            shared_s[i] = {0, 0, 0, 0, 0, 0, 1};
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(b_seg + 8 * i, 1);
@@ -288,7 +290,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
         const int half = warp >> 2, rt = threadIdx.x & 127;  // half of the tile, row of the half
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + lanes + half * 128, tO = tmem + lanes + 256 + half * 128;
-        uint32_t ph_s = 0, ph_o = 0, ph_q = 0;
+        uint32_t ph_s = 0, ph_o = 0;
+        int checks = 0;  // units checked for values that are not finite
         int unit = 0;   // units of the block so far, for the scales' ring
         for (int n = 0;; ++n) {
             const ManySeg* const sg = segment(n);
@@ -309,15 +312,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                               lastr = many_row(a, q, tl, sg->r0 + min(half * 128 + 127, nr - 1), true);
                 const int cmin = min(first.c, lastr.c), bmax = lastr.b, amin = first.a;
 
-                if (!many_wait(b_q + 8 * half, ph_q, ok)) break;
-                ph_q ^= 1;
-                const float rs = rsc[(n & 1) * 256 + r];
+                float rs = 0.f;
                 float m = -INFINITY;
                 float2 l2 = make_float2(0.f, 0.f);
                 for (int st = lo; st < hi; ++st) {
                     if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
                     ph_s ^= 1;
                     tc_fence_after();
+                    // the queries and their factors came before this unit's products; their own barrier may be two
+                    // segments further by now, so it cannot be waited for here
+                    if (st == lo) rs = rsc[(n & 1) * 256 + r];
                     float ev = 0.f;
                     const float4 *ksc = nullptr, *vsc = nullptr;
                     if constexpr (I8) {
@@ -433,11 +437,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) odd |= (y[k] & E) == E || ((y[k] >> 16) & E) == E;
                             }
-                            asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %0, 0;\nbarrier.cta.red.or.pred q, %1, 128, p;\n"
-                                         "selp.u32 %0, 1, 0, q;\n}"
-                                         : "+r"(odd)
-                                         : "r"(2 + half)
-                                         : "memory");
+                            // the half's four warps decide together: three flags in turn, each cleared a check ahead
+                            int* const flag = misc + 4 + 3 * half;
+                            if (__any_sync(0xffffffffu, odd != 0) && ln == 0) flag[checks % 3] = 1;
+                            if (rt == 0) flag[(checks + 1) % 3] = 0;
+                            __syncwarp();
+                            if (ln == 0) mbar_arrive(b_chk + 8 * half);
+                            if (!many_wait(b_chk + 8 * half, checks & 1, ok)) break;
+                            odd = *(volatile int*)&flag[checks % 3];
+                            ++checks;
                             if (rt == 0) misc[2 + half] = (int)odd;  // read by the products' thread after the arrivals
                             if (odd) many_product<BF, D>(tO, tS, vtile, st == lo);
                         } else if (rt == 0) {
@@ -490,15 +498,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             if (!ok) break;
             give_back(n);
         }
-        // ---- tiles that several blocks share: the last of them joins
+        // ---- tiles that several blocks share: the last of them joins.  One thread decides for all, so that they
+        // meet at the same barriers even where a wait has run out.
         __threadfence();
         named_bar_sync(1, 256);
         for (int x = 0; x < 2; ++x) {
             const AttnShared sh = shared_s[x];
-            if (!sh.valid) continue;
             const int bf = share.owner(sh.u_item), bl = share.owner(sh.u_item + sh.units - 1);
             if (threadIdx.x == 0) {
-                misc[1] = atomicAdd(a.count + bf, 1) == bl - bf;
+                misc[1] = ok && sh.valid && atomicAdd(a.count + bf, 1) == bl - bf;
                 if (misc[1]) a.count[bf] = 0;
                 __threadfence();
             }

@@ -334,6 +334,8 @@ static int flag_error(hc_engine* e, int flag) {
         if (flag & 1)
             return hc_set_error(HC_ERR_RANGE,
                                 "an activation magnitude reached 65504 (outside the f16 range of the tensor-core split)");
+        // a block that gave up may have left its tiles' counters behind
+        if ((flag & 2) && e->attn_cnt.p) HC_CUDA(cudaMemset(e->attn_cnt.p, 0, e->attn_cnt.cap));
         if (flag & 2) return hc_set_error(HC_ERR_TIMEOUT, "a bounded device wait expired");
         if (flag & 4)
             return hc_set_error(HC_ERR_INVALID, "kv batch: a page number, length or offset on the device is out of range");
