@@ -767,7 +767,8 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     static_assert(most <= 227 * 1024 - 1024, "shared memory of a block");
     static_assert(most >= 4 * HC_KV_SEQS, "the schedule's prefix lies in the rings");
     static_assert((size_t)F::PS * 4 * 2 * (F::W + 1) <= kFewPartBytes, "the workspace of a block");
-    const cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    static SmemOptIn opted;
+    const cudaError_t e = opted(reinterpret_cast<const void*>(attn_few_kernel<T, C, D, NT>), most);
     if (e != cudaSuccess) return e;
     attn_few_kernel<T, C, D, NT><<<blocks, 32 * F::W, most, s>>>(a);
     return cudaGetLastError();

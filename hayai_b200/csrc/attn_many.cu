@@ -810,7 +810,8 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     constexpr int bytes = ManyCfg<C, D>::BYTES;
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
     static_assert(sizeof(float) * 2 * kManyRows * (D + 2) <= kManyPartBytes, "the workspace of a block");
-    const cudaError_t e = cudaFuncSetAttribute(attn_many_kernel<T, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static SmemOptIn opted;
+    const cudaError_t e = opted(reinterpret_cast<const void*>(attn_many_kernel<T, C, D>), bytes);
     if (e != cudaSuccess) return e;
     AttnArgs b = a;
     b.over = 2;  // a tile's start and end cost about what two of its units do

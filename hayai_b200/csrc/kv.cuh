@@ -44,34 +44,56 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatchDev& b, int cap, int s) {
     return r;
 }
 
-// The sequence whose new tokens include t, or -1: the largest s with q_start[s] <= t (of empty
-// sequences at the same offset the last, which is the one that is not empty), found by GL lanes
-// together, GL candidates per step.  All lanes of the group call it with the same t.
+// The sequence whose new tokens include t (or -1), with q_start of the next and its length, found by
+// GL lanes together.  A step of single tokens has s = t, so that place is looked at first, while the
+// first of the search's steps is on its way: the largest s with q_start[s] <= t (of empty sequences
+// at the same offset the last, which is the one that is not empty), GL candidates per step.  All
+// lanes of the group call it with the same t.
+struct KvPlace {
+    int s, next, len;
+};
 template <int GL>
-__device__ __forceinline__ int kv_find_seq(const KvBatchDev& b, int t) {
+__device__ __forceinline__ KvPlace kv_find_seq(const KvBatchDev& b, int t) {
     const int l = lane_id() & (GL - 1), g0 = lane_id() & ~(GL - 1);
     const uint32_t mask = GL == 32 ? 0xffffffffu : ((1u << GL) - 1u) << g0;
-    int lo = 0, n = b.n_seq;
-    bool any = __ldg(b.q_start) <= t;
-    while (n > 1) {
-        const int step = (n + GL - 1) / GL;
-        const bool le = l * step < n && __ldg(b.q_start + lo + l * step) <= t;
+    KvPlace p;
+    p.s = min(t, b.n_seq - 1);
+    const int at = __ldg(b.q_start + p.s);
+    p.next = __ldg(b.q_start + p.s + 1);
+    p.len = __ldg(b.kv_len + p.s);
+    int lo = 0, n = b.n_seq, step = (n + GL - 1) / GL;
+    bool le = l * step < n && __ldg(b.q_start + l * step) <= t;
+    if (at <= t && t < p.next) return p;
+    for (;;) {
         const int c = __popc(__ballot_sync(mask, le) & mask);
         if (c == 0) break;
         lo += (c - 1) * step;
         n = min(step, n - (c - 1) * step);
+        if (n <= 1) break;
+        step = (n + GL - 1) / GL;
+        le = l * step < n && __ldg(b.q_start + lo + l * step) <= t;
     }
-    return any && t < __ldg(b.q_start + lo + 1) ? lo : -1;
+    const int first = __ldg(b.q_start + lo);
+    p.next = __ldg(b.q_start + lo + 1);
+    p.len = __ldg(b.kv_len + lo);
+    p.s = first <= t && t < p.next ? lo : -1;
+    return p;
 }
 
 // ---------------------------------------------------------------- 8 elements of a row
+// (raw as loaded, so that many rows wait in few registers; as values)
 template <class T>
 struct Elem;
 template <>
 struct Elem<float> {
-    static __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    struct Raw {
+        float4 a, b;
+    };
+    static __device__ __forceinline__ Raw load8(const float* p) {
+        return {__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)};
+    }
+    static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
+        x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w, x[4] = r.b.x, x[5] = r.b.y, x[6] = r.b.z, x[7] = r.b.w;
     }
     static __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
         reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -80,9 +102,10 @@ struct Elem<float> {
 };
 template <>
 struct Elem<__half> {
-    static __device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    using Raw = uint4;
+    static __device__ __forceinline__ Raw load8(const __half* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+    static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = __half22float2(u32_as_h2(w[i]));
@@ -100,9 +123,10 @@ __device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
 }
 template <>
 struct Elem<__nv_bfloat16> {
-    static __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    using Raw = uint4;
+    static __device__ __forceinline__ Raw load8(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+    static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[2 * i] = __uint_as_float(w[i] << 16);
@@ -116,10 +140,11 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<int8_t> {  // codes as they are
-    static __device__ __forceinline__ void load8(const int8_t* p, float (&x)[8]) {
-        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
+    using Raw = uint2;
+    static __device__ __forceinline__ Raw load8(const int8_t* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
+    static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s8_to_f32_flipped((i < 4 ? a.x : a.y) ^ 0x80808080u, i & 3);
+        for (int i = 0; i < 8; ++i) x[i] = s8_to_f32_flipped((i < 4 ? r.x : r.y) ^ 0x80808080u, i & 3);
     }
 };
 

@@ -14,13 +14,13 @@ namespace hc {
 // Where the batch's token t lives: its page's and row's offset in the cache (64-byte units, of
 // head 0) and in the scales, or false where it has no place.
 template <int GL>
-__device__ __forceinline__ bool kv_slot(const KvDev& c, const KvBatchDev& b, int t, uint32_t& at, long long& sat) {
-    const int s = kv_find_seq<GL>(b, t);
-    if (s < 0) return false;
-    const int len = __ldg(b.kv_len + s), pos = len - __ldg(b.q_start + s + 1) + t;
-    if (pos < 0) return false;
-    const int p = pos / c.page_size, r = pos - p * c.page_size;
-    const int page = p < b.max_pages ? __ldg(b.table + s * b.table_stride + p) : -1;
+__device__ __forceinline__ bool kv_slot(const KvDev& c, const KvBatchDev& b, const FastDiv& by_page, int t, uint32_t& at,
+                                        long long& sat) {
+    const KvPlace k = kv_find_seq<GL>(b, t);
+    const int pos = k.len - k.next + t;
+    if (k.s < 0 || pos < 0) return false;
+    const int p = by_page(pos), r = pos - p * c.page_size;
+    const int page = p < b.max_pages ? __ldg(b.table + k.s * b.table_stride + p) : -1;
     if ((unsigned)page >= (unsigned)c.n_pages) {
         atomicOr(b.err, kErrKvRange);
         return false;
@@ -35,10 +35,37 @@ __device__ __forceinline__ C* kv_elem(uint8_t* base, uint32_t units) {
     return reinterpret_cast<C*>(base + (unsigned long long)units * 64);
 }
 
+// Codes of 8 values of a row with largest |x| m and scale s, four to a word.  The code is the nearest
+// whole number to fl(x / s); x * (1 / s) is within 127 * 2^-21 of the quotient, so that its nearest
+// whole number is the same unless it lies that near to a half: only then are the values divided
+// (three instructions a value instead of about twelve).  1.5 * 2^23 added leaves the whole number in
+// the low bits, in two's complement.
+__device__ __forceinline__ void kv_codes(const float (&x)[8], float m, float s, uint32_t (&q)[2]) {
+    constexpr float kMagic = 12582912.f;
+    const float inv = __fdividef(1.f, s);
+    float f[8];
+    bool near = m < 1e-30f || !(s > 0.f);  // a scale that is not a normal number, 0 or NaN
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float y = x[i] * inv;
+        f[i] = y + kMagic;
+        near |= fabsf(y - (f[i] - kMagic)) > 0.4999f;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            f[i] = (s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f) : 0.f) + kMagic;
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+        q[w] = prmt(prmt(__float_as_uint(f[4 * w]), __float_as_uint(f[4 * w + 1]), 0x0040u),
+                    prmt(__float_as_uint(f[4 * w + 2]), __float_as_uint(f[4 * w + 3]), 0x0040u), 0x5410u);
+}
+
 // One group of D / 8 lanes per (token, U heads): each lane holds 8 values of each row, k and v.
 // Bound by memory: every value is read once and written once.
 template <class T, class C, int D, int U>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, KvRows r) {
+__global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, KvRows r, FastDiv by_page) {
     constexpr int GL = D / 8;
     const int chunks = (c.n_heads + U - 1) / U;
     const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL;
@@ -46,54 +73,45 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, K
     const int t = (int)min(g / chunks, (long long)b.n_tok - 1), h0 = (int)(g % chunks) * U;
     const bool real = g < (long long)b.n_tok * chunks;
     const T* src[2] = {(const T*)r.k + t * r.ldk + l * 8, (const T*)r.v + t * r.ldv + l * 8};
-    float x[2][U][8];
+    typename Elem<T>::Raw raw[2][U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) Elem<T>::load8(src[w] + min(h0 + u, c.n_heads - 1) * D, x[w][u]);
+        for (int w = 0; w < 2; ++w) raw[w][u] = Elem<T>::load8(src[w] + min(h0 + u, c.n_heads - 1) * D);
     uint32_t at = 0;
     long long sat = 0;
-    const bool has = kv_slot<GL>(c, b, t, at, sat) && real;
+    const bool has = kv_slot<GL>(c, b, by_page, t, at, sat) && real;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int h = h0 + u;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
+            float x[8];
+            Elem<T>::values(raw[w][u], x);
             C* dst = kv_elem<C>(w ? c.v : c.k, at + (uint32_t)h * c.head) + l * 8;
             if constexpr (sizeof(C) == 1) {
-                float m = 0.f;
-                bool fin = true;
+                uint32_t top = 0;  // the bits of |x| order as the values do, infinity and NaN above all
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    m = fmaxf(m, fabsf(x[w][u][i]));
-                    fin = fin && fabsf(x[w][u][i]) <= 3.402823466e38f;
-                }
+                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-                for (int o = GL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const uint32_t all = __ballot_sync(0xffffffffu, fin), mine = (GL == 8 ? 0xffu : 0xffffu) << (lane_id() & ~(GL - 1));
-                fin = (all & mine) == mine;
-                const float scale = fin ? m * (1.f / 127.f) : __int_as_float(0x7fffffff);
-                uint32_t q[2] = {0, 0};
-                if (scale > 0.f) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float v = fminf(fmaxf(rintf(__fdiv_rn(x[w][u][i], scale)), -127.f), 127.f);
-                        q[i >> 2] |= ((uint32_t)(int)v & 255u) << (8 * (i & 3));
-                    }
-                }
+                for (int o = GL / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float m = __uint_as_float(top);
+                const float scale = top < 0x7f800000u ? m * (1.f / 127.f) : __int_as_float(0x7fffffff);
+                uint32_t q[2];
+                kv_codes(x, m, scale, q);
                 if (has && h < c.n_heads) {
                     *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
                     if (l == 0) (w ? c.vs : c.ks)[sat + (long long)h * c.page_size] = scale;
                 }
             } else {
-                if (has && h < c.n_heads) Elem<C>::store8(dst, x[w][u]);
+                if (has && h < c.n_heads) Elem<C>::store8(dst, x);
             }
         }
     }
 }
 
 template <class T, class C, int D, int U>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvRows r) {
+__global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvRows r, FastDiv by_page) {
     constexpr int GL = D / 8;
     const int chunks = (c.n_heads + U - 1) / U;
     const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL;
@@ -101,14 +119,15 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvR
     const int t = (int)min(g / chunks, (long long)b.n_tok - 1), h0 = (int)(g % chunks) * U;
     uint32_t at = 0;
     long long sat = 0;
-    if (!kv_slot<GL>(c, b, t, at, sat) || g >= (long long)b.n_tok * chunks) return;
-    float x[2][U][8], sc[2][U];
+    if (!kv_slot<GL>(c, b, by_page, t, at, sat) || g >= (long long)b.n_tok * chunks) return;
+    typename Elem<C>::Raw raw[2][U];
+    float sc[2][U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const int h = min(h0 + u, c.n_heads - 1);
-            Elem<C>::load8(kv_elem<C>(w ? c.v : c.k, at + (uint32_t)h * c.head) + l * 8, x[w][u]);
+            raw[w][u] = Elem<C>::load8(kv_elem<C>(w ? c.v : c.k, at + (uint32_t)h * c.head) + l * 8);
             if constexpr (sizeof(C) == 1) sc[w][u] = __ldg((w ? c.vs : c.ks) + sat + (long long)h * c.page_size);
         }
 #pragma unroll
@@ -116,25 +135,35 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvR
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             if (h0 + u >= c.n_heads) continue;
+            float x[8];
+            Elem<C>::values(raw[w][u], x);
             if constexpr (sizeof(C) == 1)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[w][u][i] *= sc[w][u];
-            Elem<T>::store8((T*)(w ? r.v : r.k) + t * (w ? r.ldv : r.ldk) + (h0 + u) * D + l * 8, x[w][u]);
+                for (int i = 0; i < 8; ++i) x[i] *= sc[w][u];
+            Elem<T>::store8((T*)(w ? r.v : r.k) + t * (w ? r.ldv : r.ldk) + (h0 + u) * D + l * 8, x);
         }
 }
 
 namespace {
 
-template <class T, class C, int D>
-cudaError_t launch(bool write, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
-    constexpr int U = 2;
+template <class T, class C, int D, int U>
+cudaError_t start(bool write, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
     const long long groups = (long long)b.n_tok * ((c.n_heads + U - 1) / U);
     const unsigned grid = (unsigned)((groups * (D / 8) + 255) / 256);
+    const FastDiv by_page((uint32_t)c.page_size);
     if (write)
-        kv_append_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r);
+        kv_append_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r, by_page);
     else
-        kv_read_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r);
+        kv_read_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r, by_page);
     return cudaGetLastError();
+}
+
+// A thread's rows: one where all rows fit the GPU's threads at once (the call's time is its chain of
+// loads), two (f32) or four where they do not (the chain is paid once for more bytes on their way).
+template <class T, class C, int D>
+cudaError_t launch(bool write, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
+    if ((long long)b.n_tok * c.n_heads * (D / 8) <= 148 * 2048) return start<T, C, D, 1>(write, c, b, r, s);
+    return start<T, C, D, sizeof(T) == 4 ? 2 : 4>(write, c, b, r, s);
 }
 
 template <class T, int D>

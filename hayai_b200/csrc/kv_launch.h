@@ -1,6 +1,8 @@
 // kv_launch.h -- launchers of the paged key/value cache's kernels.
 #pragma once
 
+#include <atomic>
+
 #include "kv.cuh"
 
 namespace hc {
@@ -30,6 +32,20 @@ struct FastDiv {
     }
     __device__ __forceinline__ int operator()(int n) const {
         return (int)(((unsigned long long)(uint32_t)n * m) >> (31 + k));
+    }
+};
+
+// A kernel's shared-memory opt-in, once per device (a call of it costs about a microsecond).
+struct SmemOptIn {
+    std::atomic<unsigned long long> done{0};
+    cudaError_t operator()(const void* kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (e != cudaSuccess || (done.load() & bit)) return e;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit);
+        return e;
     }
 };
 

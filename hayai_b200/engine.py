@@ -185,6 +185,9 @@ class CudaEngine:
         _check(lib().hc_engine_init(device, ctypes.byref(h)))
         self.handle = h
         self.device = device
+        # the calls of a decode step's every layer, looked up once
+        self._kv_append, self._kv_read, self._attn_paged = (lib().hc_kv_append_dev, lib().hc_kv_read_dev,
+                                                            lib().hc_attn_paged_dev)
 
     def close(self) -> None:
         if self.handle:
@@ -421,11 +424,15 @@ class CudaEngine:
     def kv_append_dev(self, cache, batch, k, v) -> None:
         """Store the new tokens' rows k, v [n_tok][n_heads][head_dim] in the cache's pages (KvCache,
         KvBatch); an 8-bit cache gets codes and one scale per row."""
-        _check(lib().hc_kv_append_dev(self.handle, cache.ref, batch.ref, *cache.pair(batch, k, v)))
+        rc = self._kv_append(self.handle, cache.ref, batch.ref, *cache.pair(batch, k, v))
+        if rc:
+            _check(rc)
 
     def kv_read_dev(self, cache, batch, k, v) -> None:
         """Gather the same rows back out of the cache into k, v, as the values they stand for."""
-        _check(lib().hc_kv_read_dev(self.handle, cache.ref, batch.ref, *cache.pair(batch, k, v)))
+        rc = self._kv_read(self.handle, cache.ref, batch.ref, *cache.pair(batch, k, v))
+        if rc:
+            _check(rc)
 
     def attn_paged_dev(self, cache, batch, q, out, scale: float | None = None, causal: bool = True, window: int = 0,
                        sink: int = 0, lse=None) -> None:
@@ -433,14 +440,16 @@ class CudaEngine:
         out (same shape and type).  scale: 1 / sqrt(head_dim) unless given.  causal: a token sees the
         positions up to its own, of which window > 0 leaves the last ``window`` and the first
         ``sink``.  lse: None, or a float32 [n_tok][n_heads] that receives the scores' log-sum-exp."""
-        t, ldq = cache.rows(batch, q, "q")
-        to, ldo = cache.rows(batch, out, "out")
-        heads = q.shape[1]
-        if to != t or out.shape[1] != heads:
-            raise ValueError("q and out need one type and number of heads")
-        _check(lib().hc_attn_paged_dev(self.handle, cache.ref, batch.ref, t, heads, q.data_ptr(), ldq, out.data_ptr(),
-                                       ldo, cache.lse_ptr(lse, q),
-                                       cache.default_scale if scale is None else scale, causal, window, sink))
+        heads = q.shape[1] if q.dim() == 3 else 0
+        t, ldq = cache.rows(batch, q, heads, "q")
+        to, ldo = cache.rows(batch, out, heads, "out")
+        if to != t:
+            raise ValueError("q and out need one type")
+        rc = self._attn_paged(self.handle, cache.ref, batch.ref, t, heads, q.data_ptr(), ldq, out.data_ptr(), ldo,
+                              None if lse is None else cache.lse_ptr(lse, q),
+                              cache.default_scale if scale is None else scale, causal, window, sink)
+        if rc:
+            _check(rc)
 
     def router_scores_dev(self, router_w, x, scores, n_tok: int) -> None:
         E, D = router_w.shape

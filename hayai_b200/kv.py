@@ -61,7 +61,7 @@ class KvCache:
         strides = [s if n > 1 else max(64, head_dim) for s, n in zip(k.stride(), k.shape)]
         _need(all(s >= 0 for s in strides), "negative strides")
         self._keep = (k, v, k_scale, v_scale)
-        self.device, self.n_heads, self.head_dim = k.device, n_heads, head_dim
+        self.index, self.n_heads, self.head_dim = k.get_device(), n_heads, head_dim
         self.default_scale = float(head_dim) ** -0.5 if head_dim else 0.0
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         self.struct = _Cache(_CACHE_TYPES[k.dtype], n_pages, n_heads, page_size, head_dim, ptr(k), ptr(v), ptr(k_scale),
@@ -69,29 +69,29 @@ class KvCache:
                              0 if k_scale is None else max(k_scale.stride(0), n_heads * page_size if n_pages == 1 else 0))
         self.ref = ctypes.addressof(self.struct)
 
-    def rows(self, batch, x, what: str):
+    def rows(self, batch, x, heads: int, what: str):
         """(type id, leading dimension) of packed rows x [n_tok][heads][head_dim]."""
         t = _ROW_TYPES.get(x.dtype)
-        if t is None or x.dim() != 3 or x.shape[0] != batch.n_tok or x.shape[2] != self.head_dim:
-            raise ValueError(f"{what} must be float32, float16 or bfloat16 [n_tok={batch.n_tok}][heads]"
-                             f"[head_dim={self.head_dim}]")
-        st = x.stride()
-        if x.device != self.device or (st[2] != 1) or (st[1] != self.head_dim and x.shape[1] > 1):
-            raise ValueError(f"{what} must be on the cache's device with contiguous rows (the token axis may be strided)")
-        return t, st[0] if x.shape[0] > 1 else x.shape[1] * self.head_dim
+        if t is None or x.shape != (batch.n_tok, heads, self.head_dim) or x.get_device() != self.index:
+            raise ValueError(f"{what} must be float32, float16 or bfloat16 [n_tok={batch.n_tok}][heads={heads}]"
+                             f"[head_dim={self.head_dim}] on the cache's device")
+        ld, head, one = x.stride()
+        if one != 1 or (head != self.head_dim and heads > 1):
+            raise ValueError(f"{what} must have contiguous rows (only the token axis may be strided)")
+        return t, ld if batch.n_tok > 1 else heads * self.head_dim
 
     def pair(self, batch, k, v):
         """Arguments (type, k, ldk, v, ldv) of the new tokens' key and value rows."""
-        t, ldk = self.rows(batch, k, "k")
-        tv, ldv = self.rows(batch, v, "v")
-        if tv != t or k.shape[1] != self.n_heads or v.shape[1] != self.n_heads:
-            raise ValueError(f"k and v need one type and the cache's {self.n_heads} heads")
+        t, ldk = self.rows(batch, k, self.n_heads, "k")
+        tv, ldv = self.rows(batch, v, self.n_heads, "v")
+        if tv != t:
+            raise ValueError("k and v need one type")
         return t, k.data_ptr(), ldk, v.data_ptr(), ldv
 
     def lse_ptr(self, lse, q):
         if lse is None:
             return None
-        if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.device != q.device:
+        if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.get_device() != self.index:
             raise ValueError("lse must be a contiguous float32 tensor [n_tok][n_heads] on q's device")
         return lse.data_ptr()
 
