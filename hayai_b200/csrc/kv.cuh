@@ -95,11 +95,22 @@ struct Elem<float> {
     static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
         x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w, x[4] = r.b.x, x[5] = r.b.y, x[6] = r.b.z, x[7] = r.b.w;
     }
+    // The largest |x| as f32 bits, whose order is that of the values, infinity and NaN above all.
+    static __device__ __forceinline__ uint32_t top(const Raw& r) {
+        auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
+        return max(max(max(bits(r.a.x), bits(r.a.y)), max(bits(r.a.z), bits(r.a.w))),
+                   max(max(bits(r.b.x), bits(r.b.y)), max(bits(r.b.z), bits(r.b.w))));
+    }
     static __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
         reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
         reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
 };
+// The larger of the 16-bit magnitudes of 8 packed values.
+__device__ __forceinline__ uint32_t top16(const uint4& r) {
+    const uint32_t m = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+}
 template <>
 struct Elem<__half> {
     using Raw = uint4;
@@ -112,6 +123,7 @@ struct Elem<__half> {
             x[2 * i] = f.x, x[2 * i + 1] = f.y;
         }
     }
+    static __device__ __forceinline__ uint32_t top(const Raw& r) { return __float_as_uint(h2f((uint16_t)top16(r))); }
     static __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
         *reinterpret_cast<uint4*>(p) =
             make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
@@ -133,6 +145,7 @@ struct Elem<__nv_bfloat16> {
             x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
+    static __device__ __forceinline__ uint32_t top(const Raw& r) { return top16(r) << 16; }
     static __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
         *reinterpret_cast<uint4*>(p) =
             make_uint4(pack_b2(x[0], x[1]), pack_b2(x[2], x[3]), pack_b2(x[4], x[5]), pack_b2(x[6], x[7]));

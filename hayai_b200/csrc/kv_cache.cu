@@ -35,23 +35,25 @@ __device__ __forceinline__ C* kv_elem(uint8_t* base, uint32_t units) {
     return reinterpret_cast<C*>(base + (unsigned long long)units * 64);
 }
 
-// Codes of 8 values of a row with largest |x| m and scale s, four to a word.  The code is the nearest
-// whole number to fl(x / s); x * (1 / s) is within 127 * 2^-21 of the quotient, so that its nearest
-// whole number is the same unless it lies that near to a half: only then are the values divided
-// (three instructions a value instead of about twelve).  1.5 * 2^23 added leaves the whole number in
-// the low bits, in two's complement.
+// Codes of 8 values of a row with largest |x| m and scale s, four to a word.  The quotient rounded as
+// IEEE division rounds it takes three instructions a value where the row shares the divisor, by
+// Markstein's theorem (IBM J. Res. Dev. 34, 1990): with r the reciprocal of s rounded to nearest and
+// q = x r, fma(fma(-q, s, x), r, q) is x / s rounded to nearest, unless s has a significand of all
+// ones.  That, and rows whose scale or remainders are not normal numbers, are divided.  (An estimate
+// with a division where it lies near a half is slower: ratios of 8-bit significands meet halves in
+// two of three warps.)  1.5 * 2^23 added rounds to whole numbers, ties to even, and leaves them in the
+// low bits in two's complement.
 __device__ __forceinline__ void kv_codes(const float (&x)[8], float m, float s, uint32_t (&q)[2]) {
     constexpr float kMagic = 12582912.f;
-    const float inv = __fdividef(1.f, s);
     float f[8];
-    bool near = m < 1e-30f || !(s > 0.f);  // a scale that is not a normal number, 0 or NaN
+    if (m >= 1e-30f && m <= 1e30f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu) {
+        const float r = __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = x[i] * inv;
-        f[i] = y + kMagic;
-        near |= fabsf(y - (f[i] - kMagic)) > 0.4999f;
-    }
-    if (near) {
+        for (int i = 0; i < 8; ++i) {
+            const float y = x[i] * r;
+            f[i] = fmaf(fmaf(-y, s, x[i]), r, y) + kMagic;
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             f[i] = (s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f) : 0.f) + kMagic;
@@ -90,9 +92,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, K
             Elem<T>::values(raw[w][u], x);
             C* dst = kv_elem<C>(w ? c.v : c.k, at + (uint32_t)h * c.head) + l * 8;
             if constexpr (sizeof(C) == 1) {
-                uint32_t top = 0;  // the bits of |x| order as the values do, infinity and NaN above all
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+                uint32_t top = Elem<T>::top(raw[w][u]);
 #pragma unroll
                 for (int o = GL / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const float m = __uint_as_float(top);
