@@ -33,8 +33,9 @@
 // The workers of the line (attn_rows.cuh) are warps, one block of 8 or 12 of them per SM.  A warp
 // streams its units through a ring of 16-byte asynchronous copies of its own, whose issue runs ahead
 // over tile boundaries, and meets the others only once: a tile that it has whole it writes itself;
-// of its first and last tile's pieces the partial (m, l, O) go to the workspace, where after one
-// block barrier the block joins its warps' pieces, and the last block of a tile the blocks'.
+// of its first and last tile's pieces it leaves the partial (m, l, O) in shared memory or in the
+// workspace, where after one barrier the block joins its warps' pieces, and the last block of a
+// tile's row the blocks'.
 // (Tiles shared by all warps of a block, with a barrier and a joining at each tile's end, took
 // 160 us where this takes 9x us: 64 sequences of 300 to 12000 tokens, 64 heads on 8.)
 #include <math.h>
@@ -136,6 +137,27 @@ __device__ __forceinline__ float lds32f(uint32_t a) {
     return r;
 }
 
+// Four adjacent values of a query row, as loaded.
+template <class T>
+struct FewRaw {
+    using type = uint2;
+    static __device__ __forceinline__ void values(const uint2& u, float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint16_t b = (uint16_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
+            if constexpr (__is_same(T, __half))
+                x[i] = h2f(b);
+            else
+                x[i] = __uint_as_float((uint32_t)b << 16);
+        }
+    }
+};
+template <>
+struct FewRaw<float> {
+    using type = float4;
+    static __device__ __forceinline__ void values(const float4& f, float (&x)[4]) { x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w; }
+};
+
 // Places of 16-byte chunks in a stage, permuted so that the 8 lanes of a load's phase (two rows by
 // four chunks of K, four rows by two chunks of V) touch all banks once.
 template <int CPR>
@@ -181,15 +203,19 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
     constexpr int W = F::W, THREADS = 32 * W, ST = F::ST, CPR = F::CPR, MT = ST / 16, KS = D / 16, ROWS = 8 * NT, I8 = F::ES == 1;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ AttnShared shared_s[W + 1];  // tiles that start in warp w and go on past it; the block's first
-    __shared__ int last_s[2];
     __shared__ __align__(8) int scratch[32];
     const int w = threadIdx.x >> 5, ln = lane_id(), g = ln >> 2, t4 = ln & 3;
     const uint32_t ring = smem_addr(smem) + w * F::WB;
     uint8_t* const qf = smem + w * F::WB + F::NS * F::SB;
     float* const rscale = reinterpret_cast<float*>(qf + F::QB);  // [ROWS], and [ROWS] of -1152 sum q
 
+    __shared__ float* place_s[W][2];  // where a warp's last (0) and first (1) piece of a shared tile is
+
+    // few sequences (a single one above all, whose call is short): every warp schedules for itself
+    const bool lanes = a.b.n_seq <= 32 && a.max_rows <= 8 * ROWS;
     int* const pre = reinterpret_cast<int*>(smem);
-    const int U = attn_schedule<THREADS>(a, ROWS, ST, pre, scratch);
+    AttnLanes lv;
+    const int U = lanes ? attn_schedule_lanes(a, ROWS, ST, lv) : attn_schedule<THREADS>(a, ROWS, ST, pre, scratch);
     const int G = min((int)gridDim.x, max(1, U / W)), c = blockIdx.x;
     if (U <= 0 || c >= G) return;
     FewWalk pw;  // the copies' walk: units are issued NS - 1 ahead
@@ -198,7 +224,10 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
     pw.b1 = share.begin(c * W + w + 1);
     pw.live = pw.b0 < pw.b1;
     if (pw.live) {
-        pw.it.seek(a, pre, pw.b0, ROWS, ST);
+        if (lanes)
+            pw.it.seek(a, lv, pw.b0, ROWS, ST);
+        else
+            pw.it.seek(a, pre, pw.b0, ROWS, ST);
         pw.enter();
     }
     if (threadIdx.x <= W) shared_s[threadIdx.x].valid = 0;
@@ -249,6 +278,22 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         }
         cp_async_commit();
     };
+    // The tile's query rows as loaded, 4 values to a lane: all on their way at once, before the copies that
+    // wait for page numbers.
+    using Raw = typename FewRaw<T>::type;
+    Raw raw[ROWS];
+    auto load_queries = [&]() {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            raw[r] = Raw{};
+            if (r < it.t.nr && ln < D / 4) {
+                const int row = it.t.r0 + r, tr = a.by_group(row);
+                raw[r] = __ldg(reinterpret_cast<const Raw*>((const T*)a.q + (long long)(it.q.q0 + tr) * a.ldq +
+                                                            (it.hk * a.group + row - tr * a.group) * D + 4 * ln));
+            }
+        }
+    };
+    if (b0 < b1) load_queries();
     look_up();
 #pragma unroll
     for (int i = 0; i < F::NS - 1; ++i) issue();
@@ -260,41 +305,16 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         if (lo >= hi) {
             if (it.u_item + tl.span >= b1) break;
             it.next(a, ROWS, ST);
+            load_queries();
             continue;
         }
         // ---- the query tile as B operands
-#pragma unroll 4
+#pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            if (r >= tl.nr) {  // no row: zeros, so that what is there before does not move the maxima
-                if (ln == 0) rscale[r] = rscale[ROWS + r] = 0.f;
-#pragma unroll
-                for (int i = ln; i < KS * X::Q * 4; i += 32)
-                    *reinterpret_cast<uint2*>(qf + (((i >> 2) / X::Q * NT + (r >> 3)) * X::Q + (i >> 2) % X::Q) * 256 +
-                                              ((r & 7) * 4 + (i & 3)) * 8) = make_uint2(0, 0);
-                continue;
-            }
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if (ln < D / 4) {
-                const int row = tl.r0 + r, tr = a.by_group(row), tok = it.q.q0 + tr, h = it.hk * a.group + row - tr * a.group;
-                const T* q = (const T*)a.q + (long long)tok * a.ldq + h * D + 4 * ln;
-                if constexpr (sizeof(T) == 4) {
-                    const float4 f = __ldg(reinterpret_cast<const float4*>(q));
-                    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-                } else {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(q));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint16_t b = (uint16_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
-                        if constexpr (__is_same(T, __half))
-                            x[i] = h2f(b);
-                        else
-                            x[i] = __uint_as_float((uint32_t)b << 16);
-                    }
-                }
-            }
+            float x[4];
+            FewRaw<T>::values(raw[r], x);
             float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // not negative: order as bits
             // the power of two of m, taken out of the row (none for 0, infinity and the smallest)
             const uint32_t e = __float_as_uint(m) >> 23;
             const bool norm = e >= 2 && e <= 252;
@@ -663,7 +683,12 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 
         // ---- the tile's end: lane (g, t4) holds values 64 cg + 8 g + x (8-bit: (D / 8) g + x) of rows 2 t4 + e
         const bool whole = lo == 0 && hi == tl.units;
-        float* const part = a.part + (size_t)(2 * (c * W + w) + (lo == 0)) * F::PS;
+        // a piece goes to the workspace, or, the warp's last, to its own ring, which is done with
+        const bool done = it.u_item + tl.span >= b1;
+        if (done) asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        float* const part = done ? reinterpret_cast<float*>(smem + w * F::WB)
+                                 : a.part + (size_t)(2 * (c * W + w) + (lo == 0)) * F::PS;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -688,73 +713,66 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m[n][e], l[n][e]);
                 }
             }
-        if (!whole && ln == 0 && (lo == 0 || w == 0))
-            shared_s[lo == 0 ? w : W] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units};
-        if (it.u_item + tl.span >= b1) break;
+        if (!whole && ln == 0) {
+            place_s[w][lo == 0] = part;
+            if (lo == 0 || w == 0) shared_s[lo == 0 ? w : W] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units};
+        }
+        if (done) break;
         it.next(a, ROWS, ST);
+        load_queries();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 
-    // ---- the block's tiles of several warps: a row per warp at a time, its D values over D / 4 lanes
+    // ---- the tiles of several warps: a row per warp at a time, its D values over D / 4 lanes; a tile of several
+    // blocks is joined from their results, row by row, by the block whose row comes last
     float* const bpart = a.part + (size_t)2 * gridDim.x * W * F::PS;  // the blocks' partial results, two each
-    int crossing = 0, turn = 0;
+    int turn = 0;
+#pragma unroll 1
     for (int x = 0; x <= W; ++x) {
         const AttnShared sh = shared_s[x];
         if (!sh.valid) continue;
-        const int wf = share.owner(sh.u_item), wl = share.owner(sh.u_item + sh.units - 1);
-        const bool cross = wf / W != c || wl / W != c;
-        crossing |= cross ? 1 << (x == W ? 0 : 1) : 0;
+        const int wf = share.owner(sh.u_item), wl = share.owner(sh.u_item + sh.units - 1), bf = wf / W, bl = wl / W;
+        // of fewer places than warps some warps have none, and no piece
+        const int q0 = max(wf, c * W), q1 = min(wl, c * W + W - 1);
+#pragma unroll 1
         for (int r = 0; r < sh.nr; ++r) {
             if (turn++ % W != w) continue;
-            // of fewer places than warps some warps have none, and no piece
-            const int q0 = max(wf, c * W), q1 = min(wl, c * W + W - 1);
             AttnJoin j;
+            auto piece = [&](int i) { return place_s[q0 + i - c * W][q0 + i == wf]; };
             j.join(q1 - q0 + 1, ln < D / 4,
-                   [&](int i) -> const float* {
-                       const int q = q0 + i;
-                       if (share.q == 0 && q >= share.rem) return nullptr;
-                       return a.part + (size_t)(2 * q + (q == wf)) * F::PS + ROWS * D + 2 * r;
+                   [&](int i) {
+                       return share.q == 0 && q0 + i >= share.rem ? make_float2(-INFINITY, 0.f)
+                                                                  : *reinterpret_cast<const float2*>(piece(i) + ROWS * D + 2 * r);
                    },
-                   [&](int i) { return a.part + (size_t)(2 * (q0 + i) + (q0 + i == wf)) * F::PS + r * D; });
-            if (ln >= D / 4) continue;
-            if (cross) {
-                float* p = bpart + (size_t)(2 * c + (wf / W == c)) * F::PS;
-                *reinterpret_cast<float4*>(p + r * D + 4 * ln) = make_float4(j.y[0], j.y[1], j.y[2], j.y[3]);
+                   [&](int i) {
+                       return share.q == 0 && q0 + i >= share.rem ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                                  : reinterpret_cast<const float4*>(piece(i) + r * D)[ln];
+                   });
+            if (bf != bl) {
+                float* p = bpart + (size_t)(2 * c + (bf == c)) * F::PS;
+                if (ln < D / 4) reinterpret_cast<float4*>(p + r * D)[ln] = make_float4(j.y[0], j.y[1], j.y[2], j.y[3]);
                 if (ln == 0) *reinterpret_cast<float2*>(p + ROWS * D + 2 * r) = make_float2(j.m, j.l);
-            } else {
-                attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
-                if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
+                __threadfence();
+                __syncwarp();
+                int* const cnt = a.count + bf * 32 + r;
+                int last = 0;
+                if (ln == 0) {
+                    last = atomicAdd(cnt, 1) == bl - bf;
+                    if (last) *cnt = 0;
+                }
+                if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+                __threadfence();
+                auto block = [&](int i) { return bpart + (size_t)(2 * (bf + i) + (i == 0)) * F::PS; };
+                j = AttnJoin();
+                j.join(bl - bf + 1, ln < D / 4,
+                       [&](int i) { return __ldcg(reinterpret_cast<const float2*>(block(i) + ROWS * D + 2 * r)); },
+                       [&](int i) { return __ldcg(reinterpret_cast<const float4*>(block(i) + r * D) + ln); });
             }
+            if (ln >= D / 4) continue;
+            attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
+            if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
         }
-    }
-    if (!crossing) return;
-    // ---- tiles of several blocks: the last of them joins
-    __threadfence();
-    __syncthreads();
-    for (int x = 0; x <= W; ++x) {
-        const AttnShared sh = shared_s[x];
-        if (!sh.valid) continue;
-        const int bf = share.owner(sh.u_item) / W, bl = share.owner(sh.u_item + sh.units - 1) / W;
-        if (bf == bl) continue;
-        if (threadIdx.x == 0) {
-            last_s[0] = atomicAdd(a.count + bf, 1) == bl - bf;
-            if (last_s[0]) a.count[bf] = 0;
-            __threadfence();
-        }
-        __syncthreads();
-        if (last_s[0]) {
-            for (int r = w; r < sh.nr; r += W) {
-                AttnJoin j;
-                auto piece = [&](int i) { return bpart + (size_t)(2 * (bf + i) + (i == 0)) * F::PS; };
-                j.join(bl - bf + 1, ln < D / 4, [&](int i) -> const float* { return piece(i) + ROWS * D + 2 * r; },
-                       [&](int i) { return piece(i) + r * D; });
-                if (ln >= D / 4) continue;
-                attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
-                if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
-            }
-        }
-        __syncthreads();
     }
 }
 
@@ -765,6 +783,7 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     using F = FewCfg<T, C, D, NT>;
     constexpr int most = F::W * F::WB;
     static_assert(most <= 227 * 1024 - 1024, "shared memory of a block");
+    static_assert(F::WB >= F::PS * 4, "a warp's last piece lies in its own part");
     static_assert(most >= 4 * HC_KV_SEQS, "the schedule's prefix lies in the rings");
     static_assert((size_t)F::PS * 4 * 2 * (F::W + 1) <= kFewPartBytes, "the workspace of a block");
     static SmemOptIn opted;

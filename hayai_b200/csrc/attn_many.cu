@@ -515,8 +515,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 for (int r = warp; r < sh.nr; r += 8) {
                     AttnJoin j;
                     auto piece = [&](int i) { return a.part + (size_t)(2 * (bf + i) + (i == 0)) * PS; };
-                    j.join(bl - bf + 1, ln < D / 4, [&](int i) -> const float* { return piece(i) + ROWS * D + 2 * r; },
-                           [&](int i) { return piece(i) + r * D; });
+                    j.join(bl - bf + 1, ln < D / 4,
+                           [&](int i) { return __ldcg(reinterpret_cast<const float2*>(piece(i) + ROWS * D + 2 * r)); },
+                           [&](int i) { return __ldcg(reinterpret_cast<const float4*>(piece(i) + r * D) + ln); });
                     if (ln >= D / 4) continue;
                     attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
                     if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);

@@ -104,6 +104,36 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
     return (int)carry_s;
 }
 
+// The same for at most 32 sequences of few tiles, by every warp for itself and without a barrier:
+// lane s gets its sequence, and the places up to its end.
+struct AttnLanes {
+    KvSeq q;
+    int pre;
+};
+__device__ __forceinline__ int attn_schedule_lanes(const AttnArgs& a, int rows, int unit, AttnLanes& v) {
+    const int ln = lane_id();
+    v.q = {0, 0, 0};
+    unsigned long long x = 0;
+    if (ln < a.b.n_seq) {
+        v.q = kv_seq(a.b, a.b.max_pages * a.c.page_size, ln);
+        const int n = attn_tiles(a, v.q, rows);
+        for (int t = 0; t < n; ++t) x += attn_tile(a, v.q, t, rows, unit).span;
+    }
+    x = min(x * a.c.n_heads, 0x7fffffffull);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (ln >= o) x += y;
+    }
+    v.pre = (int)min(x, 0x7fffffffull);
+    const int U = __shfl_sync(0xffffffffu, v.pre, 31);
+    if (U == 0x7fffffff) {
+        if (ln == 0) atomicOr(a.b.err, kErrKvRange);
+        return -1;
+    }
+    return U;
+}
+
 // A tile that several workers share, for the joining.
 struct AttnShared {
     int valid, q0, hk, r0, nr, u_item, units;
@@ -130,7 +160,19 @@ struct AttnIter {
         }
         s = lo;
         seq(a, rows);
-        const int before = s ? pre[s - 1] : 0, w = (pre[s] - before) / a.c.n_heads;
+        enter(a, s ? pre[s - 1] : 0, pre[s], u, rows, unit);
+    }
+    __device__ __forceinline__ void seek(const AttnArgs& a, const AttnLanes& v, int u, int rows, int unit) {
+        s = __popc(__ballot_sync(0xffffffffu, v.pre <= u));
+        q = {__shfl_sync(0xffffffffu, v.q.q0, s), __shfl_sync(0xffffffffu, v.q.q1, s), __shfl_sync(0xffffffffu, v.q.len, s)};
+        n_tiles = attn_tiles(a, q, rows);
+        tile = 0;
+        const int before = __shfl_sync(0xffffffffu, v.pre, s ? s - 1 : 0);
+        enter(a, s ? before : 0, __shfl_sync(0xffffffffu, v.pre, s), u, rows, unit);
+    }
+    // The item of sequence s, whose places are [before, end), that holds place u.
+    __device__ __forceinline__ void enter(const AttnArgs& a, int before, int end, int u, int rows, int unit) {
+        const int w = (end - before) / a.c.n_heads;
         hk = (u - before) / w;
         u_item = before + hk * w;
         t = attn_tile(a, q, 0, rows, unit);
@@ -208,21 +250,19 @@ __device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk
             l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
 }
 
-// One row of n partial results joined by a warp: piece i has (m, l) at ml(i) (or none) and D values at y(i),
-// of which the lane gets 4 (4 lane ..).  All (m, l) are loaded together and the values eight pieces
-// at a time: with one piece after the other the trips to L2 took 8 to 15 us of a call.
+// One row of n partial results joined by a warp: ml(i) gives piece i's (m, l), (-inf, 0) if it has
+// none, and y(i) the lane's 4 of its D values.  All (m, l) are loaded together and the values eight
+// pieces at a time: with one piece after the other the trips to L2 took 8 to 15 us of a call.
 struct AttnJoin {
     float m = -INFINITY, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
     template <class ML, class Y>
     __device__ __forceinline__ void join(int n, bool mine, ML ml, Y at) {
         const int ln = lane_id();
+#pragma unroll 1
         for (int i0 = 0; i0 < n; i0 += 32) {
             const int cnt = min(32, n - i0);
             float2 v = make_float2(-INFINITY, 0.f);
-            if (ln < cnt) {
-                const float* p = ml(i0 + ln);
-                if (p) v = __ldcg(reinterpret_cast<const float2*>(p));
-            }
+            if (ln < cnt) v = ml(i0 + ln);
             float top = v.x;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -234,12 +274,13 @@ struct AttnJoin {
             m = top;
 #pragma unroll
             for (int k = 0; k < 4; ++k) y[k] = old == 0.f ? 0.f : y[k] * old;
+#pragma unroll 1
             for (int i = 0; i < cnt; i += 8) {
                 float4 x[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (mine && i + k < cnt) x[k] = __ldcg(reinterpret_cast<const float4*>(at(i0 + i + k)) + ln);
+                    if (mine && i + k < cnt) x[k] = at(i0 + i + k);
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {

@@ -129,7 +129,7 @@ static int attn_workspace(hc_engine* e, AttnArgs* a) {
         const int rc = e->attn_part.ensure(part);
         if (rc) return rc;
     }
-    const size_t cnt = (size_t)e->num_sms * sizeof(int);
+    const size_t cnt = (size_t)e->num_sms * 32 * sizeof(int);  // one for each row of a block's first split tile
     if (cnt > e->attn_cnt.cap) {
         const int rc = e->attn_cnt.ensure(cnt);
         if (rc) return rc;

@@ -64,7 +64,7 @@ struct AttnArgs {
     int row_min, row_max;  // sequences with fewer or more rows are left to another kernel
     int over;              // places of the line that stand for a tile's start and end
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
-    int* count;            // one counter per block, zero between calls
+    int* count;            // 32 counters per block, zero between calls
 };
 
 // Partial results of the kernel for few rows: bytes for each block.
