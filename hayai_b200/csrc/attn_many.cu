@@ -174,6 +174,19 @@ struct ManySeg {
     int pad[2];
 };
 
+// 32 bytes to global memory: in one store where they lie on 32 bytes (a thread per row stores to as
+// many lines as it has lanes, and each line once instead of twice).
+__device__ __forceinline__ void many_store32(void* p, const uint32_t (&y)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+                     "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+}
+
 // The range of a row's visible positions in the tile's count v: v < c and (v >= b or v < a).
 struct ManyRow {
     int a, b, c;
@@ -240,7 +253,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     // the schedule's prefix sums lie in the last key and value tile until warp 13 has its place
     int* const pre_s = reinterpret_cast<int*>(smem + F::oKV + (NB - 1) * TILE);
     const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 16);
-    const int G = min((int)gridDim.x, U);
+    // blocks: enough of the line for each, and a tile not in so many pieces that joining them takes longer
+    const int G = max(1, min(min((int)gridDim.x, U / 4), 16 * misc[16 + 18]));
     if (U <= 0 || c >= G) return;
     const AttnShares share(U, G);
     if (threadIdx.x == 0) {
@@ -299,23 +313,60 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             if (!ok || lo == hi) break;
             const int kvt = 2 * unit;  // key and value tiles before this segment's
             unit += hi - lo;
+            const KvSeq q{sg->q0, sg->q1, sg->len};
+            const int r0 = sg->r0, hk = sg->hk, whole = sg->whole, slot = sg->slot;
+            AttnTile tl;
+            tl.lo = sg->vlo, tl.n1 = sg->n1;
+            give_back(n);  // here: an arrival after the results' stores would wait for them
             if (half * 128 < nr) {
-                const int r = half * 128 + rt, row = sg->r0 + r;
+                const int r = half * 128 + rt, row = r0 + r;
                 const bool real = r < nr;
-                const KvSeq q{sg->q0, sg->q1, sg->len};
-                AttnTile tl;
-                tl.lo = sg->vlo, tl.n1 = sg->n1;
                 const ManyRow vis = many_row(a, q, tl, row, real);
                 // a unit is whole for this half's rows if it ends before every row's limit and starts past
                 // every row's window (or lies in the first tokens that all see)
-                const ManyRow first = many_row(a, q, tl, sg->r0 + half * 128, true),
-                              lastr = many_row(a, q, tl, sg->r0 + min(half * 128 + 127, nr - 1), true);
+                const ManyRow first = many_row(a, q, tl, r0 + half * 128, true),
+                              lastr = many_row(a, q, tl, r0 + min(half * 128 + 127, nr - 1), true);
                 const int cmin = min(first.c, lastr.c), bmax = lastr.b, amin = first.a;
 
                 float rs = 0.f;
                 float m = -INFINITY;
                 float2 l2 = make_float2(0.f, 0.f);
                 for (int st = lo; st < hi; ++st) {
+                    const int v0 = st * UNIT;
+                    const bool full = v0 + UNIT <= cmin && (v0 >= bmax || v0 + UNIT <= amin);
+                    uint32_t odd = 0;
+                    const uint8_t* vtile = nullptr;
+                    if constexpr (!I8) {
+                        // A value that is not finite, in a unit that some row does not see whole: 0 * infinity must not
+                        // reach a masked row, so that the unit's product is then done by the rows' threads (rare).  The
+                        // look at V comes before the wait for the scores.
+                        if (!full) {
+                            const int vt = kvt + 2 * (st - lo) + 1;
+                            if (!many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok)) break;
+                            vtile = smem + F::oKV + (vt % NB) * TILE;
+                            constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+                            if (v0 + rt >= cmin || bmax > v0) {  // a position that all rows see is no matter
+#pragma unroll 4
+                                for (int i = 0; i < D / 8; ++i) {
+                                    const uint4 x = *reinterpret_cast<const uint4*>(vtile + (i >> 3) * HALF + rt * 128 +
+                                                                                    (((i + rt) & 7) << 4));
+                                    const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) odd |= (y[k] & E) == E || ((y[k] >> 16) & E) == E;
+                                }
+                            }
+                            // the half's four warps decide together: three flags in turn, each cleared a check ahead
+                            int* const flag = misc + 4 + 3 * half;
+                            if (__any_sync(0xffffffffu, odd != 0) && ln == 0) flag[checks % 3] = 1;
+                            if (rt == 0) flag[(checks + 1) % 3] = 0;
+                            __syncwarp();
+                            if (ln == 0) mbar_arrive(b_chk + 8 * half);
+                            if (!many_wait(b_chk + 8 * half, checks & 1, ok)) break;
+                            odd = *(volatile int*)&flag[checks % 3];
+                            ++checks;
+                        }
+                        if (rt == 0) misc[2 + half] = (int)odd;  // read by the products' warp after the arrivals
+                    }
                     if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
                     ph_s ^= 1;
                     tc_fence_after();
@@ -339,8 +390,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         ev = (float)((int)(__float_as_uint(top) >> 23) - 126);  // log2 of a power of two over it
                     }
-                    const int v0 = st * UNIT;
-                    const bool full = v0 + UNIT <= cmin && (v0 >= bmax || v0 + UNIT <= amin);
                     const int vc = vis.c - v0, vb = vis.b - v0, va = vis.a - v0;
                     // 32 scores from TMEM: times their K scales, masked
                     auto scores = [&](int k, float* s) {
@@ -361,20 +410,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                             }
                         }
                     };
-                    float sa[4][32];
+                    // 16-bit caches hold S in registers; with scales to multiply by that is more than a thread has, and S
+                    // is read twice, 32 columns at a time with the next 32 on their way
+                    float sa[I8 ? 2 : 4][32];
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if constexpr (I8) {
+                        tc_ld32(tS, sa[0]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_ld32(tS + 32 * k, sa[k]);
-                    tc_wait_ld32(sa[0]);
-                    tc_wait_ld32(sa[1]);
-                    tc_wait_ld32(sa[2]);
-                    tc_wait_ld32(sa[3]);
+                        for (int k = 0; k < 4; ++k) {
+                            float* s = sa[k & 1];
+                            tc_wait_ld32(s);
+                            tc_ld32(tS + (k < 3 ? 32 * (k + 1) : 0), sa[(k + 1) & 1]);  // last: the second pass's first
+                            scores(k, s);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float* s = sa[k];
-                        scores(k, s);
+                            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
+                        }
+                        tc_wait_ld32(sa[0]);  // before other loads and waits
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
+                        for (int k = 0; k < 4; ++k) tc_ld32(tS + 32 * k, sa[k]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) tc_wait_ld32(sa[k]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float* s = sa[k];
+                            scores(k, s);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
+                        }
                     }
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     const float cand = top == -INFINITY ? top : top * rs + ev;
@@ -399,8 +462,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     const float2 rs2 = make_float2(rs, rs), nm2 = make_float2(-mm, -mm);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float* s = sa[k];
+                        float* s = sa[I8 ? k & 1 : k];
+                        if constexpr (I8) {
+                            if (k > 0) tc_wait_ld32(s);
+                            if (k < 3) tc_ld32(tS + 32 * (k + 1), sa[(k + 1) & 1]);
+                            scores(k, s);
+                        }
                         uint32_t pk[16];
+                        float4 vs4 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int e = 2 * i;
@@ -408,8 +477,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                             float2 p = make_float2(ex2(x.x), ex2(x.y));
                             l2 = add2(l2, p);
                             if constexpr (I8) {
-                                const float2 f = reinterpret_cast<const float2*>(vsc)[16 * k + i];
-                                p = mul2(p, f);
+                                if ((i & 1) == 0) vs4 = vsc[8 * k + (i >> 1)];
+                                p = mul2(p, i & 1 ? make_float2(vs4.z, vs4.w) : make_float2(vs4.x, vs4.y));
                                 if (!full) {  // whatever a masked position's scale is
                                     if (s[e] == -INFINITY) p.x = 0.f;
                                     if (s[e + 1] == -INFINITY) p.y = 0.f;
@@ -420,38 +489,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         tc_st16(tS + 16 * k, pk);
                     }
                     tc_wait_st();
-                    if constexpr (!I8) {
-                        // a value that is not finite, in a unit that some row does not see whole: 0 * infinity must
-                        // not reach a masked row, so that the unit's product is done here (rare)
-                        if (!full) {
-                            const int vt = kvt + 2 * (st - lo) + 1;
-                            if (!many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok)) break;
-                            const uint8_t* vtile = smem + F::oKV + (vt % NB) * TILE;
-                            constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-                            uint32_t odd = 0;
-#pragma unroll 4
-                            for (int i = 0; i < D / 8; ++i) {
-                                const uint4 x = *reinterpret_cast<const uint4*>(vtile + (i >> 3) * HALF + rt * 128 +
-                                                                                (((i + rt) & 7) << 4));
-                                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) odd |= (y[k] & E) == E || ((y[k] >> 16) & E) == E;
-                            }
-                            // the half's four warps decide together: three flags in turn, each cleared a check ahead
-                            int* const flag = misc + 4 + 3 * half;
-                            if (__any_sync(0xffffffffu, odd != 0) && ln == 0) flag[checks % 3] = 1;
-                            if (rt == 0) flag[(checks + 1) % 3] = 0;
-                            __syncwarp();
-                            if (ln == 0) mbar_arrive(b_chk + 8 * half);
-                            if (!many_wait(b_chk + 8 * half, checks & 1, ok)) break;
-                            odd = *(volatile int*)&flag[checks % 3];
-                            ++checks;
-                            if (rt == 0) misc[2 + half] = (int)odd;  // read by the products' thread after the arrivals
-                            if (odd) many_product<BF, D>(tO, tS, vtile, st == lo);
-                        } else if (rt == 0) {
-                            misc[2 + half] = 0;
-                        }
-                    }
+                    if constexpr (!I8)
+                        if (odd) many_product<BF, D>(tO, tS, vtile, st == lo);
                     tc_fence_before();
                     __syncwarp();
                     if (ln == 0) mbar_arrive(b_p + 8 * half);
@@ -461,11 +500,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 ph_o ^= 1;
                 tc_fence_after();
                 const float l = l2.x + l2.y;
-                const bool whole = sg->whole;
                 const float k1 = l == 0.f ? 0.f : 1.f / l;
+                const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.ldo * 2)) & 31) == 0;  // rows start on 32 bytes
                 const int tr = a.by_group(row);
-                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + (sg->hk * a.group + row - tr * a.group) * D;
-                float* const part = a.part + (size_t)(2 * c + sg->slot) * PS;
+                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + (hk * a.group + row - tr * a.group) * D;
+                float* const part = a.part + (size_t)(2 * c + slot) * PS;
 #pragma unroll 1
                 for (int k = 0; k < D / 32; ++k) {
                     float o[32];
@@ -474,11 +513,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     if (!real || !ok) continue;
                     if (whole) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float y[8];
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t y[8];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : o[8 * i + e] * k1;
-                            Elem<T>::store8(out + 32 * k + 8 * i, y);
+                            for (int e = 0; e < 8; ++e) {
+                                const float u = l == 0.f ? 0.f : o[16 * i + 2 * e] * k1, v = l == 0.f ? 0.f : o[16 * i + 2 * e + 1] * k1;
+                                y[e] = __is_same(T, __half) ? pack_h2(u, v) : pack_b2(u, v);
+                            }
+                            many_store32(out + 32 * k + 16 * i, y, wide);
                         }
                     } else {
 #pragma unroll
@@ -490,13 +532,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 tc_fence_before();
                 if (real && ok) {
                     if (whole)
-                        attn_store_lse(a, q.q0, sg->hk, row, m, l);
+                        attn_store_lse(a, q.q0, hk, row, m, l);
                     else
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m, l);
                 }
             }
             if (!ok) break;
-            give_back(n);
         }
         // ---- tiles that several blocks share: the last of them joins.  One thread decides for all, so that they
         // meet at the same barriers even where a wait has run out.
@@ -512,15 +553,64 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             }
             named_bar_sync(1, 256);
             if (misc[1]) {
-                for (int r = warp; r < sh.nr; r += 8) {
-                    AttnJoin j;
-                    auto piece = [&](int i) { return a.part + (size_t)(2 * (bf + i) + (i == 0)) * PS; };
-                    j.join(bl - bf + 1, ln < D / 4,
-                           [&](int i) { return __ldcg(reinterpret_cast<const float2*>(piece(i) + ROWS * D + 2 * r)); },
-                           [&](int i) { return __ldcg(reinterpret_cast<const float4*>(piece(i) + r * D) + ln); });
-                    if (ln >= D / 4) continue;
-                    attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
-                    if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
+                // The pieces' weights of every row first (into the rings, which are done with), by a thread per row;
+                // then a thread per four values of a row, eight of them on their way at once.  (A row per warp, or
+                // one value after the other, waits for L2 so often that a joining took 80000 cycles.)
+                const int n = bl - bf + 1;
+                const float* const p0 = a.part + (size_t)(2 * bf + 1) * PS;  // the first piece; the i-th: p0 + (2 i - 1) PS
+                auto piece = [&](int i) { return p0 + (i ? (size_t)(2 * i - 1) * PS : 0); };
+                constexpr int WT = 64;  // pieces whose weights fit the rings of every variant; of more they are made again
+                float* const wt = reinterpret_cast<float*>(smem + F::oKV);  // [piece][row]
+                float* const tops = wt + WT * 256;                          // [row] maxima, [row] sums
+                static_assert((WT + 2) * 1024 <= F::oRS - F::oKV, "the joining's table");
+                {
+                    const int r = threadIdx.x;
+                    float m = -INFINITY, l = 0.f;
+                    if (r < sh.nr) {
+#pragma unroll 4
+                        for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(piece(i) + ROWS * D + 2 * r));
+#pragma unroll 4
+                        for (int i = 0; i < n; ++i) {
+                            const float2 v = __ldcg(reinterpret_cast<const float2*>(piece(i) + ROWS * D + 2 * r));
+                            // a piece that saw nothing has m = -inf and l = 0
+                            const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : ex2(v.x - m);
+                            l += v.y * f;
+                            if (i < WT) wt[i * 256 + r] = f;
+                        }
+                        tops[r] = m;
+                        tops[256 + r] = l;
+                        attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, m, l);
+                    }
+                }
+                named_bar_sync(1, 256);
+#pragma unroll 1
+                for (int e0 = threadIdx.x; e0 < sh.nr * (D / 4); e0 += 8 * 256) {
+                    float y[8][4];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k][0] = y[k][1] = y[k][2] = y[k][3] = 0.f;
+#pragma unroll 1
+                    for (int i = 0; i < n; ++i) {
+                        float4 o[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int e = e0 + 256 * k;
+                            o[k] = e < sh.nr * (D / 4) ? __ldcg(reinterpret_cast<const float4*>(piece(i)) + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int e = e0 + 256 * k;
+                            if (e >= sh.nr * (D / 4)) continue;
+                            const int r = e / (D / 4);
+                            const float f = i < WT ? wt[i * 256 + r] : ex2(__ldcg(piece(i) + ROWS * D + 2 * r) - tops[r]);
+                            if (f == 0.f) continue;
+                            y[k][0] += o[k].x * f, y[k][1] += o[k].y * f, y[k][2] += o[k].z * f, y[k][3] += o[k].w * f;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int e = e0 + 256 * k, r = e / (D / 4);
+                        if (e < sh.nr * (D / 4)) attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[256 + r]);
+                    }
                 }
             }
             named_bar_sync(1, 256);

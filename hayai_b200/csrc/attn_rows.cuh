@@ -49,12 +49,16 @@ __device__ __forceinline__ int attn_tiles(const AttnArgs& a, const KvSeq& q, int
 
 // Places of every sequence, as an inclusive prefix sum in `pre` (n_seq ints of shared memory);
 // returns U, or -1 (and the error flag) if they do not fit 31 bits.  The whole block calls it, with 32
-// words of shared memory as scratch.
+// words of shared memory as scratch; word 18 then holds the number of items (of 2^16 and more: at
+// least that).
 template <int THREADS>
 __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int unit, int* pre, int* scratch) {
     static_assert(THREADS <= 32 * 16, "scratch");
     long long& carry_s = *reinterpret_cast<long long*>(scratch);
     int* const wsum = scratch + 2;
+    int* const items = scratch + 18;  // the number of items, at most 2^16 counted
+    if (threadIdx.x == 0) *items = 0;
+    __syncthreads();
     const int cap = a.b.max_pages * a.c.page_size, tid = threadIdx.x, wid = tid >> 5, ln = tid & 31;
     const bool by_warp = a.max_rows > 8 * rows;  // many tiles in a sequence: its tiles over a warp's lanes
     if (by_warp) {
@@ -65,7 +69,10 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
             for (int t = ln; t < n; t += 32) w += attn_tile(a, q, t, rows, unit).span;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-            if (ln == 0) pre[s] = (int)min(w * a.c.n_heads, 0x7fffffffll);
+            if (ln == 0) {
+                pre[s] = (int)min(w * a.c.n_heads, 0x7fffffffll);
+                if (n && *(volatile int*)items < 1 << 16) atomicAdd(items, min(n * a.c.n_heads, 1 << 16));
+            }
         }
     } else {
         for (int s = tid; s < a.b.n_seq; s += THREADS) {
@@ -74,6 +81,7 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
             long long w = 0;
             for (int t = 0; t < n; ++t) w += attn_tile(a, q, t, rows, unit).span;
             pre[s] = (int)min(w * a.c.n_heads, 0x7fffffffll);
+            if (n && *(volatile int*)items < 1 << 16) atomicAdd(items, min(n * a.c.n_heads, 1 << 16));
         }
     }
     if (tid == 0) carry_s = 0;
