@@ -425,6 +425,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                               (tl.p_lo == tl.p_hi || !a.causal ||
                                (j1 <= tl.p_lo && (!a.window || v1 <= tl.n1 || (v0 >= tl.n1 && j0 > tl.p_hi - a.window))));
             float vsc[MT][2];
+            bool vodd = false;  // a V scale that is not finite in a unit that some row does not see whole
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 float ksc[2] = {1.f, 1.f};
@@ -441,12 +442,23 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         s[i][n][e] *= I8 ? rs[n][e & 1] * ksc[e >> 1] : rs[n][e & 1];
-                        if (!full) {
-                            const int v = v0 + 16 * i + 8 * (e >> 1) + g;
-                            const int j = v < tl.n1 ? v : v - tl.n1 + tl.lo;
-                            const bool see = v < tl.nvis && j <= lim[n][e & 1] && (j >= wlo[n][e & 1] || j < a.sink);
-                            if (!see) s[i][n][e] = -INFINITY;
-                        }
+                    }
+            }
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int v = v0 + 16 * i + 8 * h + g;
+                        const int j = v < tl.n1 ? v : v - tl.n1 + tl.lo;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const bool see = v < tl.nvis && j <= lim[n][e] && (j >= wlo[n][e] || j < a.sink);
+                                if (!see) s[i][n][2 * h + e] = -INFINITY;
+                            }
+                        if (I8 && !(fabsf(vsc[i][h]) <= 3e38f)) vodd = true;
                     }
             }
             // ---- move the maxima where a score passes them by 8
@@ -492,11 +504,15 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                     for (int e = 0; e < 4; ++e) {
                         p[i][e] = ex2(s[i][n][e] - (e & 1 ? m1 : m0));
                         l[n][e & 1] += p[i][e];
-                        if constexpr (I8) {
-                            p[i][e] *= vsc[i][e >> 1];
-                            if (!full && s[i][n][e] == -INFINITY) p[i][e] = 0.f;  // whatever a masked token's scale is
-                        }
+                        if constexpr (I8) p[i][e] *= vsc[i][e >> 1];
                     }
+                if (I8 && vodd) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (s[i][n][e] == -INFINITY) p[i][e] = 0.f;
+                }
                 unit[n][0] = unit[n][1] = 1.f;
                 if constexpr (X::kBias) {
 #pragma unroll

@@ -28,6 +28,8 @@
 // bf16 on f16 products are scaled by a power of two to have their largest element in [1, 2).
 #include <math.h>
 
+#include <type_traits>
+
 #include "attn_rows.cuh"
 #include "tc5.cuh"
 
@@ -460,6 +462,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     }
                     const float mm = m == -INFINITY ? 0.f : m;
                     const float2 rs2 = make_float2(rs, rs), nm2 = make_float2(-mm, -mm);
+                    auto weights = [&](auto masked) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         float* s = sa[I8 ? k & 1 : k];
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                             if constexpr (I8) {
                                 if ((i & 1) == 0) vs4 = vsc[8 * k + (i >> 1)];
                                 p = mul2(p, i & 1 ? make_float2(vs4.z, vs4.w) : make_float2(vs4.x, vs4.y));
-                                if (!full) {  // whatever a masked position's scale is
+                                if constexpr (decltype(masked)::value) {  // whatever a masked position's scale is
                                     if (s[e] == -INFINITY) p.x = 0.f;
                                     if (s[e + 1] == -INFINITY) p.y = 0.f;
                                 }
@@ -488,6 +491,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         }
                         tc_st16(tS + 16 * k, pk);
                     }
+                    };
+                    if (I8 && !full)
+                        weights(std::true_type());
+                    else
+                        weights(std::false_type());
                     tc_wait_st();
                     if constexpr (!I8)
                         if (odd) many_product<BF, D>(tO, tS, vtile, st == lo);
@@ -623,7 +631,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
         const int pw = warp - 8;
         const int own = (ln / RPW) * 4 * RPW + pw * RPW + ln % RPW;  // this lane's row of the 128
         const int sub = pw * RPW + ln / CPR, ch = ln % CPR;          // its row (of 4 RPW) and chunk of a copy
-        constexpr int AHEAD = 2;      // tiles on their way behind the one that is waited for
+        constexpr int AHEAD = 3;      // tiles on their way; the oldest is handed on before another is waited for
         int t_issue = 0, t_done = 0;  // tiles whose copies are issued; tiles handed on
         // A tile has arrived: 16-bit tiles are operands already, codes are converted by the threads that copied them.
         auto hand_on = [&]() {
@@ -692,12 +700,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 pg = page_of(st + 1, r);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv) {
+                    if (t_issue - t_done == AHEAD) {
+                        cp_async_wait(AHEAD - 1);
+                        hand_on();
+                    }
                     const int t = t_issue++;
                     if constexpr (!I8) {
                         if (t >= NB && !many_wait(b_empty + 8 * (t % NB), ((t / NB) - 1) & 1, ok)) break;
                     } else {
-                        // the slot's last readers, of four units before, were done before the tile that was handed
-                        // on last could be (its buffer held the keys of three units before)
+                        // the slot's last readers, of four units before, were done before the tile three before this one
+                        // could be handed on (its buffer had held a tile of three units before)
                         reinterpret_cast<float*>(smem + F::oSC + ((t >> 1) & 3) * 1024 + kv * 512)[own] = kv ? sc[1] : sc[0];
                     }
                     const uint32_t dst = I8 ? sb + F::oSTG + (t % max(F::NSTG, 1)) * F::STG : sb + F::oKV + (t % NB) * TILE;
@@ -713,15 +725,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         cp16_or_zero(d, src + at, have);
                     }
                     cp_async_commit();
-                    if (t_issue - t_done > AHEAD) {
-                        cp_async_wait(AHEAD);
-                        hand_on();
-                    }
                 }
             }
         }
+        while (t_done < t_issue && ok) {
+            cp_async_wait(t_issue - t_done - 1);
+            hand_on();
+        }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        while (t_done < t_issue && ok) hand_on();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsLow));
         if (warp == 12) {
