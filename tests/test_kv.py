@@ -1,0 +1,52 @@
+"""CPU tests of the paged cache's host side: the structures that Python hands to the library have the
+header's layout, descriptions refuse what the kernels do not take, and calls without an engine fail
+with a status."""
+import ctypes
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import hayai_b200 as hb
+from hayai_b200 import _lib, kv
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("name,struct", [("hc_kv_cache", kv._Cache), ("hc_kv_batch", kv._Batch)])
+def test_structures_match_the_header(tmp_path, name, struct):
+    fields = [f for f, _ in struct._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include "hayai_cuda.h"\nint main(void) {\n'
+                   + "".join(f'printf("%zu ", offsetof({name}, {f}));\n' for f in fields)
+                   + f'printf("%zu\\n", sizeof({name}));\nreturn 0; }}\n')
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [getattr(struct, f).offset for f in fields] + [ctypes.sizeof(struct)]
+
+
+def test_rust_structures_name_the_same_fields():
+    text = open(os.path.join(ROOT, "integration", "hayai-cuda", "src", "ffi.rs")).read()
+    for name, struct in (("hc_kv_cache", kv._Cache), ("hc_kv_batch", kv._Batch)):
+        body = re.search(r"pub struct " + name + r" \{(.*?)\}", text, re.S).group(1)
+        assert [f.replace("ggml_type", "type") for f in re.findall(r"pub (\w+):", body)] == [f for f, _ in struct._fields_]
+
+
+def test_descriptions_need_device_tensors():
+    x = torch.zeros(2, 1, 16, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        hb.KvCache(x, x)
+    t = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        hb.KvBatch(t, t[0], t[0, :1], 1)
+
+
+def test_calls_without_an_engine_return_a_status():
+    L = _lib.lib()
+    assert L.hc_kv_append_dev(None, None, None, 0, None, 0, None, 0) == _lib.HC_ERR_INVALID
+    assert L.hc_kv_read_dev(None, None, None, 0, None, 0, None, 0) == _lib.HC_ERR_INVALID
+    assert L.hc_attn_paged_dev(None, None, None, 0, 1, None, 0, None, 0, None, 1.0, 1, 0, 0) == _lib.HC_ERR_INVALID
+    assert b"engine" in L.hc_last_error()
