@@ -278,22 +278,23 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         }
         cp_async_commit();
     };
-    // The tile's query rows as loaded, 4 values to a lane: all on their way at once, before the copies that
-    // wait for page numbers.
+    // Eight of the tile's query rows as loaded, 4 values to a lane: on their way at once, the first eight before
+    // the copies that wait for page numbers.  (All rows of a large tile in one straight run are so much code that a
+    // short call spends its time fetching instructions: 70 us for tiles of 32 rows.)
     using Raw = typename FewRaw<T>::type;
-    Raw raw[ROWS];
-    auto load_queries = [&]() {
+    Raw raw[8];
+    auto load_queries = [&](int r0) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
+        for (int r = 0; r < 8; ++r) {
             raw[r] = Raw{};
-            if (r < it.t.nr && ln < D / 4) {
-                const int row = it.t.r0 + r, tr = a.by_group(row);
+            if (r0 + r < it.t.nr && ln < D / 4) {
+                const int row = it.t.r0 + r0 + r, tr = a.by_group(row);
                 raw[r] = __ldg(reinterpret_cast<const Raw*>((const T*)a.q + (long long)(it.q.q0 + tr) * a.ldq +
                                                             (it.hk * a.group + row - tr * a.group) * D + 4 * ln));
             }
         }
     };
-    if (b0 < b1) load_queries();
+    if (b0 < b1) load_queries(0);
     look_up();
 #pragma unroll
     for (int i = 0; i < F::NS - 1; ++i) issue();
@@ -305,39 +306,44 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         if (lo >= hi) {
             if (it.u_item + tl.span >= b1) break;
             it.next(a, ROWS, ST);
-            load_queries();
+            load_queries(0);
             continue;
         }
         // ---- the query tile as B operands
+#pragma unroll 1
+        for (int n = 0; n < NT; ++n) {
+            if (n) load_queries(8 * n);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            float x[4];
-            FewRaw<T>::values(raw[r], x);
-            float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // not negative: order as bits
-            // the power of two of m, taken out of the row (none for 0, infinity and the smallest)
-            const uint32_t e = __float_as_uint(m) >> 23;
-            const bool norm = e >= 2 && e <= 252;
-            const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
-            const float up = norm ? __uint_as_float(e << 23) : 1.f;
+            for (int q = 0; q < 8; ++q) {
+                const int r = 8 * n + q;
+                float x[4];
+                FewRaw<T>::values(raw[q], x);
+                float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // not negative: order as bits
+                // the power of two of m, taken out of the row (none for 0, infinity and the smallest)
+                const uint32_t e = __float_as_uint(m) >> 23;
+                const bool norm = e >= 2 && e <= 252;
+                const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
+                const float up = norm ? __uint_as_float(e << 23) : 1.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] *= down;
-            if (ln == 0) rscale[r] = up * a.scale * 1.44269504f;
-            if constexpr (X::kBias) {
-                float sum = 0.f;
+                for (int i = 0; i < 4; ++i) x[i] *= down;
+                if (ln == 0) rscale[r] = up * a.scale * 1.44269504f;
+                if constexpr (X::kBias) {
+                    float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum += __half2float(__float2half_rn(x[i]));
-                sum = warp_sum(sum);
-                if (ln == 0) rscale[ROWS + r] = -1152.f * sum;
-            }
-            if (ln < D / 4) {
-                // d = 4 ln + i: 16-byte chunk of the cache row, its k step and the lane that holds it
-                const int ch = I8 ? ln >> 2 : ln >> 1, j = I8 ? 4 * (ch >> 2) + (ln & 3) : 2 * (ch >> 2) + (ln & 1);
-                uint8_t* dst = qf + (j * NT + (r >> 3)) * X::Q * 256 + ((r & 7) * 4 + (ch & 3)) * 8;
+                    for (int i = 0; i < 4; ++i) sum += __half2float(__float2half_rn(x[i]));
+                    sum = warp_sum(sum);
+                    if (ln == 0) rscale[ROWS + r] = -1152.f * sum;
+                }
+                if (ln < D / 4) {
+                    // d = 4 ln + i: 16-byte chunk of the cache row, its k step and the lane that holds it
+                    const int ch = I8 ? ln >> 2 : ln >> 1, j = I8 ? 4 * (ch >> 2) + (ln & 3) : 2 * (ch >> 2) + (ln & 1);
+                    uint8_t* dst = qf + (j * NT + n) * X::Q * 256 + (q * 4 + (ch & 3)) * 8;
 #pragma unroll
-                for (int s = 0; s < X::Q; ++s)
-                    *reinterpret_cast<uint2*>(dst + s * 256) =
-                        make_uint2(split_pair<X::kBf>(x[0], x[1]), split_pair<X::kBf>(x[2], x[3]));
+                    for (int s = 0; s < X::Q; ++s)
+                        *reinterpret_cast<uint2*>(dst + s * 256) =
+                            make_uint2(split_pair<X::kBf>(x[0], x[1]), split_pair<X::kBf>(x[2], x[3]));
+                }
             }
         }
         __syncwarp();
@@ -735,7 +741,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         }
         if (done) break;
         it.next(a, ROWS, ST);
-        load_queries();
+        load_queries(0);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();

@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     float y[8][4];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) y[k][0] = y[k][1] = y[k][2] = y[k][3] = 0.f;
-#pragma unroll 1
+#pragma unroll 2
                     for (int i = 0; i < n; ++i) {
                         float4 o[8];
 #pragma unroll
