@@ -14,11 +14,11 @@
 // of tokens come from two rows by PRMT, with no transposed copy.  S^T's accumulators become P^T's
 // operand with one MOVMATRIX per 8 tokens.
 //
-// Formats.  8-bit codes are exact in f16 and in bf16.  For 16-bit results they go in as f16 1152 +
-// code (one PRMT and no subtraction: bits 0x6400 + code + 128), and the product's accumulator starts
-// at -1152 sum q or -1152 sum p of the operand as rounded, so that the codes' own product is left
-// (the larger sums cost about 2^-24 * 1152 / 40 of a result's size).  A token's K scale multiplies
-// its score and its V scale its weights; a unit's weights of a row are then brought to at most 1 by a
+// Formats.  8-bit codes are exact in f16 and in bf16.  For 16-bit results V's go in as f16 1152 + code
+// (no subtraction: bits 0x6400 + code + 128), and the product's accumulator starts at -1152 sum p of
+// the weights as rounded, so that the codes' own product is left (the larger sums cost about 2^-24 *
+// 1152 / 40 of a result's size; K's codes are taken as they are, as the lse is f32 whatever the
+// results are).  A token's K scale multiplies its score and its V scale its weights; a unit's weights of a row are then brought to at most 1 by a
 // power of two, which multiplies the unit's product, so that f16 holds them whatever the scales are
 // (what is under 2^-25 of the unit's largest is lost).  For f32 results the codes are taken as they
 // are, and the weights times scales as bf16 terms, whose range needs no such care.  Query rows are
@@ -37,7 +37,7 @@
 // workspace, where after one barrier the block joins its warps' pieces, and the last block of a
 // tile's row the blocks'.
 // (Tiles shared by all warps of a block, with a barrier and a joining at each tile's end, took
-// 160 us where this takes 9x us: 64 sequences of 300 to 12000 tokens, 64 heads on 8.)
+// 160 us where this takes 100 us: 64 sequences of 300 to 12000 tokens, 64 heads on 8.)
 #include <math.h>
 
 #include "attn_rows.cuh"
@@ -50,7 +50,7 @@ struct FewTerms {
     static constexpr int Q = sizeof(T) == 4 ? (kBf ? 3 : 2) : (kBf && __is_same(T, __half)) ? 2 : 1;
     static constexpr bool pBf = kBf || (sizeof(C) == 1 && sizeof(T) == 4);       // bf16 products for the result
     static constexpr int P = sizeof(T) == 4 ? (pBf ? 3 : 2) : (pBf && __is_same(T, __half)) ? 2 : 1;
-    static constexpr bool kBias = sizeof(C) == 1 && sizeof(T) == 2;  // codes as 1152 + code
+    static constexpr bool kBias = sizeof(C) == 1 && sizeof(T) == 2;  // V's codes as 1152 + code
 };
 
 template <class T, class C, int D, int NT>
@@ -62,7 +62,7 @@ struct FewCfg {
     static constexpr int W = NT == 1 && FewTerms<T, C>::Q == 1 ? 12 : 8;  // warps of a block
     static constexpr int NS = CPR == 4 ? 4 : 2;                   // stages of a warp's ring
     static constexpr int QB = D / 16 * NT * FewTerms<T, C>::Q * 256;  // a query tile as B operands
-    static constexpr int WB = NS * SB + QB + 64 * NT;  // bytes of a warp: ring, queries, rows' scales and biases
+    static constexpr int WB = NS * SB + QB + 32 * NT;  // bytes of a warp: ring, queries, rows' scales
     static constexpr int PS = 8 * NT * (D + 2);  // floats of a partial result: rows of D values, then (m, l) of each
 };
 
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
     const int w = threadIdx.x >> 5, ln = lane_id(), g = ln >> 2, t4 = ln & 3;
     const uint32_t ring = smem_addr(smem) + w * F::WB;
     uint8_t* const qf = smem + w * F::WB + F::NS * F::SB;
-    float* const rscale = reinterpret_cast<float*>(qf + F::QB);  // [ROWS], and [ROWS] of -1152 sum q
+    float* const rscale = reinterpret_cast<float*>(qf + F::QB);  // [ROWS]
 
     __shared__ float* place_s[W][2];  // where a warp's last (0) and first (1) piece of a shared tile is
 
@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         cp_async_commit();
     };
     // Eight of the tile's query rows as loaded, 4 values to a lane: on their way at once, the first eight before
-    // the copies that wait for page numbers.  (All rows of a large tile in one straight run are so much code that a
-    // short call spends its time fetching instructions: 70 us for tiles of 32 rows.)
+    // the copies that wait for page numbers.  (All rows of a tile in one straight run are so much code that a short
+    // call spends its time fetching instructions.)
     using Raw = typename FewRaw<T>::type;
     Raw raw[8];
     auto load_queries = [&](int r0) {
@@ -328,13 +328,6 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] *= down;
                 if (ln == 0) rscale[r] = up * a.scale * 1.44269504f;
-                if constexpr (X::kBias) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum += __half2float(__float2half_rn(x[i]));
-                    sum = warp_sum(sum);
-                    if (ln == 0) rscale[ROWS + r] = -1152.f * sum;
-                }
                 if (ln < D / 4) {
                     // d = 4 ln + i: 16-byte chunk of the cache row, its k step and the lane that holds it
                     const int ch = I8 ? ln >> 2 : ln >> 1, j = I8 ? 4 * (ch >> 2) + (ln & 3) : 2 * (ch >> 2) + (ln & 1);
@@ -347,7 +340,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
             }
         }
         __syncwarp();
-        float m[NT][2], l[NT][2], o[KS][NT][4], rs[NT][2], qb[NT][2];
+        float m[NT][2], l[NT][2], o[KS][NT][4], rs[NT][2];
         int lim[NT][2], wlo[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -357,7 +350,6 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                 m[n][e] = -INFINITY;
                 l[n][e] = 0.f;
                 rs[n][e] = rscale[r];
-                qb[n][e] = X::kBias ? rscale[ROWS + r] : 0.f;
                 const int pos = it.q.len - (it.q.q1 - it.q.q0) + a.by_group(tl.r0 + r);
                 lim[n][e] = r >= tl.nr ? -1 : a.causal ? pos : it.q.len - 1;
                 wlo[n][e] = a.window ? pos - a.window + 1 : 0;
@@ -398,9 +390,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                             A[i][1] = prmt(fc, 0x64646464u, 0x4140u);
                             A[i][2] = prmt(fa, 0x64646464u, 0x4342u);
                             A[i][3] = prmt(fc, 0x64646464u, 0x4342u);
-                            if constexpr (!X::kBias)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) A[i][e] = hsub2_u32(A[i][e], 0x64806480u);
+                            for (int e = 0; e < 4; ++e) A[i][e] = hsub2_u32(A[i][e], 0x64806480u);
                         } else {
                             A[i][0] = wa[2 * jj];
                             A[i][1] = wc[2 * jj];
@@ -417,7 +408,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 #pragma unroll
                             for (int i = 0; i < MT; ++i) {
                                 if (j == 0 && q == 0)
-                                    mma_from<X::kBf>(s[i][n], A[i], b.x, b.y, qb[n][0], qb[n][1]);
+                                    mma_from<X::kBf>(s[i][n], A[i], b.x, b.y, 0.f, 0.f);
                                 else
                                     mma_any<X::kBf>(s[i][n], A[i], b.x, b.y);
                             }
@@ -815,13 +806,10 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// Tiles of 8, 16 or 32 rows, by the batch's largest sequence; of more terms (f32 rows) at most 16,
-// whose operands fill the shared memory.
+// Tiles of 8 or 16 rows, by the batch's largest sequence.  (Tiles of 32 need more registers than a thread has.)
 template <class T, class C, int D>
 cudaError_t by_rows(const AttnArgs& a, int blocks, cudaStream_t s) {
     if (a.max_rows <= 8) return launch<T, C, D, 1>(a, blocks, s);
-    if constexpr (FewTerms<T, C>::Q == 1)
-        if (a.max_rows > 16) return launch<T, C, D, 4>(a, blocks, s);
     return launch<T, C, D, 2>(a, blocks, s);
 }
 

@@ -68,7 +68,7 @@ struct AttnArgs {
 };
 
 // Partial results of the kernel for few rows: bytes for each block.
-constexpr size_t kFewPartBytes = 2 * 9 * 32 * (128 + 2) * 4;
+constexpr size_t kFewPartBytes = 2 * 13 * 16 * (128 + 2) * 4;
 constexpr size_t kManyPartBytes = 2 * 256 * (128 + 2) * 4;
 constexpr size_t kAttnPartBytes = kFewPartBytes > kManyPartBytes ? kFewPartBytes : kManyPartBytes;
 

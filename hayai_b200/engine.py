@@ -421,15 +421,21 @@ class CudaEngine:
         return rw
 
     # ---------------------------------------------------------------- paged key/value cache
+    def _kv_here(self, cache, batch) -> None:
+        if cache.index != self.device or batch.index != self.device:
+            raise ValueError(f"the cache and the batch must be on the engine's device {self.device}")
+
     def kv_append_dev(self, cache, batch, k, v) -> None:
         """Store the new tokens' rows k, v [n_tok][n_heads][head_dim] in the cache's pages (KvCache,
         KvBatch); an 8-bit cache gets codes and one scale per row."""
+        self._kv_here(cache, batch)
         rc = self._kv_append(self.handle, cache.ref, batch.ref, *cache.pair(batch, k, v))
         if rc:
             _check(rc)
 
     def kv_read_dev(self, cache, batch, k, v) -> None:
         """Gather the same rows back out of the cache into k, v, as the values they stand for."""
+        self._kv_here(cache, batch)
         rc = self._kv_read(self.handle, cache.ref, batch.ref, *cache.pair(batch, k, v))
         if rc:
             _check(rc)
@@ -440,6 +446,7 @@ class CudaEngine:
         out (same shape and type).  scale: 1 / sqrt(head_dim) unless given.  causal: a token sees the
         positions up to its own, of which window > 0 leaves the last ``window`` and the first
         ``sink``.  lse: None, or a float32 [n_tok][n_heads] that receives the scores' log-sum-exp."""
+        self._kv_here(cache, batch)
         heads = q.shape[1] if q.dim() == 3 else 0
         t, ldq = cache.rows(batch, q, heads, "q")
         to, ldo = cache.rows(batch, out, heads, "out")

@@ -111,7 +111,7 @@ class KvBatch:
         _need(kv_len.shape[0] == n_seq and q_start.shape[0] == n_seq + 1, "kv_len must hold n_seq and q_start n_seq + 1")
         _need(n_tok >= 0 and max_new >= 0, "n_tok and max_new must not be negative")
         self._keep = (page_table, q_start, kv_len)
-        self.n_tok = int(n_tok)
+        self.n_tok, self.index = int(n_tok), page_table.get_device()
         stride = page_table.stride(0) if n_seq > 1 else max_pages
         _need(stride >= max_pages, "page_table rows overlap")
         self.struct = _Batch(n_seq, n_tok, max_new, max_pages, page_table.data_ptr(), stride, q_start.data_ptr(),

@@ -50,3 +50,17 @@ def test_calls_without_an_engine_return_a_status():
     assert L.hc_kv_read_dev(None, None, None, 0, None, 0, None, 0) == _lib.HC_ERR_INVALID
     assert L.hc_attn_paged_dev(None, None, None, 0, 1, None, 0, None, 0, None, 1.0, 1, 0, 0) == _lib.HC_ERR_INVALID
     assert b"engine" in L.hc_last_error()
+
+
+def test_a_cache_of_another_device_is_refused():
+    """The kernels run on the engine's GPU: descriptions of another one never reach them."""
+    class Elsewhere:
+        index = 1
+
+    class Here:
+        index = device = 0
+
+    for cache, batch in ((Elsewhere, Here), (Here, Elsewhere)):
+        with pytest.raises(ValueError, match="device"):
+            hb.CudaEngine._kv_here(Here, cache, batch)
+    hb.CudaEngine._kv_here(Here, Here, Here)
