@@ -36,6 +36,8 @@
 // of its first and last tile's pieces it leaves the partial (m, l, O) in shared memory or in the
 // workspace, where after one barrier the block joins its warps' pieces, and the last block of a
 // tile's row the blocks'.
+// Measured: 64 sequences of 300 to 12000 8-bit tokens 100 us (4.2 TB/s, 66 % of the copy rate), one of
+// 131071 f16 tokens 57 us (4.7 TB/s, 73 %), one of 1001 8-bit tokens 11.5 us in a graph.
 // (Tiles shared by all warps of a block, with a barrier and a joining at each tile's end, took
 // 160 us where this takes 100 us: 64 sequences of 300 to 12000 tokens, 64 heads on 8.)
 #include <math.h>
