@@ -102,7 +102,6 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The wait for loads still in flight, tied to their registers so that no use moves before it.
 __device__ __forceinline__ void tc_wait_ld32(float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -628,7 +627,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int e = e0 + 256 * k, r = e / (D / 4);
-                        if (e < sh.nr * (D / 4)) attn_store<T, 4>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[256 + r]);
+                        if (e < sh.nr * (D / 4)) attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[256 + r]);
                     }
                 }
             }

@@ -228,28 +228,23 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
-// N (4 or 2) adjacent values of the weighted sum of row `row` of an item's kv head, over l.
-template <class T, int N>
-__device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[N],
+// Four adjacent values of the weighted sum of row `row` of an item's kv head, over l.
+template <class T>
+__device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[4],
                                            float l) {
     const bool none = l == 0.f;  // saw nothing (a sum that is not a number is kept)
     const float k = none ? 0.f : 1.f / l;
     const int t = a.by_group(row);
     T* out = (T*)a.out + (long long)(q0 + t) * a.ldo + (hk * a.group + row - t * a.group) * D + d;
-    float z[N];
+    float z[4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = none ? 0.f : y[i] * k;
-    uint32_t u[N / 2];
-    if constexpr (sizeof(T) == 4) {
-        if constexpr (N == 4) *reinterpret_cast<float4*>(out) = make_float4(z[0], z[1], z[2], z[3]);
-        else *reinterpret_cast<float2*>(out) = make_float2(z[0], z[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i)
-            u[i] = __is_same(T, __half) ? pack_h2(z[2 * i], z[2 * i + 1]) : pack_b2(z[2 * i], z[2 * i + 1]);
-        if constexpr (N == 4) *reinterpret_cast<uint2*>(out) = make_uint2(u[0], u[1]);
-        else *reinterpret_cast<uint32_t*>(out) = u[0];
-    }
+    for (int i = 0; i < 4; ++i) z[i] = none ? 0.f : y[i] * k;
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(out) = make_float4(z[0], z[1], z[2], z[3]);
+    else if constexpr (__is_same(T, __half))
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2(z[0], z[1]), pack_h2(z[2], z[3]));
+    else
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_b2(z[0], z[1]), pack_b2(z[2], z[3]));
 }
 __device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l) {
     const int t = a.by_group(row);
