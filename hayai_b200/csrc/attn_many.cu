@@ -371,9 +371,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                             odd = *(volatile int*)&flag[checks % 3];
                             ++checks;
                         }
-                        if (rt == 0) misc[2 + half] = (int)odd;  // read by the products' warp after the arrivals
                     }
                     if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
+                    // read by the products' warp after the arrivals; it has read the last unit's before it issued this S
+                    if (!I8 && rt == 0) misc[2 + half] = (int)odd;
                     ph_s ^= 1;
                     tc_fence_after();
                     // the queries and their factors came before this unit's products; their own barrier may be two

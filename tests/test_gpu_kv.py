@@ -328,6 +328,30 @@ def test_not_finite_where_masked(engine, lens, cache, dtype):
     assert out[n - 3:].isnan().any(-1).all()
 
 
+@pytest.mark.parametrize("window", [70, 300])
+@pytest.mark.parametrize("at", [610, 650, 767, 768])
+@pytest.mark.parametrize("cache,dtype", [("f16", "f16"), ("bf16", "bf16"), ("i8", "bf16")])
+def test_not_finite_outside_a_window(engine, cache, dtype, at, window):
+    """One value that is not finite among units that rows see in part, one after the other: the rows
+    whose window does not reach it are as without it."""
+    s = Setup([(300, 900)], 2, 128, 16, cache)
+    q = s.q(4, dtype)
+    ref, _, amp = s.attention(q, window=window)
+    p, r = int(s.table[0, at // 16]), at % 16
+    if cache == "i8":
+        s.scale[1][p, :, r] = math.inf
+    else:
+        s.pool[1][p, :, r, 5] = math.inf
+    out = torch.empty_like(q)
+    for _ in range(3):
+        engine.attn_paged_dev(s.cache, s.batch, q, out, window=window)
+        engine.sync()
+        pos = torch.arange(600, 900, device=DEV)
+        sees = (pos >= at) & (pos - at < window)
+        assert ((out.double() - ref).abs()[~sees] <= (2.0 ** -8 * (amp + ref.abs()))[~sees]).all()
+        assert not torch.isfinite(out[sees][..., 5]).any()
+
+
 @pytest.mark.parametrize("order", ["prhd", "both"])
 @pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "bf16")])
 def test_orders_of_the_pool(engine, order, cache, dtype):
