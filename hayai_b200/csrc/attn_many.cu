@@ -35,6 +35,7 @@
 
 #include <type_traits>
 
+#include "attn_phases.h"
 #include "attn_rows.cuh"
 #include "tc5.cuh"
 
@@ -47,7 +48,7 @@ struct ManyCfg {
     static constexpr int ES = sizeof(C);
     static constexpr bool I8 = ES == 1, BF = ES == 2 && !__is_same(C, __half);
     static constexpr int TILE = 128 * D * 2;                 // an operand tile: 128 rows of D 16-bit values
-    static constexpr int NB = I8 ? 3 : D == 64 ? 6 : 5;      // ring of key and value tiles
+    static constexpr int NB = many_ring(I8, D);              // ring of key and value tiles
     static constexpr int CPR = D * ES / 16;                  // 16-byte chunks of a cache row
     static constexpr int STG = I8 ? 128 * D : 0, NSTG = I8 ? 3 : 0;  // staging ring of tiles of codes
     static constexpr int oQ = 0, oKV = 2 * TILE, oSTG = oKV + NB * TILE, oSC = oSTG + NSTG * STG;
@@ -345,8 +346,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     if constexpr (!I8) {
                         // A value that is not finite, in a unit that some row does not see whole: 0 * infinity must not
                         // reach a masked row, so that the unit's product is then done by the rows' threads (rare).  The
-                        // look at V comes before the wait for the scores.
+                        // look at V comes before the wait for the scores where that is sound (attn_phases.h); elsewhere
+                        // the scores are waited for here, and found there again below: this half has to give its weights
+                        // before their barrier goes on.
                         if (!full) {
+                            if (!many_early_look(st, lo) && !many_wait(b_s + 8 * half, ph_s, ok)) break;
                             const int vt = kvt + 2 * (st - lo) + 1;
                             if (!many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok)) break;
                             vtile = smem + F::oKV + (vt % NB) * TILE;

@@ -485,3 +485,30 @@ def test_refusals(engine):
             f()
         assert e.value.code == code, str(e.value)
     engine.sync()
+
+
+@pytest.mark.parametrize("cache,dtype", [("f16", "f16"), ("bf16", "bf16"), ("f16", "bf16")])
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 1), (128, 3)])
+def test_not_finite_in_a_tile_after_short_ones(engine, cache, dtype, dim, group):
+    """Tiles of at most 128 rows and several units, which half of a block's row threads pass over, and
+    next to them tiles whose second half has rows that must not see a value that is not finite."""
+    lens = [(260 // group + 13 * i % 110 // group, 520 + 37 * i % 480) for i in range(40)]
+    s = Setup(lens, 4, dim, 16, cache)
+    q = s.q(4 * group, dtype)
+    ref, _, amp = s.attention(q)
+    sees = torch.zeros(s.rows, dtype=torch.bool, device=DEV)
+    done = 0
+    for i, (n, k) in enumerate(lens):
+        at = k - n + 250 // group  # its row is the 250th of the sequence's first tile, or near it
+        s.pool[1][int(s.table[i, at // 16]), :, at % 16, 7] = math.inf
+        sees[done + at - (k - n):done + n] = True
+        done += n
+    first = None
+    for _ in range(4):
+        out = torch.full_like(q, 5.0)
+        engine.attn_paged_dev(s.cache, s.batch, q, out)
+        engine.sync()
+        assert ((out.double() - ref).abs()[~sees] <= (2.0 ** -8 * (amp + ref.abs()))[~sees]).all()
+        assert not torch.isfinite(out[sees][..., 7]).any()
+        assert first is None or torch.equal(out.view(torch.int16), first)
+        first = out.view(torch.int16).clone()

@@ -64,3 +64,22 @@ def test_a_cache_of_another_device_is_refused():
         with pytest.raises(ValueError, match="device"):
             hb.CudaEngine._kv_here(Here, cache, batch)
     hb.CudaEngine._kv_here(Here, Here, Here)
+
+
+def replay(tmp_path, *flags):
+    exe = tmp_path / "replay"
+    subprocess.run(["g++", "-O2", "-std=c++17", *flags, "-I", os.path.join(ROOT, "hayai_b200", "csrc"),
+                    os.path.join(ROOT, "tests", "attn_phases.cpp"), "-o", str(exe)], check=True)
+    return [int(x) for x in subprocess.run([str(exe), "2000", "7"], capture_output=True, text=True, check=True).stdout.split()]
+
+
+def test_waits_of_the_prompt_kernel_are_sound(tmp_path):
+    """Barriers are waited for by parity: in replays of the kernel's roles over random lists of segments no
+    wait is more than one phase away from what it waits for, and none waits for ever."""
+    assert replay(tmp_path) == [0, 0]
+
+
+def test_the_replay_sees_a_wait_that_is_not_sound(tmp_path):
+    """Looking at V ahead of the scores in a segment's first unit is found out."""
+    unsound, stuck = replay(tmp_path, "-DEARLY=1")
+    assert unsound > 0 and stuck == 0
