@@ -29,7 +29,8 @@
 //
 // Formats: products of f16 (f16 and 8-bit caches) or bf16.  8-bit codes are exact in f16; a K scale
 // multiplies its column of S, a V scale its column of P, and m follows the largest score + log2 of the
-// unit's largest V scale, so that P times scale stays under 2^8 whatever the scales are.  Rows of
+// unit's largest V scale, so that P times scale stays under 2^8 whatever the scales are; scales under
+// 2^-80, zero above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of
 // bf16 on f16 products are scaled by a power of two to have their largest element in [1, 2).
 #include <math.h>
 
@@ -399,7 +400,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         float top = fmaxf(fmaxf(size(v.x), size(v.y)), fmaxf(size(v.z), size(v.w)));
 #pragma unroll
                         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        ev = (float)((int)(__float_as_uint(top) >> 23) - 126);  // log2 of a power of two over it
+                        // log2 of a power of two over it, but of scales near zero no less than -80: a weight is then
+                        // up to 2^88, and the sum of 2^30 of them finite
+                        ev = (float)max((int)(__float_as_uint(top) >> 23) - 126, -80);
                     }
                     const int vc = vis.c - v0, vb = vis.b - v0, va = vis.a - v0;
                     // 32 scores from TMEM: times their K scales, masked

@@ -512,3 +512,34 @@ def test_not_finite_in_a_tile_after_short_ones(engine, cache, dtype, dim, group)
         assert not torch.isfinite(out[sees][..., 7]).any()
         assert first is None or torch.equal(out.view(torch.int16), first)
         first = out.view(torch.int16).clone()
+
+
+def places(s, pos, i=0):
+    return s.table[i].long()[pos // s.page], pos % s.page
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,zero", [((150, 700), (0, 128)), ((150, 700), (128, 256)), ((150, 700), (0, 300)), ((150, 700), (0, 700)),
+                                       ((40, 9001), (0, 4000)), ((40, 9001), (0, 9001)), ((150, 20000), (3000, 16000))])
+def test_values_of_zero(engine, dtype, lens, zero):
+    """Rows of zeros have scale 0: whole units of them, a block's share, a split tile, all values."""
+    s = Setup([lens], 2, 128, 16, "i8")
+    pos = torch.arange(*zero, device=DEV)
+    p, r = places(s, pos)
+    s.pool[1][p, :, r] = 0
+    s.scale[1][p, :, r] = 0.0
+    check(engine, s, 8, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", [(0.0, 1e-38, 1e-20, 1.0), (1e-38, 1e-38, 0.0, 1e-38), (0.0, 1e-35, 1e-30, 1e-38)])
+def test_values_with_scales_near_zero(engine, dtype, sizes):
+    """Scales from zero to f32's smallest, mixed in a unit; what they leave is under the bound's floor or
+    beside ordinary values."""
+    for lens in ((150, 700), (40, 9001)):
+        s = Setup([lens], 2, 128, 16, "i8")
+        for i, size in enumerate(sizes):
+            pos = torch.arange(i, lens[1], len(sizes), device=DEV)
+            p, r = places(s, pos)
+            s.scale[1][p, :, r] *= size
+        check(engine, s, 8, dtype)
