@@ -28,9 +28,11 @@
 // are not all under the products.
 //
 // Formats: products of f16 (f16 and 8-bit caches) or bf16.  8-bit codes are exact in f16; a K scale
-// multiplies its column of S, a V scale its column of P, and m follows the largest score + log2 of the
-// unit's largest V scale, so that P times scale stays under 2^8 whatever the scales are; scales under
-// 2^-80, zero above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of
+// multiplies its column of S, a V scale its column of P, and m follows the largest score + log2 of its V
+// scale, so that P times scale stays under 2^8 whatever the scales are, and near it for the largest.
+// Where a unit's scales lie within 2^6 of each other the largest stands for all; elsewhere each
+// position counts with its own, as a large one may have no weight or be masked.  Scales under 2^-80, zero
+// above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of
 // bf16 on f16 products are scaled by a power of two to have their largest element in [1, 2).
 #include <math.h>
 
@@ -385,7 +387,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     // the queries and their factors came before this unit's products; their own barrier may be two
                     // segments further by now, so it cannot be waited for here
                     if (st == lo) rs = rsc[(n & 1) * 256 + r];
+                    auto size = [](float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; };  // what is not finite has none
+                    // log2 of a power of two over a size (its bits), but near zero no less than -80: a weight is then up to
+                    // 2^88, and the sum of 2^30 of them finite
+                    auto size_log2 = [](uint32_t bits) { return max((int)(bits >> 23) - 126, -80); };
                     float ev = 0.f;
+                    bool mixed = false;
                     const float4 *ksc = nullptr, *vsc = nullptr;
                     if constexpr (I8) {
                         // V's tile is not given back before this unit's weights, so its barrier is at its phase (K's
@@ -396,13 +403,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         ksc = reinterpret_cast<const float4*>(sc);
                         vsc = reinterpret_cast<const float4*>(sc + 512);
                         const float4 v = vsc[ln];
-                        auto size = [](float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; };  // what is not finite has none
-                        float top = fmaxf(fmaxf(size(v.x), size(v.y)), fmaxf(size(v.z), size(v.w)));
+                        const float vs[4] = {v.x, v.y, v.z, v.w};
+                        uint32_t most = 0, least = 0x7f7fffffu;
 #pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        // log2 of a power of two over it, but of scales near zero no less than -80: a weight is then
-                        // up to 2^88, and the sum of 2^30 of them finite
-                        ev = (float)max((int)(__float_as_uint(top) >> 23) - 126, -80);
+                        for (int i = 0; i < 4; ++i) {
+                            if (v0 + 4 * ln + i >= lastr.c) continue;  // no row of this half sees it
+                            const uint32_t b = __float_as_uint(size(vs[i]));
+                            most = max(most, b);
+                            least = min(least, b);
+                        }
+                        const int top = size_log2(__reduce_max_sync(0xffffffffu, most));
+                        ev = (float)top;
+                        mixed = size_log2(__reduce_min_sync(0xffffffffu, least)) < top - 6;
                     }
                     const int vc = vis.c - v0, vb = vis.b - v0, va = vis.a - v0;
                     // 32 scores from TMEM: times their K scales, masked
@@ -454,7 +466,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         }
                     }
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const float cand = top == -INFINITY ? top : top * rs + ev;
+                    float cand = top == -INFINITY ? top : top * rs + ev;
+                    if constexpr (I8) {
+                        if (mixed) {  // rare: the largest score + log2 of its own scale
+                            cand = -INFINITY;
+#pragma unroll 1
+                            for (int k = 0; k < 4; ++k) {
+                                float* s = sa[1];
+                                tc_ld32(tS + 32 * k, s);
+                                tc_wait_ld32(s);
+                                scores(k, s);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float x = reinterpret_cast<const float*>(vsc)[32 * k + i];
+                                    const int e = size_log2(__float_as_uint(size(x)));
+                                    cand = fmaxf(cand, s[i] == -INFINITY ? s[i] : fmaf(s[i], rs, (float)e));
+                                }
+                            }
+                        }
+                    }
                     if (__any_sync(0xffffffffu, cand > m + 8.f)) {
                         const float mn = fmaxf(m, cand), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                         m = mn;

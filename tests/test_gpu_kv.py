@@ -543,3 +543,46 @@ def test_values_with_scales_near_zero(engine, dtype, sizes):
             p, r = places(s, pos)
             s.scale[1][p, :, r] *= size
         check(engine, s, 8, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("large", [2.0 ** 20, 2.0 ** 30])
+@pytest.mark.parametrize("where", ["seen", "masked"])
+def test_large_values_with_no_weight(engine, dtype, large, where):
+    """A token that has nearly all weight beside one of a far larger value that has next to none of it (a weight
+    of e^-56); and one of a far larger value that all rows but the last are masked from."""
+    s = Setup([(150, 700)], 2, 128, 16, "i8")
+    q = s.q(8, dtype)
+    q[..., 0] = 8.0
+    for at, key in ((600, 40.0), (603, -40.0)) if where == "seen" else ((699, -40.0),):
+        p, r = int(s.table[0, at // 16]), at % 16
+        s.pool[0][p, :, r] = 0
+        s.pool[0][p, :, r, 0] = 127 if key > 0 else -127
+        s.scale[0][p, :, r] = abs(key) / 127
+        if key < 0:
+            s.scale[1][p, :, r] *= large
+    check(engine, s, 8, dtype, q=q)
+
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_strong_token_without_a_value(engine, dtype):
+    """A first token with 2^30 times the weight of any other and a value of zero: the results are the
+    others' (bound by their own sizes, as the zero adds nothing)."""
+    s = Setup([(150, 700)], 2, 128, 16, "i8")
+    p = int(s.table[0, 0])
+    s.pool[0][p, :, 0] = 0
+    s.pool[0][p, :, 0, 0] = 127
+    s.scale[0][p, :, 0] = 30 * math.log(2.0) * 128 ** 0.5 / 8.0 / 127
+    s.pool[1][p, :, 0], s.scale[1][p, :, 0] = 0, 0.0
+    q = s.q(8, dtype) * 0.1
+    q[..., 0] = 8.0
+    out = torch.empty_like(q)
+    # results near 2^-30 * 700: under f16's range, so the others' values are made as large
+    pos = torch.arange(1, 700, device=DEV)
+    pp, r = places(s, pos)
+    s.scale[1][pp, :, r] *= 2.0 ** 24
+    engine.attn_paged_dev(s.cache, s.batch, q, out)
+    engine.sync()
+    ref, _, amp = s.attention(q)
+    assert ((out.double() - ref).abs() <= 2.0 ** -8 * (amp + ref.abs())).all()
