@@ -18,10 +18,12 @@
 // (no subtraction: bits 0x6400 + code + 128), and the product's accumulator starts at -1152 sum p of
 // the weights as rounded, so that the codes' own product is left (the larger sums cost about 2^-24 *
 // 1152 / 40 of a result's size; K's codes are taken as they are, as the lse is f32 whatever the
-// results are).  A token's K scale multiplies its score and its V scale its weights; a unit's weights of a row are then brought to at most 1 by a
-// power of two, which multiplies the unit's product, so that f16 holds them whatever the scales are
-// (what is under 2^-25 of the unit's largest is lost).  For f32 results the codes are taken as they
-// are, and the weights times scales as bf16 terms, whose range needs no such care.  Query rows are
+// results are).  A token's K scale multiplies its score and its V scale its weights.  For f32 results the
+// codes are taken as they are, and the weights times scales as bf16 terms.  Where weights go in as f16, a
+// unit's weights of a row are first brought to a fixed size by a power of two, which multiplies the unit's
+// product: f16 then holds them however far they are under the row's maximum and whatever the scales are
+// (8-bit: to at most 1, and what is under 2^-25 of the unit's largest is lost; 16-bit: to 2^15, and 2^-40);
+// bf16 terms need no such care.  Query rows are
 // scaled by a power of two to have their largest element in [1, 2) and rounded to the products'
 // type: f16 and bf16 rows are exact or keep 11 bits in f16; f32 rows are split into 2 f16 terms (22
 // bits) or 3 bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11 bits of 16).  Weights are
@@ -53,6 +55,8 @@ struct FewTerms {
     static constexpr bool pBf = kBf || (sizeof(C) == 1 && sizeof(T) == 4);       // bf16 products for the result
     static constexpr int P = sizeof(T) == 4 ? (pBf ? 3 : 2) : (pBf && __is_same(T, __half)) ? 2 : 1;
     static constexpr bool kBias = sizeof(C) == 1 && sizeof(T) == 2;  // V's codes as 1152 + code
+    static constexpr bool kNorm = !pBf;                          // f16 products for the result: weights brought to f16's range
+    static constexpr int kTop = kBias ? 1 : -14;                 // a unit's largest weight is divided by 2^kTop times its power of two
 };
 
 template <class T, class C, int D, int NT>
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
             }
             // ---- weights, and P^T as B operands
             uint32_t pb[MT][NT][X::P][2];
-            float unit[NT][2];  // 8-bit: what the unit's weights of a row are divided by
+            float unit[NT][2];  // f16: what the unit's weights of a row are divided by
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
@@ -513,16 +517,17 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                             if (s[i][n][e] == -INFINITY) p[i][e] = 0.f;
                 }
                 unit[n][0] = unit[n][1] = 1.f;
-                if constexpr (X::kBias) {
+                if constexpr (X::kNorm) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float x = fmaxf(fmaxf(fabsf(p[0][e]), fabsf(p[0][e + 2])),
                                         fmaxf(fabsf(p[MT - 1][e]), fabsf(p[MT - 1][e + 2])));
 #pragma unroll
                         for (int q = 4; q < 32; q <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, q));
-                        const uint32_t b = min(max(__float_as_uint(x) & 0x7f800000u, 0x01000000u), 0x7e000000u);
-                        unit[n][e] = __uint_as_float(b + 0x00800000u);
-                        const float inv = __uint_as_float(0x7e800000u - b);
+                        // exponents that leave the power and its reciprocal normal numbers
+                        const uint32_t b = min(max(__float_as_uint(x) >> 23, X::kBias ? 2u : 15u), 252u);
+                        unit[n][e] = __uint_as_float((b + X::kTop) << 23);
+                        const float inv = __uint_as_float((254 - X::kTop - b) << 23);
 #pragma unroll
                         for (int i = 0; i < MT; ++i) {
                             p[i][e] *= inv;
@@ -581,7 +586,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                             }
                     }
             } else {
-                constexpr bool EXACT = sizeof(T) == 4;
+                constexpr bool OWN = sizeof(T) == 4 || X::kNorm;  // a unit's products are added to zero, then to the sum
                 if constexpr (I8) {
                     uint4 vw[MT][4];  // 16 (D = 128) or 8 (D = 64) adjacent values of four tokens
 #pragma unroll
@@ -668,7 +673,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) z[n][e] = EXACT ? 0.f : o[d][n][e];
+                                for (int e = 0; e < 4; ++e) z[n][e] = OWN ? 0.f : o[d][n][e];
 #pragma unroll
                             for (int i = 0; i < MT; ++i) {
                                 uint32_t A[4];
@@ -688,7 +693,10 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) o[d][n][e] = EXACT ? o[d][n][e] + z[n][e] : z[n][e];
+                                for (int e = 0; e < 4; ++e)
+                                    o[d][n][e] = X::kNorm ? fmaf(z[n][e], unit[n][e & 1], o[d][n][e])
+                                                 : OWN    ? o[d][n][e] + z[n][e]
+                                                          : z[n][e];
                         }
                     }
                 }

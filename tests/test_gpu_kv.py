@@ -564,7 +564,6 @@ def test_large_values_with_no_weight(engine, dtype, large, where):
     check(engine, s, 8, dtype, q=q)
 
 
-
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_a_strong_token_without_a_value(engine, dtype):
     """A first token with 2^30 times the weight of any other and a value of zero: the results are the
@@ -586,3 +585,62 @@ def test_a_strong_token_without_a_value(engine, dtype):
     engine.sync()
     ref, _, amp = s.attention(q)
     assert ((out.double() - ref).abs() <= 2.0 ** -8 * (amp + ref.abs())).all()
+
+
+def strong_token(engine, dtype, new, tokens, bits):
+    """The first token has 2^bits times the weight of any other and a small value, so that results are made
+    of the others' weights.  In the 2-norm: f32 as everywhere; 16-bit results have their own rounding and that of
+    weights to 11 bits, each 2^-12 (bf16: 2^-9 and 2^-12) at most and of random sign."""
+    s = Setup([(new, tokens)], 1, 128, 64, "f16")
+    pos = torch.arange(tokens, device=DEV)
+    p, r = places(s, pos)
+    s.pool[0][p, :, r] *= 0.1
+    s.pool[0][p, :, r, 0] = 0
+    s.pool[0][p[0], :, r[0]] = 0
+    s.pool[0][p[0], :, r[0], 0] = bits * math.log(2.0) * 128 ** 0.5 / 4.0
+    s.pool[1][p[0], :, r[0]] = 1e-3
+    q = s.q(4, dtype)
+    q[..., 0] = 4.0
+    out = torch.empty_like(q)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    engine.attn_paged_dev(s.cache, s.batch, q, out, lse=lse)
+    engine.sync()
+    ref, ref_lse, _ = s.attention(q)
+    rel = ((out.double() - ref).norm() / ref.norm()).item()
+    assert rel <= {"f32": 1e-5, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype], rel
+    assert ((lse.double() - ref_lse).abs() <= 2.0 ** -12 + ref_lse.abs() * 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("tokens,bits", [(1000, 10), (8000, 14), (131071, 18)])
+def test_one_strong_token(engine, dtype, tokens, bits):
+    strong_token(engine, dtype, 1, tokens, bits)
+
+
+@pytest.mark.parametrize("tokens,bits", [(1000, 10), (8000, 14), (20000, 18)])
+def test_one_strong_token_before_f32_rows(engine, tokens, bits):
+    strong_token(engine, "f32", 64, tokens, bits)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_one_strong_token_in_many_sequences(engine, dtype):
+    """The same for single tokens, where each warp streams a thousand positions: 600 sequences of the same 3000
+    positions, the first with 2^18 times the weight of any other and no value."""
+    s = Setup([(600, 3000)], 1, 128, 64, "f16")
+    pos = torch.arange(3000, device=DEV)
+    p, r = places(s, pos)
+    s.pool[0][p, :, r] *= 0.1
+    s.pool[0][p, :, r, 0] = 0
+    s.pool[0][p[0], :, r[0]] = 0
+    s.pool[0][p[0], :, r[0], 0] = 18 * math.log(2.0) * 128 ** 0.5 / 4.0
+    s.pool[1][p[0], :, r[0]] = 0
+    q = s.q(4, dtype)
+    q[..., 0] = 4.0
+    batch = hb.KvBatch(s.table.repeat(600, 1), torch.arange(601, dtype=torch.int32, device=DEV),
+                       torch.full((600,), 3000, dtype=torch.int32, device=DEV), 600, 1)
+    out = torch.empty_like(q)
+    engine.attn_paged_dev(s.cache, batch, q, out)
+    engine.sync()
+    ref, _, _ = s.attention(q, causal=False)
+    rel = ((out.double() - ref).norm() / ref.norm()).item()
+    assert rel <= {"f32": 1e-5, "f16": 2.0 ** -11}[dtype], rel
