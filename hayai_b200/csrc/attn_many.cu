@@ -27,9 +27,12 @@
 // of both halves takes about 4400 cycles (8-bit: 6000): the softmax's trips through TMEM and its chain
 // are not all under the products.
 //
-// Formats: products of f16 (f16 and 8-bit caches) or bf16.  8-bit codes are exact in f16; a K scale
+// Formats: products of f16 (f16 and 8-bit caches) or bf16.  f16 weights are taken 2^7 times as large, P =
+// 2^(s - m + 7), which with the lag of m is up to 2^15: they keep their 11 bits down to 2^-21 of the row's
+// maximum, and below it are off by up to 2^-32 of it (O stands in TMEM for the whole tile, so a unit cannot have a
+// factor of its own as in attn_few.cu).  8-bit codes are exact in f16; a K scale
 // multiplies its column of S, a V scale its column of P, and m follows the largest score + log2 of its V
-// scale, so that P times scale stays under 2^8 whatever the scales are, and near it for the largest.
+// scale, so that P times scale stays under 2^15 whatever the scales are, and near it for the largest.
 // Where a unit's scales lie within 2^6 of each other the largest stands for all; elsewhere each
 // position counts with its own, as a large one may have no weight or be masked.  Scales under 2^-80, zero
 // above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of
@@ -338,6 +341,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                               lastr = many_row(a, q, tl, r0 + min(half * 128 + 127, nr - 1), true);
                 const int cmin = min(first.c, lastr.c), bmax = lastr.b, amin = first.a;
 
+                constexpr float kLift = BF ? 0.f : 7.f;  // log2 of the weights' common factor
                 float rs = 0.f;
                 float m = -INFINITY;
                 float2 l2 = make_float2(0.f, 0.f);
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     if (st == lo) rs = rsc[(n & 1) * 256 + r];
                     auto size = [](float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; };  // what is not finite has none
                     // log2 of a power of two over a size (its bits), but near zero no less than -80: a weight is then up to
-                    // 2^88, and the sum of 2^30 of them finite
+                    // 2^95, and the sum of 2^30 of them finite
                     auto size_log2 = [](uint32_t bits) { return max((int)(bits >> 23) - 126, -80); };
                     float ev = 0.f;
                     bool mixed = false;
@@ -503,7 +507,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         }
                     }
                     const float mm = m == -INFINITY ? 0.f : m;
-                    const float2 rs2 = make_float2(rs, rs), nm2 = make_float2(-mm, -mm);
+                    const float2 rs2 = make_float2(rs, rs), nm2 = make_float2(kLift - mm, kLift - mm);
                     auto weights = [&](auto masked) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -550,6 +554,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 ph_o ^= 1;
                 tc_fence_after();
                 const float l = l2.x + l2.y;
+                m -= kLift;  // the sums are of 2^(s - m)
                 const float k1 = l == 0.f ? 0.f : 1.f / l;
                 const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.ldo * 2)) & 31) == 0;  // rows start on 32 bytes
                 const int tr = a.by_group(row);

@@ -644,3 +644,9 @@ def test_one_strong_token_in_many_sequences(engine, dtype):
     ref, _, _ = s.attention(q, causal=False)
     rel = ((out.double() - ref).norm() / ref.norm()).item()
     assert rel <= {"f32": 1e-5, "f16": 2.0 ** -11}[dtype], rel
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,bits", [(1000, 10), (8000, 14), (131071, 18)])
+def test_one_strong_token_before_a_chunk(engine, dtype, tokens, bits):
+    strong_token(engine, dtype, 64, tokens, bits)
