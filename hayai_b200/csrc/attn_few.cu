@@ -24,9 +24,10 @@
 // product: f16 then holds them however far they are under the row's maximum and whatever the scales are
 // (8-bit: to at most 1, and what is under 2^-25 of the unit's largest is lost; 16-bit: to 2^15, and 2^-40);
 // bf16 terms need no such care.  Query rows are
-// scaled by a power of two to have their largest element in [1, 2) and rounded to the products'
-// type: f16 and bf16 rows are exact or keep 11 bits in f16; f32 rows are split into 2 f16 terms (22
-// bits) or 3 bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11 bits of 16).  Weights are
+// scaled by a power of two to have their largest element in [2^14, 2^15), f16's largest, and rounded to the
+// products' type: f16 and bf16 rows are exact to 2^-39 of the largest element; f32 rows are split into 2 f16
+// terms (22 bits, and 2^-39 of the largest) or 3 bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11
+// bits of 16).  Weights are
 // rounded to one term of the cache's type, of the order of the 16-bit results' own rounding (f16
 // results on a bf16 cache: two), for f32 results to two f16 or three bf16 terms.  All sums are f32;
 // for f32 results a unit's products are added to zero and then to the running sum in FADD, as the
@@ -326,14 +327,11 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                 FewRaw<T>::values(raw[q], x);
                 float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
                 m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // not negative: order as bits
-                // the power of two of m, taken out of the row (none for 0, infinity and the smallest)
-                const uint32_t e = __float_as_uint(m) >> 23;
-                const bool norm = e >= 2 && e <= 252;
-                const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
-                const float up = norm ? __uint_as_float(e << 23) : 1.f;
+                // m brought to [2^14, 2^15) (none for infinity and NaN; the smallest to less)
+                const RowSize size(__float_as_uint(m));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] *= down;
-                if (ln == 0) rscale[r] = up * a.scale * 1.44269504f;
+                for (int i = 0; i < 4; ++i) x[i] *= size.by;
+                if (ln == 0) rscale[r] = size.back * a.scale * 1.44269504f;
                 if (ln < D / 4) {
                     // d = 4 ln + i: 16-byte chunk of the cache row, its k step and the lane that holds it
                     const int ch = I8 ? ln >> 2 : ln >> 1, j = I8 ? 4 * (ch >> 2) + (ln & 3) : 2 * (ch >> 2) + (ln & 1);

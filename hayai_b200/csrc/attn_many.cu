@@ -35,8 +35,8 @@
 // scale, so that P times scale stays under 2^15 whatever the scales are, and near it for the largest.
 // Where a unit's scales lie within 2^6 of each other the largest stands for all; elsewhere each
 // position counts with its own, as a large one may have no weight or be masked.  Scales under 2^-80, zero
-// above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of
-// bf16 on f16 products are scaled by a power of two to have their largest element in [1, 2).
+// above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of bf16 on f16 products are
+// scaled by a power of two to have their largest element in [2^14, 2^15), and are exact to 2^-39 of it.
 #include <math.h>
 
 #include <type_traits>
@@ -926,14 +926,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                                     for (int k = 0; k < 4; ++k) m = max(m, max(y[k] & 0x7fffu, (y[k] >> 16) & 0x7fffu));
 #pragma unroll
                                     for (int o = CH / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                                    const uint32_t e = m >> 7;
-                                    const bool norm = e >= 2 && e <= 252;
-                                    const float down = norm ? __uint_as_float((254 - e) << 23) : 1.f;
-                                    if (norm) rs = fmaxf(rs * __uint_as_float(e << 23), 1e-30f);
+                                    const RowSize size(m << 16);
+                                    rs = fmaxf(rs * size.back, 1e-30f);
 #pragma unroll
                                     for (int k = 0; k < 4; ++k)
-                                        y[k] = pack_h2(__uint_as_float(y[k] << 16) * down,
-                                                       __uint_as_float(y[k] & 0xffff0000u) * down);
+                                        y[k] = pack_h2(__uint_as_float(y[k] << 16) * size.by,
+                                                       __uint_as_float(y[k] & 0xffff0000u) * size.by);
                                 }
                                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(place(r)), "r"(y[0] ^ flip),
                                              "r"(y[1] ^ flip), "r"(y[2] ^ flip), "r"(y[3] ^ flip)

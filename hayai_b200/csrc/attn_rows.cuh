@@ -217,6 +217,19 @@ struct AttnShares {
     }
 };
 
+// The power of two that brings a query row whose largest |x| has the bits m to [2^14, 2^15), and its reciprocal:
+// in f16 the other elements then have the most room below.  Rows that are not finite stay as they are.
+struct RowSize {
+    float by = 1.f, back = 1.f;
+    __device__ __forceinline__ explicit RowSize(uint32_t m) {
+        const uint32_t e = max(m >> 23, 15u);  // of rows under 2^-112 the power alone stays a normal number
+        if (e < 255) {
+            by = __uint_as_float((268 - e) << 23);
+            back = __uint_as_float((e - 14) << 23);
+        }
+    }
+};
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

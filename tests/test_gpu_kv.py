@@ -650,3 +650,15 @@ def test_one_strong_token_in_many_sequences(engine, dtype):
 @pytest.mark.parametrize("tokens,bits", [(1000, 10), (8000, 14), (131071, 18)])
 def test_one_strong_token_before_a_chunk(engine, dtype, tokens, bits):
     strong_token(engine, dtype, 64, tokens, bits)
+
+
+@pytest.mark.parametrize("cache,dtype", [("f16", "f32"), ("i8", "f32"), ("f16", "bf16"), ("i8", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("new", [1, 150])
+def test_queries_of_uneven_size(engine, cache, dtype, new):
+    """One element of every query is 2^20 (f16: 2^14) times the others and meets keys of zero: the scores are
+    made of the others, which keep their bits (f32: 2^-19 of them)."""
+    s = Setup([(new, 400)], 2, 128, 16, cache)
+    s.pool[0][..., 5] = 0
+    q = s.q(8, dtype)
+    q[..., 5] = 2.0 ** (14 if dtype == "f16" else 20)
+    check(engine, s, 8, dtype, q=q)
