@@ -171,8 +171,9 @@ extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv
     a.by_group = FastDiv((uint32_t)a.group);
     a.by_page = FastDiv((uint32_t)c->page_size);
     a.causal = causal != 0;
-    a.window = window;
-    a.sink = window ? sink : 0;
+    // no sequence holds more than 2^30 tokens, and positions less a window of that stay within 32 bits
+    a.window = window < (1 << 30) ? window : 1 << 30;
+    a.sink = window ? (sink < (1 << 30) ? sink : 1 << 30) : 0;
     a.scale = scale;
     const long long rows = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
     a.max_rows = (int)(rows < INT32_MAX ? rows : INT32_MAX);

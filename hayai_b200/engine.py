@@ -31,6 +31,13 @@ TYPE_LABELS = {F32: "f32", Q8_0: "q8_0", Q4_K: "q4_k", Q6_K: "q6_k", IQ2_XXS: "i
                Q5_1: "q5_1", Q2_K: "q2_k", Q3_K: "q3_k", Q5_K: "q5_k", IQ4_NL: "iq4_nl", IQ4_XS: "iq4_xs",
                F16: "f16", BF16: "bf16", Q8_1: "q8_1", Q8_K: "q8_k"}
 LABEL_TYPES = {v: k for k, v in TYPE_LABELS.items()}
+
+
+def _positions(n: int) -> int:
+    """A number of positions as the library takes it: no sequence has more than 2^30."""
+    return min(max(n, -1), 1 << 30)
+
+
 # (elements, bytes) per block: gemv_row_bytes (compute.rs:877-907)
 BLOCK = {F32: (1, 4), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210), IQ2_XXS: (256, 66), IQ2_XS: (256, 74),
          IQ2_S: (256, 82), IQ3_XXS: (256, 98), IQ3_S: (256, 110), Q4_0: (32, 18), Q4_1: (32, 20), Q5_0: (32, 22),
@@ -445,7 +452,7 @@ class CudaEngine:
         """Attention of the new tokens' query rows q [n_tok][n_heads][head_dim] over the cache, into
         out (same shape and type).  scale: 1 / sqrt(head_dim) unless given.  causal: a token sees the
         positions up to its own, of which window > 0 leaves the last ``window`` and the first
-        ``sink``.  lse: None, or a float32 [n_tok][n_heads] that receives the scores' log-sum-exp."""
+        ``sink`` (any whole numbers; a sequence has at most 2^30 tokens).  lse: None, or a float32 [n_tok][n_heads] that receives the scores' log-sum-exp."""
         self._kv_here(cache, batch)
         heads = q.shape[1] if q.dim() == 3 else 0
         t, ldq = cache.rows(batch, q, heads, "q")
@@ -454,7 +461,7 @@ class CudaEngine:
             raise ValueError("q and out need one type")
         rc = self._attn_paged(self.handle, cache.ref, batch.ref, t, heads, q.data_ptr(), ldq, out.data_ptr(), ldo,
                               None if lse is None else cache.lse_ptr(lse, q),
-                              cache.default_scale if scale is None else scale, causal, window, sink)
+                              cache.default_scale if scale is None else scale, causal, _positions(window), _positions(sink))
         if rc:
             _check(rc)
 

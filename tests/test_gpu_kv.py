@@ -662,3 +662,10 @@ def test_queries_of_uneven_size(engine, cache, dtype, new):
     q = s.q(8, dtype)
     q[..., 5] = 2.0 ** (14 if dtype == "f16" else 20)
     check(engine, s, 8, dtype, q=q)
+
+
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 1, 1 << 31, (1 << 32) + 5])
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("f16", "f16"), ("i8", "bf16")])
+def test_windows_longer_than_any_sequence(engine, window, cache, dtype):
+    """Also with tokens before the first position, from whose place such a window starts far below zero."""
+    check(engine, Setup([(6, 2), (140, 10), (3, 0), (1, 5), (40, 300)], 2, 64, 16, cache), 4, dtype, window=window)
