@@ -729,14 +729,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             const int nvis = sg->nvis, n1 = sg->n1, vlo = sg->vlo, hk = sg->hk;
             const int* const table = a.b.table + sg->s * a.b.table_stride;
             give_back(n);
-            auto page_of = [&](int st, int& r) {  // page and row of this lane's position of unit st, -1 if it has none
+            // page and row of this lane's position of unit st, and whether it has one (any page number may stand in a table)
+            auto page_of = [&](int st, int& r, bool& has) {
                 const int v = st * UNIT + own;
-                if (v >= nvis || st >= hi) return -1;
+                has = v < nvis && st < hi;
+                if (!has) return -1;
                 const int j = v < n1 ? v : v - n1 + vlo, p = a.by_page(j);
                 r = j - p * a.c.page_size;
                 return __ldg(table + p);
             };
-            int r = 0, pg = page_of(lo, r);
+            int r = 0;
+            bool has;
+            int pg = page_of(lo, r, has);
             for (int st = lo; st < hi && ok; ++st) {
                 uint32_t off = 0xffffffffu;
                 float sc[2] = {0.f, 0.f};
@@ -747,10 +751,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         sc[0] = __ldg(a.c.ks + so);
                         sc[1] = __ldg(a.c.vs + so);
                     }
-                } else if (pg != -1) {
+                } else if (has) {
                     atomicOr(a.b.err, kErrKvRange);
                 }
-                pg = page_of(st + 1, r);
+                pg = page_of(st + 1, r, has);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv) {
                     if (t_issue - t_done == AHEAD) {

@@ -669,3 +669,23 @@ def test_queries_of_uneven_size(engine, cache, dtype, new):
 def test_windows_longer_than_any_sequence(engine, window, cache, dtype):
     """Also with tokens before the first position, from whose place such a window starts far below zero."""
     check(engine, Setup([(6, 2), (140, 10), (3, 0), (1, 5), (40, 300)], 2, 64, 16, cache), 4, dtype, window=window)
+
+
+@pytest.mark.parametrize("page", [-1, -(1 << 31), 5000])
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("i8", "f16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("new", [1, 150])
+def test_pages_out_of_range_are_reported(engine, page, cache, dtype, new):
+    """Every number outside the pool, -1 (a page that is not mapped) among them, where a token sees it; and
+    none where no token does."""
+    s = Setup([(new, 200), (new, 250)], 2, 64, 16, cache)
+    q = s.q(4, dtype)
+    out = torch.empty_like(q)
+    s.table[0, 13:] = page  # past the first sequence's 200 tokens
+    engine.attn_paged_dev(s.cache, s.batch, q, out)
+    engine.sync()
+    s.table[0, 5] = page
+    with pytest.raises(hb.CudaError) as e:
+        engine.attn_paged_dev(s.cache, s.batch, q, out)
+        engine.sync()
+    assert e.value.code == _lib.HC_ERR_INVALID
+    engine.sync()
