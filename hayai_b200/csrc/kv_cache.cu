@@ -33,6 +33,14 @@ __device__ __forceinline__ bool kv_slot(const KvDev& c, const KvBatchDev& b, con
     return true;
 }
 
+// The grid's last block looks the batch's offsets and lengths over (the others read no more of them than their
+// tokens' places take) and sets the error flag where attention would cut them.
+__device__ __forceinline__ bool kv_check_block(const KvDev& c, const KvBatchDev& b) {
+    if (blockIdx.x != gridDim.x - 1) return false;
+    for (int s = threadIdx.x; s < b.n_seq; s += blockDim.x) kv_seq(b, b.max_pages * c.page_size, s);
+    return true;
+}
+
 template <class C>
 __device__ __forceinline__ C* kv_elem(uint8_t* base, uint32_t units) {
     return reinterpret_cast<C*>(base + (unsigned long long)units * 64);
@@ -72,6 +80,7 @@ __device__ __forceinline__ void kv_codes(const float (&x)[8], float m, float s, 
 template <class T, class C, int D, int U>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, KvRows r, FastDiv by_page) {
     constexpr int GL = D / 8;
+    if (kv_check_block(c, b)) return;
     const int chunks = (c.n_heads + U - 1) / U;
     const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL;
     const int l = threadIdx.x & (GL - 1);
@@ -116,6 +125,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, K
 template <class T, class C, int D, int U>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvRows r, FastDiv by_page) {
     constexpr int GL = D / 8;
+    if (kv_check_block(c, b)) return;
     const int chunks = (c.n_heads + U - 1) / U;
     const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL;
     const int l = threadIdx.x & (GL - 1);
@@ -152,7 +162,7 @@ namespace {
 template <class T, class C, int D, int U>
 cudaError_t start(bool write, const KvDev& c, const KvBatchDev& b, const KvRows& r, cudaStream_t s) {
     const long long groups = (long long)b.n_tok * ((c.n_heads + U - 1) / U);
-    const unsigned grid = (unsigned)((groups * (D / 8) + 255) / 256);
+    const unsigned grid = (unsigned)((groups * (D / 8) + 255) / 256) + 1;  // and kv_check_block's
     const FastDiv by_page((uint32_t)c.page_size);
     if (write)
         kv_append_kernel<T, C, D, U><<<grid, 256, 0, s>>>(c, b, r, by_page);

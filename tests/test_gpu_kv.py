@@ -689,3 +689,33 @@ def test_pages_out_of_range_are_reported(engine, page, cache, dtype, new):
         engine.sync()
     assert e.value.code == _lib.HC_ERR_INVALID
     engine.sync()
+
+
+@pytest.mark.parametrize("what,at,value", [("table", 0, -1), ("table", 0, 1 << 20), ("kv_len", 1, -5), ("kv_len", 0, 100000),
+                                           ("q_start", 0, -3), ("q_start", 1, 0x7fffffff), ("q_start", 2, 1 << 20), ("q_start", 1, -1)])
+@pytest.mark.parametrize("call", ["append", "read", "attend"])
+@pytest.mark.parametrize("cache", ["i8", "f16"])
+def test_every_call_reports_values_out_of_range(engine, call, what, at, value, cache):
+    s = Setup([(40, 200), (40, 250)], 2, 64, 16, cache)
+    getattr(s, what).view(-1)[at] = value
+    if what == "table":
+        s.table[:] = value
+    x, q = s.q(2, "f16"), s.q(4, "f16")
+    with pytest.raises(hb.CudaError) as e:
+        if call == "attend":
+            engine.attn_paged_dev(s.cache, s.batch, q, torch.empty_like(q))
+        else:
+            (engine.kv_append_dev if call == "append" else engine.kv_read_dev)(s.cache, s.batch, x, x.clone())
+        engine.sync()
+    assert e.value.code == _lib.HC_ERR_INVALID
+    engine.sync()  # reported once
+
+
+@pytest.mark.parametrize("call", ["append", "read"])
+def test_sequences_that_fit_are_not_reported(engine, call):
+    """Tokens before the first position, sequences without tokens or new ones, rows of no sequence."""
+    s = Setup([(6, 2), (0, 0), (3, 0), (0, 9), (1, 5)], 2, 64, 16, "f16")
+    batch = hb.KvBatch(s.table, s.q_start + 1, s.kv_len, s.rows + 4, 6)
+    x = torch.randn(s.rows + 4, 2, 64, device=DEV).half()
+    (engine.kv_append_dev if call == "append" else engine.kv_read_dev)(s.cache, batch, x, x.clone())
+    engine.sync()
