@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             }
         }
     }
-    if (!ok) atomicOr(a.b.err, 2);
+    if (!ok) atomicOr(a.b.err, kErrWait);
     tc_fence_before();
     __syncthreads();
     if (warp == 12) {

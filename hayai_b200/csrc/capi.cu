@@ -17,6 +17,7 @@
 #include "../../include/hayai_cuda.h"
 #include "common.cuh"
 #include "engine.h"
+#include "err_flags.h"
 #include "gemv_launch.h"
 #include "gemv_mma.cuh"
 
@@ -331,15 +332,9 @@ int hc_finish_sync(hc_engine* e) {
 static int flag_error(hc_engine* e, int flag) {
     if (flag) {
         HC_CUDA(cudaMemset(e->d_err, 0, sizeof(int)));
-        if (flag & 1)
-            return hc_set_error(HC_ERR_RANGE,
-                                "an activation magnitude reached 65504 (outside the f16 range of the tensor-core split)");
-        // a block that gave up may have left its tiles' counters behind
-        if ((flag & 2) && e->attn_cnt.p) HC_CUDA(cudaMemset(e->attn_cnt.p, 0, e->attn_cnt.cap));
-        if (flag & 2) return hc_set_error(HC_ERR_TIMEOUT, "a bounded device wait expired");
-        if (flag & 4)
-            return hc_set_error(HC_ERR_INVALID, "kv batch: a page number, length or offset on the device is out of range");
-        return hc_set_error(HC_ERR_CUDA, "device error flag 0x%x", flag);
+        const ErrReport r = err_report(flag);
+        if (r.clear_counters && e->attn_cnt.p) HC_CUDA(cudaMemset(e->attn_cnt.p, 0, e->attn_cnt.cap));
+        return r.code == HC_ERR_CUDA ? hc_set_error(r.code, "device error flag 0x%x", flag) : hc_set_error(r.code, "%s", r.text);
     }
     return HC_OK;
 }

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "err_flags.h"
 
 namespace hc {
 
@@ -26,8 +27,6 @@ struct KvBatchDev {
     int n_seq, n_tok, max_pages;
     int* err;
 };
-
-constexpr int kErrKvRange = 4;  // device error flag: a page number, length or offset out of range
 
 // A sequence's new tokens [q0, q1) of the batch and its length, with offsets and lengths that do
 // not fit the batch cut to it (and the error flag set).

@@ -83,3 +83,18 @@ def test_the_replay_sees_a_wait_that_is_not_sound(tmp_path):
     """Looking at V ahead of the scores in a segment's first unit is found out."""
     unsound, stuck = replay(tmp_path, "-DEARLY=1")
     assert unsound > 0 and stuck == 0
+
+
+def test_counters_are_cleared_whatever_is_reported(tmp_path):
+    """A wait that ran out may leave joining counters behind: they are cleared also where another flag is up
+    and gives the report."""
+    src = tmp_path / "flags.cpp"
+    src.write_text('#include <stdio.h>\n#include "err_flags.h"\nint main() { for (int f = 1; f < 16; ++f) {'
+                   'const hc::ErrReport r = hc::err_report(f); printf("%d %d\\n", r.code, r.clear_counters); } }\n')
+    exe = tmp_path / "flags"
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "hayai_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    rows = [line.split() for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines()]
+    for flag, (code, clear) in enumerate(rows, 1):
+        want = _lib.HC_ERR_RANGE if flag & 1 else _lib.HC_ERR_TIMEOUT if flag & 2 else _lib.HC_ERR_INVALID if flag & 4 else None
+        assert want is None or int(code) == want
+        assert int(clear) == (flag >> 1 & 1)
