@@ -754,7 +754,6 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
         const AttnShared sh = shared_s[x];
         if (!sh.valid) continue;
         const int wf = share.owner(sh.u_item), wl = share.owner(sh.u_item + sh.units - 1), bf = wf / W, bl = wl / W;
-        // of fewer places than warps some warps have none, and no piece
         const int q0 = max(wf, c * W), q1 = min(wl, c * W + W - 1);
 #pragma unroll 1
         for (int r = 0; r < sh.nr; ++r) {
@@ -762,14 +761,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
             AttnJoin j;
             auto piece = [&](int i) { return place_s[q0 + i - c * W][q0 + i == wf]; };
             j.join(q1 - q0 + 1, ln < D / 4,
-                   [&](int i) {
-                       return share.q == 0 && q0 + i >= share.rem ? make_float2(-INFINITY, 0.f)
-                                                                  : *reinterpret_cast<const float2*>(piece(i) + ROWS * D + 2 * r);
-                   },
-                   [&](int i) {
-                       return share.q == 0 && q0 + i >= share.rem ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                                  : reinterpret_cast<const float4*>(piece(i) + r * D)[ln];
-                   });
+                   [&](int i) { return *reinterpret_cast<const float2*>(piece(i) + ROWS * D + 2 * r); },
+                   [&](int i) { return reinterpret_cast<const float4*>(piece(i) + r * D)[ln]; });
             if (bf != bl) {
                 float* p = bpart + (size_t)(2 * c + (bf == c)) * F::PS;
                 if (ln < D / 4) reinterpret_cast<float4*>(p + r * D)[ln] = make_float4(j.y[0], j.y[1], j.y[2], j.y[3]);
