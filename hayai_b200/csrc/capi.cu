@@ -231,8 +231,12 @@ extern "C" int hc_engine_free(hc_engine* e) {
     e->sk_cnt.release();
     e->stack_bar.release();
     e->ws_tc.release();
-    e->attn_part.release();
-    e->attn_cnt.release();
+    while (AttnWs* w = e->attn_ws) {
+        e->attn_ws = w->next;
+        w->part.release();
+        w->count.release();
+        delete w;
+    }
     hc_peer_release(e);
     for (auto& kv : e->ptr_tables) cudaFree(kv.second);
     e->ptr_tables.clear();
@@ -333,7 +337,8 @@ static int flag_error(hc_engine* e, int flag) {
     if (flag) {
         HC_CUDA(cudaMemset(e->d_err, 0, sizeof(int)));
         const ErrReport r = err_report(flag);
-        if (r.clear_counters && e->attn_cnt.p) HC_CUDA(cudaMemset(e->attn_cnt.p, 0, e->attn_cnt.cap));
+        if (r.clear_counters)
+            for (AttnWs* w = e->attn_ws; w; w = w->next) HC_CUDA(cudaMemset(w->count.p, 0, w->count.cap));
         return r.code == HC_ERR_CUDA ? hc_set_error(r.code, "device error flag 0x%x", flag) : hc_set_error(r.code, "%s", r.text);
     }
     return HC_OK;

@@ -2,6 +2,8 @@
 // (include/hayai_cuda.h): the arguments' checks and the launches.
 #include <math.h>
 
+#include <new>
+
 #include "../../include/hayai_cuda.h"
 #include "engine.h"
 #include "kv_launch.h"
@@ -121,22 +123,44 @@ extern "C" int hc_kv_read_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_ba
     return kv_rows(e, c, b, dtype, k, ldk, v, ldv, false);
 }
 
-// The split tiles' partial results and counters: as much as any call of any kernel takes, so that
-// they never move under a captured graph.
+// A new workspace, as much as any call of any kernel takes, so that it never moves under a captured graph.  Its
+// counters are zero before any stream gets it.
+static int attn_make_workspace(const hc_engine* e, AttnWs* w) {
+    int rc = w->part.ensure(kAttnPartBytes * e->num_sms);
+    if (!rc) rc = w->count.ensure((size_t)e->num_sms * 32 * sizeof(int));  // one for each row of a block's first split tile
+    if (rc) return rc;
+    HC_CUDA(cudaMemsetAsync(w->count.p, 0, w->count.cap, cudaStreamPerThread));
+    HC_CUDA(cudaStreamSynchronize(cudaStreamPerThread));
+    return HC_OK;
+}
+
+// The workspace of the engine's stream, or of the captures on it.
 static int attn_workspace(hc_engine* e, AttnArgs* a) {
-    const size_t part = kAttnPartBytes * e->num_sms;
-    if (part > e->attn_part.cap) {
-        const int rc = e->attn_part.ensure(part);
+    cudaStreamCaptureStatus status;
+    HC_CUDA(cudaStreamIsCapturing(e->stream, &status));
+    const bool captured = status != cudaStreamCaptureStatusNone;
+    AttnWs* w = e->attn_ws;
+    while (w && (w->stream != e->stream || w->captured != captured)) w = w->next;
+    if (!w) {
+        // a capture forbids its thread to allocate unless it says that it means to, outside the graph
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        HC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        w = new (std::nothrow) AttnWs;
+        const int rc = w ? attn_make_workspace(e, w) : hc_set_error(HC_ERR_CUDA, "attn_paged: out of host memory");
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (rc && w) {
+            w->part.release();
+            w->count.release();
+            delete w;
+        }
         if (rc) return rc;
+        w->stream = e->stream;
+        w->captured = captured;
+        w->next = e->attn_ws;
+        e->attn_ws = w;
     }
-    const size_t cnt = (size_t)e->num_sms * 32 * sizeof(int);  // one for each row of a block's first split tile
-    if (cnt > e->attn_cnt.cap) {
-        const int rc = e->attn_cnt.ensure(cnt);
-        if (rc) return rc;
-        HC_CUDA(cudaMemsetAsync(e->attn_cnt.p, 0, cnt, e->stream));
-    }
-    a->part = (float*)e->attn_part.p;
-    a->count = (int*)e->attn_cnt.p;
+    a->part = (float*)w->part.p;
+    a->count = (int*)w->count.p;
     return HC_OK;
 }
 

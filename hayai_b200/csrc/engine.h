@@ -37,6 +37,15 @@ struct PeerState {
     uint32_t flow_phases = 0;    // of those, the phases run by the dataflow stack kernel
 };
 
+// Paged attention's partial results of split tiles and their counters (zero between calls): one for the calls
+// on a stream, and one for the calls captured on it, whose graphs may run beside the stream's own calls.
+struct AttnWs {
+    cudaStream_t stream = nullptr;
+    bool captured = false;
+    DevBuf part, count;
+    AttnWs* next = nullptr;
+};
+
 // One GPU + stream: the counterpart of OpenClEngine (crates/hayai-opencl/src/context.rs:23).
 struct hc_engine {
     int device = 0;
@@ -54,7 +63,7 @@ struct hc_engine {
     DevBuf stack_bar;             // grid-barrier counter of the persistent FFN-stack kernel
     DevBuf ws_tc;                 // batched Q8_0 tensor-core GEMM: canonical activations + partials
     DevBuf ws_tp;                 // tensor parallelism at batch > 1: this rank's down partial
-    DevBuf attn_part, attn_cnt;   // paged attention: partial results of split tiles, and their counters
+    AttnWs* attn_ws = nullptr;    // paged attention: workspaces of the streams that it ran on
     bool use_stack_kernel = true; // batch-1 stacks run as one persistent kernel when they fit
     bool use_tc = true;           // batches of 8+ rows of Q8_0/Q4_K/Q6_K on the tcgen05 GEMM
     HostBuf hs_out;

@@ -452,7 +452,9 @@ class CudaEngine:
         """Attention of the new tokens' query rows q [n_tok][n_heads][head_dim] over the cache, into
         out (same shape and type).  scale: 1 / sqrt(head_dim) unless given.  causal: a token sees the
         positions up to its own, of which window > 0 leaves the last ``window`` and the first
-        ``sink`` (any whole numbers; a sequence has at most 2^30 tokens).  lse: None, or a float32 [n_tok][n_heads] that receives the scores' log-sum-exp."""
+        ``sink`` (any whole numbers; a sequence has at most 2^30 tokens).  lse: None, or a float32 [n_tok][n_heads] that receives the scores' log-sum-exp.
+        Calls on two streams (set_stream) may be in flight together, and a captured graph beside them;
+        graphs that were captured on the same stream may not."""
         self._kv_here(cache, batch)
         heads = q.shape[1] if q.dim() == 3 else 0
         t, ldq = cache.rows(batch, q, heads, "q")

@@ -311,8 +311,10 @@ int hc_kv_read_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* 
  * the cache's (query head h reads kv head h / (n_heads / cache heads)).  causal: a token sees the
  * positions up to its own, of which window > 0 leaves the last `window` and the first `sink`; else
  * all kv_len.  lse (NULL or [n_tok][n_heads]) receives log sum_j exp(scale q_i . k_j).  A token
- * that sees nothing gets out 0 and lse -inf.  out must not overlap q.  The engine's workspace for
- * partial results is made by the first call: make it before a stream capture. */
+ * that sees nothing gets out 0 and lse -inf.  out must not overlap q.  Partial results lie in the
+ * engine, about 40 MB for the calls on each stream and as much for those captured on it, made by the
+ * first such call (also inside a capture) and kept: calls on two streams, and a graph beside direct
+ * calls, may be in flight together, but of the graphs captured on one stream only one at a time. */
 int hc_attn_paged_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, int dtype, size_t n_heads,
                       const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale, int causal, int window,
                       int sink);

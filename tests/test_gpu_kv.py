@@ -719,3 +719,41 @@ def test_sequences_that_fit_are_not_reported(engine, call):
     x = torch.randn(s.rows + 4, 2, 64, device=DEV).half()
     (engine.kv_append_dev if call == "append" else engine.kv_read_dev)(s.cache, batch, x, x.clone())
     engine.sync()
+
+
+def split_work(seed):
+    """A batch whose sequences are split over blocks, its queries, and their results alone."""
+    s = Setup([(1, 9000 + 37 * seed), (1, 3), (90, 5000 + 11 * seed)], 2, 128, 16, "i8", seed=seed)
+    return s, s.q(8, "f16")
+
+
+def test_two_streams_at_once(engine):
+    """Calls on two streams are in flight together, and a graph captured on one of them beside both: each has
+    partial results of its own, so that all get the bits that they get alone."""
+    work = [split_work(i) for i in (1, 2, 3)]
+    alone = []
+    for s, q in work:
+        alone.append(torch.empty_like(q))
+        engine.attn_paged_dev(s.cache, s.batch, q, alone[-1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[torch.zeros_like(q) for _ in range(20)] for _, q in work]
+    g = torch.cuda.CUDAGraph()
+    engine.set_stream(streams[0])
+    with torch.cuda.graph(g, stream=streams[0]):  # the stream's first call, in a capture
+        for o in outs[2]:
+            engine.attn_paged_dev(work[2][0].cache, work[2][0].batch, work[2][1], o)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(streams[2]):
+            g.replay()
+        for i in range(20):
+            for k in range(2):
+                engine.set_stream(streams[k])
+                engine.attn_paged_dev(work[k][0].cache, work[k][0].batch, work[k][1], outs[k][i])
+        torch.cuda.synchronize()
+        for k in range(3):
+            for o in outs[k]:
+                assert torch.equal(o, alone[k]), k
+                o.zero_()
+    engine.sync()
