@@ -8,6 +8,7 @@ from .engine import (BF16, BLOCK, F16, F32, IQ2_S, IQ2_XS, IQ2_XXS, IQ3_S, IQ3_X
                      Q3_K, Q4_0, Q4_1, Q4_K, Q5_0, Q5_1, Q5_K, Q6_K, Q8_0, Q8_1, Q8_K, TYPE_LABELS, BoundStack, CudaEngine,
                      CudaError,
                      PendingGemv, QuantMatrix, ResidentWeights, device_count, row_bytes)
+from .kv import KvBatch, KvCache
 from .orchestrator import EngineOrchestrator
 
 __all__ = ["BoundStack", "CudaEngine", "CudaError", "EngineOrchestrator", "KvBatch", "KvCache", "PendingGemv", "QuantMatrix", "ResidentWeights",
@@ -15,11 +16,3 @@ __all__ = ["BoundStack", "CudaEngine", "CudaError", "EngineOrchestrator", "KvBat
            "IQ3_S", "Q4_0", "Q4_1", "Q5_0", "Q5_1", "Q2_K", "Q3_K", "Q5_K", "IQ4_NL", "IQ4_XS", "F16", "BF16",
            "Q8_1", "Q8_K", "BLOCK",
            "TYPE_LABELS"]
-
-
-def __getattr__(name):  # the paged cache's descriptions are the part that needs torch to import
-    if name in ("KvBatch", "KvCache"):
-        from . import kv
-
-        return getattr(kv, name)
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -11,13 +11,17 @@ from __future__ import annotations
 
 import ctypes
 
-import torch
-
-from . import _lib
-
 F32, F16, I8, BF16 = 0, 1, 24, 30  # GgmlType ids
-_ROW_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-_CACHE_TYPES = {torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8}
+_ROW_TYPES, _CACHE_TYPES = {}, {}  # by torch's types: the package imports without torch, descriptions need it
+
+
+def _torch():
+    import torch
+
+    if not _ROW_TYPES:
+        _ROW_TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _CACHE_TYPES.update({torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8})
+    return torch
 
 
 class _Cache(ctypes.Structure):
@@ -44,6 +48,7 @@ class KvCache:
     of the scales only the page axis."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
+        torch = _torch()
         _need(k.is_cuda and v.is_cuda and k.device == v.device, "k and v must be CUDA tensors of one device")
         _need(k.dtype in _CACHE_TYPES and v.dtype == k.dtype, "k and v must both be float16, bfloat16 or int8")
         _need(k.dim() == 4 and v.shape == k.shape, "k and v must be [n_pages][n_heads][page_size][head_dim]")
@@ -91,7 +96,7 @@ class KvCache:
     def lse_ptr(self, lse, q):
         if lse is None:
             return None
-        if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.get_device() != self.index:
+        if _ROW_TYPES.get(lse.dtype) != F32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.get_device() != self.index:
             raise ValueError("lse must be a contiguous float32 tensor [n_tok][n_heads] on q's device")
         return lse.data_ptr()
 
@@ -103,6 +108,7 @@ class KvBatch:
     new tokens, where the program knows one (1 when decoding)."""
 
     def __init__(self, page_table, q_start, kv_len, n_tok: int, max_new: int = 0):
+        torch = _torch()
         for t, d in ((page_table, 2), (q_start, 1), (kv_len, 1)):
             _need(t.is_cuda and t.dtype == torch.int32 and t.dim() == d and t.device == page_table.device,
                   "page_table, q_start and kv_len must be int32 CUDA tensors of one device, of 2, 1 and 1 axes")

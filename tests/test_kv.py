@@ -5,6 +5,7 @@ import ctypes
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -98,3 +99,11 @@ def test_counters_are_cleared_whatever_is_reported(tmp_path):
         want = _lib.HC_ERR_RANGE if flag & 1 else _lib.HC_ERR_TIMEOUT if flag & 2 else _lib.HC_ERR_INVALID if flag & 4 else None
         assert want is None or int(code) == want
         assert int(clear) == (flag >> 1 & 1)
+
+
+def test_the_package_imports_without_torch():
+    """All public names, and no torch loaded by them: only the cache's descriptions need it."""
+    code = "import sys; sys.modules['torch'] = None\nfrom hayai_b200 import *\nCudaEngine, KvCache, KvBatch"
+    subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True)
+    code = "import sys\nfrom hayai_b200 import *\nassert 'torch' not in sys.modules"
+    subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True)
