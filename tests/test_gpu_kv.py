@@ -757,3 +757,38 @@ def test_two_streams_at_once(engine):
                 assert torch.equal(o, alone[k]), k
                 o.zero_()
     engine.sync()
+
+
+# ------------------------------------------------------------------ sizes of prompts
+@pytest.mark.parametrize("cache", ["i8", "f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,kv_heads,page", [(128, 8, 64), (64, 5, 24), (128, 3, 100)])
+def test_append_then_read_prompts(engine, cache, dtype, dim, kv_heads, page):
+    """More rows than threads at once: several rows to a thread, and heads that they do not divide."""
+    s = Setup([(6000, 6100), (1, 7), (4003, 4003)], kv_heads, dim, page, cache)
+    x = [s.q(kv_heads, dtype) for _ in range(2)]
+    engine.kv_append_dev(s.cache, s.batch, *x)
+    back = [torch.full_like(t, math.nan) for t in x]
+    engine.kv_read_dev(s.cache, s.batch, *back)
+    engine.sync()
+    for w in range(2):
+        v = x[w].float()
+        if cache == "i8":
+            codes, scale = quantised(v)
+            v = codes.float() * scale[..., None]
+        assert torch.equal(back[w], v.to(T[cache]).float().to(T[dtype]) if cache != "i8" else v.to(T[dtype]))
+
+
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "f32"), ("f16", "f32"), ("bf16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_of_thousands(engine, cache, dtype, dim):
+    check(engine, Setup([(2500, 2500), (700, 3001), (1, 40)], 1, dim, 64, cache), 4, dtype)
+
+
+@pytest.mark.parametrize("cache,dtype", [("i8", "f16"), ("f16", "f16"), ("bf16", "bf16")])
+def test_a_tile_in_more_than_64_pieces(engine, cache, dtype):
+    """One long sequence beside short ones: nearly all blocks have a piece of its one tile."""
+    s = Setup([(40, 300000)] + [(40, 60 + i) for i in range(9)], 1, 64, 64, cache)
+    q = s.q(4, dtype)
+    a, b = check(engine, s, 4, dtype, q=q), check(engine, s, 4, dtype, q=q)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
