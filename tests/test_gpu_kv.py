@@ -792,3 +792,21 @@ def test_a_tile_in_more_than_64_pieces(engine, cache, dtype):
     q = s.q(4, dtype)
     a, b = check(engine, s, 4, dtype, q=q), check(engine, s, 4, dtype, q=q)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_lse_where_values_are_not_finite(engine, dtype, bad):
+    """V scales that are not finite, over a whole unit: the results that see them are not finite, the scores'
+    log-sum-exp is as without them."""
+    s = Setup([(150, 700), (1, 300)], 2, 128, 16, "i8")
+    for i in range(2):
+        p, r = places(s, torch.arange(130, device=DEV), i)
+        s.scale[1][p, :, r] = bad
+    q = s.q(8, dtype)
+    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device=DEV)
+    engine.attn_paged_dev(s.cache, s.batch, q, out, lse=lse)
+    engine.sync()
+    _, ref_lse, _ = s.attention(q)
+    assert not torch.isfinite(out).any()
+    assert ((lse.double() - ref_lse).abs() <= 2.0 ** -12 + ref_lse.abs() * 2.0 ** -20).all()
