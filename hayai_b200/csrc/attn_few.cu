@@ -16,22 +16,22 @@
 //
 // Formats.  8-bit codes are exact in f16 and in bf16.  For 16-bit results V's go in as f16 1152 + code
 // (no subtraction: bits 0x6400 + code + 128), and the product's accumulator starts at -1152 sum p of
-// the weights as rounded, so that the codes' own product is left (the larger sums cost about 2^-24 *
-// 1152 / 40 of a result's size; K's codes are taken as they are, as the lse is f32 whatever the
-// results are).  A token's K scale multiplies its score and its V scale its weights.  For f32 results the
-// codes are taken as they are, and the weights times scales as bf16 terms.  Where weights go in as f16, a
-// unit's weights of a row are first brought to a fixed size by a power of two, which multiplies the unit's
-// product: f16 then holds them however far they are under the row's maximum and whatever the scales are
-// (8-bit: to at most 1, and what is under 2^-25 of the unit's largest is lost; 16-bit: to 2^15, and 2^-40);
-// bf16 terms need no such care.  Query rows are
-// scaled by a power of two to have their largest element in [2^14, 2^15), f16's largest, and rounded to the
-// products' type: f16 and bf16 rows are exact to 2^-39 of the largest element; f32 rows are split into 2 f16
-// terms (22 bits, and 2^-39 of the largest) or 3 bf16 terms (24 bits), f16 rows on a bf16 cache into 2 (11
-// bits of 16).  Weights are
-// rounded to one term of the cache's type, of the order of the 16-bit results' own rounding (f16
-// results on a bf16 cache: two), for f32 results to two f16 or three bf16 terms.  All sums are f32;
-// for f32 results a unit's products are added to zero and then to the running sum in FADD, as the
-// tensor cores' own chained additions truncate.
+// the weights as rounded, so that the codes' own product is left.  (The larger sums are rounded to about 1e-4
+// of a code, 1e-6 of the values' largest, also where a result is nearly zero; K's codes are taken as they are,
+// as the lse is f32 whatever the results are.)  A token's K scale multiplies its score and its V scale its
+// weights.  For f32 results the codes are taken as they are, and the weights times scales as bf16 terms.
+//
+// Query rows are scaled by a power of two to have their largest element in [2^14, 2^15), the top of f16, and
+// rounded to the products' type: f16 and bf16 rows are exact to 2^-39 of the largest element; f32 rows are
+// split into 2 f16 terms (22 bits, and 2^-39 of the largest) or 3 bf16 terms (24 bits), f16 rows on a bf16
+// cache into 2 (11 bits of 16).  Weights are rounded to one term of the cache's type, of the order of the
+// 16-bit results' own rounding (f16 results on a bf16 cache: two), for f32 results to two f16 or three bf16
+// terms.  Where they go in as f16, a unit's weights of a row are first brought to a fixed size by a power of
+// two, which multiplies the unit's product: f16 then holds them however far they are under the row's maximum
+// and whatever the scales are (8-bit: to at most 1, and what is under 2^-25 of the unit's largest is lost;
+// 16-bit: to 2^15, and 2^-40); bf16 terms need no such care.  All sums are f32; for f32 results and f16
+// weights a unit's products are added to zero and then to the running sum in FADD, as the tensor cores' own
+// chained additions truncate.
 //
 // The workers of the line (attn_rows.cuh) are warps, one block of 8 or 12 of them per SM.  A warp
 // streams its units through a ring of 16-byte asynchronous copies of its own, whose issue runs ahead
@@ -40,7 +40,7 @@
 // workspace, where after one barrier the block joins its warps' pieces, and the last block of a
 // tile's row the blocks'.
 // Measured: 64 sequences of 300 to 12000 8-bit tokens 100 us (4.2 TB/s, 66 % of the copy rate), one of
-// 131071 f16 tokens 57 us (4.7 TB/s, 73 %), one of 1001 8-bit tokens 11.5 us in a graph.
+// 131071 f16 tokens 58 us (4.6 TB/s, 72 %), one of 1001 8-bit tokens 11.7 us in a graph.
 // (Tiles shared by all warps of a block, with a barrier and a joining at each tile's end, took
 // 160 us where this takes 100 us: 64 sequences of 300 to 12000 tokens, 64 heads on 8.)
 #include <math.h>

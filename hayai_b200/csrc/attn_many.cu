@@ -6,7 +6,7 @@
 // halves of 128 with their own accumulators, and units of 128 positions; one block of 16 warps per SM
 // takes an equal share of the line of units.
 //
-//   warps 0-3, 4-7   one thread per row of half 0 and 1: S from TMEM, weights P = 2^(s - m) back into
+//   warps 0-3, 4-7   one thread per row of half 0 and 1: S from TMEM, weights P (below) back into
 //                    the same TMEM columns in 16 bits, m and the sum in registers; the row's O in TMEM
 //                    is rescaled by its thread in the rare units where m moves;
 //   warps 8-11       bring keys and values in: 16-byte asynchronous copies (8-bit pages: by way of a
@@ -22,21 +22,22 @@
 // the special function unit: the two pipes are equally loaded, and the rest of the softmax has to fit
 // under them.
 //
-// Measured: 10.9k prompt tokens in 4 sequences (32 heads on 8 of 128, bf16) 394 us, 640 TFLOP/s of the
-// visible pairs (39 % of cuBLAS's rate); 2048 tokens over 30k cached 8-bit ones 404 us, 609 TFLOP/s.  A unit
+// Measured: 10.9k prompt tokens in 4 sequences (32 heads on 8 of 128, bf16) 397 us, 636 TFLOP/s of the
+// visible pairs (38 % of cuBLAS's rate); 2048 tokens over 30k cached 8-bit ones 410 us, 600 TFLOP/s.  A unit
 // of both halves takes about 4400 cycles (8-bit: 6000): the softmax's trips through TMEM and its chain
 // are not all under the products.
 //
-// Formats: products of f16 (f16 and 8-bit caches) or bf16.  f16 weights are taken 2^7 times as large, P =
-// 2^(s - m + 7), which with the lag of m is up to 2^15: they keep their 11 bits down to 2^-21 of the row's
-// maximum, and below it are off by up to 2^-32 of it (O stands in TMEM for the whole tile, so a unit cannot have a
-// factor of its own as in attn_few.cu).  8-bit codes are exact in f16; a K scale
-// multiplies its column of S, a V scale its column of P, and m follows the largest score + log2 of its V
-// scale, so that P times scale stays under 2^15 whatever the scales are, and near it for the largest.
-// Where a unit's scales lie within 2^6 of each other the largest stands for all; elsewhere each
-// position counts with its own, as a large one may have no weight or be masked.  Scales under 2^-80, zero
-// above all, count as 2^-80, so that P's own sum stays in f32's range.  Rows of bf16 on f16 products are
-// scaled by a power of two to have their largest element in [2^14, 2^15), and are exact to 2^-39 of it.
+// Formats: products of f16 (f16 and 8-bit caches) or bf16; P = 2^(s - m) is rounded to that type, of the
+// order of the 16-bit results' own rounding, and summed in f32.  f16 weights are taken 2^7 times as large,
+// with the lag of m up to 2^15: they keep their 11 bits down to 2^-21 of the row's maximum, and below it are
+// off by up to 2^-32 of it (O stands in TMEM for the whole tile, so a unit cannot have a factor of its own as
+// in attn_few.cu).  8-bit codes are exact in f16; a K scale multiplies its column of S, a V scale its column
+// of P, and m follows the largest score + log2 of its V scale, so that P times scale stays under 2^15
+// whatever the scales are.  Where a unit's scales lie within 2^6 of each other the largest stands for all,
+// which may take that much of the room; elsewhere each position counts with its own, as a large one may have
+// no weight or be masked.  Scales under 2^-80, zero above all, count as 2^-80, so that the weights' own sum
+// stays in f32's range.  Rows of bf16 on f16 products are scaled by a power of two to have their largest
+// element in [2^14, 2^15), and are exact to 2^-39 of it.
 #include <math.h>
 
 #include <type_traits>

@@ -4,12 +4,12 @@
 // One row is one token's head_dim values of one head.  An 8-bit cache holds
 //     scale = max|x| * r, r = f32(1/127),   code = x / scale rounded to nearest (ties to even)
 // with the product and the quotient rounded to f32 as IEEE rounds them and codes held to [-127,
-// 127], so that they do not depend on the kernel; a row of zeros has scale 0 and codes 0, and a row that is not finite has scale NaN, so
-// that it reads back as NaN and is not hidden.  The scale stays in f32: 4 bytes beside 64 to 128.
+// 127], so that they do not depend on the kernel; a row of zeros has scale 0 and codes 0, and a row that
+// is not finite has scale NaN, so that it reads back as NaN and is not hidden.  The scale stays in f32: 4 bytes beside 64 to 128.
 // Reading back gives code * scale, rounded once to the type of the rows.
 //
-// Measured: 30080 tokens of 8 heads of 128 from bf16 into 8-bit pages about 41 us (4.5 TB/s), 31720
-// back into bf16 36 us (5.4 TB/s, 84 % of the copy rate); one token 1.7 us in a graph.
+// Measured: 30080 tokens of 8 heads of 128 from bf16 into 8-bit pages 43 us in a graph (4.3 TB/s), 31720
+// back into bf16 36 us (5.4 TB/s, 84 % of the copy rate); one token 1.8 us in a graph.
 #include "kv_launch.h"
 
 namespace hc {
