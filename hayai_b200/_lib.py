@@ -28,6 +28,7 @@ _P = ctypes.c_void_p
 _S = ctypes.c_size_t
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 _PP = ctypes.POINTER(ctypes.c_void_p)
 
 # name -> argtypes (all return int status except hc_last_error)
@@ -75,6 +76,14 @@ SIGNATURES: dict[str, list] = {
     "hc_kv_append_dev": [_P, _P, _P, _I, _P, _S, _P, _S],
     "hc_kv_read_dev": [_P, _P, _P, _I, _P, _S, _P, _S],
     "hc_attn_paged_dev": [_P, _P, _P, _I, _S, _P, _S, _P, _S, _P, _F, _I, _I, _I],
+    "hc_attn_shared_dev": [_P, _P, _P, _P, _I, _S, _P, _S, _P, _S, _P, _F],
+    "hc_rope_init": [_P, _I, _I, _I, _D, _D, _D, _D, _D, _P, _F],
+    "hc_rope_dev": [_P, _P, _I, _S, _S, _P, _P, _S, _P, _S],
+    "hc_kv_append_rope_dev": [_P, _P, _P, _P, _I, _S, _P, _S, _P, _S, _P, _S, _P, _S],
+    "hc_kv_pages_scratch": [_I, ctypes.POINTER(_S)],
+    "hc_kv_fork_dev": [_P, _P, _I, _P, _P],
+    "hc_kv_resize_dev": [_P, _P, _I, _P, _P],
+    "hc_kv_compact_dev": [_P, _P, _P],
     "hc_synth_normal_dev": [_P, ctypes.c_uint64, _S, _F, _F, _P],
     "hc_quantize_dev": [_P, _I, _P, _S, _P],
 }

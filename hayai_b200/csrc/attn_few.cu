@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
             const int j = v < pw.it.t.n1 ? v : v - pw.it.t.n1 + pw.it.t.lo;
             const int p = a.by_page(j);
             pr = j - p * a.c.page_size;
-            pg = __ldg(a.b.table + pw.it.s * a.b.table_stride + p);
+            pg = __ldg(a.b.table + (a.table_row ? __ldg(a.table_row + pw.it.s) : pw.it.s) * a.b.table_stride + p);
             if ((unsigned)pg >= (unsigned)a.c.n_pages) {
                 atomicOr(a.b.err, kErrKvRange);
                 pg = -1;
@@ -723,20 +723,20 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                     const int col = I8 ? (D / 8) * g + 2 * d : 64 * (d >> 2) + 8 * g + 2 * (d & 3);
                     const float y[4] = {o[d][n][e], o[d][n][e + 2], o[d + 1][n][e], o[d + 1][n][e + 2]};
                     if (whole)
-                        attn_store<T>(a, it.q.q0, it.hk, tl.r0 + r, D, col, y, l[n][e]);
+                        attn_store<T>(a, it.q.q0, it.hk, tl.r0 + r, D, col, y, m[n][e], l[n][e], attn_adds(a, tl.lo));
                     else
                         *reinterpret_cast<float4*>(part + r * D + col) = make_float4(y[0], y[1], y[2], y[3]);
                 }
                 if (g == 0) {
                     if (whole)
-                        attn_store_lse(a, it.q.q0, it.hk, tl.r0 + r, m[n][e], l[n][e]);
+                        attn_store_lse(a, it.q.q0, it.hk, tl.r0 + r, m[n][e], l[n][e], attn_adds(a, tl.lo));
                     else
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m[n][e], l[n][e]);
                 }
             }
         if (!whole && ln == 0) {
             place_s[w][lo == 0] = part;
-            if (lo == 0 || w == 0) shared_s[lo == 0 ? w : W] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units};
+            if (lo == 0 || w == 0) shared_s[lo == 0 ? w : W] = {1, it.q.q0, it.hk, tl.r0, tl.nr, it.u_item, tl.units, tl.lo};
         }
         if (done) break;
         it.next(a, ROWS, ST);
@@ -784,8 +784,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                        [&](int i) { return __ldcg(reinterpret_cast<const float4*>(block(i) + r * D) + ln); });
             }
             if (ln >= D / 4) continue;
-            attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l);
-            if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l);
+            attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.m, j.l, attn_adds(a, sh.lo));
+            if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l, attn_adds(a, sh.lo));
         }
     }
 }

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             mbar_init(b_qf + 8 * i, 1);
             mbar_init(b_chk + 8 * i, 4);
             misc[4 + 3 * i] = misc[5 + 3 * i] = misc[6 + 3 * i] = 0;
-            shared_s[i] = {0, 0, 0, 0, 0, 0, 1};
+            shared_s[i] = {0, 0, 0, 0, 0, 0, 1, 0};
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(b_seg + 8 * i, 1);
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             if (!ok || lo == hi) break;
             const int kvt = 2 * unit;  // key and value tiles before this segment's
             unit += hi - lo;
-            const KvSeq q{sg->q0, sg->q1, sg->len};
+            const KvSeq q{sg->q0, sg->q1, sg->len, 0};
             const int r0 = sg->r0, hk = sg->hk, whole = sg->whole, slot = sg->slot;
             AttnTile tl;
             tl.lo = sg->vlo, tl.n1 = sg->n1;
@@ -558,8 +558,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 m -= kLift;  // the sums are of 2^(s - m)
                 const float k1 = l == 0.f ? 0.f : 1.f / l;
                 const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.ldo * 2)) & 31) == 0;  // rows start on 32 bytes
-                const int tr = a.by_group(row);
-                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + (hk * a.group + row - tr * a.group) * D;
+                const int tr = a.by_group(row), head = hk * a.group + row - tr * a.group;
+                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + head * D;
+                // a shared prefix: its own results, or what it adds to a row's
+                const bool adds = attn_adds(a, tl.lo);
+                const long long at = (long long)(q.q0 + tr) * a.heads + head;
+                const AttnAdd add(m, l, adds && real && whole ? __ldcg(a.base_lse + at) : -INFINITY);
+                float* const base = a.base + at * D;
                 float* const part = a.part + (size_t)(2 * c + slot) * PS;
 #pragma unroll 1
                 for (int k = 0; k < D / 32; ++k) {
@@ -567,7 +572,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     tc_ld32(tO + 32 * k, o);
                     tc_wait_ld32(o);
                     if (!real || !ok) continue;
-                    if (whole) {
+                    if (whole && a.to_base) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(base + 32 * k + 4 * i) =
+                                l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                         : make_float4(o[4 * i] * k1, o[4 * i + 1] * k1, o[4 * i + 2] * k1, o[4 * i + 3] * k1);
+                    } else if (whole && adds) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 b = __ldcg(reinterpret_cast<const float4*>(base + 32 * k + 4 * i));
+                            const float u = add(o[4 * i], b.x), v = add(o[4 * i + 1], b.y), w = add(o[4 * i + 2], b.z),
+                                        x = add(o[4 * i + 3], b.w);
+                            *reinterpret_cast<uint2*>(out + 32 * k + 4 * i) =
+                                __is_same(T, __half) ? make_uint2(pack_h2(u, v), pack_h2(w, x)) : make_uint2(pack_b2(u, v), pack_b2(w, x));
+                        }
+                    } else if (whole) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             uint32_t y[8];
@@ -588,7 +608,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 tc_fence_before();
                 if (real && ok) {
                     if (whole)
-                        attn_store_lse(a, q.q0, hk, row, m, l);
+                        attn_store_lse(a, q.q0, hk, row, m, l, adds);
                     else
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m, l);
                 }
@@ -635,7 +655,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         }
                         tops[r] = m;
                         tops[256 + r] = l;
-                        attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, m, l);
+                        attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, m, l, attn_adds(a, sh.lo));
                     }
                 }
                 named_bar_sync(1, 256);
@@ -671,7 +691,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int e = e0 + 256 * k, r = e / (D / 4);
-                        if (e < sh.nr * (D / 4)) attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[256 + r]);
+                        if (e < sh.nr * (D / 4)) attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[r], tops[256 + r], attn_adds(a, sh.lo));
                     }
                 }
             }
@@ -728,7 +748,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             const int lo = sg->lo, hi = sg->hi;
             if (!ok || lo == hi) break;
             const int nvis = sg->nvis, n1 = sg->n1, vlo = sg->vlo, hk = sg->hk;
-            const int* const table = a.b.table + sg->s * a.b.table_stride;
+            const int* const table = a.b.table + (a.table_row ? __ldg(a.table_row + sg->s) : sg->s) * a.b.table_stride;
             give_back(n);
             // page and row of this lane's position of unit st, and whether it has one (any page number may stand in a table)
             auto page_of = [&](int st, int& r, bool& has) {
@@ -859,7 +879,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         const bool whole = lo == 0 && hi == it.t.units;
                         segs[n & 3] = {lo, hi, it.t.nr, it.t.r0, it.q.q0, it.q.q1, it.q.len, it.s, it.hk, it.t.lo, it.t.n1,
                                        it.t.nvis, whole, lo == 0, {0, 0}};
-                        if (!whole) shared_s[lo == 0] = {1, it.q.q0, it.hk, it.t.r0, it.t.nr, it.u_item, it.t.units};
+                        if (!whole) shared_s[lo == 0] = {1, it.q.q0, it.hk, it.t.r0, it.t.nr, it.u_item, it.t.units, it.t.lo};
                         mbar_arrive(b_seg + 8 * (n & 3));
                     }
                     ++n;

@@ -34,7 +34,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
     t.p_lo = q.len - n + a.by_group(t.r0);
     t.p_hi = q.len - n + a.by_group(t.r0 + t.nr - 1);
     const int end = a.causal ? max(min(q.len, t.p_hi + 1), 0) : q.len;
-    t.lo = a.window ? min(max(t.p_lo - a.window + 1, 0), end) : 0;
+    t.lo = a.window ? min(max(t.p_lo - a.window + 1, 0), end) : min(q.first, end);
     t.n1 = min(a.sink, t.lo);
     t.nvis = t.n1 + end - t.lo;
     t.units = max(1, (t.nvis + unit - 1) / unit);  // a tile that sees nothing still has to write zeros
@@ -42,7 +42,15 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
     return t;
 }
 
+// A sequence, and where what it sees starts.
+__device__ __forceinline__ KvSeq attn_seq(const AttnArgs& a, int s) {
+    KvSeq q = kv_seq(a.b, a.b.max_pages * a.c.page_size, s);
+    if (a.first) q.first = __ldg(a.first + s);
+    return q;
+}
+
 __device__ __forceinline__ int attn_tiles(const AttnArgs& a, const KvSeq& q, int rows) {
+    if (a.to_base && q.len == 0) return 0;  // nothing shared: nothing to add
     const int r = (q.q1 - q.q0) * a.group;
     return r >= a.row_min && r <= a.row_max ? (r + rows - 1) / rows : 0;
 }
@@ -59,11 +67,11 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
     int* const items = scratch + 18;  // the number of items, at most 2^16 counted
     if (threadIdx.x == 0) *items = 0;
     __syncthreads();
-    const int cap = a.b.max_pages * a.c.page_size, tid = threadIdx.x, wid = tid >> 5, ln = tid & 31;
+    const int tid = threadIdx.x, wid = tid >> 5, ln = tid & 31;
     const bool by_warp = a.max_rows > 8 * rows;  // many tiles in a sequence: its tiles over a warp's lanes
     if (by_warp) {
         for (int s = wid; s < a.b.n_seq; s += THREADS / 32) {
-            const KvSeq q = kv_seq(a.b, cap, s);
+            const KvSeq q = attn_seq(a, s);
             const int n = attn_tiles(a, q, rows);
             long long w = 0;
             for (int t = ln; t < n; t += 32) w += attn_tile(a, q, t, rows, unit).span;
@@ -76,7 +84,7 @@ __device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int un
         }
     } else {
         for (int s = tid; s < a.b.n_seq; s += THREADS) {
-            const KvSeq q = kv_seq(a.b, cap, s);
+            const KvSeq q = attn_seq(a, s);
             const int n = attn_tiles(a, q, rows);
             long long w = 0;
             for (int t = 0; t < n; ++t) w += attn_tile(a, q, t, rows, unit).span;
@@ -120,10 +128,10 @@ struct AttnLanes {
 };
 __device__ __forceinline__ int attn_schedule_lanes(const AttnArgs& a, int rows, int unit, AttnLanes& v) {
     const int ln = lane_id();
-    v.q = {0, 0, 0};
+    v.q = {0, 0, 0, 0};
     unsigned long long x = 0;
     if (ln < a.b.n_seq) {
-        v.q = kv_seq(a.b, a.b.max_pages * a.c.page_size, ln);
+        v.q = attn_seq(a, ln);
         const int n = attn_tiles(a, v.q, rows);
         for (int t = 0; t < n; ++t) x += attn_tile(a, v.q, t, rows, unit).span;
     }
@@ -144,7 +152,7 @@ __device__ __forceinline__ int attn_schedule_lanes(const AttnArgs& a, int rows, 
 
 // A tile that several workers share, for the joining.
 struct AttnShared {
-    int valid, q0, hk, r0, nr, u_item, units;
+    int valid, q0, hk, r0, nr, u_item, units, lo;
 };
 
 // An item of the line, (sequence, kv head, tile), and its first place.
@@ -154,7 +162,7 @@ struct AttnIter {
     AttnTile t;
 
     __device__ __forceinline__ void seq(const AttnArgs& a, int rows) {
-        q = kv_seq(a.b, a.b.max_pages * a.c.page_size, s);
+        q = attn_seq(a, s);
         n_tiles = attn_tiles(a, q, rows);
         hk = tile = 0;
     }
@@ -172,7 +180,8 @@ struct AttnIter {
     }
     __device__ __forceinline__ void seek(const AttnArgs& a, const AttnLanes& v, int u, int rows, int unit) {
         s = __popc(__ballot_sync(0xffffffffu, v.pre <= u));
-        q = {__shfl_sync(0xffffffffu, v.q.q0, s), __shfl_sync(0xffffffffu, v.q.q1, s), __shfl_sync(0xffffffffu, v.q.len, s)};
+        q = {__shfl_sync(0xffffffffu, v.q.q0, s), __shfl_sync(0xffffffffu, v.q.q1, s), __shfl_sync(0xffffffffu, v.q.len, s),
+             __shfl_sync(0xffffffffu, v.q.first, s)};
         n_tiles = attn_tiles(a, q, rows);
         tile = 0;
         const int before = __shfl_sync(0xffffffffu, v.pre, s ? s - 1 : 0);
@@ -241,17 +250,48 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
-// Four adjacent values of the weighted sum of row `row` of an item's kv head, over l.
+// Does a tile that starts at position `lo` add a shared prefix's results?  (The start of a window does not.)
+__device__ __forceinline__ bool attn_adds(const AttnArgs& a, int lo) { return a.first && lo > 0; }
+
+// What a row's own weighted sum and the result over its shared prefix count for in the two's result.  Own: sum y
+// and l of weights 2^(s - m); the prefix: a result with log 2 of its weights' sum.
+struct AttnAdd {
+    float own, pre, m, l;  // result = y * own + prefix's * pre; m and l of both together
+    __device__ __forceinline__ AttnAdd(float m0, float l0, float lse) {
+        m = fmaxf(m0, lse);
+        const float f = m0 == -INFINITY && l0 == 0.f ? 0.f : ex2(m0 - m), g = lse == -INFINITY ? 0.f : ex2(lse - m);
+        l = l0 * f + g;
+        const float k = l == 0.f ? 0.f : 1.f / l;
+        own = f * k;
+        pre = g * k;
+    }
+    // a weight of zero takes nothing, whatever the value is
+    __device__ __forceinline__ float operator()(float y, float b) const {
+        return (own == 0.f ? 0.f : y * own) + (pre == 0.f ? 0.f : b * pre);
+    }
+};
+
+// Four adjacent values of the weighted sum y of row `row` of an item's kv head, over l; adds: with the prefix's.
 template <class T>
 __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[4],
-                                           float l) {
+                                           float m, float l, bool adds) {
     const bool none = l == 0.f;  // saw nothing (a sum that is not a number is kept)
     const float k = none ? 0.f : 1.f / l;
-    const int t = a.by_group(row);
-    T* out = (T*)a.out + (long long)(q0 + t) * a.ldo + (hk * a.group + row - t * a.group) * D + d;
+    const int t = a.by_group(row), h = hk * a.group + row - t * a.group;
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = none ? 0.f : y[i] * k;
+    const long long at = (long long)(q0 + t) * a.heads + h;
+    if (a.to_base) {
+        *reinterpret_cast<float4*>(a.base + at * D + d) = make_float4(z[0], z[1], z[2], z[3]);
+        return;
+    }
+    if (adds) {
+        const AttnAdd w(m, l, __ldcg(a.base_lse + at));
+        const float4 b = __ldcg(reinterpret_cast<const float4*>(a.base + at * D + d));
+        z[0] = w(y[0], b.x), z[1] = w(y[1], b.y), z[2] = w(y[2], b.z), z[3] = w(y[3], b.w);
+    }
+    T* out = (T*)a.out + (long long)(q0 + t) * a.ldo + h * D + d;
     if constexpr (sizeof(T) == 4)
         *reinterpret_cast<float4*>(out) = make_float4(z[0], z[1], z[2], z[3]);
     else if constexpr (__is_same(T, __half))
@@ -259,11 +299,18 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, in
     else
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_b2(z[0], z[1]), pack_b2(z[2], z[3]));
 }
-__device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l) {
+__device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l, bool adds) {
     const int t = a.by_group(row);
-    if (a.lse)
-        a.lse[(long long)(q0 + t) * a.heads + hk * a.group + row - t * a.group] =
-            l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
+    const long long at = (long long)(q0 + t) * a.heads + hk * a.group + row - t * a.group;
+    if (a.to_base) {
+        a.base_lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+    } else if (a.lse) {
+        if (adds) {
+            const AttnAdd w(m, l, __ldcg(a.base_lse + at));
+            m = w.m, l = w.l;
+        }
+        a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
+    }
 }
 
 // One row of n partial results joined by a warp: ml(i) gives piece i's (m, l), (-inf, 0) if it has

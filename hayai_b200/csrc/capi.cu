@@ -235,6 +235,7 @@ extern "C" int hc_engine_free(hc_engine* e) {
         e->attn_ws = w->next;
         w->part.release();
         w->count.release();
+        w->base.release();
         delete w;
     }
     hc_peer_release(e);

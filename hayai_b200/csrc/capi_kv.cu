@@ -1,5 +1,5 @@
-// capi_kv.cu -- C ABI of the paged key/value cache and of the attention over it
-// (include/hayai_cuda.h): the arguments' checks and the launches.
+// capi_kv.cu -- C ABI of the paged key/value cache, its bookkeeping, rotary positions and the attention
+// over it (include/hayai_cuda.h): the arguments' checks and the launches.
 #include <math.h>
 
 #include <new>
@@ -134,92 +134,396 @@ static int attn_make_workspace(const hc_engine* e, AttnWs* w) {
     return HC_OK;
 }
 
-// The workspace of the engine's stream, or of the captures on it.
-static int attn_workspace(hc_engine* e, AttnArgs* a) {
+// The workspace of the engine's stream, or of the captures on it, with `base` bytes for a shared prefix.
+static int attn_workspace(hc_engine* e, AttnArgs* a, size_t base, void** base_at) {
     cudaStreamCaptureStatus status;
     HC_CUDA(cudaStreamIsCapturing(e->stream, &status));
     const bool captured = status != cudaStreamCaptureStatusNone;
     AttnWs* w = e->attn_ws;
-    while (w && (w->stream != e->stream || w->captured != captured)) w = w->next;
-    if (!w) {
+    while (w && (w->stream != e->stream || w->captured != captured || (captured && w->base.cap < base))) w = w->next;
+    if (!w || w->base.cap < base) {
+        size_t size = base ? (size_t)1 << 20 : 0;  // a power of two: it grows few times
+        while (size < base) size *= 2;
         // a capture forbids its thread to allocate unless it says that it means to, outside the graph
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         HC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-        w = new (std::nothrow) AttnWs;
-        const int rc = w ? attn_make_workspace(e, w) : hc_set_error(HC_ERR_CUDA, "attn_paged: out of host memory");
+        const bool fresh = !w;
+        if (fresh) w = new (std::nothrow) AttnWs;
+        int rc = !w ? hc_set_error(HC_ERR_CUDA, "attn_paged: out of host memory") : fresh ? attn_make_workspace(e, w) : HC_OK;
+        if (!rc && size) rc = w->base.ensure(size);  // (freeing what was there waits for the calls that use it)
         cudaThreadExchangeStreamCaptureMode(&mode);
-        if (rc && w) {
+        if (rc && w && fresh) {
             w->part.release();
             w->count.release();
             delete w;
         }
         if (rc) return rc;
-        w->stream = e->stream;
-        w->captured = captured;
-        w->next = e->attn_ws;
-        e->attn_ws = w;
+        if (fresh) {
+            w->stream = e->stream;
+            w->captured = captured;
+            w->next = e->attn_ws;
+            e->attn_ws = w;
+        }
     }
     a->part = (float*)w->part.p;
     a->count = (int*)w->count.p;
+    if (base_at) *base_at = w->base.p;
     return HC_OK;
+}
+
+// What the attention calls have in common: their checks, and the arguments that both kernels get.  *none: nothing to do.
+static int attn_args(const char* what, hc_engine* e, const hc_kv_cache* c, const hc_kv_batch* b, int dtype, size_t n_heads,
+                     const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale, AttnArgs* a, bool* none) {
+    int rc = hc_engine_activate(e);
+    if (!rc) rc = check_cache(c, &a->c);
+    if (!rc) rc = check_batch(e, c, b, &a->b);
+    if (rc) return rc;
+    if ((unsigned long long)b->n_tok * n_heads > INT32_MAX)
+        return hc_set_error(HC_ERR_INVALID, "%s: %d tokens of %zu heads are past 2^31 rows", what, b->n_tok, n_heads);
+    if (n_heads == 0 || n_heads % (size_t)c->n_heads || n_heads > 65535)
+        return hc_set_error(HC_ERR_INVALID, "%s: %zu query heads on %d kv heads", what, n_heads, c->n_heads);
+    if (!isfinite(scale)) return hc_set_error(HC_ERR_INVALID, "%s: scale is not finite", what);
+    *none = b->n_tok == 0 || b->n_seq == 0;
+    if (*none) return HC_OK;
+    const size_t width = n_heads * c->head_dim;
+    rc = check_rows(what, dtype, q, ldq, width);
+    if (!rc) rc = check_rows(what, dtype, out, ldo, width);
+    if (rc) return rc;
+    a->q = q;
+    a->out = out;
+    a->lse = lse;
+    a->ldq = (long long)ldq;
+    a->ldo = (long long)ldo;
+    a->heads = (int)n_heads;
+    a->group = (int)(n_heads / c->n_heads);
+    a->by_group = FastDiv((uint32_t)a->group);
+    a->by_page = FastDiv((uint32_t)c->page_size);
+    a->causal = 1;
+    a->scale = scale;
+    return HC_OK;
+}
+
+// Sequences with up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
+// ones to the other (tiles of 256): both are launched where the batch may have both.  At 16 rows, 16
+// sequences of 3000 to 8000 8-bit tokens take 67 us in the first and 145 in the second (bf16: 79 and
+// 113); at 32 rows, in tiles of 32, 182 and 147 (bf16: 115 and 116).
+static cudaError_t attn_run(const hc_engine* e, const hc_kv_cache* c, int dtype, AttnArgs a, int max_new) {
+    constexpr int kFewRows = 16;
+    const long long rows = (long long)(max_new && max_new < a.b.n_tok ? max_new : a.b.n_tok) * a.group;
+    a.max_rows = (int)(rows < INT32_MAX ? rows : INT32_MAX);
+    const bool many = attn_many_supported(c->type, dtype) && a.max_rows > kFewRows;
+    cudaError_t ce = cudaSuccess;
+    if (many) {
+        a.row_min = a.b.n_seq > 1 ? kFewRows + 1 : 1;
+        a.row_max = INT32_MAX;
+        ce = launch_attn_many(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
+    }
+    if (ce == cudaSuccess && (!many || a.b.n_seq > 1)) {
+        a.row_min = 1;
+        a.row_max = many ? kFewRows : INT32_MAX;
+        if (many) a.max_rows = kFewRows;
+        ce = launch_attn_few(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
+    }
+    return ce;
 }
 
 extern "C" int hc_attn_paged_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_batch* b, int dtype, size_t n_heads,
                                  const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale, int causal,
                                  int window, int sink) {
     AttnArgs a{};
-    int rc = hc_engine_activate(e);
-    if (!rc) rc = check_cache(c, &a.c);
-    if (!rc) rc = check_batch(e, c, b, &a.b);
-    if (rc) return rc;
-    if ((unsigned long long)b->n_tok * n_heads > INT32_MAX)
-        return hc_set_error(HC_ERR_INVALID, "attn_paged: %d tokens of %zu heads are past 2^31 rows", b->n_tok, n_heads);
-    if (n_heads == 0 || n_heads % (size_t)c->n_heads || n_heads > 65535)
-        return hc_set_error(HC_ERR_INVALID, "attn_paged: %zu query heads on %d kv heads", n_heads, c->n_heads);
+    bool none;
     if (window < 0 || sink < 0 || (window && !causal))
         return hc_set_error(HC_ERR_INVALID, "attn_paged: window %d and sink %d must not be negative, and a window needs causal",
                             window, sink);
-    if (!isfinite(scale)) return hc_set_error(HC_ERR_INVALID, "attn_paged: scale is not finite");
-    if (b->n_tok == 0 || b->n_seq == 0) return HC_OK;
-    const size_t width = n_heads * c->head_dim;
-    rc = check_rows("attn_paged", dtype, q, ldq, width);
-    if (!rc) rc = check_rows("attn_paged", dtype, out, ldo, width);
-    if (rc) return rc;
-    a.q = q;
-    a.out = out;
-    a.lse = lse;
-    a.ldq = (long long)ldq;
-    a.ldo = (long long)ldo;
-    a.heads = (int)n_heads;
-    a.group = (int)(n_heads / c->n_heads);
-    a.by_group = FastDiv((uint32_t)a.group);
-    a.by_page = FastDiv((uint32_t)c->page_size);
+    int rc = attn_args("attn_paged", e, c, b, dtype, n_heads, q, ldq, out, ldo, lse, scale, &a, &none);
+    if (rc || none) return rc;
     a.causal = causal != 0;
     // no sequence holds more than 2^30 tokens, and positions less a window of that stay within 32 bits
     a.window = window < (1 << 30) ? window : 1 << 30;
     a.sink = window ? (sink < (1 << 30) ? sink : 1 << 30) : 0;
-    a.scale = scale;
-    const long long rows = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
-    a.max_rows = (int)(rows < INT32_MAX ? rows : INT32_MAX);
-    rc = attn_workspace(e, &a);
+    rc = attn_workspace(e, &a, 0, nullptr);
     if (rc) return rc;
-    // Sequences of up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
-    // ones to the other (tiles of 256): both are launched where the batch may have both.  At 16 rows, 16
-    // sequences of 3000 to 8000 8-bit tokens take 67 us in the first and 145 in the second (bf16: 79 and
-    // 113); at 32 rows, in tiles of 32, 182 and 147 (bf16: 115 and 116).
-    constexpr int kFewRows = 16;
-    const bool many = attn_many_supported(c->type, dtype) && a.max_rows > kFewRows;
-    cudaError_t ce = cudaSuccess;
-    if (many) {
-        a.row_min = b->n_seq > 1 ? kFewRows + 1 : 1;
-        a.row_max = INT32_MAX;
-        ce = launch_attn_many(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
-    }
-    if (ce == cudaSuccess && (!many || b->n_seq > 1)) {
-        a.row_min = 1;
-        a.row_max = many ? kFewRows : INT32_MAX;
-        if (many) a.max_rows = kFewRows;
-        ce = launch_attn_few(c->type, dtype, c->head_dim, a, e->num_sms, e->stream);
-    }
+    const cudaError_t ce = attn_run(e, c, dtype, a, b->max_new);
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_paged launch");
+}
+
+extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_batch* b, const hc_kv_shared* g, int dtype,
+                                  size_t n_heads, const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale) {
+    AttnArgs a{};
+    bool none;
+    int rc = attn_args("attn_shared", e, c, b, dtype, n_heads, q, ldq, out, ldo, lse, scale, &a, &none);
+    if (rc) return rc;
+    if (!g) return hc_set_error(HC_ERR_INVALID, "attn_shared: null groups");
+    if (g->n_groups < 0 || g->max_new < 0)
+        return hc_set_error(HC_ERR_INVALID, "attn_shared: negative size n_groups=%d max_new=%d", g->n_groups, g->max_new);
+    if (g->n_groups > HC_KV_MAX_SEQ)
+        return hc_set_error(HC_ERR_INVALID, "attn_shared: %d groups (at most %d)", g->n_groups, HC_KV_MAX_SEQ);
+    if (g->n_groups && (!g->seq_start || !g->length)) return hc_set_error(HC_ERR_INVALID, "attn_shared: null seq_start or length");
+    if (none) return HC_OK;
+    // the batch's firsts and the groups' arrays, then the prefixes' sums and results
+    const size_t rows = (size_t)b->n_tok * n_heads, lse_at = (kSharedInts * 4 + 255) / 256 * 256,
+                 out_at = (lse_at + rows * 4 + 255) / 256 * 256;
+    const bool shares = g->n_groups > 0 && b->n_seq > 1;
+    void* base = nullptr;
+    rc = attn_workspace(e, &a, shares ? out_at + rows * c->head_dim * 4 : 0, &base);
+    if (rc) return rc;
+    cudaError_t ce = cudaSuccess;
+    if (shares) {
+        KvSharedDev d{};
+        d.seq_start = g->seq_start;
+        d.length = g->length;
+        d.n = g->n_groups;
+        d.first = (int*)base;
+        d.q_start = d.first + HC_KV_SEQS;
+        d.len = d.q_start + HC_KV_SEQS + 4;
+        d.row = d.len + HC_KV_SEQS;
+        a.base_lse = (float*)((uint8_t*)base + lse_at);
+        a.base = (float*)((uint8_t*)base + out_at);
+        ce = launch_attn_groups(a.b, d, b->max_pages * c->page_size, e->stream);
+        AttnArgs p = a;
+        p.b.q_start = d.q_start;
+        p.b.kv_len = d.len;
+        p.b.n_seq = d.n;
+        p.table_row = d.row;
+        p.causal = 0;
+        p.to_base = 1;
+        if (ce == cudaSuccess) ce = attn_run(e, c, dtype, p, g->max_new);
+        a.first = d.first;
+    }
+    if (ce == cudaSuccess) ce = attn_run(e, c, dtype, a, b->max_new);
+    return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
+}
+
+// ------------------------------------------------------------------ rotary positions
+static int check_rope(const hc_rope* r, RopeDev* d) {
+    if (!r) return hc_set_error(HC_ERR_INVALID, "null rope");
+    if (r->layout != HC_ROPE_HALF && r->layout != HC_ROPE_PAIRS)
+        return hc_set_error(HC_ERR_INVALID, "rope: layout %d (HC_ROPE_HALF or HC_ROPE_PAIRS)", r->layout);
+    if (r->head_dim < 2 || r->head_dim > 2 * HC_ROPE_MAX || r->head_dim % 2 || r->rot_dim < 2 || r->rot_dim % 2 ||
+        r->rot_dim > r->head_dim)
+        return hc_set_error(HC_ERR_INVALID, "rope: rot_dim %d of head_dim %d (even, at most %d)", r->rot_dim, r->head_dim,
+                            2 * HC_ROPE_MAX);
+    if (!isfinite(r->amplitude)) return hc_set_error(HC_ERR_INVALID, "rope: amplitude is not finite");
+    d->pairs = r->layout == HC_ROPE_PAIRS;
+    d->dim = r->head_dim;
+    d->rot = r->rot_dim;
+    d->amplitude = r->amplitude;
+    for (int i = 0; i < r->rot_dim / 2; ++i) d->turns[i] = r->turns[i];
+    return HC_OK;
+}
+// Are values turned in chunks of 8, or of 8 and their 8 partners?
+static bool rope_chunks(const RopeDev& r) { return r.dim % 16 == 0 && r.rot % (r.pairs ? 8 : 16) == 0; }
+
+extern "C" int hc_rope_init(hc_rope* out, int layout, int head_dim, int rot_dim, double base, double factor, double original,
+                            double low, double high, const float* factors, float amplitude) {
+    if (!out) return hc_set_error(HC_ERR_INVALID, "null out pointer");
+    hc_rope r{};
+    r.layout = layout;
+    r.head_dim = head_dim;
+    r.rot_dim = rot_dim ? rot_dim : head_dim;
+    r.amplitude = amplitude;
+    RopeDev unused;
+    const int rc = check_rope(&r, &unused);
+    if (rc) return rc;
+    if (!(base > 0) || !isfinite(base) || !(factor > 0) || !isfinite(factor))
+        return hc_set_error(HC_ERR_INVALID, "rope: base %g and factor %g must be positive", base, factor);
+    if (!(original >= 0) || !isfinite(original) || (original > 0 && !(low < high && isfinite(low) && isfinite(high))))
+        return hc_set_error(HC_ERR_INVALID, "rope: original context %g must not be negative, and needs low < high (%g, %g)",
+                            original, low, high);
+    const long double tau = 6.283185307179586476925286766559L;
+    for (int i = 0; i < r.rot_dim / 2; ++i) {
+        if (factors && (!(factors[i] > 0) || !isfinite(factors[i])))
+            return hc_set_error(HC_ERR_INVALID, "rope: factors must be positive");
+        long double t = powl((long double)base, -2.0L * i / r.rot_dim) / (factors ? factors[i] : 1.0L);
+        if (original > 0) {
+            long double g = ((long double)original * t / tau - low) / ((long double)high - low);
+            g = g < 0 ? 0 : g > 1 ? 1 : g;
+            t *= (1 - g) / factor + g;
+        } else {
+            t /= factor;
+        }
+        const long double turn = t / tau;  // whole turns make no difference
+        if (!(turn < 0x1p62L)) return hc_set_error(HC_ERR_INVALID, "rope: frequency %d is out of range", i);
+        const long double part = roundl((turn - floorl(turn)) * 0x1p64L);
+        r.turns[i] = part >= 0x1p64L ? 0 : (uint64_t)part;
+    }
+    *out = r;
+    return HC_OK;
+}
+
+// May rows be written at `out` while rows are read at `x`?  Where both are the same rows, or no row of the one touches
+// a row of the other (slices of one array's rows, or apart altogether).
+static bool rows_apart(const void* x, size_t ldx, size_t wx, const void* out, size_t ldo, size_t wo, size_t n, size_t es) {
+    const uint64_t a = (uint64_t)(uintptr_t)x, b = (uint64_t)(uintptr_t)out;
+    if (n == 0 || a + ((n - 1) * ldx + wx) * es <= b || b + ((n - 1) * ldo + wo) * es <= a) return true;
+    if (ldx != ldo) return false;
+    const uint64_t pitch = ldx * es, off = b >= a ? (b - a) % pitch : (pitch - (a - b) % pitch) % pitch;
+    return off >= wx * es && off + wo * es <= pitch;
+}
+
+extern "C" int hc_rope_dev(hc_engine* e, const hc_rope* rope, int dtype, size_t n_tok, size_t n_heads, const int32_t* positions,
+                           const void* x, size_t ldx, void* out, size_t ldo) {
+    RopeDev r{};
+    int rc = hc_engine_activate(e);
+    if (!rc) rc = check_rope(rope, &r);
+    if (rc) return rc;
+    if (dtype != T_F32 && !half_type(dtype))
+        return hc_set_error(HC_ERR_UNSUPPORTED, "rope: no kernel for rows of type %d (f32, f16 or bf16)", dtype);
+    if (n_tok > INT32_MAX || n_heads > 65535 || n_tok * n_heads > INT32_MAX)
+        return hc_set_error(HC_ERR_INVALID, "rope: %zu tokens of %zu heads are past 2^31 rows", n_tok, n_heads);
+    if (n_tok == 0 || n_heads == 0) return HC_OK;
+    if (!positions || !x || !out) return hc_set_error(HC_ERR_INVALID, "rope: null positions or rows");
+    const size_t width = n_heads * r.dim, es = elem_bytes(dtype);
+    if (ldx < width || ldo < width || ldx > ((size_t)1 << 40) || ldo > ((size_t)1 << 40))
+        return hc_set_error(HC_ERR_INVALID, "rope: leading dimension %zu out of range for rows of %zu", ldx < width ? ldx : ldo, width);
+    if (((uintptr_t)x | (uintptr_t)out) % es) return hc_set_error(HC_ERR_INVALID, "rope: rows are not aligned to their type");
+    if (!(x == out && ldx == ldo) && !rows_apart(x, ldx, width, out, ldo, width, n_tok, es))
+        return hc_set_error(HC_ERR_INVALID, "rope: out must be x itself or not overlap it");
+    const bool wide = rope_chunks(r) && (((uintptr_t)x | (uintptr_t)out) & 15) == 0 && ldx * es % 16 == 0 && ldo * es % 16 == 0;
+    const RopeRows a{positions, x, out, (long long)ldx, (long long)ldo, (int)n_tok, (int)n_heads};
+    const cudaError_t ce = launch_rope(dtype, r, a, wide, e->stream);
+    return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "rope launch");
+}
+
+extern "C" int hc_kv_append_rope_dev(hc_engine* e, const hc_kv_cache* c, const hc_kv_batch* b, const hc_rope* rope, int dtype,
+                                     size_t n_heads, const void* q, size_t ldq, void* q_out, size_t ldqo, const void* k,
+                                     size_t ldk, const void* v, size_t ldv) {
+    const char* what = "kv_append_rope";
+    KvDev cd;
+    KvBatchDev bd;
+    RopeDev r{};
+    int rc = hc_engine_activate(e);
+    if (!rc) rc = check_cache(c, &cd);
+    if (!rc) rc = check_batch(e, c, b, &bd);
+    if (!rc) rc = check_rope(rope, &r);
+    if (rc) return rc;
+    if (r.dim != c->head_dim)
+        return hc_set_error(HC_ERR_INVALID, "%s: the rope's head_dim is %d, the cache's %d", what, r.dim, c->head_dim);
+    if (!rope_chunks(r))
+        return hc_set_error(HC_ERR_UNSUPPORTED, "%s: rot_dim %d (a multiple of 16, in pairs of 8; hc_rope_dev takes the others)",
+                            what, r.rot);
+    if (n_heads == 0 || n_heads > 65535 || c->n_heads > 65535 ||
+        (unsigned long long)b->n_tok * (n_heads + 2ull * c->n_heads) > INT32_MAX)
+        return hc_set_error(HC_ERR_INVALID, "%s: %d tokens of %zu query and %d kv heads", what, b->n_tok, n_heads, c->n_heads);
+    if (b->n_tok == 0 || b->n_seq == 0) return HC_OK;
+    const size_t width = n_heads * c->head_dim, kw = (size_t)c->n_heads * c->head_dim, es = elem_bytes(dtype), n = b->n_tok;
+    rc = check_rows(what, dtype, q, ldq, width);
+    if (!rc) rc = check_rows(what, dtype, q_out, ldqo, width);
+    if (!rc) rc = check_rows(what, dtype, k, ldk, kw);
+    if (!rc) rc = check_rows(what, dtype, v, ldv, kw);
+    if (rc) return rc;
+    if ((!(q == q_out && ldq == ldqo) && !rows_apart(q, ldq, width, q_out, ldqo, width, n, es)) ||
+        !rows_apart(k, ldk, kw, q_out, ldqo, width, n, es) || !rows_apart(v, ldv, kw, q_out, ldqo, width, n, es))
+        return hc_set_error(HC_ERR_INVALID, "%s: q_out must be q itself or overlap neither q, k nor v", what);
+    const RopeAppend a{q, k, v, q_out, (long long)ldq, (long long)ldqo, (long long)ldk, (long long)ldv, (int)n_heads};
+    const cudaError_t ce = launch_kv_append_rope(c->type, dtype, c->head_dim, r, cd, bd, a, e->stream);
+    return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "kv_append_rope launch");
+}
+
+// ------------------------------------------------------------------ the cache's bookkeeping
+extern "C" int hc_kv_pages_scratch(int n_pages, size_t* out) {
+    if (!out || n_pages < 1) return hc_set_error(HC_ERR_INVALID, "kv pages: n_pages %d, or a null pointer", n_pages);
+    *out = kv_pages_scratch(n_pages);
+    return HC_OK;
+}
+
+// The pages' description, and its layers by kMaxLayers (room for `most` such groups).
+static int check_pages(const char* what, hc_engine* e, const hc_kv_pages* p, PagesDev* d, KvLayers* layers, int most, int* groups) {
+    int rc = hc_engine_activate(e);
+    if (rc) return rc;
+    if (!p) return hc_set_error(HC_ERR_INVALID, "%s: null pages", what);
+    if (p->n_layers < 1 || !p->layers) return hc_set_error(HC_ERR_INVALID, "%s: no layers", what);
+    if (p->n_layers > most * kMaxLayers)
+        return hc_set_error(HC_ERR_INVALID, "%s: %d layers (at most %d)", what, p->n_layers, most * kMaxLayers);
+    const hc_kv_cache* const c0 = p->layers;
+    for (int i = 0; i < p->n_layers; ++i) {
+        const hc_kv_cache* const c = p->layers + i;
+        KvDev k;
+        rc = check_cache(c, &k);
+        if (rc) return rc;
+        if (c->type != c0->type || c->n_pages != c0->n_pages || c->n_heads != c0->n_heads || c->page_size != c0->page_size ||
+            c->head_dim != c0->head_dim || c->page_stride != c0->page_stride || c->head_stride != c0->head_stride ||
+            c->row_stride != c0->row_stride || c->scale_page_stride != c0->scale_page_stride)
+            return hc_set_error(HC_ERR_INVALID, "%s: layer %d has another shape than the first", what, i);
+        KvLayers& y = layers[i / kMaxLayers];
+        const int at = i % kMaxLayers;
+        y.k[at] = k.k;
+        y.v[at] = k.v;
+        y.ks[at] = c->type == T_I8 ? k.ks : nullptr;
+        y.vs[at] = c->type == T_I8 ? k.vs : nullptr;
+        if (at == 0) {
+            y.page = k.page;
+            y.head = k.head;
+            y.row = k.row;
+            y.spage = k.spage;
+            y.n_heads = c->n_heads;
+            y.row_bytes = c->head_dim * (c->type == T_I8 ? 1 : 2);
+        }
+        y.n = at + 1;
+    }
+    *groups = (p->n_layers + kMaxLayers - 1) / kMaxLayers;
+    if (p->n_slots < 0 || p->max_pages < 0)
+        return hc_set_error(HC_ERR_INVALID, "%s: negative size n_slots=%d max_pages=%d", what, p->n_slots, p->max_pages);
+    if ((long long)p->max_pages * c0->page_size > (1 << 30))
+        return hc_set_error(HC_ERR_INVALID, "%s: %d pages of %d reach past 2^30 tokens", what, p->max_pages, c0->page_size);
+    if (p->n_slots && (!p->page_table || !p->kv_len))
+        return hc_set_error(HC_ERR_INVALID, "%s: null page table or kv_len", what);
+    if (!p->refs || !p->scratch) return hc_set_error(HC_ERR_INVALID, "%s: null refs or scratch", what);
+    if (p->table_stride < (size_t)p->max_pages)
+        return hc_set_error(HC_ERR_INVALID, "%s: table stride %zu < max_pages %d", what, p->table_stride, p->max_pages);
+    d->table = p->page_table;
+    d->stride = (long long)p->table_stride;
+    d->len = p->kv_len;
+    d->refs = p->refs;
+    d->n_slots = p->n_slots;
+    d->max_pages = p->max_pages;
+    d->n_pages = c0->n_pages;
+    d->page_size = c0->page_size;
+    d->by_page = FastDiv((uint32_t)c0->page_size);
+    const size_t moves = d->n_pages > HC_KV_SEQS ? d->n_pages : HC_KV_SEQS;
+    d->moves = p->scratch;
+    d->item = d->moves + 16;
+    d->src = d->item + 4 * HC_KV_SEQS;
+    d->dst = d->src + moves;
+    d->rows = d->dst + moves;
+    d->free = d->rows + moves;
+    d->err = e->d_err;
+    return HC_OK;
+}
+constexpr int kLayerGroups = 4;
+
+static int check_items(const char* what, int n, const void* a, const void* b) {
+    if (n < 0 || n > HC_KV_MAX_SEQ) return hc_set_error(HC_ERR_INVALID, "%s: %d sequences (at most %d)", what, n, HC_KV_MAX_SEQ);
+    if (n && (!a || !b)) return hc_set_error(HC_ERR_INVALID, "%s: null array", what);
+    return HC_OK;
+}
+
+extern "C" int hc_kv_fork_dev(hc_engine* e, const hc_kv_pages* p, int n, const int32_t* parents, const int32_t* children) {
+    PagesDev d{};
+    KvLayers y[kLayerGroups];
+    int groups = 0, rc = check_pages("kv_fork", e, p, &d, y, kLayerGroups, &groups);
+    if (!rc) rc = check_items("kv_fork", n, parents, children);
+    if (rc || n == 0) return rc;
+    const cudaError_t ce = launch_kv_fork(d, y, groups, n, parents, children, e->num_sms, e->stream);
+    return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "kv_fork launch");
+}
+
+extern "C" int hc_kv_resize_dev(hc_engine* e, const hc_kv_pages* p, int n, const int32_t* slots, const int32_t* lens) {
+    PagesDev d{};
+    KvLayers y[kLayerGroups];
+    int groups = 0, rc = check_pages("kv_resize", e, p, &d, y, kLayerGroups, &groups);
+    if (!rc) rc = check_items("kv_resize", n, slots, lens);
+    if (rc || n == 0) return rc;
+    const cudaError_t ce = launch_kv_resize(d, y, groups, n, slots, lens, e->num_sms, e->stream);
+    return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "kv_resize launch");
+}
+
+extern "C" int hc_kv_compact_dev(hc_engine* e, const hc_kv_pages* p, int32_t* moved) {
+    PagesDev d{};
+    KvLayers y[kLayerGroups];
+    int groups = 0;
+    const int rc = check_pages("kv_compact", e, p, &d, y, kLayerGroups, &groups);
+    if (rc) return rc;
+    const cudaError_t ce = launch_kv_compact(d, y, groups, moved, e->num_sms, e->stream);
+    return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "kv_compact launch");
 }

@@ -38,11 +38,13 @@ struct PeerState {
 };
 
 // Paged attention's partial results of split tiles and their counters (zero between calls): one for the calls
-// on a stream, and one for the calls captured on it, whose graphs may run beside the stream's own calls.
+// on a stream, and one for the calls captured on it, whose graphs may run beside the stream's own calls.  `base`: what
+// attention over a shared prefix keeps between its kernels.  It grows with the calls; as a captured graph holds its
+// address, a captured call that needs more than there is gets a new workspace.
 struct AttnWs {
     cudaStream_t stream = nullptr;
     bool captured = false;
-    DevBuf part, count;
+    DevBuf part, count, base;
     AttnWs* next = nullptr;
 };
 

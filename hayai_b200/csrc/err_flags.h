@@ -8,6 +8,7 @@ namespace hc {
 constexpr int kErrRange = 1;    // an activation outside f16's range
 constexpr int kErrWait = 2;     // a bounded wait ran out
 constexpr int kErrKvRange = 4;  // a page number, length or offset out of range
+constexpr int kErrKvFull = 8;   // no free page was left
 
 struct ErrReport {
     int code;
@@ -23,6 +24,7 @@ constexpr ErrReport err_report(int flag) {
     if (flag & kErrWait) return {HC_ERR_TIMEOUT, "a bounded device wait expired", clear};
     if (flag & kErrKvRange)
         return {HC_ERR_INVALID, "kv batch: a page number, length or offset on the device is out of range", clear};
+    if (flag & kErrKvFull) return {HC_ERR_INVALID, "kv pages: no free page was left for all that was asked for", clear};
     return {HC_ERR_CUDA, "unknown device error flag", clear};
 }
 

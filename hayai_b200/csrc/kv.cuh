@@ -32,9 +32,10 @@ struct KvBatchDev {
 // not fit the batch cut to it (and the error flag set).
 struct KvSeq {
     int q0, q1, len;
+    int first;  // attention over what comes behind a shared prefix: its first position
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvBatchDev& b, int cap, int s) {
-    KvSeq r;
+    KvSeq r{};
     const int a = __ldg(b.q_start + s), e = __ldg(b.q_start + s + 1), n = __ldg(b.kv_len + s);
     r.q0 = min(max(a, 0), b.n_tok);
     r.q1 = min(max(e, r.q0), b.n_tok);

@@ -10,70 +10,9 @@
 //
 // Measured: 30080 tokens of 8 heads of 128 from bf16 into 8-bit pages 43 us in a graph (4.3 TB/s), 31720
 // back into bf16 36 us (5.4 TB/s, 84 % of the copy rate); one token 1.8 us in a graph.
-#include "kv_launch.h"
+#include "kv_rows.cuh"
 
 namespace hc {
-
-// Where the batch's token t lives: its page's and row's offset in the cache (64-byte units, of
-// head 0) and in the scales, or false where it has no place.
-template <int GL>
-__device__ __forceinline__ bool kv_slot(const KvDev& c, const KvBatchDev& b, const FastDiv& by_page, int t, uint32_t& at,
-                                        long long& sat) {
-    const KvPlace k = kv_find_seq<GL>(b, t);
-    const int pos = k.len - k.next + t;
-    if (k.s < 0 || pos < 0) return false;
-    const int p = by_page(pos), r = pos - p * c.page_size;
-    const int page = p < b.max_pages ? __ldg(b.table + k.s * b.table_stride + p) : -1;
-    if ((unsigned)page >= (unsigned)c.n_pages) {
-        atomicOr(b.err, kErrKvRange);
-        return false;
-    }
-    at = (uint32_t)page * c.page + (uint32_t)r * c.row;
-    sat = page * c.spage + r;
-    return true;
-}
-
-// The grid's last block looks the batch's offsets and lengths over (the others read no more of them than their
-// tokens' places take) and sets the error flag where attention would cut them.
-__device__ __forceinline__ bool kv_check_block(const KvDev& c, const KvBatchDev& b) {
-    if (blockIdx.x != gridDim.x - 1) return false;
-    for (int s = threadIdx.x; s < b.n_seq; s += blockDim.x) kv_seq(b, b.max_pages * c.page_size, s);
-    return true;
-}
-
-template <class C>
-__device__ __forceinline__ C* kv_elem(uint8_t* base, uint32_t units) {
-    return reinterpret_cast<C*>(base + (unsigned long long)units * 64);
-}
-
-// Codes of 8 values of a row with largest |x| m and scale s, four to a word.  The quotient rounded as
-// IEEE division rounds it takes three instructions a value where the row shares the divisor, by
-// Markstein's theorem (IBM J. Res. Dev. 34, 1990): with r the reciprocal of s rounded to nearest and
-// q = x r, fma(fma(-q, s, x), r, q) is x / s rounded to nearest, unless s has a significand of all
-// ones.  That, and rows whose scale or remainders are not normal numbers, are divided.  (An estimate
-// with a division where it lies near a half is slower: ratios of 8-bit significands meet halves in
-// two of three warps.)  1.5 * 2^23 added rounds to whole numbers, ties to even, and leaves them in the
-// low bits in two's complement.
-__device__ __forceinline__ void kv_codes(const float (&x)[8], float m, float s, uint32_t (&q)[2]) {
-    constexpr float kMagic = 12582912.f;
-    float f[8];
-    if (m >= 1e-30f && m <= 1e30f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu) {
-        const float r = __frcp_rn(s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float y = x[i] * r;
-            f[i] = fmaf(fmaf(-y, s, x[i]), r, y) + kMagic;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            f[i] = (s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f) : 0.f) + kMagic;
-    }
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-        q[w] = prmt(prmt(__float_as_uint(f[4 * w]), __float_as_uint(f[4 * w + 1]), 0x0040u),
-                    prmt(__float_as_uint(f[4 * w + 2]), __float_as_uint(f[4 * w + 3]), 0x0040u), 0x5410u);
-}
 
 // One group of D / 8 lanes per (token, U heads): each lane holds 8 values of each row, k and v.
 // Bound by memory: every value is read once and written once.
@@ -94,7 +33,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvDev c, KvBatchDev b, K
         for (int w = 0; w < 2; ++w) raw[w][u] = Elem<T>::load8(src[w] + min(h0 + u, c.n_heads - 1) * D);
     uint32_t at = 0;
     long long sat = 0;
-    const bool has = kv_slot<GL>(c, b, by_page, t, at, sat) && real;
+    int pos;
+    const bool has = kv_slot<GL>(c, b, by_page, t, at, sat, pos) && real;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int h = h0 + u;
@@ -132,7 +72,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvDev c, KvBatchDev b, KvR
     const int t = (int)min(g / chunks, (long long)b.n_tok - 1), h0 = (int)(g % chunks) * U;
     uint32_t at = 0;
     long long sat = 0;
-    if (!kv_slot<GL>(c, b, by_page, t, at, sat) || g >= (long long)b.n_tok * chunks) return;
+    int pos;
+    if (!kv_slot<GL>(c, b, by_page, t, at, sat, pos) || g >= (long long)b.n_tok * chunks) return;
     typename Elem<C>::Raw raw[2][U];
     float sc[2][U];
 #pragma unroll

@@ -21,6 +21,30 @@ cudaError_t launch_kv_append(int cache_type, int dtype, int head_dim, const KvDe
 cudaError_t launch_kv_read(int cache_type, int dtype, int head_dim, const KvDev& c, const KvBatchDev& b,
                            const KvRows& r, cudaStream_t s);
 
+// hc_rope as the kernels get it.
+struct RopeDev {
+    int pairs, dim, rot;
+    float amplitude;
+    unsigned long long turns[128];
+};
+struct RopeRows {
+    const int* pos;
+    const void* x;
+    void* out;
+    long long ldx, ldo;
+    int n_tok, heads;
+};
+struct RopeAppend {
+    const void *q, *k, *v;
+    void* q_out;
+    long long ldq, ldqo, ldk, ldv;
+    int heads;
+};
+// wide: sizes, strides and addresses in whole 16 bytes and chunks of 8 values.
+cudaError_t launch_rope(int dtype, const RopeDev& r, const RopeRows& a, bool wide, cudaStream_t s);
+cudaError_t launch_kv_append_rope(int cache_type, int dtype, int head_dim, const RopeDev& r, const KvDev& c,
+                                  const KvBatchDev& b, const RopeAppend& a, cudaStream_t s);
+
 // Division of 0 <= n < 2^31 by d >= 1 as a multiplication: with 2^k >= d and m = ceil(2^(31+k) / d),
 // floor(n m / 2^(31+k)) = floor(n / d), as m d - 2^(31+k) < d <= 2^k.
 struct FastDiv {
@@ -49,6 +73,37 @@ struct SmemOptIn {
     }
 };
 
+// hc_kv_pages as the kernels get it, with its scratch divided.
+struct PagesDev {
+    int* table;  // [n_slots][stride]
+    long long stride;
+    int *len, *refs;  // [n_slots], [n_pages]
+    int n_slots, max_pages, n_pages, page_size;
+    FastDiv by_page;
+    int* moves;             // the number of copies
+    int* item;              // 4 x HC_KV_SEQS
+    int *src, *dst, *rows;  // the copies: pages, and rows from the first (null: all)
+    int* free;              // free pages that the call takes
+    int* err;
+};
+constexpr size_t kv_pages_scratch(int n_pages) {
+    return 16 + 4 * (size_t)HC_KV_SEQS + 3 * (size_t)(n_pages > HC_KV_SEQS ? n_pages : HC_KV_SEQS) + n_pages;
+}
+// Layers of one shape: strides in 64-byte units as in KvDev.
+constexpr int kMaxLayers = 64;
+struct KvLayers {
+    uint8_t *k[kMaxLayers], *v[kMaxLayers];
+    float *ks[kMaxLayers], *vs[kMaxLayers];  // null: 16-bit pages
+    uint32_t page, head, row;
+    long long spage;
+    int n, n_heads, row_bytes;
+};
+cudaError_t launch_kv_fork(const PagesDev& p, const KvLayers* layers, int groups, int n, const int* parents,
+                           const int* children, int sms, cudaStream_t s);
+cudaError_t launch_kv_resize(const PagesDev& p, const KvLayers* layers, int groups, int n, const int* slots,
+                             const int* lens, int sms, cudaStream_t s);
+cudaError_t launch_kv_compact(const PagesDev& p, const KvLayers* layers, int groups, int* moved, int sms, cudaStream_t s);
+
 struct AttnArgs {
     KvDev c;
     KvBatchDev b;
@@ -63,9 +118,25 @@ struct AttnArgs {
     int max_rows;          // the host's bound on a sequence's rows of one kv head (new tokens x group)
     int row_min, row_max;  // sequences with fewer or more rows are left to another kernel
     int over;              // places of the line that stand for a tile's start and end
+    // A shared prefix (attn_shared.cu).  One call writes the groups' results to `base`, the other starts every
+    // sequence behind its prefix and adds them.
+    const int* first;      // [n_seq] positions that a sequence leaves out, or null
+    const int* table_row;  // [n_seq] rows of the page table, or null: a sequence's own
+    float *base, *base_lse;  // [n_tok * heads][head_dim] and log 2 of the weights' sums
+    int to_base;
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
     int* count;            // 32 counters per block, zero between calls
 };
+
+// hc_kv_shared as the kernels get it, and the groups as sequences of their own.
+struct KvSharedDev {
+    const int *seq_start, *length;
+    int n;
+    int *first;                // [n_seq]
+    int *q_start, *len, *row;  // [n + 1], [n], [n]
+};
+constexpr size_t kSharedInts = 4 * (size_t)HC_KV_SEQS + 4;
+cudaError_t launch_attn_groups(const KvBatchDev& b, const KvSharedDev& g, int cap, cudaStream_t s);
 
 // Partial results of the kernel for few rows: bytes for each block.
 constexpr size_t kFewPartBytes = 2 * 13 * 16 * (128 + 2) * 4;

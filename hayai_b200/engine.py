@@ -195,6 +195,8 @@ class CudaEngine:
         # the calls of a decode step's every layer, looked up once
         self._kv_append, self._kv_read, self._attn_paged = (lib().hc_kv_append_dev, lib().hc_kv_read_dev,
                                                             lib().hc_attn_paged_dev)
+        self._attn_shared, self._rope, self._kv_append_rope = (lib().hc_attn_shared_dev, lib().hc_rope_dev,
+                                                               lib().hc_kv_append_rope_dev)
 
     def close(self) -> None:
         if self.handle:
@@ -466,6 +468,80 @@ class CudaEngine:
                               cache.default_scale if scale is None else scale, causal, _positions(window), _positions(sink))
         if rc:
             _check(rc)
+
+    def attn_shared_dev(self, cache, batch, shared, q, out, scale: float | None = None, lse=None) -> None:
+        """attn_paged_dev (causal) where groups of the batch's sequences share their first tokens (KvShared), which
+        are read once for a group.  The same calls may be in flight together as of attn_paged_dev."""
+        self._kv_here(cache, batch)
+        if shared.index != self.device:
+            raise ValueError(f"the groups must be on the engine's device {self.device}")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        t, ldq = cache.rows(batch, q, heads, "q")
+        to, ldo = cache.rows(batch, out, heads, "out")
+        if to != t:
+            raise ValueError("q and out need one type")
+        rc = self._attn_shared(self.handle, cache.ref, batch.ref, shared.ref, t, heads, q.data_ptr(), ldq, out.data_ptr(), ldo,
+                               None if lse is None else cache.lse_ptr(lse, q),
+                               cache.default_scale if scale is None else scale)
+        if rc:
+            _check(rc)
+
+    # ---------------------------------------------------------------- rotary positions
+    def rope_dev(self, rope, positions, x, out=None) -> None:
+        """Turn rows x [n_tok][n_heads][head_dim] by int32 positions [n_tok] (Rope), into out or in place."""
+        out = x if out is None else out
+        n = positions.shape[0] if positions.dim() == 1 else -1
+        if str(positions.dtype) != "torch.int32" or n < 0 or (n > 1 and positions.stride(0) != 1):
+            raise ValueError("positions must be a contiguous int32 tensor [n_tok]")
+        t, heads, ldx = rope.rows(x, "x", n)
+        _, _, ldo = rope.rows(out, "out", n, x)
+        if not x.get_device() == out.get_device() == positions.get_device() == self.device:
+            raise ValueError(f"positions, x and out must be on the engine's device {self.device}")
+        rc = self._rope(self.handle, rope.ref, t, n, heads, positions.data_ptr(), x.data_ptr(), ldx, out.data_ptr(), ldo)
+        if rc:
+            _check(rc)
+
+    def kv_append_rope_dev(self, cache, batch, rope, q, k, v, q_out=None) -> None:
+        """kv_append_dev for keys that are turned by their positions in the cache on the way, and the queries
+        q [n_tok][n_heads][head_dim] with them (into q_out or in place), in one launch."""
+        self._kv_here(cache, batch)
+        q_out = q if q_out is None else q_out
+        heads = q.shape[1] if q.dim() == 3 else 0
+        t, ldq = cache.rows(batch, q, heads, "q")
+        to, ldqo = cache.rows(batch, q_out, heads, "q_out")
+        tk, *kv = cache.pair(batch, k, v)
+        if not t == to == tk:
+            raise ValueError("q, k, v and q_out need one type")
+        rc = self._kv_append_rope(self.handle, cache.ref, batch.ref, rope.ref, t, heads, q.data_ptr(), ldq, q_out.data_ptr(),
+                                  ldqo, *kv)
+        if rc:
+            _check(rc)
+
+    # ---------------------------------------------------------------- the cache's bookkeeping
+    def _pages_here(self, pages) -> None:
+        if pages.index != self.device:
+            raise ValueError(f"the pages must be on the engine's device {self.device}")
+
+    def kv_fork_dev(self, pages, parents, children) -> None:
+        """Slot children[i] becomes a copy of slot parents[i] (KvPages; int32 tensors): whole pages are shared, a
+        partly filled last page is copied to one of the child's own, in every layer.  Children hold nothing before."""
+        self._pages_here(pages)
+        _check(lib().hc_kv_fork_dev(self.handle, pages.ref, *pages.items(parents, children, "parents and children")))
+
+    def kv_resize_dev(self, pages, slots, lens) -> None:
+        """Slot slots[i] gets the length lens[i] (int32 tensors): pages are taken, the lowest free ones first, or
+        given back; a length of 0 lets the slot go."""
+        self._pages_here(pages)
+        _check(lib().hc_kv_resize_dev(self.handle, pages.ref, *pages.items(slots, lens, "slots and lens")))
+
+    def kv_compact_dev(self, pages, moved=None) -> None:
+        """The pages in use move to the lowest numbers, in every layer, and the tables follow.  moved: None, or
+        an int32 tensor [n_pages] that receives every page's new number."""
+        self._pages_here(pages)
+        if moved is not None and (str(moved.dtype) != "torch.int32" or moved.shape != (pages.n_pages,) or
+                                  moved.get_device() != self.device or not moved.is_contiguous()):
+            raise ValueError("moved must be a contiguous int32 tensor [n_pages] on the engine's device")
+        _check(lib().hc_kv_compact_dev(self.handle, pages.ref, None if moved is None else moved.data_ptr()))
 
     def router_scores_dev(self, router_w, x, scores, n_tok: int) -> None:
         E, D = router_w.shape

@@ -2,14 +2,20 @@
 
 ``KvCache`` is one layer's pool of pages and ``KvBatch`` the sequences of a step
 (hc_kv_cache and hc_kv_batch of include/hayai_cuda.h); ``CudaEngine.kv_append_dev``,
-``kv_read_dev`` and ``attn_paged_dev`` take both.  They keep references to their tensors and
-no copies: a step that changes page numbers, lengths or offsets in place needs no new batch.
+``kv_read_dev`` and ``attn_paged_dev`` take both.  ``KvShared`` names the sequences of a batch that
+share their first tokens, for ``attn_shared_dev``; ``KvPages`` is the bookkeeping of all layers' pools,
+which ``kv_fork_dev``, ``kv_resize_dev`` and ``kv_compact_dev`` change; ``Rope`` says how queries and keys
+are turned by their positions (``rope_dev``, ``kv_append_rope_dev``).  They keep references to their
+tensors and no copies: a step that changes page numbers, lengths or offsets in place needs no new batch.
 The reference keeps a sink-and-window INT8 cache of one sequence on the host
 (crates/hayai-cpu/src/kv_cache.rs).
 """
 from __future__ import annotations
 
 import ctypes
+import math
+
+from . import _lib
 
 F32, F16, I8, BF16 = 0, 1, 24, 30  # GgmlType ids
 _ROW_TYPES, _CACHE_TYPES = {}, {}  # by torch's types: the package imports without torch, descriptions need it
@@ -34,6 +40,22 @@ class _Batch(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("n_seq", "n_tok", "max_new", "max_pages")] + \
                [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_size_t), ("q_start", ctypes.c_void_p),
                 ("kv_len", ctypes.c_void_p)]
+
+
+class _Shared(ctypes.Structure):
+    _fields_ = [("n_groups", ctypes.c_int), ("max_new", ctypes.c_int), ("seq_start", ctypes.c_void_p),
+                ("length", ctypes.c_void_p)]
+
+
+class _Pages(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_slots", "max_pages", "n_layers")] + \
+               [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_size_t)] + \
+               [(n, ctypes.c_void_p) for n in ("kv_len", "refs", "scratch", "layers")]
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("layout", "head_dim", "rot_dim")] + \
+               [("amplitude", ctypes.c_float), ("turns", ctypes.c_uint64 * 128)]
 
 
 def _need(ok: bool, what: str) -> None:
@@ -123,3 +145,106 @@ class KvBatch:
         self.struct = _Batch(n_seq, n_tok, max_new, max_pages, page_table.data_ptr(), stride, q_start.data_ptr(),
                              kv_len.data_ptr())
         self.ref = ctypes.addressof(self.struct)
+
+
+class KvShared:
+    """Groups of a batch's sequences that share their first tokens: group g is the sequences
+    seq_start[g] to seq_start[g + 1] (int32 [n_groups + 1]), whose first length[g] positions (int32
+    [n_groups]) are the same, and are read by the first one's pages.  max_new: a bound on any group's new
+    tokens, where the program knows one."""
+
+    def __init__(self, seq_start, length, max_new: int = 0):
+        torch = _torch()
+        for t in (seq_start, length):
+            _need(t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.device == seq_start.device,
+                  "seq_start and length must be int32 CUDA tensors of one device and one axis")
+            _need(t.shape[0] <= 1 or t.stride(0) == 1, "seq_start and length must be contiguous")
+        _need(seq_start.shape[0] == length.shape[0] + 1, "length must hold n_groups and seq_start n_groups + 1")
+        _need(max_new >= 0, "max_new must not be negative")
+        self._keep = (seq_start, length)
+        self.index = seq_start.get_device()
+        self.struct = _Shared(length.shape[0], min(max_new, 2**31 - 1), seq_start.data_ptr(), length.data_ptr())
+        self.ref = ctypes.addressof(self.struct)
+
+
+class KvPages:
+    """The bookkeeping of a pool that sequences share in every layer: caches, a KvCache for each layer, all
+    of one shape; page_table int32 [n_slots][max_pages], kv_len int32 [n_slots] (the tokens that a slot
+    holds, 0 for an unused one) and refs int32 [n_pages] (how many table entries in use name a page, 0
+    for a free one).  The calls change the three in place; page_table and kv_len serve as a KvBatch's."""
+
+    def __init__(self, caches, page_table, kv_len, refs):
+        torch = _torch()
+        caches = list(caches)
+        _need(len(caches) > 0, "caches must hold at least one KvCache")
+        for t, d in ((page_table, 2), (kv_len, 1), (refs, 1)):
+            _need(t.is_cuda and t.dtype == torch.int32 and t.dim() == d and t.device == page_table.device,
+                  "page_table, kv_len and refs must be int32 CUDA tensors of one device, of 2, 1 and 1 axes")
+            _need(t.shape[-1] <= 1 or t.stride(-1) == 1, "page_table rows, kv_len and refs must be contiguous")
+        n_slots, max_pages = page_table.shape
+        self.index, self.n_pages = page_table.get_device(), caches[0].struct.n_pages
+        _need(all(c.index == self.index for c in caches), "the caches must be on page_table's device")
+        _need(kv_len.shape[0] == n_slots and refs.shape[0] == self.n_pages, "kv_len must hold n_slots and refs n_pages")
+        stride = page_table.stride(0) if n_slots > 1 else max_pages
+        _need(stride >= max_pages, "page_table rows overlap")
+        size = ctypes.c_size_t()
+        rc = _lib.lib().hc_kv_pages_scratch(self.n_pages, ctypes.byref(size))
+        _need(rc == 0, "the caches hold no pages")
+        scratch = torch.empty(size.value, dtype=torch.int32, device=page_table.device)
+        layers = (_Cache * len(caches))(*[c.struct for c in caches])
+        self._keep = (caches, page_table, kv_len, refs, scratch, layers)
+        self.struct = _Pages(n_slots, max_pages, len(caches), page_table.data_ptr(), stride, kv_len.data_ptr(),
+                             refs.data_ptr(), scratch.data_ptr(), ctypes.addressof(layers))
+        self.ref = ctypes.addressof(self.struct)
+
+    def items(self, a, b, what: str):
+        """(n, pointers) of a call's two int32 arrays."""
+        for t in (a, b):
+            if t.dim() != 1 or t.shape != a.shape or str(t.dtype) != "torch.int32" or t.get_device() != self.index or \
+                    (t.shape[0] > 1 and t.stride(0) != 1):
+                raise ValueError(f"{what} must be contiguous int32 tensors of one length on the pages' device")
+        return a.shape[0], a.data_ptr(), b.data_ptr()
+
+
+class Rope:
+    """Rotary positions: how the first rot_dim values of a head (0: all) are turned, in pairs (i, i + rot_dim / 2)
+    (layout "half") or (2 i, 2 i + 1) ("pairs"), by the angles position * base^(-2 i / rot_dim) / factors[i].
+
+    Longer contexts: ``factor`` alone divides every frequency (linear scaling).  With ``original``, the
+    context that the model was trained with, a frequency that made r turns there is divided by bands: wholly
+    where r <= low, not at all where r >= high, and in proportion between.  ``amplitude`` multiplies the
+    turned values (0.1 ln factor + 1 with bands: YaRN).  factors: a sequence of rot_dim / 2 positive numbers,
+    as a GGUF file's rope_freqs."""
+
+    LAYOUTS = {"half": 0, "pairs": 1}
+
+    def __init__(self, head_dim: int, rot_dim: int = 0, base: float = 10000.0, layout: str = "half", factor: float = 1.0,
+                 original: float = 0, low: float = 0.0, high: float = 0.0, factors=None, amplitude: float = 1.0):
+        _need(layout in self.LAYOUTS, f"layout must be one of {sorted(self.LAYOUTS)}")
+        _need(math.isfinite(amplitude), "amplitude must be finite")
+        rot_dim = rot_dim or head_dim
+        given = None
+        if factors is not None:
+            factors = [float(f) for f in factors]
+            _need(len(factors) == rot_dim // 2, "factors must hold rot_dim / 2 numbers")
+            given = (ctypes.c_float * len(factors))(*factors)
+        self.struct = _Rope()
+        rc = _lib.lib().hc_rope_init(ctypes.addressof(self.struct), self.LAYOUTS[layout], head_dim, rot_dim, base, factor,
+                                     original, low, high, given, amplitude)
+        _need(rc == 0, _lib.lib().hc_last_error().decode(errors="replace"))
+        self.ref = ctypes.addressof(self.struct)
+        self.head_dim, self.rot_dim = head_dim, rot_dim
+
+    def rows(self, x, what: str, n: int, like=None):
+        """(type id, heads, leading dimension) of packed rows x [n_tok][heads][head_dim]."""
+        _torch()
+        t = _ROW_TYPES.get(x.dtype)
+        if t is None or not x.is_cuda or x.dim() != 3 or x.shape[0] != n or x.shape[2] != self.head_dim or \
+                (like is not None and (x.shape != like.shape or x.dtype != like.dtype)):
+            raise ValueError(f"{what} must be float32, float16 or bfloat16 [n_tok={n}][heads][head_dim={self.head_dim}] on the "
+                             "engine's device, and rows that go together of one shape and type")
+        ld, head, one = x.stride()
+        heads = x.shape[1]
+        if x.numel() and (one != 1 or (head != self.head_dim and heads > 1)):
+            raise ValueError(f"{what} must have contiguous rows (only the token axis may be strided)")
+        return t, heads, ld if n > 1 else heads * self.head_dim

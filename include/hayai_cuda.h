@@ -319,6 +319,93 @@ int hc_attn_paged_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batc
                       const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale, int causal, int window,
                       int sink);
 
+/* Sequences of a batch that share their first tokens (an instruction, a document): group g is the batch's
+ * sequences [seq_start[g], seq_start[g+1]) (seq_start ascends; sequences in no group share nothing), whose
+ * first length[g] positions hold the same keys and values, as hc_kv_fork_dev leaves them.  They are read by the
+ * first sequence's pages.  Of a length past the tokens that every sequence of the group had before its new ones,
+ * that much is shared.  max_new is the host's bound on any group's new tokens (0: n_tok); a group with more is
+ * still computed, at lower speed. */
+typedef struct hc_kv_shared {
+    int n_groups, max_new;
+    const int32_t *seq_start, *length; /* n_groups + 1, n_groups; device */
+} hc_kv_shared;
+
+/* hc_attn_paged_dev (causal, without a window) for groups of sequences with shared tokens, which are read once
+ * for the group and seen by all its rows together.  Its notes hold here too.  Between the call's kernels the
+ * prefixes' results lie in the engine, in a workspace of about n_tok * n_heads * (head_dim + 1) floats that grows
+ * with the calls. */
+int hc_attn_shared_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, const hc_kv_shared* shared,
+                       int dtype, size_t n_heads, const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale);
+
+/* ---- rotary positions -----------------------------------------------------------------
+ * Counterpart of the reference's RoPE (crates/hayai-cpu/src/attention.rs).  The first rot_dim values of a head
+ * are rot_dim / 2 pairs, (i, i + rot_dim / 2) in the half layout, (2 i, 2 i + 1) in pairs; at position p pair i,
+ * (a, b), becomes amplitude * (a c - b s, a s + b c) with c = cos(p t_i), s = sin(p t_i).  The rest of a head
+ * stays.  The frequencies are kept as fractions of a turn, 2^64 to the turn, so that every position of 32
+ * bits, negative ones as well, has its angle to 2^-32 of a turn. */
+#define HC_ROPE_HALF 0
+#define HC_ROPE_PAIRS 1
+#define HC_ROPE_MAX 128
+typedef struct hc_rope {
+    int layout, head_dim, rot_dim; /* both even, head_dim at most 2 * HC_ROPE_MAX */
+    float amplitude;
+    uint64_t turns[HC_ROPE_MAX]; /* t_i / 2 pi of a turn */
+} hc_rope;
+
+/* Fill in *out (host memory only): t_i = base^(-2 i / rot_dim) / factors[i] (NULL: ones; rot_dim / 2 of them, as a
+ * GGUF file's rope_freqs), rot_dim 0 for the whole head.  Longer contexts: original = 0 divides every t_i by `factor`
+ * (linear scaling); original > 0, the context that the model was trained with, divides by bands: with the r =
+ * original * t_i / 2 pi turns that it made there and g = (r - low) / (high - low) held to [0, 1], t_i becomes
+ * t_i * ((1 - g) / factor + g).  (With amplitude 0.1 ln factor + 1 that is YaRN, Peng et al. 2023.) */
+int hc_rope_init(hc_rope* out, int layout, int head_dim, int rot_dim, double base, double factor, double original,
+                 double low, double high, const float* factors, float amplitude);
+
+/* Turn the rows x [n_tok][n_heads * head_dim] (leading dimension ldx; dtype F32, F16 or BF16) by positions [n_tok]
+ * into out, which is x itself or does not overlap it. */
+int hc_rope_dev(hc_engine* eng, const hc_rope* rope, int dtype, size_t n_tok, size_t n_heads, const int32_t* positions,
+                const void* x, size_t ldx, void* out, size_t ldo);
+
+/* hc_kv_append_dev for keys that are turned by their positions in the cache on the way, and the n_heads query heads
+ * with them, in one launch: q [n_tok][n_heads * head_dim] into q_out (q itself, or overlapping none of the rows).
+ * rot_dim is a multiple of 16, in pairs of 8.  8-bit codes are of the turned values, unrounded. */
+int hc_kv_append_rope_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, const hc_rope* rope, int dtype,
+                          size_t n_heads, const void* q, size_t ldq, void* q_out, size_t ldqo, const void* k, size_t ldk,
+                          const void* v, size_t ldv);
+
+/* ---- the cache's bookkeeping ------------------------------------------------------------
+ * Page tables, lengths and holders of the pool's pages, on the device.  Slot s holds kv_len[s] tokens in the pages
+ * page_table[s * table_stride + 0 ..]; refs[p] is the number of table entries in use that name page p, 0 for a free
+ * page.  Every layer's cache has the same shape and follows the same tables.  A slot's last page, where it is partly
+ * filled, belongs to the slot alone, so that appending never writes what another slot reads; whole pages may be
+ * shared.  An array of slots, kv_len and the page table serve as a hc_kv_batch's with n_seq = n_slots.
+ * Calls on one hc_kv_pages are made on one stream, or in an order that the caller sees to; they keep their plan in
+ * `scratch`.  What is out of range on the device (slots, lengths, page numbers), a slot twice in a call, and a fork
+ * into a slot that holds tokens are left out, and hc_sync reports HC_ERR_INVALID; so are items for which no free
+ * page is left, with all later ones that take pages. */
+typedef struct hc_kv_pages {
+    int n_slots, max_pages, n_layers;
+    int32_t* page_table; /* [n_slots][table_stride] */
+    size_t table_stride;
+    int32_t *kv_len, *refs;    /* [n_slots], [n_pages] */
+    int32_t* scratch;          /* hc_kv_pages_scratch(n_pages) ints */
+    const hc_kv_cache* layers; /* host array, at most 256 */
+} hc_kv_pages;
+int hc_kv_pages_scratch(int n_pages, size_t* out);
+
+/* Slot children[i] becomes a copy of slot parents[i] (device arrays; n at most HC_KV_MAX_SEQ): it shares the whole
+ * pages and gets the rest copied to a page of its own, the lowest free one, in the order of i.  Parents are taken as
+ * they were before the call. */
+int hc_kv_fork_dev(hc_engine* eng, const hc_kv_pages* pages, int n, const int32_t* parents, const int32_t* children);
+
+/* Slot slots[i] gets the length lens[i]: pages are taken (the lowest that were free before the call, in the order
+ * of i and of the table) or given back; a length of 0 lets the slot go.  Where the last page kept is shared and
+ * partly filled then, the slot gets a copy of it. */
+int hc_kv_resize_dev(hc_engine* eng, const hc_kv_pages* pages, int n, const int32_t* slots, const int32_t* lens);
+
+/* The pages in use move to the lowest numbers: of u of them, those numbered u and more go, in ascending order, to the
+ * free ones below.  The tables follow, and moved (NULL or [n_pages]) receives every page's new number. */
+int hc_kv_compact_dev(hc_engine* eng, const hc_kv_pages* pages, int32_t* moved);
+
 /* ---- synthetic data ----------------------------------------------------------------
  * Seeded N(mean, std^2) floats on the device (splitmix64 at a position + Box-Muller in
  * double; the same stream as the test oracle's generator up to last-bit differences of

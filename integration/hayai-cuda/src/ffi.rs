@@ -42,7 +42,36 @@ pub struct hc_kv_batch {
     pub q_start: *const i32,
     pub kv_len: *const i32,
 }
+#[repr(C)]
+pub struct hc_kv_shared {
+    pub n_groups: c_int,
+    pub max_new: c_int,
+    pub seq_start: *const i32,
+    pub length: *const i32,
+}
+#[repr(C)]
+pub struct hc_rope {
+    pub layout: c_int,
+    pub head_dim: c_int,
+    pub rot_dim: c_int,
+    pub amplitude: f32,
+    pub turns: [u64; 128],
+}
+#[repr(C)]
+pub struct hc_kv_pages {
+    pub n_slots: c_int,
+    pub max_pages: c_int,
+    pub n_layers: c_int,
+    pub page_table: *mut i32,
+    pub table_stride: usize,
+    pub kv_len: *mut i32,
+    pub refs: *mut i32,
+    pub scratch: *mut i32,
+    pub layers: *const hc_kv_cache,
+}
 
+pub const HC_ROPE_HALF: c_int = 0;
+pub const HC_ROPE_PAIRS: c_int = 1;
 pub const HC_KV_MAX_SEQ: c_int = 2048;
 pub const HC_OK: c_int = 0;
 pub const HC_ERR_INVALID: c_int = 1;
@@ -142,6 +171,23 @@ extern "C" {
     pub fn hc_attn_paged_dev(eng: *mut hc_engine, cache: *const hc_kv_cache, batch: *const hc_kv_batch, dtype: c_int,
                              n_heads: usize, q: *const c_void, ldq: usize, out: *mut c_void, ldo: usize,
                              lse: *mut f32, scale: f32, causal: c_int, window: c_int, sink: c_int) -> c_int;
+    pub fn hc_attn_shared_dev(eng: *mut hc_engine, cache: *const hc_kv_cache, batch: *const hc_kv_batch,
+                              shared: *const hc_kv_shared, dtype: c_int, n_heads: usize, q: *const c_void, ldq: usize,
+                              out: *mut c_void, ldo: usize, lse: *mut f32, scale: f32) -> c_int;
+    pub fn hc_rope_init(out: *mut hc_rope, layout: c_int, head_dim: c_int, rot_dim: c_int, base: f64, factor: f64,
+                        original: f64, low: f64, high: f64, factors: *const f32, amplitude: f32) -> c_int;
+    pub fn hc_rope_dev(eng: *mut hc_engine, rope: *const hc_rope, dtype: c_int, n_tok: usize, n_heads: usize,
+                       positions: *const i32, x: *const c_void, ldx: usize, out: *mut c_void, ldo: usize) -> c_int;
+    pub fn hc_kv_append_rope_dev(eng: *mut hc_engine, cache: *const hc_kv_cache, batch: *const hc_kv_batch,
+                                 rope: *const hc_rope, dtype: c_int, n_heads: usize, q: *const c_void, ldq: usize,
+                                 q_out: *mut c_void, ldqo: usize, k: *const c_void, ldk: usize, v: *const c_void,
+                                 ldv: usize) -> c_int;
+    pub fn hc_kv_pages_scratch(n_pages: c_int, out: *mut usize) -> c_int;
+    pub fn hc_kv_fork_dev(eng: *mut hc_engine, pages: *const hc_kv_pages, n: c_int, parents: *const i32,
+                          children: *const i32) -> c_int;
+    pub fn hc_kv_resize_dev(eng: *mut hc_engine, pages: *const hc_kv_pages, n: c_int, slots: *const i32,
+                            lens: *const i32) -> c_int;
+    pub fn hc_kv_compact_dev(eng: *mut hc_engine, pages: *const hc_kv_pages, moved: *mut i32) -> c_int;
     pub fn hc_synth_normal_dev(eng: *mut hc_engine, seed: u64, n: usize, mean: f32, stdv: f32, out: *mut f32) -> c_int;
     pub fn hc_quantize_dev(eng: *mut hc_engine, ggml_type: c_int, x: *const f32, n: usize, out: *mut u8) -> c_int;
 }
