@@ -723,13 +723,13 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                     const int col = I8 ? (D / 8) * g + 2 * d : 64 * (d >> 2) + 8 * g + 2 * (d & 3);
                     const float y[4] = {o[d][n][e], o[d][n][e + 2], o[d + 1][n][e], o[d + 1][n][e + 2]};
                     if (whole)
-                        attn_store<T>(a, it.q.q0, it.hk, tl.r0 + r, D, col, y, m[n][e], l[n][e], attn_adds(a, tl.lo));
+                        attn_store<T>(a, it.q.q0, it.hk, tl.r0 + r, D, col, y, l[n][e], attn_part(a, tl.lo));
                     else
                         *reinterpret_cast<float4*>(part + r * D + col) = make_float4(y[0], y[1], y[2], y[3]);
                 }
                 if (g == 0) {
                     if (whole)
-                        attn_store_lse(a, it.q.q0, it.hk, tl.r0 + r, m[n][e], l[n][e], attn_adds(a, tl.lo));
+                        attn_store_lse(a, it.q.q0, it.hk, tl.r0 + r, m[n][e], l[n][e], attn_part(a, tl.lo));
                     else
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m[n][e], l[n][e]);
                 }
@@ -784,8 +784,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
                        [&](int i) { return __ldcg(reinterpret_cast<const float4*>(block(i) + r * D) + ln); });
             }
             if (ln >= D / 4) continue;
-            attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.m, j.l, attn_adds(a, sh.lo));
-            if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l, attn_adds(a, sh.lo));
+            attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, 4 * ln, j.y, j.l, attn_part(a, sh.lo));
+            if (ln == 0) attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, j.m, j.l, attn_part(a, sh.lo));
         }
     }
 }

@@ -250,46 +250,22 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
-// Does a tile that starts at position `lo` add a shared prefix's results?  (The start of a window does not.)
-__device__ __forceinline__ bool attn_adds(const AttnArgs& a, int lo) { return a.first && lo > 0; }
+// Does a tile's result go to `base`, to be joined?  Those of a prefix do, and those of what comes behind one.
+__device__ __forceinline__ bool attn_part(const AttnArgs& a, int lo) { return a.to_base || (a.first && lo > 0); }
 
-// What a row's own weighted sum and the result over its shared prefix count for in the two's result.  Own: sum y
-// and l of weights 2^(s - m); the prefix: a result with log 2 of its weights' sum.
-struct AttnAdd {
-    float own, pre, m, l;  // result = y * own + prefix's * pre; m and l of both together
-    __device__ __forceinline__ AttnAdd(float m0, float l0, float lse) {
-        m = fmaxf(m0, lse);
-        const float f = m0 == -INFINITY && l0 == 0.f ? 0.f : ex2(m0 - m), g = lse == -INFINITY ? 0.f : ex2(lse - m);
-        l = l0 * f + g;
-        const float k = l == 0.f ? 0.f : 1.f / l;
-        own = f * k;
-        pre = g * k;
-    }
-    // a weight of zero takes nothing, whatever the value is
-    __device__ __forceinline__ float operator()(float y, float b) const {
-        return (own == 0.f ? 0.f : y * own) + (pre == 0.f ? 0.f : b * pre);
-    }
-};
-
-// Four adjacent values of the weighted sum y of row `row` of an item's kv head, over l; adds: with the prefix's.
+// Four adjacent values of the weighted sum of row `row` of an item's kv head, over l.
 template <class T>
 __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[4],
-                                           float m, float l, bool adds) {
+                                           float l, bool part) {
     const bool none = l == 0.f;  // saw nothing (a sum that is not a number is kept)
     const float k = none ? 0.f : 1.f / l;
     const int t = a.by_group(row), h = hk * a.group + row - t * a.group;
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = none ? 0.f : y[i] * k;
-    const long long at = (long long)(q0 + t) * a.heads + h;
-    if (a.to_base) {
-        *reinterpret_cast<float4*>(a.base + at * D + d) = make_float4(z[0], z[1], z[2], z[3]);
+    if (part) {
+        *reinterpret_cast<float4*>(a.base + ((long long)(q0 + t) * a.heads + h) * D + d) = make_float4(z[0], z[1], z[2], z[3]);
         return;
-    }
-    if (adds) {
-        const AttnAdd w(m, l, __ldcg(a.base_lse + at));
-        const float4 b = __ldcg(reinterpret_cast<const float4*>(a.base + at * D + d));
-        z[0] = w(y[0], b.x), z[1] = w(y[1], b.y), z[2] = w(y[2], b.z), z[3] = w(y[3], b.w);
     }
     T* out = (T*)a.out + (long long)(q0 + t) * a.ldo + h * D + d;
     if constexpr (sizeof(T) == 4)
@@ -299,18 +275,14 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, in
     else
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_b2(z[0], z[1]), pack_b2(z[2], z[3]));
 }
-__device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l, bool adds) {
+__device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l, bool part) {
     const int t = a.by_group(row);
     const long long at = (long long)(q0 + t) * a.heads + hk * a.group + row - t * a.group;
-    if (a.to_base) {
-        a.base_lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
-    } else if (a.lse) {
-        if (adds) {
-            const AttnAdd w(m, l, __ldcg(a.base_lse + at));
-            m = w.m, l = w.l;
-        }
-        a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
-    }
+    const float y = l == 0.f ? -INFINITY : m + log2f(l);
+    if (part)
+        a.base_lse[at] = y;
+    else if (a.lse)
+        a.lse[at] = y * 0.693147181f;
 }
 
 // One row of n partial results joined by a warp: ml(i) gives piece i's (m, l), (-inf, 0) if it has

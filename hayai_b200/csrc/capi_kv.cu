@@ -203,12 +203,13 @@ static int attn_args(const char* what, hc_engine* e, const hc_kv_cache* c, const
     return HC_OK;
 }
 
+constexpr int kFewRows = 16;
+
 // Sequences with up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
 // ones to the other (tiles of 256): both are launched where the batch may have both.  At 16 rows, 16
 // sequences of 3000 to 8000 8-bit tokens take 67 us in the first and 145 in the second (bf16: 79 and
 // 113); at 32 rows, in tiles of 32, 182 and 147 (bf16: 115 and 116).
 static cudaError_t attn_run(const hc_engine* e, const hc_kv_cache* c, int dtype, AttnArgs a, int max_new) {
-    constexpr int kFewRows = 16;
     const long long rows = (long long)(max_new && max_new < a.b.n_tok ? max_new : a.b.n_tok) * a.group;
     a.max_rows = (int)(rows < INT32_MAX ? rows : INT32_MAX);
     const bool many = attn_many_supported(c->type, dtype) && a.max_rows > kFewRows;
@@ -260,37 +261,81 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         return hc_set_error(HC_ERR_INVALID, "attn_shared: %d groups (at most %d)", g->n_groups, HC_KV_MAX_SEQ);
     if (g->n_groups && (!g->seq_start || !g->length)) return hc_set_error(HC_ERR_INVALID, "attn_shared: null seq_start or length");
     if (none) return HC_OK;
-    // the batch's firsts and the groups' arrays, then the prefixes' sums and results
-    const size_t rows = (size_t)b->n_tok * n_heads, lse_at = (kSharedInts * 4 + 255) / 256 * 256,
-                 out_at = (lse_at + rows * 4 + 255) / 256 * 256;
-    const bool shares = g->n_groups > 0 && b->n_seq > 1;
-    void* base = nullptr;
-    rc = attn_workspace(e, &a, shares ? out_at + rows * c->head_dim * 4 : 0, &base);
-    if (rc) return rc;
-    cudaError_t ce = cudaSuccess;
-    if (shares) {
-        KvSharedDev d{};
-        d.seq_start = g->seq_start;
-        d.length = g->length;
-        d.n = g->n_groups;
-        d.first = (int*)base;
-        d.q_start = d.first + HC_KV_SEQS;
-        d.len = d.q_start + HC_KV_SEQS + 4;
-        d.row = d.len + HC_KV_SEQS;
-        a.base_lse = (float*)((uint8_t*)base + lse_at);
-        a.base = (float*)((uint8_t*)base + out_at);
-        ce = launch_attn_groups(a.b, d, b->max_pages * c->page_size, e->stream);
-        AttnArgs p = a;
-        p.b.q_start = d.q_start;
-        p.b.kv_len = d.len;
-        p.b.n_seq = d.n;
-        p.table_row = d.row;
-        p.causal = 0;
-        p.to_base = 1;
-        if (ce == cudaSuccess) ce = attn_run(e, c, dtype, p, g->max_new);
-        a.first = d.first;
+    if (g->n_groups == 0 || b->n_seq < 2 || b->n_tok < 2) {  // nothing that two sequences could share
+        rc = attn_workspace(e, &a, 0, nullptr);
+        if (rc) return rc;
+        const cudaError_t ce = attn_run(e, c, dtype, a, b->max_new);
+        return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
     }
+    // Prefixes of up to kFewRows rows per kv head go to the kernel for few rows, the others to attn_prefix.cu (both
+    // launched where the batch may have both); so do all of f32 rows, whose terms its operands do not hold.
+    const int sms = e->num_sms;
+    const long long rows = (long long)b->n_tok * (long long)n_heads, kv = c->n_heads;
+    const long long most = (long long)(g->max_new && g->max_new < b->n_tok ? g->max_new : b->n_tok) * a.group;
+    const bool tc = attn_many_supported(c->type, dtype) && most > kFewRows, few = !tc || g->n_groups > 1;
+    long long shared = b->n_seq / 2;  // groups that share anything: two sequences with new tokens each
+    if (shared > b->n_tok / 2) shared = b->n_tok / 2;
+    if (shared > g->n_groups) shared = g->n_groups;
+    const long long tiles = rows / 256 + shared * kv;
+    // a row's result in a piece or two (narrow tiles), and where a block's share ends in a tile, its rows once more
+    const long long narrow = shared * kv * 128 < rows ? shared * kv * 128 : rows;
+    const long long pieces = tc ? rows + narrow + (long long)sms * 256 : 0;
+    size_t size = 0;
+    auto room = [&](size_t n) {
+        const size_t at = size;
+        size += (n * 4 + 255) / 256 * 256;
+        return at;
+    };
+    const size_t at_first = room(HC_KV_SEQS), at_q = room(HC_KV_SEQS + 1), at_len = room(HC_KV_SEQS), at_row = room(HC_KV_SEQS),
+                 at_line = room(kLineInts), at_block = room((size_t)sms), at_tiles = room((size_t)tiles * sizeof(PrefixTile) / 4),
+                 at_lse = room((size_t)rows), at_out = room((size_t)rows * c->head_dim), at_flse = room(few ? (size_t)rows : 0),
+                 at_few = room(few ? (size_t)rows * c->head_dim : 0), at_ml = room((size_t)pieces * 2),
+                 at_part = room((size_t)pieces * c->head_dim);
+    void* base = nullptr;
+    rc = attn_workspace(e, &a, size, &base);
+    if (rc) return rc;
+    auto place = [&](size_t at) { return (void*)((uint8_t*)base + at); };
+    KvSharedDev d{};
+    d.seq_start = g->seq_start;
+    d.length = g->length;
+    d.n = g->n_groups;
+    d.first = (int*)place(at_first);
+    d.q_start = (int*)place(at_q);
+    d.len = (int*)place(at_len);
+    d.row = (int*)place(at_row);
+    d.heads = a.heads;
+    d.kv_heads = c->n_heads;
+    d.few_rows = !tc ? INT32_MAX : few ? kFewRows : 0;
+    d.blocks = sms;
+    d.max_tiles = (int)(tiles < INT32_MAX ? tiles : INT32_MAX);
+    d.max_pieces = (int)(pieces < INT32_MAX ? pieces : INT32_MAX);
+    d.tiles = (PrefixTile*)place(at_tiles);
+    d.line = (int*)place(at_line);
+    d.first_tile = (int*)place(at_block);
+    cudaError_t ce = launch_attn_groups(a.b, d, b->max_pages * c->page_size, e->stream);
+    const PrefixArgs p{d.tiles, d.line, d.first_tile, (float*)place(at_part), (float*)place(at_ml), (float*)place(at_few),
+                       (float*)place(at_flse)};
+    if (ce == cudaSuccess && tc) ce = launch_attn_prefix(c->type, dtype, c->head_dim, a, p, sms, e->stream);
+    if (ce == cudaSuccess && few) {
+        AttnArgs x = a;
+        x.b.q_start = d.q_start;
+        x.b.kv_len = d.len;
+        x.b.n_seq = d.n;
+        x.table_row = d.row;
+        x.causal = 0;
+        x.to_base = 1;
+        x.base = (float*)place(at_few);
+        x.base_lse = (float*)place(at_flse);
+        x.row_min = 1;
+        x.row_max = d.few_rows;
+        x.max_rows = (int)(most < d.few_rows ? most : d.few_rows);
+        ce = launch_attn_few(c->type, dtype, c->head_dim, x, sms, e->stream);
+    }
+    a.first = d.first;
+    a.base = (float*)place(at_out);
+    a.base_lse = (float*)place(at_lse);
     if (ce == cudaSuccess) ce = attn_run(e, c, dtype, a, b->max_new);
+    if (ce == cudaSuccess) ce = launch_attn_join(dtype, c->head_dim, a, p, sms, e->stream);
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
 }
 

@@ -118,12 +118,11 @@ struct AttnArgs {
     int max_rows;          // the host's bound on a sequence's rows of one kv head (new tokens x group)
     int row_min, row_max;  // sequences with fewer or more rows are left to another kernel
     int over;              // places of the line that stand for a tile's start and end
-    // A shared prefix (attn_shared.cu).  One call writes the groups' results to `base`, the other starts every
-    // sequence behind its prefix and adds them.
-    const int* first;      // [n_seq] positions that a sequence leaves out, or null
-    const int* table_row;  // [n_seq] rows of the page table, or null: a sequence's own
+    // A shared prefix (attn_shared.cu): results over a part of the positions go to `base`, to be joined.
+    const int* first;        // [n_seq] positions that a sequence leaves out, or null
+    const int* table_row;    // [n_seq] rows of the page table, or null: a sequence's own
     float *base, *base_lse;  // [n_tok * heads][head_dim] and log 2 of the weights' sums
-    int to_base;
+    int to_base;             // the sequences are prefixes: all their results, but nothing of empty ones
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
     int* count;            // 32 counters per block, zero between calls
 };
@@ -133,10 +132,37 @@ struct KvSharedDev {
     const int *seq_start, *length;
     int n;
     int *first;                // [n_seq]
-    int *q_start, *len, *row;  // [n + 1], [n], [n]
+    int *q_start, *len, *row;  // [n + 1], [n], [n]: the prefixes that go to the kernel for few rows
+    int heads, kv_heads;       // query heads, and those that the keys have
+    int few_rows;              // a prefix with more rows per kv head goes to attn_prefix.cu
+    int blocks, max_tiles;     // of attn_prefix.cu; tiles that there is room for
+    int max_pieces;            // rows of pieces that there is room for
+    struct PrefixTile* tiles;
+    int *line, *first_tile;    // kLine...; [blocks] the tile that a block starts in
 };
-constexpr size_t kSharedInts = 4 * (size_t)HC_KV_SEQS + 4;
+// Rows of a kv head of a prefix, up to 256 of them.
+struct PrefixTile {
+    int place, units;    // the first of its places on the line (attn_prefix.cu); units of 128 positions, 0: not on it
+    int cost;            // places of a unit: 2, or 1 for up to 128 rows
+    int q0, hk, r0, nr;  // the group's first token; the kv head; the tile's first row and number of rows
+    int len, row;        // the prefix's length, and its row of the page table
+    int piece, pieces;   // its first row in the pieces, and how many there are; 0: it is in the few rows' `base`
+    int c0;              // the block that has its first unit
+    int pad[4];
+};
+enum { kLineTiles, kLinePlaces, kLineBlocks, kLineInts = 16 };
+// What attn_prefix.cu and the joining get besides: pieces (O, then m and l of a row), and the other parts' results.
+struct PrefixArgs {
+    const PrefixTile* tiles;
+    const int *line, *first_tile;
+    float *part, *part_ml;
+    const float *few, *few_lse;  // of prefixes with few rows
+};
 cudaError_t launch_attn_groups(const KvBatchDev& b, const KvSharedDev& g, int cap, cudaStream_t s);
+cudaError_t launch_attn_prefix(int cache_type, int dtype, int head_dim, const AttnArgs& a, const PrefixArgs& p, int blocks,
+                               cudaStream_t s);
+// out and lse of the rows with a prefix, from `base` (what they have behind it) and the prefix's pieces.
+cudaError_t launch_attn_join(int dtype, int head_dim, const AttnArgs& a, const PrefixArgs& p, int sms, cudaStream_t s);
 
 // Partial results of the kernel for few rows: bytes for each block.
 constexpr size_t kFewPartBytes = 2 * 13 * 16 * (128 + 2) * 4;

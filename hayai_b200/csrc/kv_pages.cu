@@ -10,6 +10,7 @@
 //
 // Bound by: the copies' bytes (read once, written once) where there are many, or else two launches and
 // the first kernel's walk over the holders.
+#include "block_scan.cuh"
 #include "kv_launch.h"
 
 namespace hc {
@@ -18,36 +19,6 @@ namespace {
 
 constexpr int kPlanThreads = 1024, kItems = HC_KV_SEQS, kWorkThreads = 256;
 static_assert(kItems == 2 * kPlanThreads, "two items to a thread");
-
-// Exclusive prefix sum over the block; `total` is the sum.  `scratch`: 33 numbers of shared memory.
-template <class I>
-__device__ __forceinline__ I block_scan(I x, long long* scratch, I& total) {
-    const int w = threadIdx.x >> 5, l = lane_id();
-    I y = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const I z = __shfl_up_sync(0xffffffffu, y, o);
-        if (l >= o) y += z;
-    }
-    if (l == 31) scratch[w] = y;
-    __syncthreads();
-    if (w == 0) {
-        I v = (I)scratch[l];
-        const I own = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const I z = __shfl_up_sync(0xffffffffu, v, o);
-            if (l >= o) v += z;
-        }
-        scratch[l] = v - own;
-        if (l == 31) scratch[32] = v;
-    }
-    __syncthreads();
-    total = (I)scratch[32];
-    const I before = (I)scratch[w] + y - x;
-    __syncthreads();
-    return before;
-}
 
 constexpr int kRun = 8;  // pages of a thread at a time
 
