@@ -218,6 +218,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 
     __shared__ float* place_s[W][2];  // where a warp's last (0) and first (1) piece of a shared tile is
 
+    if (a.early) after_previous();
+    if (a.first) let_next_start();
     // few sequences (a single one above all, whose call is short): every warp schedules for itself
     const bool lanes = a.b.n_seq <= 32 && a.max_rows <= 8 * ROWS;
     int* const pre = reinterpret_cast<int*>(smem);
@@ -803,6 +805,7 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     static SmemOptIn opted;
     const cudaError_t e = opted(reinterpret_cast<const void*>(attn_few_kernel<T, C, D, NT>), most);
     if (e != cudaSuccess) return e;
+    if (a.early) return launch_early(attn_few_kernel<T, C, D, NT>, blocks, 32 * F::W, most, s, a);
     attn_few_kernel<T, C, D, NT><<<blocks, 32 * F::W, most, s>>>(a);
     return cudaGetLastError();
 }

@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     AttnShared* const shared_s = reinterpret_cast<AttnShared*>(misc + 64);  // the block's first and last tile, where shared
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
 
+    if (a.early) after_previous();
+    if (a.first) let_next_start();
     // the schedule's prefix sums lie in the last key and value tile until warp 13 has its place
     int* const pre_s = reinterpret_cast<int*>(smem + F::oKV + (NB - 1) * TILE);
     const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 16);
@@ -867,6 +869,7 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     AttnArgs b = a;
     b.over = 2;  // a tile's start and end cost about what two of its units do
+    if (a.early) return launch_early(attn_many_kernel<T, C, D>, blocks, kManyThreads, bytes, s, b);
     attn_many_kernel<T, C, D><<<blocks, kManyThreads, bytes, s>>>(b);
     return cudaGetLastError();
 }

@@ -19,9 +19,6 @@
 //                    where they wait for the same units in turn: 5000 cycles a unit, 3400 so); warps 13-15 are there for the
 //                    register split, which goes by four warps
 //
-// A quarter of the exponentials is made by polynomials: of a wide unit's 32768, at 16 a cycle, the special function unit
-// would have as much to do (2048 cycles) as the tensor cores, and the chain of each half would wait for both.
-//
 // Formats as in attn_many.cu: products of f16 (f16 and 8-bit caches) or bf16, weights rounded to that type and
 // summed in f32; f16 weights are taken 2^7 times as large.  8-bit codes are exact in f16; a K scale multiplies its column of
 // S, a V scale its column of P, and m follows the largest score + log2 of its V scale, so that P times scale
@@ -62,17 +59,17 @@ struct PfxWalk {
     int lo, hi;  // units [lo, hi)
     bool wide;
     __device__ __forceinline__ PfxWalk(const PrefixArgs& args, const AttnShares& share, int c) : p(args) {
-        t = p.first_tile[c] - 1;
-        n = p.line[kLineTiles];
+        t = __ldcg(p.first_tile + c) - 1;
+        n = __ldcg(p.line + kLineTiles);
         b0 = share.begin(c);
         b1 = share.begin(c + 1);
     }
     __device__ __forceinline__ bool next() {
         while (++t < n) {
             const int4* const s = reinterpret_cast<const int4*>(p.tiles + t);
-            reinterpret_cast<int4*>(&x)[0] = __ldg(s);
-            reinterpret_cast<int4*>(&x)[1] = __ldg(s + 1);
-            reinterpret_cast<int4*>(&x)[2] = __ldg(s + 2);
+            reinterpret_cast<int4*>(&x)[0] = __ldcg(s);
+            reinterpret_cast<int4*>(&x)[1] = __ldcg(s + 1);
+            reinterpret_cast<int4*>(&x)[2] = __ldcg(s + 2);
             if (x.place >= b1) return false;
             wide = x.cost == 2;
             // a unit belongs to the block that has its first place
@@ -83,13 +80,8 @@ struct PfxWalk {
         }
         return false;
     }
-    // Places of a run's tiles in the ring's order, the order in which the products need them.  Wide: K0 V0 K1 V1 ...;
-    // narrow: K0 K1 V0 K2 V1 ... V.
-    __device__ __forceinline__ int k_at(int unit) const { return wide ? 2 * unit : unit ? 2 * unit - 1 : 0; }
-    __device__ __forceinline__ int v_at(int unit) const {
-        const int last = 2 * (hi - lo) - 1;
-        return wide ? 2 * unit + 1 : min(2 * unit + 2, last);
-    }
+    // The i-th of a run's tiles in the ring, where they lie in the order in which the products need them.  Wide: K0 V0 K1
+    // V1 ...; narrow: K0 K1 V0 K2 V1 ... V.
     __device__ __forceinline__ void tile_at(int i, int& unit, bool& v) const {
         const int last = 2 * (hi - lo) - 1;
         if (wide)
@@ -103,32 +95,6 @@ struct PfxWalk {
     }
 };
 
-// 2^x on the FMA pipe: the nearest whole number by adding 1.5 * 2^23, 2^f of the rest on [-1/2, 1/2] by a
-// polynomial (least squares of the relative error, reweighted to level it: 7.5e-5 at degree 3, where weights are rounded to
-// bf16's 8 bits; 2.6e-6 at degree 4), times 2^n.  x under -126 counts as that; NaN stays (max.NaN, and a product at the end).
-template <bool BF>
-__device__ __forceinline__ float2 pfx_ex2(float2 x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-    const float2 magic = make_float2(12582912.f, 12582912.f), less = make_float2(-12582912.f, -12582912.f);
-    const float2 t = add2(x, magic), r = add2(t, less);
-    const float2 f = fma2(r, make_float2(-1.f, -1.f), x);
-    float2 p;
-    if constexpr (BF) {
-        p = fma2(f, make_float2(0.0551716648f, 0.0551716648f), make_float2(0.242611125f, 0.242611125f));
-        p = fma2(p, f, make_float2(0.693260968f, 0.693260968f));
-        p = fma2(p, f, make_float2(0.999928057f, 0.999928057f));
-    } else {
-        p = fma2(f, make_float2(0.0095701013f, 0.0095701013f), make_float2(0.0559178591f, 0.0559178591f));
-        p = fma2(p, f, make_float2(0.240247443f, 0.240247443f));
-        p = fma2(p, f, make_float2(0.693121791f, 0.693121791f));
-        p = fma2(p, f, make_float2(0.999999285f, 0.999999285f));
-    }
-    const float2 e = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                                 __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-    return mul2(p, e);
-}
-
 template <class T, class C, int D>
 __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __grid_constant__ AttnArgs a,
                                                                      const __grid_constant__ PrefixArgs p) {
@@ -138,13 +104,16 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sb = smem_addr(smem), bars = sb + F::oBAR;
     // barriers: key and value tiles full and empty; S ready, P's first and second part ready, O ready (of each half);
-    // queries in, queries free; a unit's scales there
+    // queries in, queries free; 8-bit pages: a unit's scales there and done with, a tile of codes there and converted
     const uint32_t b_full = bars, b_empty = b_full + 8 * NB, b_s = b_empty + 8 * NB, b_p = b_s + 16, b_o = b_p + 32,
-                   b_q = b_o + 16, b_qf = b_q + 8, b_sc = b_qf + 8;
+                   b_q = b_o + 16, b_qf = b_q + 8, b_sc = b_qf + 8, b_scf = b_sc + 8 * NSC, b_stg = b_scf + 8 * NSC,
+                   b_stge = b_stg + 8 * F::NSTG;
     float* const rsc = reinterpret_cast<float*>(smem + F::oRS);
     int* const misc = reinterpret_cast<int*>(smem + F::oMISC);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
-    const int U = p.line[kLinePlaces], G = p.line[kLineBlocks];
+    after_previous();
+    let_next_start();
+    const int U = __ldcg(p.line + kLinePlaces), G = __ldcg(p.line + kLineBlocks);
     if (U <= 0 || c >= G) return;
     const AttnShares share(U, G);
     if (threadIdx.x == 0) {
@@ -161,8 +130,16 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
         }
         mbar_init(b_q, 8);
         mbar_init(b_qf, 1);
-        if (I8)
-            for (int i = 0; i < NSC; ++i) mbar_init(b_sc + 8 * i, 4);
+        if (I8) {
+            for (int i = 0; i < NSC; ++i) {
+                mbar_init(b_sc + 8 * i, 1);
+                mbar_init(b_scf + 8 * i, 8);  // of a narrow tile's unit the four warps of one half arrive twice
+            }
+            for (int i = 0; i < F::NSTG; ++i) {
+                mbar_init(b_stg + 8 * i, 1);
+                mbar_init(b_stge + 8 * i, 4);
+            }
+        }
         mbar_fence_init();
     }
     if (warp == 12) {
@@ -248,7 +225,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
             float m = -INFINITY;
             float2 l2 = make_float2(0.f, 0.f);
             for (int u = first; u < nu; u += step) {
-                if (!(ok = ok && mbar_wait_spin(b_s + 8 * half, ph_s))) break;
+                if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
                 ph_s ^= 1;
                 tc_fence_after();
                 float s[128];
@@ -338,11 +315,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                     for (int i = 0; i < 16; ++i) {
                         const int e = 32 * k + 2 * i;
                         const float2 x = fma2(make_float2(s[e], s[e + 1]), rs2, nm2);
-                        float2 q;
-                        if ((i & 3) == 3)
-                            q = pfx_ex2<BF>(x);
-                        else
-                            q = make_float2(ex2(x.x), ex2(x.y));
+                        float2 q = make_float2(ex2(x.x), ex2(x.y));
                         l2 = add2(l2, q);
                         if constexpr (I8) {
                             if ((i & 1) == 0) vs4 = vsc[8 * k + (i >> 1)];
@@ -356,6 +329,11 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                         tc_fence_before();
                         __syncwarp();
                         if (ln == 0) mbar_arrive(b_p + 16 * half + 8 * (k >> 1));
+                        if (I8 && k == 3 && ln == 0) {
+                            const uint32_t bar = b_scf + 8 * ((units + u) % NSC);
+                            mbar_arrive(bar);
+                            if (step == 2) mbar_arrive(bar);
+                        }
                         if (k == 1) {
                             // The second part's arithmetic is not to be moved before the first one's arrival: it takes a
                             // zero that is read behind it.
@@ -394,99 +372,118 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
             if (real) *reinterpret_cast<float2*>(p.part_ml + 2 * (size_t)piece) = make_float2(m - kLift, l2.x + l2.y);
         }
     } else if (warp < 12) {
-        // ================================================================ keys and values in
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfxRegsLow));
-        // each warp copies RPW rows of 16-byte chunks at a time; lane i owns the address of row(i)
-        constexpr int CPR = F::CPR, RPW = 32 / CPR, IT = CPR;
         const int pw = warp - 8;
-        const int mine = (ln / RPW) * 4 * RPW + pw * RPW + ln % RPW;  // this lane's row of the 128
-        const int sub = pw * RPW + ln / CPR, ch = ln % CPR;           // its row (of 4 RPW) and chunk of a copy
-        constexpr int AHEAD = 3;      // tiles on their way; the oldest is handed on before another is waited for
-        int t_issue = 0, t_done = 0;  // tiles whose copies are issued; tiles handed on
-        int units = 0;
-        // A tile has arrived: 16-bit tiles are operands already, codes are converted by the threads that copied them.
-        auto hand_on = [&]() {
-            const int t = t_done++, buf = t % NB;
-            if constexpr (I8) {
-                if (t >= NB && !many_wait(b_empty + 8 * buf, ((t / NB) - 1) & 1, ok)) return;
-                const uint32_t stg = sb + F::oSTG + (t % F::NSTG) * F::STG;
-                const uint32_t dst = sb + F::oKV + buf * TILE;
+        if constexpr (I8) {
+            // ============================================================ codes into operands
+            constexpr int CPR = F::CPR, ROWS = 128 / CPR, IT = 128 / ROWS;  // rows the four warps take at a time
+            const int r0 = (pw * 32 + ln) / CPR, ch = ln % CPR;
+            uint32_t slot = 0, ph = 0, stage = 0, ph_st = 0;  // the operands' ring and the staging ring
+            bool around = false;                              // the ring's places have been used before
+            while (ok && w.next()) {
+                const int last = 2 * (w.hi - w.lo);
+#pragma unroll 1
+                for (int i = 0; i < last; ++i) {
+                    if (!many_wait(b_stg + 8 * stage, ph_st, ok)) break;
+                    if (around && !many_wait(b_empty + 8 * slot, ph ^ 1, ok)) break;
+                    const uint32_t src = sb + F::oSTG + stage * F::STG, dst = sb + F::oKV + slot * TILE;
 #pragma unroll
-                for (int i = 0; i < IT; ++i) {
-                    const int r = i * 4 * RPW + sub;
-                    uint4 x;
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                                 : "r"(stg + r * D + ch * 16));
-                    const uint32_t y[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-                    uint32_t h[8];
+                    for (int k0 = 0; k0 < IT; k0 += 4) {  // four reads, then what they give: the trips overlap
+                        uint4 code[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        h[2 * k] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4140u), 0x64806480u);
-                        h[2 * k + 1] = hsub2_u32(prmt(y[k], 0x64646464u, 0x4342u), 0x64806480u);
+                        for (int k = 0; k < 4; ++k)
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(code[k].x), "=r"(code[k].y), "=r"(code[k].z), "=r"(code[k].w)
+                                         : "r"(src + (r0 + (k0 + k) * ROWS) * D + ch * 16));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = r0 + (k0 + k) * ROWS;
+                            const uint32_t y[4] = {code[k].x ^ 0x80808080u, code[k].y ^ 0x80808080u, code[k].z ^ 0x80808080u,
+                                                   code[k].w ^ 0x80808080u};
+                            uint32_t h[8];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                h[2 * e] = hsub2_u32(prmt(y[e], 0x64646464u, 0x4140u), 0x64806480u);
+                                h[2 * e + 1] = hsub2_u32(prmt(y[e], 0x64646464u, 0x4342u), 0x64806480u);
+                            }
+                            // chunk ch holds d = 16 ch ..: two 16-byte places of the tile's row, the second first in the
+                            // tile's upper half, so that eight lanes meet all banks
+                            const uint32_t row = dst + (ch >> 2) * HALF + r * 128;
+                            const uint32_t at[2] = {row + (((2 * (ch & 3)) ^ (r & 7)) << 4),
+                                                    row + (((2 * (ch & 3) + 1) ^ (r & 7)) << 4)};
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const bool hi = (o ^ (ch >> 2)) & 1;
+                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(hi ? at[1] : at[0]),
+                                             "r"(hi ? h[4] : h[0]), "r"(hi ? h[5] : h[1]), "r"(hi ? h[6] : h[2]),
+                                             "r"(hi ? h[7] : h[3])
+                                             : "memory");
+                            }
+                        }
                     }
-                    // chunk ch holds d = 16 ch ..: two 16-byte places of the tile's row
-                    const uint32_t row = dst + (ch >> 2) * HALF + r * 128;
-                    const int q = 2 * (ch & 3);
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((q ^ (r & 7)) << 4)), "r"(h[0]),
-                                 "r"(h[1]), "r"(h[2]), "r"(h[3])
-                                 : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((q + 1) ^ (r & 7)) << 4)), "r"(h[4]),
-                                 "r"(h[5]), "r"(h[6]), "r"(h[7])
-                                 : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (ln == 0) {
+                        mbar_arrive(b_full + 8 * slot);
+                        mbar_arrive(b_stge + 8 * stage);
+                    }
+                    if (++slot == NB) slot = 0, ph ^= 1, around = true;
+                    if (++stage == F::NSTG) stage = 0, ph_st ^= 1;
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (ln == 0) mbar_arrive(b_full + 8 * buf);
-        };
-        while (ok && w.next()) {
-            const int* const table = a.b.table + w.x.row * a.b.table_stride;
-            const int last = 2 * (w.hi - w.lo), hk = w.x.hk;
-            // page and row of this lane's position of tile i, and whether it has one (any page number may stand in a table)
-            auto page_of = [&](int i, int& r, bool& has) {
-                int unit;
-                bool v;
-                has = i < last;
-                if (has) {
-                    w.tile_at(i, unit, v);
-                    const int j = (w.lo + unit) * UNIT + mine;
-                    has = j < w.x.len;
-                    if (has) {
-                        const int q = a.by_page(j);
-                        r = j - q * a.c.page_size;
-                        return __ldg(table + q);
-                    }
-                }
-                return -1;
+        } else {
+            // ============================================================ keys and values in
+            // each warp copies RPW rows of 16-byte chunks at a time; lane i owns the address of row(i)
+            constexpr int CPR = F::CPR, RPW = 32 / CPR, IT = CPR;
+            const int mine = (ln / RPW) * 4 * RPW + pw * RPW + ln % RPW;  // this lane's row of the 128
+            const int sub = pw * RPW + ln / CPR, ch = ln % CPR;           // its row (of 4 RPW) and chunk of a copy
+            constexpr int AHEAD = 3;      // tiles on their way; the oldest is handed on before another is waited for
+            int t_issue = 0, t_done = 0;  // tiles whose copies are issued; tiles handed on
+            auto hand_on = [&]() {
+                const int t = t_done++, buf = t % NB;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (ln == 0) mbar_arrive(b_full + 8 * buf);
             };
-            int r = 0;
-            bool has;
-            int pg = page_of(0, r, has);
-#pragma unroll 1
-            for (int i = 0; i < last && ok; ++i) {
-                int unit;
-                bool v;
-                w.tile_at(i, unit, v);
-                uint32_t off = 0xffffffffu;
-                float sc[2] = {0.f, 0.f};
-                if ((unsigned)pg < (unsigned)a.c.n_pages) {
-                    off = (uint32_t)pg * a.c.page + (uint32_t)r * a.c.row + (uint32_t)hk * a.c.head;
-                    if (I8 && !v) {
-                        const long long so = pg * a.c.spage + (long long)hk * a.c.page_size + r;
-                        sc[0] = __ldg(a.c.ks + so);
-                        sc[1] = __ldg(a.c.vs + so);
+            while (ok && w.next()) {
+                const int* const table = a.b.table + w.x.row * a.b.table_stride;
+                const int last = 2 * (w.hi - w.lo), hk = w.x.hk;
+                // page and row of this lane's position of tile i, and whether it has one (any page number may stand in a table)
+                auto page_of = [&](int i, int& r, bool& has) {
+                    int unit;
+                    bool v;
+                    has = i < last;
+                    if (has) {
+                        w.tile_at(i, unit, v);
+                        const int j = (w.lo + unit) * UNIT + mine;
+                        has = j < w.x.len;
+                        if (has) {
+                            const int q = a.by_page(j);
+                            r = j - q * a.c.page_size;
+                            return __ldg(table + q);
+                        }
                     }
-                } else if (has) {
-                    atomicOr(a.b.err, kErrKvRange);
-                }
-                pg = page_of(i + 1, r, has);
-                if (t_issue - t_done == AHEAD) {
-                    cp_async_wait(AHEAD - 1);
-                    hand_on();
-                }
-                const int t = t_issue++;
-                if constexpr (!I8) {
+                    return -1;
+                };
+                int r = 0;
+                bool has;
+                int pg = page_of(0, r, has);
+#pragma unroll 1
+                for (int i = 0; i < last && ok; ++i) {
+                    int unit;
+                    bool v;
+                    w.tile_at(i, unit, v);
+                    uint32_t off = 0xffffffffu;
+                    if ((unsigned)pg < (unsigned)a.c.n_pages)
+                        off = (uint32_t)pg * a.c.page + (uint32_t)r * a.c.row + (uint32_t)hk * a.c.head;
+                    else if (has)
+                        atomicOr(a.b.err, kErrKvRange);
+                    pg = page_of(i + 1, r, has);
+                    if (t_issue - t_done == AHEAD) {
+                        cp_async_wait(AHEAD - 1);
+                        hand_on();
+                    }
+                    const int t = t_issue++;
                     if (t >= NB && !__all_sync(0xffffffffu, mbar_test(b_empty + 8 * (t % NB), ((t / NB) - 1) & 1))) {
                         // what has come meanwhile is not held back by a place that is not free yet
                         while (t_done < t && ok) {
@@ -495,38 +492,25 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                         }
                         if (!many_wait(b_empty + 8 * (t % NB), ((t / NB) - 1) & 1, ok)) break;
                     }
-                } else if (!v) {
-                    // The slot's last readers, the weights of eight units before, are done: the tiles up to three before this one
-                    // are handed on, for which those three before them were given back: keys of at most four units before, whose
-                    // products come after those with the weights of two units before them.
-                    const int slot = (units + unit) % NSC;
-                    float* const at = reinterpret_cast<float*>(smem + F::oSC + slot * 1024);
-                    at[mine] = sc[0];
-                    at[128 + mine] = sc[1];
-                    __syncwarp();
-                    if (ln == 0) mbar_arrive(b_sc + 8 * slot);
-                }
-                const uint32_t dst = I8 ? sb + F::oSTG + (t % max(F::NSTG, 1)) * F::STG : sb + F::oKV + (t % NB) * TILE;
-                const uint8_t* const src = v ? a.c.v : a.c.k;
+                    const uint32_t dst = sb + F::oKV + (t % NB) * TILE;
+                    const uint8_t* const src = v ? a.c.v : a.c.k;
 #pragma unroll
-                for (int k = 0; k < IT; ++k) {
-                    const uint32_t o = __shfl_sync(0xffffffffu, off, k * RPW + ln / CPR);
-                    const int rr = k * 4 * RPW + sub;
-                    const bool have = o != 0xffffffffu;
-                    const unsigned long long at = have ? (unsigned long long)o * 64 + ch * 16 : 0;
-                    const uint32_t d = I8 ? dst + rr * D + ch * 16
-                                          : dst + (ch >> 3) * HALF + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
-                    cp16_or_zero(d, src + at, have);
+                    for (int k = 0; k < IT; ++k) {
+                        const uint32_t o = __shfl_sync(0xffffffffu, off, k * RPW + ln / CPR);
+                        const int rr = k * 4 * RPW + sub;
+                        const bool have = o != 0xffffffffu;
+                        const unsigned long long at = have ? (unsigned long long)o * 64 + ch * 16 : 0;
+                        cp16_or_zero(dst + (ch >> 3) * HALF + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src + at, have);
+                    }
+                    cp_async_commit();
                 }
-                cp_async_commit();
             }
-            units += w.hi - w.lo;
+            while (t_done < t_issue && ok) {
+                cp_async_wait(t_issue - t_done - 1);
+                hand_on();
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        while (t_done < t_issue && ok) {
-            cp_async_wait(t_issue - t_done - 1);
-            hand_on();
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfxRegsLow));
         if (warp == 12) {
@@ -595,6 +579,84 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                         break;
                 }
             }
+        } else if (I8 && warp == 13) {
+            // ============================================================ codes in, as they lie
+            // A page's rows of a head are one piece where rows follow one another, else a row is.  What is not copied (past the
+            // prefix's end, pages out of range) stays whatever codes lay there: numbers, with no weight or a scale of zero.
+            constexpr int NS = F::NSTG ? F::NSTG : 1;
+            const bool together = a.c.row * 64 == D * F::ES;
+            int t = 0;
+            while (ok && w.next()) {
+                const int* const table = a.b.table + w.x.row * a.b.table_stride;
+                const int last = 2 * (w.hi - w.lo);
+#pragma unroll 1
+                for (int i = 0; i < last; ++i, ++t) {
+                    int unit;
+                    bool v;
+                    w.tile_at(i, unit, v);
+                    const int v0 = (w.lo + unit) * UNIT, v1 = min(v0 + UNIT, w.x.len);
+                    const uint32_t bar = b_stg + 8 * (t % NS), dst = sb + F::oSTG + (t % NS) * F::STG;
+                    if (t >= NS && !many_wait(b_stge + 8 * (t % NS), ((t / NS) - 1) & 1, ok)) break;
+                    const uint8_t* const src = (v ? a.c.v : a.c.k) + 64ull * ((uint32_t)w.x.hk * a.c.head);
+                    const int p0 = a.by_page(v0), runs = together ? a.by_page(v1 - 1) - p0 + 1 : v1 - v0;
+                    // this lane's pieces: from position `from` on, n of them, at row r of page pg
+                    auto piece = [&](int k, int& from, int& n, int& pg, int& r) {
+                        const int q = together ? p0 + k : a.by_page(v0 + k);
+                        from = together ? max(v0, q * a.c.page_size) : v0 + k;
+                        n = together ? min(v1, (q + 1) * a.c.page_size) - from : 1;
+                        r = from - q * a.c.page_size;
+                        pg = __ldg(table + q);
+                        return (unsigned)pg < (unsigned)a.c.n_pages;
+                    };
+                    int from, n, pg, r, rows = 0;
+                    for (int k = ln; k < runs; k += 32) {
+                        if (piece(k, from, n, pg, r))
+                            rows += n;
+                        else
+                            atomicOr(a.b.err, kErrKvRange);
+                    }
+                    rows = __reduce_add_sync(0xffffffffu, rows);
+                    if (ln == 0) mbar_arrive_expect_tx(bar, (uint32_t)rows * D);
+                    __syncwarp();
+                    for (int k = ln; k < runs; k += 32)
+                        if (piece(k, from, n, pg, r))
+                            bulk_g2s(dst + (from - v0) * D, src + 64ull * ((uint32_t)pg * a.c.page + (uint32_t)r * a.c.row),
+                                     (uint32_t)n * D, bar);
+                    __syncwarp();
+                }
+            }
+            // none of the copies outlives the block, whatever has become of their readers
+            bool come = true;
+            for (int k = max(t - NS, 0); k < t; ++k) many_wait(b_stg + 8 * (k % NS), (k / NS) & 1, come);
+            ok = ok && come;
+        } else if (I8 && warp == 14) {
+            // ============================================================ the scales
+            int q = 0;  // units so far
+            while (ok && w.next()) {
+                const int* const table = a.b.table + w.x.row * a.b.table_stride;
+#pragma unroll 1
+                for (int u = w.lo; u < w.hi; ++u, ++q) {
+                    float sc[2][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = u * UNIT + 32 * i + ln, p = a.by_page(j);
+                        const int pg = j < w.x.len ? __ldg(table + p) : -1;
+                        sc[0][i] = sc[1][i] = 0.f;
+                        if ((unsigned)pg < (unsigned)a.c.n_pages) {
+                            const long long so = pg * a.c.spage + (long long)w.x.hk * a.c.page_size + j - p * a.c.page_size;
+                            sc[0][i] = __ldg(a.c.ks + so);
+                            sc[1][i] = __ldg(a.c.vs + so);
+                        }
+                    }
+                    const int slot = q % NSC;
+                    if (q >= NSC && !many_wait(b_scf + 8 * slot, ((q / NSC) - 1) & 1, ok)) break;
+                    float* const at = reinterpret_cast<float*>(smem + F::oSC + slot * 1024);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) at[32 * i + ln] = sc[0][i], at[128 + 32 * i + ln] = sc[1][i];
+                    __syncwarp();
+                    if (ln == 0) mbar_arrive(b_sc + 8 * slot);
+                }
+            }
         }
     }
     if (!ok) atomicOr(a.b.err, kErrWait);
@@ -613,8 +675,7 @@ cudaError_t launch(const AttnArgs& a, const PrefixArgs& p, int blocks, cudaStrea
     static SmemOptIn opted;
     const cudaError_t e = opted(reinterpret_cast<const void*>(attn_prefix_kernel<T, C, D>), bytes);
     if (e != cudaSuccess) return e;
-    attn_prefix_kernel<T, C, D><<<blocks, kPfxThreads, bytes, s>>>(a, p);
-    return cudaGetLastError();
+    return launch_early(attn_prefix_kernel<T, C, D>, blocks, kPfxThreads, bytes, s, a, p);
 }
 
 template <class T, int D>

@@ -45,7 +45,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
 // A sequence, and where what it sees starts.
 __device__ __forceinline__ KvSeq attn_seq(const AttnArgs& a, int s) {
     KvSeq q = kv_seq(a.b, a.b.max_pages * a.c.page_size, s);
-    if (a.first) q.first = __ldg(a.first + s);
+    if (a.first) q.first = __ldcg(a.first + s);
     return q;
 }
 

@@ -24,6 +24,10 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
     __shared__ long long scratch[33];
     __shared__ int len_s[HC_KV_SEQS], tok_s[HC_KV_SEQS], tile_s[HC_KV_SEQS + 1], place_s[HC_KV_SEQS];
     const int tid = threadIdx.x, ln = lane_id(), group = g.heads / g.kv_heads;
+    let_next_start();
+    int *const from_s = tile_s, *const to_s = place_s;  // the groups' sequences, until their tiles are counted
+    __shared__ unsigned long long saved_s;
+    if (tid == 0) saved_s = 0;
     for (int s = tid; s < b.n_seq; s += 1024) g.first[s] = 0;
     __syncthreads();
     for (int i = tid >> 5; i < g.n; i += 32) {
@@ -39,8 +43,21 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
             most = min(most, q.len - (q.q1 - q.q0));
         }
         most = max(__reduce_min_sync(0xffffffffu, most), 0);
-        if (__reduce_add_sync(0xffffffffu, seqs) < 2) most = 0;
+        seqs = __reduce_add_sync(0xffffffffu, seqs);
+        if (seqs < 2) most = 0;
+        if (ln == 0) {
+            len_s[i] = most;
+            from_s[i] = s0;
+            to_s[i] = s1;
+            atomicAdd(&saved_s, (unsigned long long)most * max(seqs - 1, 0));
+        }
+    }
+    __syncthreads();
+    const bool worth = saved_s >= (unsigned long long)g.least;
+    for (int i = tid >> 5; i < g.n; i += 32) {
+        const int s0 = from_s[i], s1 = to_s[i], most = worth ? len_s[i] : 0;
         for (int s = s0 + ln; s < s1; s += 32) g.first[s] = most;
+        __syncwarp();
         if (ln == 0) {
             // its new tokens' rows, cut as kv_seq cuts them
             const int q0 = min(max(__ldg(b.q_start + s0), 0), b.n_tok), q1 = min(max(__ldg(b.q_start + s1), q0), b.n_tok);
@@ -132,46 +149,65 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
     }
 }
 
-// A warp per row of a tile, eight rows of one at a time.
+// A warp per row of a tile, eight rows of one at a time.  Bound by memory and its latency: a row's parts are asked for
+// together, before the weights that they count with are there.
 template <class T, int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, PrefixArgs p) {
-    const int n = p.line[kLineTiles], ln = lane_id();
-    constexpr int RUNS = kTileRows / 8;
-    for (int w = blockIdx.x; w < n * RUNS; w += gridDim.x) {
-        const PrefixTile x = p.tiles[w / RUNS];
+    constexpr int RUNS = kTileRows / 8, U = 8;
+    after_previous();
+    const int n_tiles = __ldcg(p.line + kLineTiles), ln = lane_id();
+    const bool mine = ln < D / 4;
+    for (int w = blockIdx.x; w < n_tiles * RUNS; w += gridDim.x) {
+        const int4* const xt = reinterpret_cast<const int4*>(p.tiles + w / RUNS);
+        PrefixTile x;
+        reinterpret_cast<int4*>(&x)[0] = __ldcg(xt);
+        reinterpret_cast<int4*>(&x)[1] = __ldcg(xt + 1);
+        reinterpret_cast<int4*>(&x)[2] = __ldcg(xt + 2);
         const int r = w % RUNS * 8 + (threadIdx.x >> 5);
         if (r >= x.nr) continue;
         const int row = x.r0 + r, t = a.by_group(row);
         const long long at = (long long)(x.q0 + t) * a.heads + x.hk * a.group + row - t * a.group;
-        AttnJoin j;
-        auto whole = [&](const float* o, const float* lse) {  // a result that is divided by its sum
-            j.join(1, ln < D / 4,
-                   [&](int) {
-                       const float y = __ldcg(lse + at);
-                       return make_float2(y, y == -INFINITY ? 0.f : 1.f);
-                   },
-                   [&](int) { return __ldcg(reinterpret_cast<const float4*>(o + at * D) + ln); });
-        };
-        const float* const o = p.part + ((size_t)x.piece + r) * D;
+        // the parts: what is behind the prefix (divided by its sum), then the prefix's pieces, or its one result
+        const int n = x.pieces;
+        const size_t step = n ? x.nr : 0;
+        const float4* const o = reinterpret_cast<const float4*>(n ? p.part + ((size_t)x.piece + r) * D : p.few + at * D) + ln;
         const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + x.piece + r;
-        if (x.pieces)
-            j.join(x.pieces, ln < D / 4, [&](int i) { return __ldcg(ml + (size_t)i * x.nr); },
-                   [&](int i) { return __ldcg(reinterpret_cast<const float4*>(o + (size_t)i * x.nr * D) + ln); });
-        else
-            whole(p.few, p.few_lse);
-        whole(a.base, a.base_lse);
-        if (ln < D / 4) attn_store<T>(a, x.q0, x.hk, row, D, 4 * ln, j.y, j.l, false);
+        float4 y0 = make_float4(0.f, 0.f, 0.f, 0.f), y[U];
+        if (mine) y0 = __ldcg(reinterpret_cast<const float4*>(a.base + at * D) + ln);
+        const float own = __ldcg(a.base_lse + at);
+        float2 v = make_float2(-INFINITY, 0.f);
+        if (n) {
+            if (ln < n) v = __ldcg(ml + ln * step);
+        } else if (ln == 0) {
+            const float e = __ldcg(p.few_lse + at);
+            v = make_float2(e, e == -INFINITY ? 0.f : 1.f);
+        }
+        const int parts = max(n, 1);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mine && k < parts) y[k] = __ldcg(o + k * step * (D / 4));
+        }
+        AttnJoin j;
+        auto ml_of = [&](int i) { return i < 32 ? v : __ldcg(ml + i * step); };  // a lane asks for its own part of a run of 32
+        auto o_of = [&](int i) {
+            if (i >= U) return __ldcg(o + i * step * (D / 4));
+            float4 z = y[0];
+#pragma unroll
+            for (int k = 1; k < U; ++k)
+                if (i == k) z = y[k];
+            return z;
+        };
+        j.join(1, mine, [&](int) { return make_float2(own, own == -INFINITY ? 0.f : 1.f); }, [&](int) { return y0; });
+        j.join(parts, mine, ml_of, o_of);
+        if (mine) attn_store<T>(a, x.q0, x.hk, row, D, 4 * ln, j.y, j.l, false);
         if (ln == 0) attn_store_lse(a, x.q0, x.hk, row, j.m, j.l, false);
     }
 }
 
 template <class T>
 cudaError_t join(int head_dim, const AttnArgs& a, const PrefixArgs& p, int sms, cudaStream_t s) {
-    if (head_dim == 64)
-        attn_join_kernel<T, 64><<<sms * 8, 256, 0, s>>>(a, p);
-    else
-        attn_join_kernel<T, 128><<<sms * 8, 256, 0, s>>>(a, p);
-    return cudaGetLastError();
+    return launch_early(head_dim == 64 ? attn_join_kernel<T, 64> : attn_join_kernel<T, 128>, sms * 8, 256, 0, s, a, p);
 }
 
 }  // namespace

@@ -205,6 +205,9 @@ static int attn_args(const char* what, hc_engine* e, const hc_kv_cache* c, const
 
 constexpr int kFewRows = 16;
 
+// Bytes of keys and values that sharing prefixes has to save.
+constexpr long long kShareBytes = 192 << 20;
+
 // Sequences with up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
 // ones to the other (tiles of 256): both are launched where the batch may have both.  At 16 rows, 16
 // sequences of 3000 to 8000 8-bit tokens take 67 us in the first and 145 in the second (bf16: 79 and
@@ -255,13 +258,18 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     int rc = attn_args("attn_shared", e, c, b, dtype, n_heads, q, ldq, out, ldo, lse, scale, &a, &none);
     if (rc) return rc;
     if (!g) return hc_set_error(HC_ERR_INVALID, "attn_shared: null groups");
-    if (g->n_groups < 0 || g->max_new < 0)
-        return hc_set_error(HC_ERR_INVALID, "attn_shared: negative size n_groups=%d max_new=%d", g->n_groups, g->max_new);
+    if (g->n_groups < 0 || g->max_new < 0 || g->least < 0)
+        return hc_set_error(HC_ERR_INVALID, "attn_shared: negative size n_groups=%d max_new=%d least=%lld", g->n_groups, g->max_new,
+                            (long long)g->least);
     if (g->n_groups > HC_KV_MAX_SEQ)
         return hc_set_error(HC_ERR_INVALID, "attn_shared: %d groups (at most %d)", g->n_groups, HC_KV_MAX_SEQ);
     if (g->n_groups && (!g->seq_start || !g->length)) return hc_set_error(HC_ERR_INVALID, "attn_shared: null seq_start or length");
     if (none) return HC_OK;
-    if (g->n_groups == 0 || b->n_seq < 2 || b->n_tok < 2) {  // nothing that two sequences could share
+    // Sharing costs several kernels' starts, and is left where what it saves is not worth them: here where the page
+    // tables do not reach so far, else by the groups' lengths, on the device.
+    const size_t token = 2 * (size_t)c->n_heads * (c->head_dim * (c->type == T_I8 ? 1 : 2) + (c->type == T_I8 ? 4 : 0));
+    const long long least = g->least ? g->least : kShareBytes / (long long)token;  // tokens whose reading has to be saved
+    if (g->n_groups == 0 || b->n_tok < 2 || (b->n_seq - 1ll) * b->max_pages * c->page_size < least) {
         rc = attn_workspace(e, &a, 0, nullptr);
         if (rc) return rc;
         const cudaError_t ce = attn_run(e, c, dtype, a, b->max_new);
@@ -272,7 +280,7 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     const int sms = e->num_sms;
     const long long rows = (long long)b->n_tok * (long long)n_heads, kv = c->n_heads;
     const long long most = (long long)(g->max_new && g->max_new < b->n_tok ? g->max_new : b->n_tok) * a.group;
-    const bool tc = attn_many_supported(c->type, dtype) && most > kFewRows, few = !tc || g->n_groups > 1;
+    const bool tc = attn_many_supported(c->type, dtype), few = !tc;
     long long shared = b->n_seq / 2;  // groups that share anything: two sequences with new tokens each
     if (shared > b->n_tok / 2) shared = b->n_tok / 2;
     if (shared > g->n_groups) shared = g->n_groups;
@@ -303,9 +311,10 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     d.q_start = (int*)place(at_q);
     d.len = (int*)place(at_len);
     d.row = (int*)place(at_row);
+    d.least = least;
     d.heads = a.heads;
     d.kv_heads = c->n_heads;
-    d.few_rows = !tc ? INT32_MAX : few ? kFewRows : 0;
+    d.few_rows = few ? INT32_MAX : 0;
     d.blocks = sms;
     d.max_tiles = (int)(tiles < INT32_MAX ? tiles : INT32_MAX);
     d.max_pieces = (int)(pieces < INT32_MAX ? pieces : INT32_MAX);
@@ -328,10 +337,11 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         x.base_lse = (float*)place(at_flse);
         x.row_min = 1;
         x.row_max = d.few_rows;
-        x.max_rows = (int)(most < d.few_rows ? most : d.few_rows);
+        x.max_rows = (int)(most < INT32_MAX ? most : INT32_MAX);
         ce = launch_attn_few(c->type, dtype, c->head_dim, x, sms, e->stream);
     }
     a.first = d.first;
+    a.early = 1;
     a.base = (float*)place(at_out);
     a.base_lse = (float*)place(at_lse);
     if (ce == cudaSuccess) ce = attn_run(e, c, dtype, a, b->max_new);

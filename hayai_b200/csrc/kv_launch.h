@@ -59,6 +59,26 @@ struct FastDiv {
     }
 };
 
+// A launch that may start while the kernel before it on the stream still runs (programmatic dependent launch): the
+// kernel waits with after_previous() before it reads what that one wrote, and of such data uses no __ldg, which may
+// be moved before the wait.  A kernel calls let_next_start() where its successor is such a launch.
+template <class... P, class... A>
+cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...);
+}
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A kernel's shared-memory opt-in, once per device (a call of it costs about a microsecond).
 struct SmemOptIn {
     std::atomic<unsigned long long> done{0};
@@ -123,6 +143,7 @@ struct AttnArgs {
     const int* table_row;    // [n_seq] rows of the page table, or null: a sequence's own
     float *base, *base_lse;  // [n_tok * heads][head_dim] and log 2 of the weights' sums
     int to_base;             // the sequences are prefixes: all their results, but nothing of empty ones
+    int early;               // a launch_early
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
     int* count;            // 32 counters per block, zero between calls
 };
@@ -133,6 +154,7 @@ struct KvSharedDev {
     int n;
     int *first;                // [n_seq]
     int *q_start, *len, *row;  // [n + 1], [n], [n]: the prefixes that go to the kernel for few rows
+    long long least;           // tokens that sharing has to save, or nothing is shared
     int heads, kv_heads;       // query heads, and those that the keys have
     int few_rows;              // a prefix with more rows per kv head goes to attn_prefix.cu
     int blocks, max_tiles;     // of attn_prefix.cu; tiles that there is room for

@@ -8,6 +8,8 @@
 // the items in order, one after the other, whatever the blocks' order: free pages are taken by a prefix
 // sum over the items, and counts of holders are whole numbers.
 //
+// Both are launched early (kv_launch.h): a call's second kernel, and the next call's first, wait for the one before
+// them on the GPU.
 // Bound by: the copies' bytes (read once, written once) where there are many, or else two launches and
 // the first kernel's walk over the holders.
 #include "block_scan.cuh"
@@ -80,11 +82,12 @@ enum { kSlot, kFrom, kHad, kGet };
 // fork: children get the parents' whole pages and a page of their own for the rest.
 // resize: slots get new lengths.
 template <bool FORK>
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagesDev p, const int* __restrict__ first, const int* __restrict__ second,
-                                                            int n) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagesDev p, const int* first, const int* second, int n) {
     __shared__ long long scratch[33];
     __shared__ int moves_s;
     __shared__ Claims claims;
+    after_previous();
+    let_next_start();
     if (threadIdx.x == 0) moves_s = 0;
     claims.clear();
     struct Item {
@@ -177,6 +180,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagesDev p, const in
 // Where compacting moves pages: those held of numbers `used` and more to the free ones below, both in order.
 __global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(PagesDev p, int* moved) {
     __shared__ long long scratch[33];
+    after_previous();
+    let_next_start();
     int n = 0, used;
     for (int b = 0; b < p.n_pages; b += kPlanThreads * kRun)
 #pragma unroll
@@ -226,7 +231,9 @@ enum Work { kForkWork, kResizeWork, kCompactWork, kCopyWork };
 // page, of keys or values, of a layer.
 template <int WORK>
 __global__ void __launch_bounds__(kWorkThreads) work_kernel(PagesDev p, const __grid_constant__ KvLayers y, int n,
-                                                            const int* __restrict__ moved) {
+                                                            const int* moved) {
+    after_previous();
+    let_next_start();
     const int runs = (p.max_pages + kWorkThreads - 1) / kWorkThreads;
     if constexpr (WORK != kCopyWork)
         for (long long w = blockIdx.x; w < (long long)n * runs; w += gridDim.x) {
@@ -311,11 +318,8 @@ __global__ void __launch_bounds__(kWorkThreads) work_kernel(PagesDev p, const __
 template <int WORK>
 cudaError_t work(const PagesDev& p, const KvLayers* layers, int groups, int n, const int* moved, int sms, cudaStream_t s) {
     for (int g = 0; g < groups; ++g) {
-        if (g == 0)
-            work_kernel<WORK><<<sms * 8, kWorkThreads, 0, s>>>(p, layers[g], n, moved);
-        else
-            work_kernel<kCopyWork><<<sms * 8, kWorkThreads, 0, s>>>(p, layers[g], 0, nullptr);
-        const cudaError_t e = cudaGetLastError();
+        const cudaError_t e = launch_early(g ? work_kernel<kCopyWork> : work_kernel<WORK>, sms * 8, kWorkThreads, 0, s, p,
+                                           layers[g], g ? 0 : n, g ? (const int*)nullptr : moved);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -325,15 +329,13 @@ cudaError_t work(const PagesDev& p, const KvLayers* layers, int groups, int n, c
 
 cudaError_t launch_kv_fork(const PagesDev& p, const KvLayers* layers, int groups, int n, const int* parents,
                            const int* children, int sms, cudaStream_t s) {
-    plan_kernel<true><<<1, kPlanThreads, 0, s>>>(p, parents, children, n);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_early(plan_kernel<true>, 1, kPlanThreads, 0, s, p, parents, children, n);
     return e != cudaSuccess ? e : work<kForkWork>(p, layers, groups, n, nullptr, sms, s);
 }
 
 cudaError_t launch_kv_resize(const PagesDev& p, const KvLayers* layers, int groups, int n, const int* slots,
                              const int* lens, int sms, cudaStream_t s) {
-    plan_kernel<false><<<1, kPlanThreads, 0, s>>>(p, slots, lens, n);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_early(plan_kernel<false>, 1, kPlanThreads, 0, s, p, slots, lens, n);
     return e != cudaSuccess ? e : work<kResizeWork>(p, layers, groups, n, nullptr, sms, s);
 }
 
@@ -342,8 +344,7 @@ cudaError_t launch_kv_compact(const PagesDev& args, const KvLayers* layers, int 
     PagesDev p = args;
     if (!moved) moved = p.rows;  // whole pages are copied: their numbers of rows are not needed
     p.rows = nullptr;
-    plan_compact_kernel<<<1, kPlanThreads, 0, s>>>(p, moved);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_early(plan_compact_kernel, 1, kPlanThreads, 0, s, p, moved);
     return e != cudaSuccess ? e : work<kCompactWork>(p, layers, groups, p.n_slots, moved, sms, s);
 }
 

@@ -20,7 +20,7 @@ namespace hc {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kRounds = 8;
 
 // cos and sin of pair j at a position, times the amplitude.
 __device__ __forceinline__ float2 rope_angle(const RopeDev& r, int j, int pos) {
@@ -161,36 +161,48 @@ __global__ void __launch_bounds__(kThreads) rope_any_kernel(const __grid_constan
     }
 }
 
-// A step's rows by their positions in the cache: a group of D / 16 lanes per (token, U rows), the rows being the
-// token's query heads, then its key heads, then its value heads.
+// A step's rows by their positions in the cache: a group of D / 16 lanes per (token, U rows), the rows being U of the
+// token's query heads, of its key heads or of its value heads.
 template <class T, class C, int D, int U>
 __global__ void __launch_bounds__(kThreads) kv_append_rope_kernel(const __grid_constant__ RopeDev r, KvDev c, KvBatchDev b,
                                                                   RopeAppend a, FastDiv by_page, int tokens) {
     constexpr int GL = D / 16, GROUPS = kThreads / GL;
+    using Raw = typename Elem<T>::Raw;
     extern __shared__ float2 cs_s[];
     __shared__ uint32_t at_s[32];
     __shared__ long long sat_s[32];
     __shared__ int pos_s[32], has_s[32];
     if (kv_check_block(c, b)) return;
-    const int half = r.rot / 2, all = a.heads + 2 * c.n_heads, hc = (all + U - 1) / U, t0 = blockIdx.x * tokens;
-    const int n = min(tokens, b.n_tok - t0), l = threadIdx.x & (GL - 1), group = threadIdx.x / GL;
+    const int half = r.rot / 2, nq = (a.heads + U - 1) / U, nk = (c.n_heads + U - 1) / U, hc = nq + 2 * nk;
+    const int t0 = blockIdx.x * tokens, n = min(tokens, b.n_tok - t0), l = threadIdx.x & (GL - 1), group = threadIdx.x / GL;
     const RopeLane ln(r, l);
-    const T *const q = (const T*)a.q, *const k = (const T*)a.k, *const v = (const T*)a.v;
-    typename Elem<T>::Raw raw[U][2];
-    auto load = [&](int item) {
-        item = min(item, n * hc - 1);
-        const int t = item / hc, h0 = (item - t * hc) * U;
+    // An item's rows: what they are (0 queries, 1 keys, 2 values), the first head, and how many there are.
+    struct Item {
+        int t, what, h0, rows;
+    };
+    auto item_of = [&](int i) {
+        Item x;
+        x.t = i / hc;
+        const int k = i - x.t * hc;
+        x.what = (k >= nq) + (k >= nq + nk);
+        x.h0 = (k - (x.what == 0 ? 0 : x.what == 1 ? nq : nq + nk)) * U;
+        x.rows = min(U, (x.what ? c.n_heads : a.heads) - x.h0);
+        return x;
+    };
+    auto load = [&](const Item& x, Raw (&raw)[U][2]) {
+        const T* const src = (x.what == 0   ? (const T*)a.q + (t0 + x.t) * a.ldq
+                              : x.what == 1 ? (const T*)a.k + (t0 + x.t) * a.ldk
+                                            : (const T*)a.v + (t0 + x.t) * a.ldv) + (long long)x.h0 * D;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = min(h0 + u, all - 1);
-            const T* src = h < a.heads               ? q + (t0 + t) * a.ldq + (long long)h * D
-                           : h < a.heads + c.n_heads ? k + (t0 + t) * a.ldk + (long long)(h - a.heads) * D
-                                                     : v + (t0 + t) * a.ldv + (long long)(h - a.heads - c.n_heads) * D;
-            raw[u][0] = Elem<T>::load8(src + ln.c0);
-            raw[u][1] = Elem<T>::load8(src + ln.c1);
+            const int o = min(u, x.rows - 1) * D;
+            raw[u][0] = Elem<T>::load8(src + o + ln.c0);
+            raw[u][1] = Elem<T>::load8(src + o + ln.c1);
         }
     };
-    load(group);  // on their way while the tokens' places and angles are found
+    Raw raw[U][2];
+    Item x = item_of(min(group, n * hc - 1));
+    load(x, raw);  // on their way while the tokens' places and angles are found
     {
         // eight lanes to a token, whatever D is: at most 32 tokens
         const int t = threadIdx.x >> 3;
@@ -206,54 +218,63 @@ __global__ void __launch_bounds__(kThreads) kv_append_rope_kernel(const __grid_c
         cs_s[i] = rope_angle(r, i - t * half, pos_s[t]);
     }
     __syncthreads();
-    const int items = n * hc;
+    const uint32_t lanes = ((1u << GL) - 1) << (threadIdx.x & 31 & ~(GL - 1));  // the group's, which exchange below
 #pragma unroll 1
-    for (int i0 = 0; i0 < items; i0 += GROUPS) {  // the whole block goes round together: lanes exchange below
-        const int item = min(i0 + group, items - 1), t = item / hc, h0 = (item - t * hc) * U;
-        const bool real = i0 + group < items && pos_s[t] >= 0, has = real && has_s[t];
-        if (i0) load(item);
+    for (int i = group; i < n * hc; i += GROUPS) {
+        if (i >= GROUPS) {
+            x = item_of(i);
+            load(x, raw);
+        }
+        if (x.what == 0) {
+            if (pos_s[x.t] < 0) continue;
+            float2 cs[8];
+            ln.angles(cs_s + x.t * half, cs);
+            T* const dst = (T*)a.q_out + (t0 + x.t) * a.ldqo + (long long)x.h0 * D;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (u >= x.rows) break;
+                float p[8], q[8];
+                Elem<T>::values(raw[u][0], p);
+                Elem<T>::values(raw[u][1], q);
+                ln.turn(r.pairs, cs, p, q);
+                Elem<T>::store8(dst + u * D + ln.c0, p);
+                Elem<T>::store8(dst + u * D + ln.c1, q);
+            }
+            continue;
+        }
+        if (!has_s[x.t]) continue;
+        const bool v = x.what == 2;
+        uint8_t* const pool = v ? c.v : c.k;
+        const uint32_t at = at_s[x.t] + (uint32_t)x.h0 * c.head;
         float2 cs[8];
-        ln.angles(cs_s + t * half, cs);
-        const uint32_t at = at_s[t];
-        const long long sat = sat_s[t];
+        if (!v) ln.angles(cs_s + x.t * half, cs);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = h0 + u, hk = h - a.heads, w = hk >= c.n_heads, head = w ? hk - c.n_heads : hk;
-            float x[8], y[8];
-            Elem<T>::values(raw[u][0], x);
-            Elem<T>::values(raw[u][1], y);
-            if (!w) ln.turn(r.pairs, cs, x, y);
-            float m = 0.f, scale = 0.f;
+            if (u >= x.rows) break;
+            float p[8], q[8];
+            Elem<T>::values(raw[u][0], p);
+            Elem<T>::values(raw[u][1], q);
+            if (!v) ln.turn(r.pairs, cs, p, q);
+            C* const dst = kv_elem<C>(pool, at + (uint32_t)u * c.head);
             if constexpr (sizeof(C) == 1) {
                 // as bits, whose order is that of the sizes, infinity and NaN above all
                 uint32_t top = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    top = max(top, max(__float_as_uint(x[i]) & 0x7fffffffu, __float_as_uint(y[i]) & 0x7fffffffu));
+                for (int k = 0; k < 8; ++k)
+                    top = max(top, max(__float_as_uint(p[k]) & 0x7fffffffu, __float_as_uint(q[k]) & 0x7fffffffu));
 #pragma unroll
-                for (int o = GL / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                m = __uint_as_float(top);
-                scale = top < 0x7f800000u ? m * (1.f / 127.f) : __int_as_float(0x7fffffff);
-            }
-            if (h < a.heads) {
-                if (real) {
-                    T* const dst = (T*)a.q_out + (t0 + t) * a.ldqo + (long long)h * D;
-                    Elem<T>::store8(dst + ln.c0, x);
-                    Elem<T>::store8(dst + ln.c1, y);
-                }
-            } else if (has && h < all) {
-                C* const dst = kv_elem<C>(w ? c.v : c.k, at + (uint32_t)head * c.head);
-                if constexpr (sizeof(C) == 1) {
-                    uint32_t e[2], f[2];
-                    kv_codes(x, m, scale, e);
-                    kv_codes(y, m, scale, f);
-                    *reinterpret_cast<uint2*>(dst + ln.c0) = make_uint2(e[0], e[1]);
-                    *reinterpret_cast<uint2*>(dst + ln.c1) = make_uint2(f[0], f[1]);
-                    if (l == 0) (w ? c.vs : c.ks)[sat + (long long)head * c.page_size] = scale;
-                } else {
-                    Elem<C>::store8(dst + ln.c0, x);
-                    Elem<C>::store8(dst + ln.c1, y);
-                }
+                for (int o = GL / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
+                const float m = __uint_as_float(top);
+                const float scale = top < 0x7f800000u ? m * (1.f / 127.f) : __int_as_float(0x7fffffff);
+                uint32_t e[2], f[2];
+                kv_codes(p, m, scale, e);
+                kv_codes(q, m, scale, f);
+                *reinterpret_cast<uint2*>(dst + ln.c0) = make_uint2(e[0], e[1]);
+                *reinterpret_cast<uint2*>(dst + ln.c1) = make_uint2(f[0], f[1]);
+                if (l == 0) (v ? c.vs : c.ks)[sat_s[x.t] + (long long)(x.h0 + u) * c.page_size] = scale;
+            } else {
+                Elem<C>::store8(dst + ln.c0, p);
+                Elem<C>::store8(dst + ln.c1, q);
             }
         }
     }
@@ -283,8 +304,9 @@ cudaError_t rows_by_size(const RopeDev& r, const RopeRows& a, bool wide, cudaStr
 
 template <class T, class C, int D, int U>
 cudaError_t append(const RopeDev& r, const KvDev& c, const KvBatchDev& b, const RopeAppend& a, cudaStream_t s) {
-    const int per = (a.heads + 2 * c.n_heads + U - 1) / U * (D / 16);
-    const int tokens = min(32, max(1, kThreads / per));
+    const int per = ((a.heads + U - 1) / U + 2 * ((c.n_heads + U - 1) / U)) * (D / 16);
+    // of many tokens a block takes several rounds: finding their places is a chain of loads that all of them share
+    const int tokens = min(32, max(max(1, kThreads / per), min(kRounds, b.n_tok / (148 * 4))));
     kv_append_rope_kernel<T, C, D, U><<<(unsigned)((b.n_tok + tokens - 1) / tokens + 1), kThreads, (size_t)tokens * r.rot * 4,
                                         s>>>(r, c, b, a, FastDiv((uint32_t)c.page_size), tokens);
     return cudaGetLastError();

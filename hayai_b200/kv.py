@@ -43,8 +43,8 @@ class _Batch(ctypes.Structure):
 
 
 class _Shared(ctypes.Structure):
-    _fields_ = [("n_groups", ctypes.c_int), ("max_new", ctypes.c_int), ("seq_start", ctypes.c_void_p),
-                ("length", ctypes.c_void_p)]
+    _fields_ = [("n_groups", ctypes.c_int), ("max_new", ctypes.c_int), ("least", ctypes.c_int64),
+                ("seq_start", ctypes.c_void_p), ("length", ctypes.c_void_p)]
 
 
 class _Pages(ctypes.Structure):
@@ -151,19 +151,20 @@ class KvShared:
     """Groups of a batch's sequences that share their first tokens: group g is the sequences
     seq_start[g] to seq_start[g + 1] (int32 [n_groups + 1]), whose first length[g] positions (int32
     [n_groups]) are the same, and are read by the first one's pages.  max_new: a bound on any group's new
-    tokens, where the program knows one."""
+    tokens, where the program knows one.  least: how many tokens of reading the sharing has to save, over all
+    groups, to be made (0: as many as its kernels' starts are worth)."""
 
-    def __init__(self, seq_start, length, max_new: int = 0):
+    def __init__(self, seq_start, length, max_new: int = 0, least: int = 0):
         torch = _torch()
         for t in (seq_start, length):
             _need(t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.device == seq_start.device,
                   "seq_start and length must be int32 CUDA tensors of one device and one axis")
             _need(t.shape[0] <= 1 or t.stride(0) == 1, "seq_start and length must be contiguous")
         _need(seq_start.shape[0] == length.shape[0] + 1, "length must hold n_groups and seq_start n_groups + 1")
-        _need(max_new >= 0, "max_new must not be negative")
+        _need(max_new >= 0 and least >= 0, "max_new and least must not be negative")
         self._keep = (seq_start, length)
         self.index = seq_start.get_device()
-        self.struct = _Shared(length.shape[0], min(max_new, 2**31 - 1), seq_start.data_ptr(), length.data_ptr())
+        self.struct = _Shared(length.shape[0], min(max_new, 2**31 - 1), min(least, 2**62), seq_start.data_ptr(), length.data_ptr())
         self.ref = ctypes.addressof(self.struct)
 
 

@@ -46,6 +46,7 @@ pub struct hc_kv_batch {
 pub struct hc_kv_shared {
     pub n_groups: c_int,
     pub max_new: c_int,
+    pub least: i64,
     pub seq_start: *const i32,
     pub length: *const i32,
 }

@@ -81,7 +81,7 @@ class Groups:
         self.cache = hb.KvCache(*self.pool, *self.scale)
         self.batch = hb.KvBatch(self.table, self.q_start, self.kv_len, self.rows, max(self.new))
         self.starts, self.length = ints(starts), ints([p for p, _ in groups])
-        self.shared = hb.KvShared(self.starts, self.length, max(sum(n for n, _ in s) for _, s in groups))
+        self.shared = hb.KvShared(self.starts, self.length, max(sum(n for n, _ in s) for _, s in groups), 1)
 
     def q(self, heads, dtype, scale=1.0):
         return (torch.randn(self.rows, heads, self.dim, generator=self.g, device=DEV) * scale).to(T[dtype])
@@ -191,16 +191,16 @@ def test_lengths_are_cut_to_what_all_new_tokens_see(engine, dtype, cache):
 def test_sequences_outside_the_groups(engine):
     s = Groups(CASES["ragged"], 2, 64, 16, "f16")
     n = len(s.new)
-    check(engine, s, 8, "f16", shared=hb.KvShared(ints([3, 5, 6]), ints([0, 200])))
-    check(engine, s, 8, "f16", shared=hb.KvShared(ints([0, 3]), ints([37]), 4))
-    check(engine, s, 8, "f16", shared=hb.KvShared(ints([n, n]), ints([37])))
-    check(engine, s, 8, "f16", shared=hb.KvShared(ints([0]), ints([])))
+    check(engine, s, 8, "f16", shared=hb.KvShared(ints([3, 5, 6]), ints([0, 200]), 0, 1))
+    check(engine, s, 8, "f16", shared=hb.KvShared(ints([0, 3]), ints([37]), 4, 1))
+    check(engine, s, 8, "f16", shared=hb.KvShared(ints([n, n]), ints([37]), 0, 1))
+    check(engine, s, 8, "f16", shared=hb.KvShared(ints([0]), ints([]), 0, 1))
 
 
 def test_without_hints_and_with_wrong_ones(engine):
     s = Groups(CASES["chunks"], 2, 128, 16, "bf16")
     for most in (0, 1, 10**9):
-        check(engine, s, 16, "bf16", shared=hb.KvShared(s.starts, s.length, most))
+        check(engine, s, 16, "bf16", shared=hb.KvShared(s.starts, s.length, most, 1))
     s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows)
     check(engine, s, 16, "bf16")
 
@@ -292,7 +292,7 @@ def test_forked_pages(engine):
     nobody = hb.KvShared(ints([0]), ints([]))
     step([101, 0, 0, 0, 0, 40], nobody)
     engine.kv_fork_dev(pages, ints([0] * 4), ints([1, 2, 3, 4]))
-    family = hb.KvShared(ints([0, 5]), ints([101]))
+    family = hb.KvShared(ints([0, 5]), ints([101]), least=1)
     for _ in range(3):
         engine.kv_resize_dev(pages, ints([0, 1, 2, 3, 4]), kv_len[:5] + 1)
         step([1] * 5 + [0], family)
@@ -352,9 +352,22 @@ def test_groups_out_of_range_are_reported(engine, starts, length):
     s = Groups([(37, [(1, 1), (2, 3), (1, 40)]), (20, [(1, 4), (1, 1)])], 2, 64, 16, "f16")
     q = s.q(4, "f16")
     out = torch.empty_like(q)
-    engine.attn_shared_dev(s.cache, s.batch, hb.KvShared(ints(starts), ints(length)), q, out)
+    engine.attn_shared_dev(s.cache, s.batch, hb.KvShared(ints(starts), ints(length), 0, 1), q, out)
     with pytest.raises(hb.CudaError, match="out of range"):
         engine.sync()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_what_sharing_has_to_save(engine, dtype):
+    """Two groups of five save 4 * 300 + 4 * 100 tokens: up to there it is made, past it not; by the library's rule it is
+    not.  All are the same results, and bit for bit where nothing is shared."""
+    s = Groups([(300, [(1, 30)] * 5), (100, [(2, 9)] * 5)], 2, 64, 16, "bf16")
+    q = s.q(8, dtype)
+    plain, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    engine.attn_paged_dev(s.cache, s.batch, q, plain, lse=lse)
+    got = [check(engine, s, 8, dtype, q=q, shared=hb.KvShared(s.starts, s.length, least=n))[0] for n in (1, 1600, 1601, 10**30, 0)]
+    assert torch.equal(got[0], got[1]) and not torch.equal(got[1], got[2])
+    assert all(torch.equal(g, plain) for g in got[2:])
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
