@@ -102,36 +102,6 @@ __device__ __forceinline__ ManyRow many_row(const AttnArgs& ar, const KvSeq& q, 
     return r;
 }
 
-// O += P V of one unit by the rows' threads, leaving out weights of zero.
-template <bool BF, int D>
-__device__ __noinline__ void many_product(uint32_t tO, uint32_t tP, const uint8_t* v, bool fresh) {
-#pragma unroll 1
-    for (int k = 0; k < D / 32; ++k) {
-        float o[32];
-        tc_ld32(tO + 32 * k, o);
-        tc_wait_ld32(o);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = fresh ? 0.f : o[i];
-#pragma unroll 1
-        for (int t = 0; t < 128; ++t) {
-            const uint32_t two = tc_ld1(tP + (t >> 1)), w = t & 1 ? two >> 16 : two & 0xffffu;
-            const float p = BF ? __uint_as_float(w << 16) : h2f((uint16_t)w);
-            if (p != 0.f) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int d = 32 * k + i;
-                    const uint16_t x = *reinterpret_cast<const uint16_t*>(v + (d >> 6) * (128 * 128) + t * 128 +
-                                                                         ((((d & 63) >> 3) ^ (t & 7)) << 4) + (d & 7) * 2);
-                    o[i] += p * (BF ? __uint_as_float((uint32_t)x << 16) : h2f(x));
-                }
-            }
-            __syncwarp();
-        }
-        tc_st32(tO + 32 * k, o);
-    }
-    tc_wait_st();
-}
-
 template <class T, class C, int D>
 __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid_constant__ AttnArgs a) {
     using F = ManyCfg<C, D>;
@@ -151,7 +121,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
 
     if (a.early) after_previous();
-    if (a.first) let_next_start();
+    if (a.early) let_next_start();
+    if ((a.unless && __ldcg(a.unless)) || (a.only && !__ldcg(a.only))) return;
     // the schedule's prefix sums lie in the last key and value tile until warp 13 has its place
     int* const pre_s = reinterpret_cast<int*>(smem + F::oKV + (NB - 1) * TILE);
     const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 16);

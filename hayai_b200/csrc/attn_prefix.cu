@@ -48,7 +48,7 @@ struct PfxCfg {
     static constexpr int NSC = 8;                                    // scales: ring of 8 units, K then V
     static constexpr int oKV = 2 * TILE, oSTG = oKV + NB * TILE, oSC = oSTG + NSTG * STG;
     static constexpr int oRS = oSC + (I8 ? NSC * 1024 : 0);  // the rows' score factors, of two runs
-    static constexpr int oBAR = oRS + 2048, oMISC = oBAR + 512, BYTES = oMISC + 64;
+    static constexpr int oBAR = oRS + 2048, oMISC = oBAR + 448, BYTES = oMISC + 64;
 };
 
 // The block's runs of units, one tile after the other; every role goes through them for itself.
@@ -67,9 +67,8 @@ struct PfxWalk {
     __device__ __forceinline__ bool next() {
         while (++t < n) {
             const int4* const s = reinterpret_cast<const int4*>(p.tiles + t);
-            reinterpret_cast<int4*>(&x)[0] = __ldcg(s);
-            reinterpret_cast<int4*>(&x)[1] = __ldcg(s + 1);
-            reinterpret_cast<int4*>(&x)[2] = __ldcg(s + 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(&x)[i] = __ldcg(s + i);
             if (x.place >= b1) return false;
             wide = x.cost == 2;
             // a unit belongs to the block that has its first place
@@ -104,11 +103,12 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sb = smem_addr(smem), bars = sb + F::oBAR;
     // barriers: key and value tiles full and empty; S ready, P's first and second part ready, O ready (of each half);
-    // queries in, queries free; 8-bit pages: a unit's scales there and done with, a tile of codes there and converted
+    // queries in, queries free; a unit checked (of each half); 8-bit pages: a unit's scales there and done with, a tile of codes there and converted
     const uint32_t b_full = bars, b_empty = b_full + 8 * NB, b_s = b_empty + 8 * NB, b_p = b_s + 16, b_o = b_p + 32,
                    b_q = b_o + 16, b_qf = b_q + 8, b_sc = b_qf + 8, b_scf = b_sc + 8 * NSC, b_stg = b_scf + 8 * NSC,
-                   b_stge = b_stg + 8 * F::NSTG;
+                   b_stge = b_stg + 8 * F::NSTG, b_chk = b_stge + 8 * F::NSTG;
     float* const rsc = reinterpret_cast<float*>(smem + F::oRS);
+    // TMEM base; a zero; [2..3] a half's product is done by hand; [4..9] what its checks found, three in turn
     int* const misc = reinterpret_cast<int*>(smem + F::oMISC);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
     after_previous();
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
     if (U <= 0 || c >= G) return;
     const AttnShares share(U, G);
     if (threadIdx.x == 0) {
-        misc[1] = 0;
+        for (int i = 1; i < 10; ++i) misc[i] = 0;
         for (int i = 0; i < NB; ++i) {
             mbar_init(b_full + 8 * i, 4);
             mbar_init(b_empty + 8 * i, 1);
@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
             mbar_init(b_p + 16 * i, 4);
             mbar_init(b_p + 16 * i + 8, 4);
             mbar_init(b_o + 8 * i, 1);
+            mbar_init(b_chk + 8 * i, 4);
         }
         mbar_init(b_q, 8);
         mbar_init(b_qf, 1);
@@ -162,7 +163,8 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
         const uint32_t tS = tmem + lanes + half * 128, tO = tmem + lanes + 256 + half * 128;
         constexpr float kLift = BF ? 0.f : 7.f;  // log2 of the weights' common factor
         uint32_t ph_s = 0, ph_o = 0;
-        int units = 0;  // of the block before this run, for the scales' ring
+        int units = 0;   // of the block before this run, for the rings
+        int checks = 0;  // units checked for values that are not finite
         // The tile's row r, where the row is this thread's: its query in and its scores' factor, once the products of the
         // run before, n - 1, have read theirs.
         auto queries = [&](int n, int r) {
@@ -216,8 +218,17 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
         if (more) queries(0, row_of());
         for (int n = 0; more && ok; ++n) {
             const int nu = w.hi - w.lo, step = w.wide ? 1 : 2, first = w.wide ? 0 : half;
-            const int r = row_of(), lo = w.lo, len = w.x.len;
-            const bool real = r < w.x.nr;
+            const int r = row_of(), kvt = 2 * units, last = 2 * nu - 1;
+            const bool real = r < w.x.nr, wide = w.wide;
+            // positions from the run's first on that a row sees: this one's, and the half's first and last row's (whose
+            // own are the fewest and the most)
+            const int start = w.x.from + w.lo * UNIT;
+            auto seen = [&](int row) {
+                return (w.x.pos0 == kAllSeen ? w.x.len : min(w.x.len, w.x.pos0 + a.by_group(w.x.r0 + row) + 1)) - start;
+            };
+            const int r_first = wide ? half * 128 : 0, sees = seen(min(r, w.x.nr - 1)), least = seen(min(r_first, w.x.nr - 1)),
+                      most_seen = seen(min(r_first + 127, w.x.nr - 1));
+            const bool idle = r_first + 32 * (warp & 3) >= w.x.nr;  // none of the warp's rows is there
             const int piece = w.x.piece + (w.wide ? c - w.x.c0 : 2 * (c - w.x.c0) + half) * w.x.nr + r;
             // a narrow tile's factors are the first half's; they are written over two runs later, when all warps are past this
             if (!many_wait(b_q, n & 1, ok)) break;
@@ -228,12 +239,64 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                 if (!many_wait(b_s + 8 * half, ph_s, ok)) break;
                 ph_s ^= 1;
                 tc_fence_after();
+                const bool full = (u + 1) * UNIT <= least;
+                uint32_t odd = 0;
+                const uint8_t* vtile = nullptr;
+                if constexpr (!I8) {
+                    // A value that is not finite, where some row does not see it: 0 * infinity must not reach that row, so
+                    // that the unit's product is then done by the rows' threads (rare).  V's tile is not given back before
+                    // this half's weights, and the tile that was in its place is before this unit's keys in the ring: its
+                    // barrier is at its phase or the one before.
+                    if (!full && least < w.x.len - start) {
+                        const int vt = kvt + (wide ? 2 * u + 1 : min(2 * u + 2, last));
+                        if (!many_wait(b_full + 8 * (vt % NB), (vt / NB) & 1, ok)) break;
+                        vtile = smem + F::oKV + (vt % NB) * TILE;
+                        constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+                        if (u * UNIT + rt >= least) {
+#pragma unroll 4
+                            for (int i = 0; i < D / 8; ++i) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(vtile + (i >> 3) * HALF + rt * 128 + (((i + rt) & 7) << 4));
+                                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) odd |= (y[k] & E) == E || ((y[k] >> 16) & E) == E;
+                            }
+                        }
+                        // the half's four warps decide together: three flags in turn, each cleared a check ahead
+                        int* const flag = misc + 4 + 3 * half;
+                        if (__any_sync(0xffffffffu, odd != 0) && ln == 0) flag[checks % 3] = 1;
+                        if (rt == 0) flag[(checks + 1) % 3] = 0;
+                        __syncwarp();
+                        if (ln == 0) mbar_arrive(b_chk + 8 * half);
+                        if (!many_wait(b_chk + 8 * half, checks & 1, ok)) break;
+                        odd = *(volatile int*)&flag[checks % 3];
+                        ++checks;
+                    }
+                    // read by the products' warp after the arrivals; it has read the last unit's before it issued this S
+                    if (rt == 0) misc[2 + half] = (int)odd;
+                }
+                auto arrive = [&](int part) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (ln == 0) {
+                        mbar_arrive(b_p + 16 * half + 8 * part);
+                        if (I8 && part == 1) {
+                            const uint32_t bar = b_scf + 8 * ((units + u) % NSC);
+                            mbar_arrive(bar);
+                            if (step == 2) mbar_arrive(bar);
+                        }
+                    }
+                };
+                if (idle) {
+                    arrive(0);
+                    arrive(1);
+                    continue;
+                }
                 float s[128];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc_ld32(tS + 32 * k, s + 32 * k);
                 auto size = [](float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; };  // what is not finite has none
                 auto size_log2 = [](uint32_t bits) { return max((int)(bits >> 23) - 126, -80); };
-                const int left = len - (lo + u) * UNIT;  // positions from the unit's first on
+                const int left = sees - u * UNIT;  // positions that the row sees from the unit's first on
                 float ev = 0.f;
                 bool mixed = false;
                 const float4 *ksc = nullptr, *vsc = nullptr;
@@ -245,17 +308,17 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                     vsc = reinterpret_cast<const float4*>(sc + 512);
                     const float4 v = vsc[ln];
                     const float vs[4] = {v.x, v.y, v.z, v.w};
-                    uint32_t most = 0, least = 0x7f7fffffu;
+                    uint32_t most = 0, fewest = 0x7f7fffffu;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (4 * ln + i >= left) continue;
+                        if (4 * ln + i >= most_seen - u * UNIT) continue;
                         const uint32_t b = __float_as_uint(size(vs[i]));
                         most = max(most, b);
-                        least = min(least, b);
+                        fewest = min(fewest, b);
                     }
                     const int top = size_log2(__reduce_max_sync(0xffffffffu, most));
                     ev = (float)top;
-                    mixed = size_log2(__reduce_min_sync(0xffffffffu, least)) < top - 6;
+                    mixed = size_log2(__reduce_min_sync(0xffffffffu, fewest)) < top - 6;
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc_wait_ld32(s + 32 * k);
@@ -268,7 +331,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                         s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = y.x, s[4 * i + 3] = y.y;
                     }
                 }
-                if (left < UNIT) {
+                if (!full) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
                         if (i >= left) s[i] = -INFINITY;
@@ -307,6 +370,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                 const float mm = m == -INFINITY ? 0.f : m;
                 const float2 rs2 = make_float2(rs, rs);
                 float2 nm2 = make_float2(kLift - mm, kLift - mm);
+                auto weights = [&](auto masked) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     uint32_t pk[16];
@@ -320,20 +384,19 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                         if constexpr (I8) {
                             if ((i & 1) == 0) vs4 = vsc[8 * k + (i >> 1)];
                             q = mul2(q, i & 1 ? make_float2(vs4.z, vs4.w) : make_float2(vs4.x, vs4.y));
+                            if constexpr (decltype(masked)::value) {  // whatever a masked position's scale is
+                                if (s[e] == -INFINITY) q.x = 0.f;
+                                if (s[e + 1] == -INFINITY) q.y = 0.f;
+                            }
                         }
                         pk[i] = BF ? pack_b2(q.x, q.y) : pack_h2(q.x, q.y);
                     }
                     tc_st16(tS + 16 * k, pk);
                     if (k & 1) {
                         tc_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (ln == 0) mbar_arrive(b_p + 16 * half + 8 * (k >> 1));
-                        if (I8 && k == 3 && ln == 0) {
-                            const uint32_t bar = b_scf + 8 * ((units + u) % NSC);
-                            mbar_arrive(bar);
-                            if (step == 2) mbar_arrive(bar);
-                        }
+                        if constexpr (!I8)
+                            if (k == 3 && odd) many_product<BF, D>(tO, tS, vtile, u == first);
+                        arrive(k >> 1);
                         if (k == 1) {
                             // The second part's arithmetic is not to be moved before the first one's arrival: it takes a
                             // zero that is read behind it.
@@ -343,6 +406,11 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                         }
                     }
                 }
+                };
+                if (I8 && !full)
+                    weights(std::true_type());
+                else
+                    weights(std::false_type());
             }
             units += nu;
             if (!ok) break;
@@ -455,7 +523,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                     has = i < last;
                     if (has) {
                         w.tile_at(i, unit, v);
-                        const int j = (w.lo + unit) * UNIT + mine;
+                        const int j = w.x.from + (w.lo + unit) * UNIT + mine;
                         has = j < w.x.len;
                         if (has) {
                             const int q = a.by_page(j);
@@ -564,13 +632,16 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                     const uint32_t tP = tmem + h * 128, tO = tP + 256, bar = b_p + 16 * h, par = (ph_p >> h) & 1;
                     if (!ready(bar, par)) break;
                     tc_fence_after();
+                    const bool by_hand = !I8 && *(volatile int*)&misc[2 + h];
+                    if (!by_hand)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)  // O += P V
-                        many_mma_ta(tO, tP + 8 * i, vd + i * 128, idO, j >= 2 || i ? 1u : 0u);
+                        for (int i = 0; i < 4; ++i)  // O += P V
+                            many_mma_ta(tO, tP + 8 * i, vd + i * 128, idO, j >= 2 || i ? 1u : 0u);
                     if (!ready(bar + 8, par)) break;
                     tc_fence_after();
+                    if (!by_hand)
 #pragma unroll
-                    for (int i = 4; i < 8; ++i) many_mma_ta(tO, tP + 8 * i, vd + i * 128, idO, 1u);
+                        for (int i = 4; i < 8; ++i) many_mma_ta(tO, tP + 8 * i, vd + i * 128, idO, 1u);
                     ph_p ^= 1u << h;
                     if (!wide || h) many_commit(vgone);
                     if (j + 2 >= nj)
@@ -594,7 +665,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                     int unit;
                     bool v;
                     w.tile_at(i, unit, v);
-                    const int v0 = (w.lo + unit) * UNIT, v1 = min(v0 + UNIT, w.x.len);
+                    const int v0 = w.x.from + (w.lo + unit) * UNIT, v1 = min(v0 + UNIT, w.x.len);
                     const uint32_t bar = b_stg + 8 * (t % NS), dst = sb + F::oSTG + (t % NS) * F::STG;
                     if (t >= NS && !many_wait(b_stge + 8 * (t % NS), ((t / NS) - 1) & 1, ok)) break;
                     const uint8_t* const src = (v ? a.c.v : a.c.k) + 64ull * ((uint32_t)w.x.hk * a.c.head);
@@ -639,7 +710,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) attn_prefix_kernel(const __gri
                     float sc[2][4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int j = u * UNIT + 32 * i + ln, p = a.by_page(j);
+                        const int j = w.x.from + u * UNIT + 32 * i + ln, p = a.by_page(j);
                         const int pg = j < w.x.len ? __ldg(table + p) : -1;
                         sc[0][i] = sc[1][i] = 0.f;
                         if ((unsigned)pg < (unsigned)a.c.n_pages) {

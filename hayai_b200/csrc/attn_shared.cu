@@ -3,11 +3,13 @@
 //
 // A group's rows see its prefix whole, so that the prefix is one more sequence, of all the group's new tokens and
 // not causal: its keys are read once for the group, and its rows fill the tensor cores' tiles.  One call is
-//     attn_groups    what every group shares for this step, and its tiles
-//     attn_prefix    prefixes of more than a few rows per kv head (attn_prefix.cu), in pieces
-//     attn_few       prefixes of few rows, one result each
-//     attn_many/few  what every sequence has behind its prefix (AttnArgs::first)
-//     attn_join      out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts
+//     attn_groups    what every group shares for this step, and the tiles: of the prefixes, then of what every sequence
+//                    has behind its own
+//     attn_prefix    the tiles (attn_prefix.cu), in pieces
+//     attn_few       of single tokens, what is behind the prefixes (AttnArgs::first), which has no tiles then
+//     attn_join      out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's pieces
+// or, of f32 rows, attn_few over the prefixes and again over what is behind them, and the joining.
+// Where nothing is shared after all, the two others find no tiles, and the paged attention's kernels behind them do the work.
 #include "attn_rows.cuh"
 #include "block_scan.cuh"
 
@@ -17,25 +19,53 @@ namespace {
 
 constexpr int kTileRows = 256, kUnit = 128, kOver = 2;
 
+// Positions that tile k of `tok` tokens sees, at `pos` and following (kAllSeen: the whole of [from, len)).
+__device__ __forceinline__ int tile_end(int k, int rows, int group, int len, int pos) {
+    if (pos == kAllSeen) return len;
+    return min(len, pos + (min((k + 1) * kTileRows, rows) - 1) / group + 1);
+}
+__device__ __forceinline__ int tile_units(int from, int end) { return end > from ? (end - from + kUnit - 1) / kUnit : 0; }
+__device__ __forceinline__ bool tile_narrow(int k, int rows) { return rows - k * kTileRows <= kTileRows / 2; }
+// Places of a kv head's first `tiles` tiles.  (Not inlined, as little of the kernel below as can be: its code runs once,
+// and fetching it is most of its time.)
+__device__ __noinline__ int tile_places(int tiles, int rows, int group, int from, int len, int pos) {
+    int w = 0;
+#pragma unroll 1
+    for (int k = 0; k < tiles; ++k) {
+        const int u = tile_units(from, tile_end(k, rows, group, len, pos));
+        if (u) w += min((tile_narrow(k, rows) ? u : 2 * u) + kOver, 0x7fffffff - w);
+    }
+    return w;
+}
+__device__ __noinline__ long long scan_1024(long long x, long long* scratch, long long& total) { return block_scan(x, scratch, total); }
+
 // A warp per group: how many tokens its sequences share for this step.  All new tokens have to see them all, so that
 // they are at most the tokens that every sequence had before; a group of one sequence shares nothing.  Then the
-// groups' tiles, in a line whose places the blocks of attn_prefix.cu share equally.
+// tiles, in a line whose places the blocks of attn_prefix.cu share equally: a unit of a wide tile is two places, of a narrow
+// one one, and starting and finishing a tile counts as two more.
 __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvSharedDev g, int cap) {
     __shared__ long long scratch[33];
-    __shared__ int len_s[HC_KV_SEQS], tok_s[HC_KV_SEQS], tile_s[HC_KV_SEQS + 1], place_s[HC_KV_SEQS];
-    const int tid = threadIdx.x, ln = lane_id(), group = g.heads / g.kv_heads;
-    let_next_start();
-    int *const from_s = tile_s, *const to_s = place_s;  // the groups' sequences, until their tiles are counted
     __shared__ unsigned long long saved_s;
+    __shared__ int runs_s;
+    extern __shared__ int ent[];
+    // entities: the groups' prefixes, then the sequences
+    const int E = g.n + b.n_seq, tid = threadIdx.x, ln = lane_id(), group = g.heads / g.kv_heads;
+    int *const tok_s = ent, *const from_s = tok_s + E, *const len_s = from_s + E, *const tile_s = len_s + E,
+               *const place_s = tile_s + E, *const q0_s = place_s + E, *const w_s = q0_s + E, *const of_s = w_s + E;  // [n_seq] a sequence's group, or -1
+    let_next_start();
     if (tid == 0) saved_s = 0;
-    for (int s = tid; s < b.n_seq; s += 1024) g.first[s] = 0;
+#pragma unroll 1
+    for (int s = tid; s < b.n_seq; s += 1024) of_s[s] = -1;
     __syncthreads();
+    int *const s0_s = tile_s, *const s1_s = place_s;  // the groups' sequences, until the tiles are counted
+#pragma unroll 1
     for (int i = tid >> 5; i < g.n; i += 32) {
         const int a0 = __ldg(g.seq_start + i), a1 = __ldg(g.seq_start + i + 1), given = __ldg(g.length + i);
         const int s0 = min(max(a0, 0), b.n_seq), s1 = min(max(a1, s0), b.n_seq);
         int most = min(max(given, 0), cap), seqs = 0;
         if (s0 != a0 || s1 != a1 || most != given)
             if (ln == 0) atomicOr(b.err, kErrKvRange);
+#pragma unroll 1
         for (int s = s0 + ln; s < s1; s += 32) {
             const KvSeq q = kv_seq(b, cap, s);
             if (q.q1 == q.q0) continue;
@@ -47,161 +77,225 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
         if (seqs < 2) most = 0;
         if (ln == 0) {
             len_s[i] = most;
-            from_s[i] = s0;
-            to_s[i] = s1;
-            atomicAdd(&saved_s, (unsigned long long)most * max(seqs - 1, 0));
+            s0_s[i] = s0;
+            s1_s[i] = s1;
+            if (most) atomicAdd(&saved_s, (unsigned long long)most * (seqs - 1));
         }
     }
     __syncthreads();
     const bool worth = saved_s >= (unsigned long long)g.least;
+    if (!worth) {
+        if (tid == 0) g.line[kLineTiles] = g.line[kLineOwn] = g.line[kLinePlaces] = 0;
+        return;
+    }
+#pragma unroll 1
     for (int i = tid >> 5; i < g.n; i += 32) {
-        const int s0 = from_s[i], s1 = to_s[i], most = worth ? len_s[i] : 0;
-        for (int s = s0 + ln; s < s1; s += 32) g.first[s] = most;
-        __syncwarp();
+        const int s0 = s0_s[i], s1 = s1_s[i], most = len_s[i];
+        if (most)
+#pragma unroll 1
+            for (int s = s0 + ln; s < s1; s += 32) of_s[s] = i;
         if (ln == 0) {
             // its new tokens' rows, cut as kv_seq cuts them
             const int q0 = min(max(__ldg(b.q_start + s0), 0), b.n_tok), q1 = min(max(__ldg(b.q_start + s1), q0), b.n_tok);
-            const int tok = most ? q1 - q0 : 0;
-            len_s[i] = most;
-            tok_s[i] = tok;
-            const bool few = (long long)tok * group <= g.few_rows;
+            tok_s[i] = most ? q1 - q0 : 0;
+            from_s[i] = 0;
+            q0_s[i] = q0;
             g.q_start[i] = q0;
             if (i == g.n - 1) g.q_start[g.n] = q1;
-            g.len[i] = few ? most : 0;
+            g.len[i] = most;
             g.row[i] = min(s0, b.n_seq - 1);
         }
     }
     __syncthreads();
-    // ---- tiles and places of every group
-    auto units_of = [&](int i) { return (len_s[i] + kUnit - 1) / kUnit; };
-    long long tiles[2] = {0, 0}, places[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        if (i >= g.n || tok_s[i] == 0) continue;
-        const long long r = (long long)tok_s[i] * group, n = (r + kTileRows - 1) / kTileRows;
-        tiles[e] = n * g.kv_heads;
-        const bool narrow = r - (n - 1) * kTileRows <= kTileRows / 2;
-        if (r > g.few_rows) places[e] = (n * (2ll * units_of(i) + kOver) - (narrow ? units_of(i) : 0)) * g.kv_heads;
+#pragma unroll 1
+    for (int s = tid; s < b.n_seq; s += 1024) {
+        const KvSeq q = kv_seq(b, cap, s);
+        const int first = of_s[s] >= 0 ? len_s[of_s[s]] : 0;
+        g.first[s] = first;
+        tok_s[g.n + s] = g.few_behind && !first ? 0 : q.q1 - q.q0;
+        from_s[g.n + s] = first;
+        len_s[g.n + s] = q.len;
+        q0_s[g.n + s] = q.q0;
     }
-    long long all_tiles, U;
-    long long at = block_scan(tiles[0] + tiles[1], scratch, all_tiles);
-    long long pl = block_scan(places[0] + places[1], scratch, U);
+    __syncthreads();
+    // ---- tiles and places of every entity; of those that the kernel for few rows does only what the joining takes
+    auto elsewhere = [&](int i) { return i < g.n ? g.few : g.few_behind; };
+    auto pos_of = [&](int i) { return i < g.n ? kAllSeen : len_s[i] - tok_s[i]; };
+    const int each = (E + 1023) / 1024, e0 = min(tid * each, E), e1 = min(e0 + each, E);
+    long long tiles = 0, places = 0, all_tiles, U;
+#pragma unroll 1
+    for (int i = e0; i < e1; ++i) {  // a kv head's tiles and places
+        const int rows = tok_s[i] * group, n = (rows + kTileRows - 1) / kTileRows;
+        tile_s[i] = elsewhere(i) ? i >= g.n && rows : n * g.kv_heads;
+        place_s[i] = w_s[i] = elsewhere(i) ? 0 : tile_places(n, rows, group, from_s[i], len_s[i], pos_of(i));
+        tiles += tile_s[i];
+        places += (long long)w_s[i] * g.kv_heads;
+    }
+    long long at = scan_1024(tiles, scratch, all_tiles), pl = scan_1024(places, scratch, U);
     const bool fits = all_tiles <= g.max_tiles && U < 0x7fffffff;
-    if (!fits && tid == 0) atomicOr(b.err, kErrKvRange);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        if (i < g.n && fits) tile_s[i] = (int)at, place_s[i] = (int)pl;
-        at += tiles[e];
-        pl += places[e];
+#pragma unroll 1
+    for (int i = e0; i < e1; ++i) {  // what is before them
+        const int n = tile_s[i], w = place_s[i];
+        tile_s[i] = (int)at, place_s[i] = (int)pl;
+        at += n;
+        pl += (long long)w * g.kv_heads;
     }
     const int n_tiles = fits ? (int)all_tiles : 0;
     const int G = fits ? max(1, min(g.blocks, (int)U / 4)) : 1;  // shares of four places and more: every one has a unit
     __syncthreads();
     const AttnShares share(max((int)(fits ? U : 0), 1), G);
     long long rows_before = 0;
+    int runs = 0;
+#pragma unroll 1
     for (int t0 = 0; t0 < n_tiles; t0 += 1024) {
         const int t = t0 + tid;
         PrefixTile x{};
         long long rows = 0;
         if (t < n_tiles) {
-            int lo = 0, hi = g.n - 1;  // the last group whose tiles start at or before t, of those at one place the last
+            int lo = 0, hi = E - 1;  // the last entity whose tiles start at or before t, of those at one place the last
+#pragma unroll 1
             while (lo < hi) {
                 const int m = (lo + hi + 1) >> 1;
                 if (tile_s[m] <= t) lo = m;
                 else hi = m - 1;
             }
-            const int r = tok_s[lo] * group, per = (r + kTileRows - 1) / kTileRows, local = t - tile_s[lo];
-            const int units = units_of(lo), rest = r - (per - 1) * kTileRows;
-            const bool few = r <= g.few_rows, narrow = rest <= kTileRows / 2;
-            x.hk = local / per;
-            const int k = local - x.hk * per;
+            const int r = tok_s[lo] * group, per = (r + kTileRows - 1) / kTileRows, local = t - tile_s[lo], s = lo - g.n;
+            const int pos = pos_of(lo);
+            const bool all = elsewhere(lo);  // all rows of a sequence, for the joining
+            x.hk = all ? -1 : local / per;
+            const int k = all ? 0 : local - x.hk * per;
             x.r0 = k * kTileRows;
-            x.nr = k == per - 1 ? rest : kTileRows;
-            x.q0 = g.q_start[lo];
-            x.len = len_s[lo];
-            x.row = g.row[lo];
-            x.cost = k == per - 1 && narrow ? 1 : 2;
-            x.place = place_s[lo];
-            if (!few) {
-                x.units = units;
-                x.place += x.hk * (per * (2 * units + kOver) - (narrow ? units : 0)) + k * (2 * units + kOver);
+            x.nr = all ? tok_s[lo] * g.heads : min(kTileRows, r - x.r0);
+            x.q0 = q0_s[lo];
+            x.from = from_s[lo];
+            x.len = tile_end(k, r, group, len_s[lo], pos);
+            x.row = lo < g.n ? g.row[lo] : s;
+            x.pos0 = pos;
+            x.pre = -1;
+            if (s >= 0 && of_s[s] >= 0) {
+                const int i = of_s[s], to_head = (tok_s[i] * group + kTileRows - 1) / kTileRows;
+                x.pre = tile_s[i] + (all ? 0 : x.hk * to_head);
+                x.pre_row = (x.q0 - q0_s[i]) * group;
+                x.cost = to_head;
+            }
+            if (!all) x.cost = tile_narrow(k, r) ? 1 : 2;
+            x.units = all ? 0 : tile_units(x.from, x.len);
+            if (s >= 0) runs = max(runs, (x.nr + 7) / 8);
+            x.place = place_s[lo] + (all ? 0 : x.hk * w_s[lo]) + (k ? tile_places(k, r, group, x.from, len_s[lo], pos) : 0);
+            if (x.units) {
                 x.c0 = share.owner(x.place);
-                x.pieces = (share.owner(x.place + x.cost * (units - 1)) - x.c0 + 1) * (x.cost == 1 ? 2 : 1);
+                x.pieces = (share.owner(x.place + x.cost * (x.units - 1)) - x.c0 + 1) * (x.cost == 1 ? 2 : 1);
                 rows = (long long)x.pieces * x.nr;
-                const int end = x.place + x.cost * units + kOver;
+                const int end = x.place + x.cost * x.units + kOver;
+#pragma unroll 1
                 for (int c = x.place ? share.owner(x.place - 1) + 1 : 0; c < G && share.begin(c) < end; ++c) g.first_tile[c] = t;
             }
         }
         long long total;
-        x.piece = (int)(rows_before + block_scan(rows, scratch, total));
+        x.piece = (int)(rows_before + scan_1024(rows, scratch, total));
         rows_before += total;
-        if (t < n_tiles) g.tiles[t] = x;
+        if (t < n_tiles)  // 16 bytes at a time: the tiles are 64 bytes apart, and every store of a warp meets 32 sectors
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(g.tiles + t)[i] = reinterpret_cast<const int4*>(&x)[i];
     }
     // groups that overlap (offsets that do not ascend) may want more room than any others: nothing is made of them
-    const bool room = rows_before <= g.max_pieces;
+    const bool room = fits && rows_before <= g.max_pieces;
+    runs = __reduce_max_sync(0xffffffffu, runs);
+    if (tid == 0) runs_s = 0;
+    __syncthreads();
+    if (ln == 0) atomicMax(&runs_s, runs);
+    __syncthreads();
     if (tid == 0) {
         if (!room) atomicOr(b.err, kErrKvRange);
         g.line[kLineTiles] = room ? n_tiles : 0;
-        g.line[kLinePlaces] = fits && room ? (int)U : 0;
+        g.line[kLineOwn] = room ? tile_s[g.n] : 0;
+        g.line[kLineRuns] = runs_s;
+        g.line[kLinePlaces] = room ? (int)U : 0;
         g.line[kLineBlocks] = G;
     }
 }
 
-// A warp per row of a tile, eight rows of one at a time.  Bound by memory and its latency: a row's parts are asked for
-// together, before the weights that they count with are there.
+// A warp per row of a tile behind the prefixes, eight rows of one at a time.  Bound by memory and its latency: four of a
+// row's parts are asked for together, the prefix's pieces and then its own, and every lane forms the weights for itself.
 template <class T, int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, PrefixArgs p) {
-    constexpr int RUNS = kTileRows / 8, U = 8;
+__global__ void __launch_bounds__(256, 4) attn_join_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PrefixArgs p) {
+    constexpr int U = 4;
     after_previous();
-    const int n_tiles = __ldcg(p.line + kLineTiles), ln = lane_id();
+    let_next_start();
+    const int n_tiles = __ldcg(p.line + kLineTiles), own = __ldcg(p.line + kLineOwn), runs = __ldcg(p.line + kLineRuns),
+              ln = lane_id();
     const bool mine = ln < D / 4;
-    for (int w = blockIdx.x; w < n_tiles * RUNS; w += gridDim.x) {
-        const int4* const xt = reinterpret_cast<const int4*>(p.tiles + w / RUNS);
+    for (int w = blockIdx.x; w < (n_tiles - own) * runs; w += gridDim.x) {
         PrefixTile x;
-        reinterpret_cast<int4*>(&x)[0] = __ldcg(xt);
-        reinterpret_cast<int4*>(&x)[1] = __ldcg(xt + 1);
-        reinterpret_cast<int4*>(&x)[2] = __ldcg(xt + 2);
-        const int r = w % RUNS * 8 + (threadIdx.x >> 5);
+        const int4* const xs = reinterpret_cast<const int4*>(p.tiles + own + w / runs);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(&x)[i] = __ldcg(xs + i);
+        const int r = w % runs * 8 + (threadIdx.x >> 5);
         if (r >= x.nr) continue;
-        const int row = x.r0 + r, t = a.by_group(row);
-        const long long at = (long long)(x.q0 + t) * a.heads + x.hk * a.group + row - t * a.group;
-        // the parts: what is behind the prefix (divided by its sum), then the prefix's pieces, or its one result
-        const int n = x.pieces;
-        const size_t step = n ? x.nr : 0;
-        const float4* const o = reinterpret_cast<const float4*>(n ? p.part + ((size_t)x.piece + r) * D : p.few + at * D) + ln;
-        const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + x.piece + r;
-        float4 y0 = make_float4(0.f, 0.f, 0.f, 0.f), y[U];
-        if (mine) y0 = __ldcg(reinterpret_cast<const float4*>(a.base + at * D) + ln);
-        const float own = __ldcg(a.base_lse + at);
-        float2 v = make_float2(-INFINITY, 0.f);
-        if (n) {
-            if (ln < n) v = __ldcg(ml + ln * step);
-        } else if (ln == 0) {
-            const float e = __ldcg(p.few_lse + at);
-            v = make_float2(e, e == -INFINITY ? 0.f : 1.f);
+        int row = x.r0 + r, hk = x.hk;
+        if (hk < 0) {  // the r-th of all (token, query head)
+            const int t = r / a.heads, h = r - t * a.heads;
+            hk = a.by_group(h);
+            row = t * a.group + h - hk * a.group;
         }
-        const int parts = max(n, 1);
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (mine && k < parts) y[k] = __ldcg(o + k * step * (D / 4));
+        const int t = a.by_group(row);
+        const long long at = (long long)(x.q0 + t) * a.heads + hk * a.group + row - t * a.group;
+        // the row's places among its own pieces and its prefix's, and from one piece to the next
+        size_t p_own = (size_t)x.piece + r, p_pre = 0;
+        int s_own = x.nr, s_pre = 0, n_own = x.pieces, n_pre = 0;
+        bool w_own = false, w_pre = false;  // one result, divided by its sum
+        if (a.base) n_own = 1, p_own = at, w_own = true;
+        if (p.few) {
+            n_pre = 1, p_pre = at, w_pre = true;
+        } else if (x.pre >= 0) {
+            const int pr = x.pre_row + row;
+            const PrefixTile* const z = p.tiles + x.pre + (x.hk < 0 ? hk * x.cost : 0) + pr / kTileRows;
+            s_pre = __ldcg(&z->nr), n_pre = __ldcg(&z->pieces);
+            p_pre = (size_t)__ldcg(&z->piece) + pr % kTileRows;
         }
-        AttnJoin j;
-        auto ml_of = [&](int i) { return i < 32 ? v : __ldcg(ml + i * step); };  // a lane asks for its own part of a run of 32
-        auto o_of = [&](int i) {
-            if (i >= U) return __ldcg(o + i * step * (D / 4));
-            float4 z = y[0];
+        float m = -INFINITY, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+        const int n = n_pre + n_own;
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += U) {
+            float2 ml[U];
+            float4 o[U];
 #pragma unroll
-            for (int k = 1; k < U; ++k)
-                if (i == k) z = y[k];
-            return z;
-        };
-        j.join(1, mine, [&](int) { return make_float2(own, own == -INFINITY ? 0.f : 1.f); }, [&](int) { return y0; });
-        j.join(parts, mine, ml_of, o_of);
-        if (mine) attn_store<T>(a, x.q0, x.hk, row, D, 4 * ln, j.y, j.l, false);
-        if (ln == 0) attn_store_lse(a, x.q0, x.hk, row, j.m, j.l, false);
+            for (int k = 0; k < U; ++k) {
+                const int i = i0 + k;
+                ml[k] = make_float2(-INFINITY, 0.f);
+                o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < n) {
+                    const bool pre = i < n_pre, whole = pre ? w_pre : w_own;
+                    const size_t q = pre ? p_pre + (size_t)i * s_pre : p_own + (size_t)(i - n_pre) * s_own;
+                    if (whole) {
+                        const float e = __ldcg((pre ? p.few_lse : a.base_lse) + q);
+                        ml[k] = make_float2(e, e == -INFINITY ? 0.f : 1.f);
+                    } else {
+                        ml[k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + q);
+                    }
+                    if (mine) o[k] = __ldcg(reinterpret_cast<const float4*>((whole ? (pre ? p.few : a.base) : p.part) + q * D) + ln);
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < U; ++k) top = fmaxf(top, ml[k].x);
+            // a part that saw nothing has m = -inf and l = 0; one of scores that are not numbers has m = -inf only
+            const float old = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - top);
+            m = top;
+            l *= old;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = old == 0.f ? 0.f : y[e] * old;
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : ex2(ml[k].x - top);
+                l += ml[k].y * f;
+                if (f == 0.f) continue;  // a weight of zero takes nothing, whatever the value is
+                y[0] = fmaf(o[k].x, f, y[0]), y[1] = fmaf(o[k].y, f, y[1]);
+                y[2] = fmaf(o[k].z, f, y[2]), y[3] = fmaf(o[k].w, f, y[3]);
+            }
+        }
+        if (mine) attn_store<T>(a, x.q0, hk, row, D, 4 * ln, y, l, false);
+        if (ln == 0) attn_store_lse(a, x.q0, hk, row, m, l, false);
     }
 }
 
@@ -213,7 +307,11 @@ cudaError_t join(int head_dim, const AttnArgs& a, const PrefixArgs& p, int sms, 
 }  // namespace
 
 cudaError_t launch_attn_groups(const KvBatchDev& b, const KvSharedDev& g, int cap, cudaStream_t s) {
-    attn_groups_kernel<<<1, 1024, 0, s>>>(b, g, cap);
+    const int bytes = (7 * (g.n + b.n_seq) + b.n_seq) * 4;
+    static SmemOptIn opted;
+    const cudaError_t e = opted(reinterpret_cast<const void*>(attn_groups_kernel), (7 * 2 * HC_KV_SEQS + HC_KV_SEQS) * 4);
+    if (e != cudaSuccess) return e;
+    attn_groups_kernel<<<1, 1024, bytes, s>>>(b, g, cap);
     return cudaGetLastError();
 }
 

@@ -2,6 +2,7 @@
 // attn_prefix.cu): products with operands in shared memory or TMEM, TMEM loads and stores, packed f32 arithmetic.
 #pragma once
 
+#include "kv.cuh"
 #include "tc5.cuh"
 
 namespace hc {
@@ -139,6 +140,36 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+
+// O += P V of one unit by the rows' threads, leaving out weights of zero.
+template <bool BF, int D>
+__device__ __noinline__ void many_product(uint32_t tO, uint32_t tP, const uint8_t* v, bool fresh) {
+#pragma unroll 1
+    for (int k = 0; k < D / 32; ++k) {
+        float o[32];
+        tc_ld32(tO + 32 * k, o);
+        tc_wait_ld32(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = fresh ? 0.f : o[i];
+#pragma unroll 1
+        for (int t = 0; t < 128; ++t) {
+            const uint32_t two = tc_ld1(tP + (t >> 1)), w = t & 1 ? two >> 16 : two & 0xffffu;
+            const float p = BF ? __uint_as_float(w << 16) : h2f((uint16_t)w);
+            if (p != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int d = 32 * k + i;
+                    const uint16_t x = *reinterpret_cast<const uint16_t*>(v + (d >> 6) * (128 * 128) + t * 128 +
+                                                                         ((((d & 63) >> 3) ^ (t & 7)) << 4) + (d & 7) * 2);
+                    o[i] += p * (BF ? __uint_as_float((uint32_t)x << 16) : h2f(x));
+                }
+            }
+            __syncwarp();
+        }
+        tc_st32(tO + 32 * k, o);
+    }
+    tc_wait_st();
 }
 
 }  // namespace hc

@@ -206,7 +206,7 @@ static int attn_args(const char* what, hc_engine* e, const hc_kv_cache* c, const
 constexpr int kFewRows = 16;
 
 // Bytes of keys and values that sharing prefixes has to save.
-constexpr long long kShareBytes = 192 << 20;
+constexpr long long kShareBytes = 384 << 20;
 
 // Sequences with up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
 // ones to the other (tiles of 256): both are launched where the batch may have both.  At 16 rows, 16
@@ -275,30 +275,34 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         const cudaError_t ce = attn_run(e, c, dtype, a, b->max_new);
         return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
     }
-    // Prefixes of up to kFewRows rows per kv head go to the kernel for few rows, the others to attn_prefix.cu (both
-    // launched where the batch may have both); so do all of f32 rows, whose terms its operands do not hold.
+    // f32 rows go to the kernel for few rows, whose terms attn_prefix.cu's operands do not hold, in two calls.
     const int sms = e->num_sms;
     const long long rows = (long long)b->n_tok * (long long)n_heads, kv = c->n_heads;
-    const long long most = (long long)(g->max_new && g->max_new < b->n_tok ? g->max_new : b->n_tok) * a.group;
-    const bool tc = attn_many_supported(c->type, dtype), few = !tc;
+    // What a sequence has behind its prefix goes there too where it has few rows (single tokens): 64 of them with 30 to
+    // 1500 8-bit tokens each take 43 us there, and 75 as tiles of attn_prefix.cu; in chunks of up to 60, 46 of them 108
+    // and 75.
+    const bool few = !attn_many_supported(c->type, dtype);
+    const bool behind = few || (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group <= kFewRows;
     long long shared = b->n_seq / 2;  // groups that share anything: two sequences with new tokens each
     if (shared > b->n_tok / 2) shared = b->n_tok / 2;
     if (shared > g->n_groups) shared = g->n_groups;
-    const long long tiles = rows / 256 + shared * kv;
-    // a row's result in a piece or two (narrow tiles), and where a block's share ends in a tile, its rows once more
-    const long long narrow = shared * kv * 128 < rows ? shared * kv * 128 : rows;
-    const long long pieces = tc ? rows + narrow + (long long)sms * 256 : 0;
+    const long long seqs = b->n_seq < b->n_tok ? b->n_seq : b->n_tok;  // with new tokens
+    const long long tiles = 2 * (rows / 256) + (shared + seqs) * kv;
+    // a row's result in a piece (of narrow tiles two) of its prefix and one behind it, and where a block's share ends
+    // in a tile, its rows once more
+    auto narrow = [&](long long n) { return n * kv * 128 < rows ? n * kv * 128 : rows; };
+    const long long pieces = few ? 0 : 2 * rows + narrow(shared) + narrow(seqs) + (long long)sms * 256;
     size_t size = 0;
     auto room = [&](size_t n) {
         const size_t at = size;
         size += (n * 4 + 255) / 256 * 256;
         return at;
     };
+    const size_t r_few = few ? (size_t)rows : 0, r_behind = behind ? (size_t)rows : 0;
     const size_t at_first = room(HC_KV_SEQS), at_q = room(HC_KV_SEQS + 1), at_len = room(HC_KV_SEQS), at_row = room(HC_KV_SEQS),
                  at_line = room(kLineInts), at_block = room((size_t)sms), at_tiles = room((size_t)tiles * sizeof(PrefixTile) / 4),
-                 at_lse = room((size_t)rows), at_out = room((size_t)rows * c->head_dim), at_flse = room(few ? (size_t)rows : 0),
-                 at_few = room(few ? (size_t)rows * c->head_dim : 0), at_ml = room((size_t)pieces * 2),
-                 at_part = room((size_t)pieces * c->head_dim);
+                 at_lse = room(r_behind), at_out = room(r_behind * c->head_dim), at_flse = room(r_few), at_few = room(r_few * c->head_dim),
+                 at_ml = room((size_t)pieces * 2), at_part = room((size_t)pieces * c->head_dim);
     void* base = nullptr;
     rc = attn_workspace(e, &a, size, &base);
     if (rc) return rc;
@@ -314,7 +318,8 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     d.least = least;
     d.heads = a.heads;
     d.kv_heads = c->n_heads;
-    d.few_rows = few ? INT32_MAX : 0;
+    d.few = few;
+    d.few_behind = behind;
     d.blocks = sms;
     d.max_tiles = (int)(tiles < INT32_MAX ? tiles : INT32_MAX);
     d.max_pieces = (int)(pieces < INT32_MAX ? pieces : INT32_MAX);
@@ -322,30 +327,43 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     d.line = (int*)place(at_line);
     d.first_tile = (int*)place(at_block);
     cudaError_t ce = launch_attn_groups(a.b, d, b->max_pages * c->page_size, e->stream);
-    const PrefixArgs p{d.tiles, d.line, d.first_tile, (float*)place(at_part), (float*)place(at_ml), (float*)place(at_few),
-                       (float*)place(at_flse)};
-    if (ce == cudaSuccess && tc) ce = launch_attn_prefix(c->type, dtype, c->head_dim, a, p, sms, e->stream);
-    if (ce == cudaSuccess && few) {
-        AttnArgs x = a;
-        x.b.q_start = d.q_start;
-        x.b.kv_len = d.len;
-        x.b.n_seq = d.n;
-        x.table_row = d.row;
-        x.causal = 0;
-        x.to_base = 1;
-        x.base = (float*)place(at_few);
-        x.base_lse = (float*)place(at_flse);
-        x.row_min = 1;
-        x.row_max = d.few_rows;
-        x.max_rows = (int)(most < INT32_MAX ? most : INT32_MAX);
-        ce = launch_attn_few(c->type, dtype, c->head_dim, x, sms, e->stream);
+    AttnArgs plain = a;  // the paged attention, where nothing is shared after all
+    plain.unless = d.line + kLineTiles;
+    plain.early = 1;
+    PrefixArgs p{d.tiles, d.line, d.first_tile, (float*)place(at_part), (float*)place(at_ml), nullptr, nullptr};
+    AttnArgs x = a;  // of the kernel for few rows
+    x.only = d.line + kLineTiles;
+    x.row_min = 1;
+    x.row_max = INT32_MAX;
+    if (few) {
+        AttnArgs y = x;
+        y.b.q_start = d.q_start;
+        y.b.kv_len = d.len;
+        y.b.n_seq = d.n;
+        y.table_row = d.row;
+        y.causal = 0;
+        y.to_base = 1;
+        y.base = (float*)place(at_few);
+        y.base_lse = (float*)place(at_flse);
+        const long long most = (long long)(g->max_new && g->max_new < b->n_tok ? g->max_new : b->n_tok) * a.group;
+        y.max_rows = (int)(most < INT32_MAX ? most : INT32_MAX);
+        p.few = y.base;
+        p.few_lse = y.base_lse;
+        if (ce == cudaSuccess) ce = launch_attn_few(c->type, dtype, c->head_dim, y, sms, e->stream);
+    } else if (ce == cudaSuccess) {
+        ce = launch_attn_prefix(c->type, dtype, c->head_dim, a, p, sms, e->stream);
     }
-    a.first = d.first;
-    a.early = 1;
-    a.base = (float*)place(at_out);
-    a.base_lse = (float*)place(at_lse);
-    if (ce == cudaSuccess) ce = attn_run(e, c, dtype, a, b->max_new);
+    if (behind) {
+        x.first = d.first;
+        x.base = a.base = (float*)place(at_out);
+        x.base_lse = a.base_lse = (float*)place(at_lse);
+        x.early = 1;
+        const long long most = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
+        x.max_rows = (int)(most < INT32_MAX ? most : INT32_MAX);
+        if (ce == cudaSuccess) ce = launch_attn_few(c->type, dtype, c->head_dim, x, sms, e->stream);
+    }
     if (ce == cudaSuccess) ce = launch_attn_join(dtype, c->head_dim, a, p, sms, e->stream);
+    if (ce == cudaSuccess) ce = attn_run(e, c, dtype, plain, b->max_new);
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
 }
 

@@ -144,46 +144,56 @@ struct AttnArgs {
     float *base, *base_lse;  // [n_tok * heads][head_dim] and log 2 of the weights' sums
     int to_base;             // the sequences are prefixes: all their results, but nothing of empty ones
     int early;               // a launch_early
+    const int *unless, *only;  // nothing is done where the one is not 0, or the other is
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
     int* count;            // 32 counters per block, zero between calls
 };
 
-// hc_kv_shared as the kernels get it, and the groups as sequences of their own.
+// hc_kv_shared as the kernels get it, and what is made of it.
 struct KvSharedDev {
     const int *seq_start, *length;
     int n;
-    int *first;                // [n_seq]
-    int *q_start, *len, *row;  // [n + 1], [n], [n]: the prefixes that go to the kernel for few rows
     long long least;           // tokens that sharing has to save, or nothing is shared
     int heads, kv_heads;       // query heads, and those that the keys have
-    int few_rows;              // a prefix with more rows per kv head goes to attn_prefix.cu
-    int blocks, max_tiles;     // of attn_prefix.cu; tiles that there is room for
-    int max_pieces;            // rows of pieces that there is room for
+    int few, few_behind;       // the prefixes, or what is behind them, go to the kernel for few rows, else to attn_prefix.cu
+    int *first;                // few_behind: [n_seq] shared tokens, where what is behind them starts
+    int *q_start, *len, *row;  // few: [n + 1], [n], [n]: the prefixes as sequences
+    int blocks;                // of attn_prefix.cu
+    int max_tiles, max_pieces;  // tiles, and rows of pieces, that there is room for
     struct PrefixTile* tiles;
-    int *line, *first_tile;    // kLine...; [blocks] the tile that a block starts in
+    int *line, *first_tile;  // kLine...; [blocks] the tile that a block starts in
 };
-// Rows of a kv head of a prefix, up to 256 of them.
-struct PrefixTile {
-    int place, units;    // the first of its places on the line (attn_prefix.cu); units of 128 positions, 0: not on it
+// Rows of a kv head, up to 256 of them, and the positions that they see together: those of a prefix all of them, those
+// behind one up to each row's own.
+struct alignas(16) PrefixTile {
+    int place, units;    // the first of its places on the line (attn_prefix.cu); units of 128 positions
     int cost;            // places of a unit: 2, or 1 for up to 128 rows
-    int q0, hk, r0, nr;  // the group's first token; the kv head; the tile's first row and number of rows
-    int len, row;        // the prefix's length, and its row of the page table
-    int piece, pieces;   // its first row in the pieces, and how many there are; 0: it is in the few rows' `base`
+    int q0;              // the first token of the group, or of the sequence
+    int hk, r0, nr;      // the kv head; the tile's first row and number of rows.  hk = -1: rows of all query heads, only for
+                         // the joining (what is behind the prefix has a result from elsewhere); nr may be any number then
+    int from, len;       // positions [from, len)
+    int row;             // of the page table
+    int piece, pieces;   // its first row in the pieces, and how many there are
     int c0;              // the block that has its first unit
-    int pad[4];
+    int pos0;            // position of token q0, or kAllSeen
+    int pre, pre_row;    // behind a prefix: its first tile of this kv head (or -1), and the row there of row 0; hk = -1: its
+                         // first tile, `cost` of them to a kv head
 };
-enum { kLineTiles, kLinePlaces, kLineBlocks, kLineInts = 16 };
-// What attn_prefix.cu and the joining get besides: pieces (O, then m and l of a row), and the other parts' results.
+constexpr int kAllSeen = 1 << 30;
+// Tiles; the first behind a prefix; what there is of those rows by eights, at most; places; blocks.
+enum { kLineTiles, kLineOwn, kLineRuns, kLinePlaces, kLineBlocks, kLineInts = 16 };
+// What attn_prefix.cu and the joining get besides: pieces (O, then m and l of a row), and where the kernel for few rows
+// made them the prefixes' results (what is behind them: AttnArgs::base).
 struct PrefixArgs {
     const PrefixTile* tiles;
     const int *line, *first_tile;
     float *part, *part_ml;
-    const float *few, *few_lse;  // of prefixes with few rows
+    const float *few, *few_lse;
 };
 cudaError_t launch_attn_groups(const KvBatchDev& b, const KvSharedDev& g, int cap, cudaStream_t s);
 cudaError_t launch_attn_prefix(int cache_type, int dtype, int head_dim, const AttnArgs& a, const PrefixArgs& p, int blocks,
                                cudaStream_t s);
-// out and lse of the rows with a prefix, from `base` (what they have behind it) and the prefix's pieces.
+// out and lse of all tiles' rows, from their own and their prefixes' pieces, or from `base` and PrefixArgs::few.
 cudaError_t launch_attn_join(int dtype, int head_dim, const AttnArgs& a, const PrefixArgs& p, int sms, cudaStream_t s);
 
 // Partial results of the kernel for few rows: bytes for each block.

@@ -247,6 +247,49 @@ def test_not_finite(engine, dtype, cache, at):
     assert bad.tolist() == ([True] * 3 if at == "prefix" else [False, True, False]) + [False, False]
 
 
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "i8"), ("bf16", "f16"), ("f32", "f16")])
+@pytest.mark.parametrize("new,own", [(40, 40), (70, 200), (3, 300)])
+@pytest.mark.parametrize("heads", [1, 4, 16])
+def test_not_finite_where_some_rows_do_not_see_it(engine, dtype, cache, new, own, heads):
+    """Infinities among a chunk's own tokens reach its later tokens, and leave the earlier ones what they were."""
+    s = Groups([(90, [(new, own), (2, 30), (1, 1)])], 1, 64, 16, cache)
+    q = s.q(heads, dtype)
+    clean, lse = check(engine, s, heads, dtype, q=q)
+    at = s.kv[0] - 2  # the chunk's last token but one
+    page, row = s.table[0, at // 16].long(), at % 16
+    if cache == "i8":
+        s.scale[1][page, 0, row] = math.nan
+    else:
+        s.pool[1][page, 0, row, 5] = math.inf
+        s.pool[1][page, 0, row, 6] = math.nan
+    out = torch.zeros_like(q)
+    engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out)
+    engine.sync()
+    bad = ~out.isfinite().all(-1).all(-1)
+    assert bad.nonzero().flatten().tolist() == [new - 2, new - 1]
+    c = 2.0 ** -13 if dtype == "f32" else 2.0 ** -10 if dtype == cache == "f16" else 2.0 ** -8
+    most = s.values(1, 1).abs().max().item()
+    keep = ~bad
+    # both are within c (A + |out|) of the definition, and |out| <= A <= the largest value
+    most = max(most, clean.abs().max().item(), 6.0)
+    assert (out[keep].double() - clean[keep].double()).abs().max().item() <= 4 * c * most
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "i8"), ("f32", "bf16")])
+def test_tokens_before_the_first_position_see_nothing(engine, dtype, cache):
+    """A sequence with more new tokens than tokens shares nothing with its group, and its first ones get zeros."""
+    s = Groups([(40, [(1, 5), (1, 9)]), (0, [(30, 12), (5, 2)])], 2, 64, 16, cache)
+    out, lse = check(engine, s, 8, dtype)
+    assert (lse[2:20] == -math.inf).all() and (out[2:20] == 0).all() and (lse[20:32] > -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "i8"), ("bf16", "f16")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunks_of_many_tiles(engine, dtype, cache, dim):
+    """Chunks whose rows are several tiles with ends of their own, beside single tokens, behind a long prefix."""
+    check(engine, Groups([(2050, [(130, 130), (1, 700), (257, 900), (16, 16), (1, 1)]), (0, [(300, 300)])], 1, dim, 24, cache), 4, dtype)
+
+
 def test_the_same_bits_every_time(engine):
     s = Groups([(3000, [(1, 50)] * 40), (500, [(3, 30)] * 7)], 2, 128, 64, "bf16")
     q = s.q(8, "bf16")
