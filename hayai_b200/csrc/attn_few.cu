@@ -218,9 +218,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 
     __shared__ float* place_s[W][2];  // where a warp's last (0) and first (1) piece of a shared tile is
 
-    if (a.early) after_previous();
-    if (a.early) let_next_start();
-    if ((a.unless && __ldcg(a.unless)) || (a.only && !__ldcg(a.only))) return;
+    if (a.shared && !attn_wanted(a)) return;
     // few sequences (a single one above all, whose call is short): every warp schedules for itself
     const bool lanes = a.b.n_seq <= 32 && a.max_rows <= 8 * ROWS;
     int* const pre = reinterpret_cast<int*>(smem);

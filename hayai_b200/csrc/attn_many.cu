@@ -120,9 +120,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
     AttnShared* const shared_s = reinterpret_cast<AttnShared*>(misc + 64);  // the block's first and last tile, where shared
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), ln = lane_id(), c = blockIdx.x;
 
-    if (a.early) after_previous();
-    if (a.early) let_next_start();
-    if ((a.unless && __ldcg(a.unless)) || (a.only && !__ldcg(a.only))) return;
+    if (a.shared && !attn_wanted(a)) return;
     // the schedule's prefix sums lie in the last key and value tile until warp 13 has its place
     int* const pre_s = reinterpret_cast<int*>(smem + F::oKV + (NB - 1) * TILE);
     const int U = attn_schedule<kManyThreads>(a, ROWS, UNIT, pre_s, misc + 16);

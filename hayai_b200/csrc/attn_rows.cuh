@@ -42,6 +42,15 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
     return t;
 }
 
+// The start of a kernel that is part of attention over a shared prefix: is it wanted?
+static __device__ __noinline__ bool attn_wanted(const AttnArgs& a) {
+    if (a.early) {
+        after_previous();
+        let_next_start();
+    }
+    return !((a.unless && __ldcg(a.unless)) || (a.only && !__ldcg(a.only)));
+}
+
 // A sequence, and where what it sees starts.
 __device__ __forceinline__ KvSeq attn_seq(const AttnArgs& a, int s) {
     KvSeq q = kv_seq(a.b, a.b.max_pages * a.c.page_size, s);
@@ -263,13 +272,10 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, in
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = none ? 0.f : y[i] * k;
-    if (part) {
-        *reinterpret_cast<float4*>(a.base + ((long long)(q0 + t) * a.heads + h) * D + d) = make_float4(z[0], z[1], z[2], z[3]);
-        return;
-    }
-    T* out = (T*)a.out + (long long)(q0 + t) * a.ldo + h * D + d;
-    if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4*>(out) = make_float4(z[0], z[1], z[2], z[3]);
+    const long long at = part ? (long long)(q0 + t) * (a.heads * D) : (long long)(q0 + t) * a.ldo;
+    T* const out = (T*)a.out + at + h * D + d;
+    if (sizeof(T) == 4 || part)
+        *reinterpret_cast<float4*>((part ? a.base : (float*)a.out) + at + h * D + d) = make_float4(z[0], z[1], z[2], z[3]);
     else if constexpr (__is_same(T, __half))
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2(z[0], z[1]), pack_h2(z[2], z[3]));
     else
@@ -278,11 +284,8 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, in
 __device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l, bool part) {
     const int t = a.by_group(row);
     const long long at = (long long)(q0 + t) * a.heads + hk * a.group + row - t * a.group;
-    const float y = l == 0.f ? -INFINITY : m + log2f(l);
-    if (part)
-        a.base_lse[at] = y;
-    else if (a.lse)
-        a.lse[at] = y * 0.693147181f;
+    float* const lse = part ? a.base_lse : a.lse;
+    if (lse) lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * (part ? 1.f : 0.693147181f);
 }
 
 // One row of n partial results joined by a warp: ml(i) gives piece i's (m, l), (-inf, 0) if it has

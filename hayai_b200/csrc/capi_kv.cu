@@ -329,9 +329,10 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     cudaError_t ce = launch_attn_groups(a.b, d, b->max_pages * c->page_size, e->stream);
     AttnArgs plain = a;  // the paged attention, where nothing is shared after all
     plain.unless = d.line + kLineTiles;
-    plain.early = 1;
+    plain.shared = plain.early = 1;
     PrefixArgs p{d.tiles, d.line, d.first_tile, (float*)place(at_part), (float*)place(at_ml), nullptr, nullptr};
     AttnArgs x = a;  // of the kernel for few rows
+    x.shared = 1;
     x.only = d.line + kLineTiles;
     x.row_min = 1;
     x.row_max = INT32_MAX;

@@ -143,6 +143,7 @@ struct AttnArgs {
     const int* table_row;    // [n_seq] rows of the page table, or null: a sequence's own
     float *base, *base_lse;  // [n_tok * heads][head_dim] and log 2 of the weights' sums
     int to_base;             // the sequences are prefixes: all their results, but nothing of empty ones
+    int shared;              // one of the kernels of such a call
     int early;               // a launch_early
     const int *unless, *only;  // nothing is done where the one is not 0, or the other is
     float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats

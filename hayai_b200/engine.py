@@ -197,6 +197,7 @@ class CudaEngine:
                                                             lib().hc_attn_paged_dev)
         self._attn_shared, self._rope, self._kv_append_rope = (lib().hc_attn_shared_dev, lib().hc_rope_dev,
                                                                lib().hc_kv_append_rope_dev)
+        self._kv_fork, self._kv_resize = lib().hc_kv_fork_dev, lib().hc_kv_resize_dev
 
     def close(self) -> None:
         if self.handle:
@@ -490,9 +491,7 @@ class CudaEngine:
     def rope_dev(self, rope, positions, x, out=None) -> None:
         """Turn rows x [n_tok][n_heads][head_dim] by int32 positions [n_tok] (Rope), into out or in place."""
         out = x if out is None else out
-        n = positions.shape[0] if positions.dim() == 1 else -1
-        if str(positions.dtype) != "torch.int32" or n < 0 or (n > 1 and positions.stride(0) != 1):
-            raise ValueError("positions must be a contiguous int32 tensor [n_tok]")
+        n = rope.count(positions)
         t, heads, ldx = rope.rows(x, "x", n)
         _, _, ldo = rope.rows(out, "out", n, x)
         if not x.get_device() == out.get_device() == positions.get_device() == self.device:
@@ -526,13 +525,17 @@ class CudaEngine:
         """Slot children[i] becomes a copy of slot parents[i] (KvPages; int32 tensors): whole pages are shared, a
         partly filled last page is copied to one of the child's own, in every layer.  Children hold nothing before."""
         self._pages_here(pages)
-        _check(lib().hc_kv_fork_dev(self.handle, pages.ref, *pages.items(parents, children, "parents and children")))
+        rc = self._kv_fork(self.handle, pages.ref, *pages.items(parents, children, "parents and children"))
+        if rc:
+            _check(rc)
 
     def kv_resize_dev(self, pages, slots, lens) -> None:
         """Slot slots[i] gets the length lens[i] (int32 tensors): pages are taken, the lowest free ones first, or
         given back; a length of 0 lets the slot go."""
         self._pages_here(pages)
-        _check(lib().hc_kv_resize_dev(self.handle, pages.ref, *pages.items(slots, lens, "slots and lens")))
+        rc = self._kv_resize(self.handle, pages.ref, *pages.items(slots, lens, "slots and lens"))
+        if rc:
+            _check(rc)
 
     def kv_compact_dev(self, pages, moved=None) -> None:
         """The pages in use move to the lowest numbers, in every layer, and the tables follow.  moved: None, or

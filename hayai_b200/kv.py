@@ -183,7 +183,7 @@ class KvPages:
                   "page_table, kv_len and refs must be int32 CUDA tensors of one device, of 2, 1 and 1 axes")
             _need(t.shape[-1] <= 1 or t.stride(-1) == 1, "page_table rows, kv_len and refs must be contiguous")
         n_slots, max_pages = page_table.shape
-        self.index, self.n_pages = page_table.get_device(), caches[0].struct.n_pages
+        self.index, self.n_pages, self.int32 = page_table.get_device(), caches[0].struct.n_pages, torch.int32
         _need(all(c.index == self.index for c in caches), "the caches must be on page_table's device")
         _need(kv_len.shape[0] == n_slots and refs.shape[0] == self.n_pages, "kv_len must hold n_slots and refs n_pages")
         stride = page_table.stride(0) if n_slots > 1 else max_pages
@@ -200,11 +200,11 @@ class KvPages:
 
     def items(self, a, b, what: str):
         """(n, pointers) of a call's two int32 arrays."""
+        n = a.numel()
         for t in (a, b):
-            if t.dim() != 1 or t.shape != a.shape or str(t.dtype) != "torch.int32" or t.get_device() != self.index or \
-                    (t.shape[0] > 1 and t.stride(0) != 1):
+            if t.dtype is not self.int32 or t.dim() != 1 or t.numel() != n or t.get_device() != self.index or not t.is_contiguous():
                 raise ValueError(f"{what} must be contiguous int32 tensors of one length on the pages' device")
-        return a.shape[0], a.data_ptr(), b.data_ptr()
+        return n, a.data_ptr(), b.data_ptr()
 
 
 class Rope:
@@ -236,9 +236,16 @@ class Rope:
         self.ref = ctypes.addressof(self.struct)
         self.head_dim, self.rot_dim = head_dim, rot_dim
 
+    def count(self, positions) -> int:
+        """How many positions there are."""
+        if positions.dtype is not _torch().int32 or positions.dim() != 1 or not positions.is_contiguous():
+            raise ValueError("positions must be a contiguous int32 tensor [n_tok]")
+        return positions.numel()
+
     def rows(self, x, what: str, n: int, like=None):
         """(type id, heads, leading dimension) of packed rows x [n_tok][heads][head_dim]."""
-        _torch()
+        if not _ROW_TYPES:
+            _torch()
         t = _ROW_TYPES.get(x.dtype)
         if t is None or not x.is_cuda or x.dim() != 3 or x.shape[0] != n or x.shape[2] != self.head_dim or \
                 (like is not None and (x.shape != like.shape or x.dtype != like.dtype)):
