@@ -157,7 +157,10 @@ static int attn_workspace(hc_engine* e, AttnArgs* a, size_t base, void** base_at
             w->count.release();
             delete w;
         }
-        if (rc) return rc;
+        if (rc) {
+            cudaGetLastError();  // reported here: the next launch's check is not to find it
+            return rc;
+        }
         if (fresh) {
             w->stream = e->stream;
             w->captured = captured;

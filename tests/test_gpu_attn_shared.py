@@ -290,6 +290,17 @@ def test_chunks_of_many_tiles(engine, dtype, cache, dim):
     check(engine, Groups([(2050, [(130, 130), (1, 700), (257, 900), (16, 16), (1, 1)]), (0, [(300, 300)])], 1, dim, 24, cache), 4, dtype)
 
 
+@pytest.mark.parametrize("dtype,cache", [("bf16", "i8"), ("f32", "f16")])
+def test_as_many_sequences_as_a_batch_takes(engine, dtype, cache):
+    """2048 sequences in 1024 groups of two, and in one group, tables wider than they need be."""
+    s = Groups([(20 + i % 7, ONE * 2) for i in range(1024)], 1, 64, 16, cache)
+    wide = torch.full((2048, 5), -1, dtype=torch.int32, device=DEV)
+    wide[:, 1:1 + s.table.shape[1]] = s.table
+    s.batch = hb.KvBatch(wide[:, 1:3], s.q_start, s.kv_len, s.rows, 1)
+    check(engine, s, 2, dtype)
+    check(engine, Groups([(333, [(1, 1 + i % 3) for i in range(2048)])], 1, 64, 16, cache), 2, dtype)
+
+
 def test_the_same_bits_every_time(engine):
     s = Groups([(3000, [(1, 50)] * 40), (500, [(3, 30)] * 7)], 2, 128, 64, "bf16")
     q = s.q(8, "bf16")

@@ -218,6 +218,30 @@ def test_random_steps(engine, seed):
             p.do(engine, call)
 
 
+def test_a_slice_of_a_wider_table(engine):
+    """Page tables and pools that are views: what lies around them stays."""
+    p = Pool(n_pages=30, slots=5, page=16, max_pages=6)
+    wide = torch.full((5, 9), 77, dtype=torch.int32, device=DEV)
+    wide[:, 2:8] = p.table
+    p.table = wide[:, 2:8]
+    p.pages = hb.KvPages(p.pages._keep[0], p.table, p.kv_len, p.refs)
+    p.do(engine, "resize", [0, 4], [90, 33], ok=True)
+    p.do(engine, "fork", [0, 4], [1, 2], ok=True)
+    p.do(engine, "resize", [0], [0], ok=True)
+    p.do(engine, "compact")
+    assert (wide[:, :2] == 77).all() and (wide[:, 8] == 77).all()
+
+
+def test_lengths_from_the_lengths_themselves(engine):
+    """kv_len as the new lengths: nothing changes, but partly filled pages that are shared become the slots' own."""
+    p = Pool(page=16)
+    p.do(engine, "resize", [0, 1], [40, 7], ok=True)
+    engine.kv_resize_dev(p.pages, ints(list(range(p.slots))), p.kv_len)
+    engine.sync()
+    assert p.resize(list(range(p.slots)), list(p.m_len))
+    p.same()
+
+
 def test_two_thousand_items(engine):
     """As many as a call takes: 2048 children of one parent, one new page each, and all of them let go."""
     p = Pool(n_pages=2200, slots=2049, page=16, layers=1, heads=1, max_pages=9)
