@@ -1,5 +1,6 @@
-// attn_prefix.cu -- attention of a group's rows over the prefix that its sequences share, on the 5th-generation
-// tensor cores.  Every row sees every position, so that nothing is masked but the last unit's end.
+// attn_prefix.cu -- attention for a call with shared prefixes, on the 5th-generation tensor cores: of a group's rows
+// over the prefix that its sequences share, which all of them see whole, and of a chunk's rows over what it has behind
+// its prefix, up to each row's own position.
 //
 //     O_i = sum_j 2^(s_ij - m_i) v_j,   l_i = sum_j 2^(s_ij - m_i),   s_ij = scale log2 e q_i . k_j
 // over the positions of a piece, with m_i near their maximum (it moves when a score passes it by 8).
@@ -8,16 +9,28 @@
 // are two halves of 128 that take every unit; a narrow one, of up to 128 rows, has its units taken by the two halves in
 // turn, each with sums of its own.  Either way a block has two independent chains S = Q K^T -> weights -> O += P V, and
 // the tensor cores work on one's products while the other's weights are made: a list of jobs, the j-th on half j & 1.
-// One block of 16 warps per SM takes an equal share of the line of units, and leaves a piece for each tile and half.
+// One block of 16 warps per SM takes an equal share of the line of units, and leaves a piece for each tile and half;
+// attn_shared.cu joins them over the whole GPU.  (A tile joined by the block that comes last, as attn_many.cu does, took
+// 100 us of a call with few tiles: one SM reads all its pieces.)
 //
 //   warps 0-3, 4-7   a thread per row of half 0 and 1: its query in (a row a thread: 256 rows are on their way at
-//                    once), then S from TMEM to registers, weights back over it in 16 bits, in two parts, so that
-//                    the first part's product runs while the second is made
-//   warps 8-11       keys and values in: 16-byte asynchronous copies (8-bit pages: by way of a staging ring, from which
-//                    each thread converts what it copied itself) into 128-byte-swizzled operand tiles
+//                    once; one warp for all took 32 us), then S from TMEM to registers, weights back over it in 16
+//                    bits, in two parts, so that the first part's product runs while the second is made
+//   warps 8-11       16-bit pages: keys and values in by 16-byte asynchronous copies into 128-byte-swizzled operand
+//                    tiles; 8-bit pages: staged codes into operands
 //   warp 12          the products, one half's after the other's (a warp for each half lets the halves fall into step,
-//                    where they wait for the same units in turn: 5000 cycles a unit, 3400 so); warps 13-15 are there for the
-//                    register split, which goes by four warps
+//                    where they wait for the same units in turn: 5000 cycles a unit against 3500 to 4000)
+//   warps 13, 14     8-bit pages: codes into the staging ring by bulk copies, a page's rows of a head in one; scales
+//   warp 15          is there for the register split, which goes by four warps
+//
+// Measured: a prefix of 60001 bf16 tokens under 100 single tokens (32 heads on 8 of 128) 132 us, 745 TFLOP/s of the
+// visible pairs (45 % of cuBLAS's rate; rows fill 400 of 512 places of their tiles); 65536 tokens under 64 of them 1.3
+// times the keys' and values' time at the copy rate from 16-bit pages, and 3 times from 8-bit ones.  A
+// unit of a wide tile takes 3500 to 4000 cycles, where its products take 2048 and its exponentials as many: each
+// half's chain (scores in, weights 1800, products 800, and the waits between) is the time, not either pipe.  Two threads per row,
+// exponentials by polynomials, and scores read twice from a shorter loop took the same time or more.  A start takes
+// 12 us and more (45 us in all for 64 sequences behind 4100 8-bit tokens, whose units are 8 us): code that is run for the
+// first time, fetched line by line.
 //
 // Formats as in attn_many.cu: products of f16 (f16 and 8-bit caches) or bf16, weights rounded to that type and
 // summed in f32; f16 weights are taken 2^7 times as large.  8-bit codes are exact in f16; a K scale multiplies its column of

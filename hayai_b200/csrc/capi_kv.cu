@@ -208,7 +208,10 @@ static int attn_args(const char* what, hc_engine* e, const hc_kv_cache* c, const
 
 constexpr int kFewRows = 16;
 
-// Bytes of keys and values that sharing prefixes has to save.
+// Bytes of keys and values that sharing prefixes has to save.  16 and 64 sequences of 32 heads on 8, as paged attention
+// and shared: behind 4096 bf16 tokens (252 MB saved) 37 and 47 us, 1024 (264 MB) 43 and 52; behind 16384 (1.0 GB) 103 and
+// 62, 4096 (1.1 GB) 109 and 57; behind 4096 8-bit tokens (134 MB) 34 and 42, 1024 (140 MB) 41 and 49, behind 16384 (535 MB)
+// 94 and 65, 4096 (561 MB) 100 and 62.
 constexpr long long kShareBytes = 384 << 20;
 
 // Sequences with up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
@@ -282,8 +285,8 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     const int sms = e->num_sms;
     const long long rows = (long long)b->n_tok * (long long)n_heads, kv = c->n_heads;
     // What a sequence has behind its prefix goes there too where it has few rows (single tokens): 64 of them with 30 to
-    // 1500 8-bit tokens each take 43 us there, and 75 as tiles of attn_prefix.cu; in chunks of up to 60, 46 of them 108
-    // and 75.
+    // 1500 8-bit tokens each take 43 us there, and 75 as tiles of attn_prefix.cu; 53 chunks of up to 60 tokens with up
+    // to 300 before them 108 in the paged attention's kernels, and 75 as tiles.
     const bool few = !attn_many_supported(c->type, dtype);
     const bool behind = few || (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group <= kFewRows;
     long long shared = b->n_seq / 2;  // groups that share anything: two sequences with new tokens each

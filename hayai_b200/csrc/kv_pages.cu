@@ -12,6 +12,10 @@
 // them on the GPU.
 // Bound by: the copies' bytes (read once, written once) where there are many, or else two launches and
 // the first kernel's walk over the holders.
+//
+// Measured in a graph: half of 96 conversations gone, 728 MB moved down in 8 layers 245 us (5.9 TB/s, 91 % of the copy
+// rate); 144 forks of 9 prompts, 87 MB of partly filled pages in 12 layers with the children let go before and grown
+// after 43 us (the copies 22); four forks in three layers, likewise three calls, 17 us.
 #include "block_scan.cuh"
 #include "kv_launch.h"
 

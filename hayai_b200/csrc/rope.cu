@@ -12,6 +12,11 @@
 //
 // Bound by memory: a row is read once and written once.  A lane holds two chunks of 8 values, in the half layout
 // the two partners, so that nothing is exchanged between lanes but an 8-bit row's largest value.
+//
+// Measured: 9000 tokens of 32 bf16 heads of 128 26 us (5.6 TB/s, 86 % of the copy rate); 15947 tokens of prompts, 32
+// query heads turned and 8 kv heads turned and stored in 8 bits, 82 us (4.4 TB/s), one token 3.6 us in a graph.
+// In blocks of one round, each of which finds its tokens' places for itself, the prompts took 139 us; in 8 rounds 82, in 32
+// 92.  Queries, keys and values in loops of their own (a row's quantising for queries as well: 151 us).
 #include <type_traits>
 
 #include "kv_rows.cuh"

@@ -325,7 +325,7 @@ int hc_attn_paged_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batc
  * first sequence's pages.  Of a length past the tokens that every sequence of the group had before its new ones,
  * that much is shared.  max_new is the host's bound on any group's new tokens (0: n_tok); a group with more is
  * still computed, at lower speed.  least: how many tokens of reading the call's sharing has to save, over all
- * groups, to be made (0: as many as its kernels' starts are worth); the results are the same either way. */
+ * groups, to be made (0: as many as its kernels' starts are worth); the results differ by roundings only. */
 typedef struct hc_kv_shared {
     int n_groups, max_new;
     int64_t least;
@@ -333,9 +333,9 @@ typedef struct hc_kv_shared {
 } hc_kv_shared;
 
 /* hc_attn_paged_dev (causal, without a window) for groups of sequences with shared tokens, which are read once
- * for the group and seen by all its rows together.  Its notes hold here too.  Between the call's kernels the
- * prefixes' results lie in the engine, in a workspace of about n_tok * n_heads * (head_dim + 1) floats that grows
- * with the calls. */
+ * for the group and seen by all its rows together.  Its notes hold here too.  Between the call's kernels partial results
+ * lie in the engine, in a workspace of up to 4 * n_tok * n_heads * (head_dim + 2) floats and 20 MB, which grows with
+ * the calls in powers of two. */
 int hc_attn_shared_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, const hc_kv_shared* shared,
                        int dtype, size_t n_heads, const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale);
 
