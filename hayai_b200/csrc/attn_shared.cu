@@ -59,28 +59,30 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
 #pragma unroll 1
     for (int s = tid; s < b.n_seq; s += 1024) of_s[s] = -1;
     __syncthreads();
-    int *const s0_s = tile_s, *const s1_s = place_s;  // the groups' sequences, until the tiles are counted
+    int *const s0_s = tile_s, *const s1_s = place_s, *const lead_s = w_s;  // the groups' sequences, until the tiles are counted
 #pragma unroll 1
     for (int i = tid >> 5; i < g.n; i += 32) {
         const int a0 = __ldg(g.seq_start + i), a1 = __ldg(g.seq_start + i + 1), given = __ldg(g.length + i);
         const int s0 = min(max(a0, 0), b.n_seq), s1 = min(max(a1, s0), b.n_seq);
-        int most = min(max(given, 0), cap), seqs = 0;
+        int most = min(max(given, 0), cap), seqs = 0, lead = b.n_seq - 1;
         if (s0 != a0 || s1 != a1 || most != given)
             if (ln == 0) atomicOr(b.err, kErrKvRange);
 #pragma unroll 1
         for (int s = s0 + ln; s < s1; s += 32) {
             const KvSeq q = kv_seq(b, cap, s);
             if (q.q1 == q.q0) continue;
-            ++seqs;
+            if (seqs++ == 0) lead = s;
             most = min(most, q.len - (q.q1 - q.q0));
         }
         most = max(__reduce_min_sync(0xffffffffu, most), 0);
         seqs = __reduce_add_sync(0xffffffffu, seqs);
+        lead = __reduce_min_sync(0xffffffffu, lead);
         if (seqs < 2) most = 0;
         if (ln == 0) {
             len_s[i] = most;
             s0_s[i] = s0;
             s1_s[i] = s1;
+            lead_s[i] = lead;
             if (most) atomicAdd(&saved_s, (unsigned long long)most * (seqs - 1));
         }
     }
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
             g.q_start[i] = q0;
             if (i == g.n - 1) g.q_start[g.n] = q1;
             g.len[i] = most;
-            g.row[i] = min(s0, b.n_seq - 1);
+            g.row[i] = lead_s[i];  // its pages hold the prefix, whatever became of the others
         }
     }
     __syncthreads();

@@ -150,9 +150,9 @@ class KvBatch:
 class KvShared:
     """Groups of a batch's sequences that share their first tokens: group g is the sequences
     seq_start[g] to seq_start[g + 1] (int32 [n_groups + 1]), whose first length[g] positions (int32
-    [n_groups]) are the same, and are read by the first one's pages.  max_new: a bound on any group's new
-    tokens, where the program knows one.  least: how many tokens of reading the sharing has to save, over all
-    groups, to be made (0: as many as its kernels' starts are worth)."""
+    [n_groups]) are the same, and are read by the pages of the first one that has new tokens.  max_new: a bound
+    on any group's new tokens, where the program knows one.  least: how many tokens of reading the sharing has
+    to save, over all groups, to be made (0: as many as its kernels' starts are worth)."""
 
     def __init__(self, seq_start, length, max_new: int = 0, least: int = 0):
         torch = _torch()

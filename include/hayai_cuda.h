@@ -322,10 +322,11 @@ int hc_attn_paged_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batc
 /* Sequences of a batch that share their first tokens (an instruction, a document): group g is the batch's
  * sequences [seq_start[g], seq_start[g+1]) (seq_start ascends; sequences in no group share nothing), whose
  * first length[g] positions hold the same keys and values, as hc_kv_fork_dev leaves them.  They are read by the
- * first sequence's pages.  Of a length past the tokens that every sequence of the group had before its new ones,
- * that much is shared.  max_new is the host's bound on any group's new tokens (0: n_tok); a group with more is
- * still computed, at lower speed.  least: how many tokens of reading the call's sharing has to save, over all
- * groups, to be made (0: as many as its kernels' starts are worth); the results differ by roundings only. */
+ * pages of the group's first sequence that has new tokens; those without may have gone.  Of a length past the tokens
+ * that every such sequence had before its new ones, that much is shared.  max_new is the host's bound on any group's
+ * new tokens (0: n_tok); a group with more is still computed, at lower speed.  least: how many tokens of reading the
+ * call's sharing has to save, over all groups, to be made (0: as many as its kernels' starts are worth); the results
+ * differ by roundings only. */
 typedef struct hc_kv_shared {
     int n_groups, max_new;
     int64_t least;

@@ -188,6 +188,16 @@ def test_lengths_are_cut_to_what_all_new_tokens_see(engine, dtype, cache):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("cache,dtype", [("i8", "bf16"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_that_have_gone(engine, cache, dtype, new):
+    """A group is read by the pages of one that is there: those without new tokens may hold nothing."""
+    s = Groups([(200, [(0, 0), (0, 0), (new, 90), (0, 0), (new, 60)]), (90, [(0, 0), (new, 70), (new, 70)])], 2, 64, 16, cache)
+    for i in (0, 1, 3, 5):
+        s.table[i], s.kv_len[i] = -1, 0
+    check(engine, s, 8, dtype)
+
+
 def test_sequences_outside_the_groups(engine):
     s = Groups(CASES["ragged"], 2, 64, 16, "f16")
     n = len(s.new)
