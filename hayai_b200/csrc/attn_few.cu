@@ -191,7 +191,8 @@ struct FewWalk {
         hi = min(b1 - it.u_item, it.t.units);
     }
     // On to the next item with a unit of this warp, if there is one.
-    __device__ __forceinline__ void settle(const AttnArgs& a, int rows, int unit) {
+    template <class A>
+    __device__ __forceinline__ void settle(const A& a, int rows, int unit) {
         while (st >= hi) {
             if (it.u_item + it.t.span >= b1) {
                 live = false;
@@ -203,8 +204,10 @@ struct FewWalk {
     }
 };
 
-template <class T, class C, int D, int NT>
-__global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kernel(const __grid_constant__ AttnArgs a) {
+// A: AttnArgs or AttnAlone.  (A sequence of 1001 tokens alone, f32 on 8-bit pages: 11.6 us; up to 0.5 more in a kernel that
+// asks for shared prefixes.)
+template <class T, class C, int D, int NT, class A>
+__global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kernel(const __grid_constant__ A a) {
     using F = FewCfg<T, C, D, NT>;
     using X = FewTerms<T, C>;
     constexpr int W = F::W, THREADS = 32 * W, ST = F::ST, CPR = F::CPR, MT = ST / 16, KS = D / 16, ROWS = 8 * NT, I8 = F::ES == 1;
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
             const int j = v < pw.it.t.n1 ? v : v - pw.it.t.n1 + pw.it.t.lo;
             const int p = a.by_page(j);
             pr = j - p * a.c.page_size;
-            pg = __ldg(a.b.table + (a.table_row ? __ldg(a.table_row + pw.it.s) : pw.it.s) * a.b.table_stride + p);
+            pg = __ldg(a.b.table + (a.shared && a.table_row ? __ldg(a.table_row + pw.it.s) : pw.it.s) * a.b.table_stride + p);
             if ((unsigned)pg >= (unsigned)a.c.n_pages) {
                 atomicOr(a.b.err, kErrKvRange);
                 pg = -1;
@@ -793,8 +796,8 @@ __global__ void __launch_bounds__(32 * FewCfg<T, C, D, NT>::W, 1) attn_few_kerne
 
 namespace {
 
-template <class T, class C, int D, int NT>
-cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
+template <class T, class C, int D, int NT, class A>
+cudaError_t launch(const A& a, int blocks, cudaStream_t s) {
     using F = FewCfg<T, C, D, NT>;
     constexpr int most = F::W * F::WB;
     static_assert(most <= 227 * 1024 - 1024, "shared memory of a block");
@@ -802,18 +805,19 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t s) {
     static_assert(most >= 4 * HC_KV_SEQS, "the schedule's prefix lies in the rings");
     static_assert((size_t)F::PS * 4 * 2 * (F::W + 1) <= kFewPartBytes, "the workspace of a block");
     static SmemOptIn opted;
-    const cudaError_t e = opted(reinterpret_cast<const void*>(attn_few_kernel<T, C, D, NT>), most);
+    const cudaError_t e = opted(reinterpret_cast<const void*>(attn_few_kernel<T, C, D, NT, A>), most);
     if (e != cudaSuccess) return e;
-    if (a.early) return launch_early(attn_few_kernel<T, C, D, NT>, blocks, 32 * F::W, most, s, a);
-    attn_few_kernel<T, C, D, NT><<<blocks, 32 * F::W, most, s>>>(a);
+    if (a.shared && a.early) return launch_early(attn_few_kernel<T, C, D, NT, A>, blocks, 32 * F::W, most, s, a);
+    attn_few_kernel<T, C, D, NT, A><<<blocks, 32 * F::W, most, s>>>(a);
     return cudaGetLastError();
 }
 
 // Tiles of 8 or 16 rows, by the batch's largest sequence.  (Tiles of 32 need more registers than a thread has.)
 template <class T, class C, int D>
 cudaError_t by_rows(const AttnArgs& a, int blocks, cudaStream_t s) {
-    if (a.max_rows <= 8) return launch<T, C, D, 1>(a, blocks, s);
-    return launch<T, C, D, 2>(a, blocks, s);
+    if (a.shared) return a.max_rows <= 8 ? launch<T, C, D, 1>(a, blocks, s) : launch<T, C, D, 2>(a, blocks, s);
+    const AttnAlone b{a};
+    return a.max_rows <= 8 ? launch<T, C, D, 1>(b, blocks, s) : launch<T, C, D, 2>(b, blocks, s);
 }
 
 template <class T>

@@ -415,10 +415,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 m -= kLift;  // the sums are of 2^(s - m)
                 const float k1 = l == 0.f ? 0.f : 1.f / l;
                 const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.ldo * 2)) & 31) == 0;  // rows start on 32 bytes
-                const int tr = a.by_group(row), head = hk * a.group + row - tr * a.group;
-                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + head * D;
-                const bool to_base = attn_part(a, tl.lo);
-                float* const base = a.base + ((long long)(q.q0 + tr) * a.heads + head) * D;
+                const int tr = a.by_group(row);
+                T* const out = (T*)a.out + (long long)(q.q0 + tr) * a.ldo + (hk * a.group + row - tr * a.group) * D;
                 float* const part = a.part + (size_t)(2 * c + slot) * PS;
 #pragma unroll 1
                 for (int k = 0; k < D / 32; ++k) {
@@ -426,13 +424,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                     tc_ld32(tO + 32 * k, o);
                     tc_wait_ld32(o);
                     if (!real || !ok) continue;
-                    if (whole && to_base) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<float4*>(base + 32 * k + 4 * i) =
-                                l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                         : make_float4(o[4 * i] * k1, o[4 * i + 1] * k1, o[4 * i + 2] * k1, o[4 * i + 3] * k1);
-                    } else if (whole) {
+                    if (whole) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             uint32_t y[8];
@@ -453,7 +445,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                 tc_fence_before();
                 if (real && ok) {
                     if (whole)
-                        attn_store_lse(a, q.q0, hk, row, m, l, to_base);
+                        attn_store_lse(a, q.q0, hk, row, m, l, false);
                     else
                         *reinterpret_cast<float2*>(part + ROWS * D + 2 * r) = make_float2(m, l);
                 }
@@ -500,7 +492,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         }
                         tops[r] = m;
                         tops[256 + r] = l;
-                        attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, m, l, attn_part(a, sh.lo));
+                        attn_store_lse(a, sh.q0, sh.hk, sh.r0 + r, m, l, false);
                     }
                 }
                 named_bar_sync(1, 256);
@@ -536,7 +528,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int e = e0 + 256 * k, r = e / (D / 4);
-                        if (e < sh.nr * (D / 4)) attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[256 + r], attn_part(a, sh.lo));
+                        if (e < sh.nr * (D / 4)) attn_store<T>(a, sh.q0, sh.hk, sh.r0 + r, D, e % (D / 4) * 4, y[k], tops[256 + r], false);
                     }
                 }
             }
@@ -593,7 +585,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
             const int lo = sg->lo, hi = sg->hi;
             if (!ok || lo == hi) break;
             const int nvis = sg->nvis, n1 = sg->n1, vlo = sg->vlo, hk = sg->hk;
-            const int* const table = a.b.table + (a.table_row ? __ldg(a.table_row + sg->s) : sg->s) * a.b.table_stride;
+            const int* const table = a.b.table + sg->s * a.b.table_stride;
             give_back(n);
             // page and row of this lane's position of unit st, and whether it has one (any page number may stand in a table)
             auto page_of = [&](int st, int& r, bool& has) {
@@ -724,7 +716,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const __grid
                         const bool whole = lo == 0 && hi == it.t.units;
                         segs[n & 3] = {lo, hi, it.t.nr, it.t.r0, it.q.q0, it.q.q1, it.q.len, it.s, it.hk, it.t.lo, it.t.n1,
                                        it.t.nvis, whole, lo == 0, {0, 0}};
-                        if (!whole) shared_s[lo == 0] = {1, it.q.q0, it.hk, it.t.r0, it.t.nr, it.u_item, it.t.units, it.t.lo};
+                        if (!whole) shared_s[lo == 0] = {1, it.q.q0, it.hk, it.t.r0, it.t.nr, it.u_item, it.t.units, 0};
                         mbar_arrive(b_seg + 8 * (n & 3));
                     }
                     ++n;

@@ -26,7 +26,8 @@ struct AttnTile {
     int units, span;   // span: units + a.over
 };
 
-__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q, int tile, int rows, int unit) {
+template <class A>
+__device__ __forceinline__ AttnTile attn_tile(const A& a, const KvSeq& q, int tile, int rows, int unit) {
     AttnTile t;
     const int n = q.q1 - q.q0;
     t.r0 = tile * rows;
@@ -34,7 +35,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const KvSeq& q,
     t.p_lo = q.len - n + a.by_group(t.r0);
     t.p_hi = q.len - n + a.by_group(t.r0 + t.nr - 1);
     const int end = a.causal ? max(min(q.len, t.p_hi + 1), 0) : q.len;
-    t.lo = a.window ? min(max(t.p_lo - a.window + 1, 0), end) : min(q.first, end);
+    t.lo = a.window ? min(max(t.p_lo - a.window + 1, 0), end) : a.shared ? min(q.first, end) : 0;
     t.n1 = min(a.sink, t.lo);
     t.nvis = t.n1 + end - t.lo;
     t.units = max(1, (t.nvis + unit - 1) / unit);  // a tile that sees nothing still has to write zeros
@@ -52,14 +53,16 @@ static __device__ __noinline__ bool attn_wanted(const AttnArgs& a) {
 }
 
 // A sequence, and where what it sees starts.
-__device__ __forceinline__ KvSeq attn_seq(const AttnArgs& a, int s) {
+template <class A>
+__device__ __forceinline__ KvSeq attn_seq(const A& a, int s) {
     KvSeq q = kv_seq(a.b, a.b.max_pages * a.c.page_size, s);
-    if (a.first) q.first = __ldcg(a.first + s);
+    if (a.shared && a.first) q.first = __ldcg(a.first + s);
     return q;
 }
 
-__device__ __forceinline__ int attn_tiles(const AttnArgs& a, const KvSeq& q, int rows) {
-    if (a.to_base && q.len == 0) return 0;  // nothing shared: nothing to add
+template <class A>
+__device__ __forceinline__ int attn_tiles(const A& a, const KvSeq& q, int rows) {
+    if (a.shared && a.to_base && q.len == 0) return 0;  // nothing shared: nothing to add
     const int r = (q.q1 - q.q0) * a.group;
     return r >= a.row_min && r <= a.row_max ? (r + rows - 1) / rows : 0;
 }
@@ -68,8 +71,8 @@ __device__ __forceinline__ int attn_tiles(const AttnArgs& a, const KvSeq& q, int
 // returns U, or -1 (and the error flag) if they do not fit 31 bits.  The whole block calls it, with 32
 // words of shared memory as scratch; word 18 then holds the number of items (of 2^16 and more: at
 // least that).
-template <int THREADS>
-__device__ __forceinline__ int attn_schedule(const AttnArgs& a, int rows, int unit, int* pre, int* scratch) {
+template <int THREADS, class A>
+__device__ __forceinline__ int attn_schedule(const A& a, int rows, int unit, int* pre, int* scratch) {
     static_assert(THREADS <= 32 * 16, "scratch");
     long long& carry_s = *reinterpret_cast<long long*>(scratch);
     int* const wsum = scratch + 2;
@@ -135,7 +138,8 @@ struct AttnLanes {
     KvSeq q;
     int pre;
 };
-__device__ __forceinline__ int attn_schedule_lanes(const AttnArgs& a, int rows, int unit, AttnLanes& v) {
+template <class A>
+__device__ __forceinline__ int attn_schedule_lanes(const A& a, int rows, int unit, AttnLanes& v) {
     const int ln = lane_id();
     v.q = {0, 0, 0, 0};
     unsigned long long x = 0;
@@ -170,13 +174,15 @@ struct AttnIter {
     KvSeq q;
     AttnTile t;
 
-    __device__ __forceinline__ void seq(const AttnArgs& a, int rows) {
+    template <class A>
+    __device__ __forceinline__ void seq(const A& a, int rows) {
         q = attn_seq(a, s);
         n_tiles = attn_tiles(a, q, rows);
         hk = tile = 0;
     }
     // The item that holds place u (0 <= u < U).
-    __device__ __forceinline__ void seek(const AttnArgs& a, const int* pre, int u, int rows, int unit) {
+    template <class A>
+    __device__ __forceinline__ void seek(const A& a, const int* pre, int u, int rows, int unit) {
         int lo = 0, hi = a.b.n_seq - 1;  // first sequence whose prefix is past u
         while (lo < hi) {
             const int m = (lo + hi) >> 1;
@@ -187,7 +193,8 @@ struct AttnIter {
         seq(a, rows);
         enter(a, s ? pre[s - 1] : 0, pre[s], u, rows, unit);
     }
-    __device__ __forceinline__ void seek(const AttnArgs& a, const AttnLanes& v, int u, int rows, int unit) {
+    template <class A>
+    __device__ __forceinline__ void seek(const A& a, const AttnLanes& v, int u, int rows, int unit) {
         s = __popc(__ballot_sync(0xffffffffu, v.pre <= u));
         q = {__shfl_sync(0xffffffffu, v.q.q0, s), __shfl_sync(0xffffffffu, v.q.q1, s), __shfl_sync(0xffffffffu, v.q.len, s),
              __shfl_sync(0xffffffffu, v.q.first, s)};
@@ -197,7 +204,8 @@ struct AttnIter {
         enter(a, s ? before : 0, __shfl_sync(0xffffffffu, v.pre, s), u, rows, unit);
     }
     // The item of sequence s, whose places are [before, end), that holds place u.
-    __device__ __forceinline__ void enter(const AttnArgs& a, int before, int end, int u, int rows, int unit) {
+    template <class A>
+    __device__ __forceinline__ void enter(const A& a, int before, int end, int u, int rows, int unit) {
         const int w = (end - before) / a.c.n_heads;
         hk = (u - before) / w;
         u_item = before + hk * w;
@@ -208,7 +216,8 @@ struct AttnIter {
         }
     }
     // The next item (there has to be one).
-    __device__ __forceinline__ void next(const AttnArgs& a, int rows, int unit) {
+    template <class A>
+    __device__ __forceinline__ void next(const A& a, int rows, int unit) {
         u_item += t.span;
         if (++tile == n_tiles) {
             tile = 0;
@@ -260,11 +269,12 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
 }
 
 // Does a tile's result go to `base`, to be joined?  Those of a prefix do, and those of what comes behind one.
-__device__ __forceinline__ bool attn_part(const AttnArgs& a, int lo) { return a.to_base || (a.first && lo > 0); }
+template <class A>
+__device__ __forceinline__ bool attn_part(const A& a, int lo) { return a.shared && (a.to_base || (a.first && lo > 0)); }
 
 // Four adjacent values of the weighted sum of row `row` of an item's kv head, over l.
-template <class T>
-__device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, int row, int D, int d, const float (&y)[4],
+template <class T, class A>
+__device__ __forceinline__ void attn_store(const A& a, int q0, int hk, int row, int D, int d, const float (&y)[4],
                                            float l, bool part) {
     const bool none = l == 0.f;  // saw nothing (a sum that is not a number is kept)
     const float k = none ? 0.f : 1.f / l;
@@ -281,7 +291,8 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, int q0, int hk, in
     else
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_b2(z[0], z[1]), pack_b2(z[2], z[3]));
 }
-__device__ __forceinline__ void attn_store_lse(const AttnArgs& a, int q0, int hk, int row, float m, float l, bool part) {
+template <class A>
+__device__ __forceinline__ void attn_store_lse(const A& a, int q0, int hk, int row, float m, float l, bool part) {
     const int t = a.by_group(row);
     const long long at = (long long)(q0 + t) * a.heads + hk * a.group + row - t * a.group;
     float* const lse = part ? a.base_lse : a.lse;

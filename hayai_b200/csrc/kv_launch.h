@@ -138,16 +138,20 @@ struct AttnArgs {
     int max_rows;          // the host's bound on a sequence's rows of one kv head (new tokens x group)
     int row_min, row_max;  // sequences with fewer or more rows are left to another kernel
     int over;              // places of the line that stand for a tile's start and end
+    int shared;            // one of the kernels of a call with shared prefixes; 0: nothing behind `count` is read
+    float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
+    int* count;            // 32 counters per block, zero between calls
     // A shared prefix (attn_shared.cu): results over a part of the positions go to `base`, to be joined.
     const int* first;        // [n_seq] positions that a sequence leaves out, or null
     const int* table_row;    // [n_seq] rows of the page table, or null: a sequence's own
     float *base, *base_lse;  // [n_tok * heads][head_dim] and log 2 of the weights' sums
     int to_base;             // the sequences are prefixes: all their results, but nothing of empty ones
-    int shared;              // one of the kernels of such a call
     int early;               // a launch_early
     const int *unless, *only;  // nothing is done where the one is not 0, or the other is
-    float* part;           // partial results: 2 slots per block of rows * (head_dim + 2) floats
-    int* count;            // 32 counters per block, zero between calls
+};
+// Those of a call of its own, for a kernel in which nothing asks for shared prefixes.
+struct AttnAlone : AttnArgs {
+    static constexpr int shared = 0;
 };
 
 // hc_kv_shared as the kernels get it, and what is made of it.
