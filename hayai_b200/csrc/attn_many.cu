@@ -1,7 +1,7 @@
 // attn_many.cu -- attention over the paged cache for sequences with many rows per kv head (prompts,
 // chunks of prompts), on the 5th-generation tensor cores.
 //
-// The mathematics is attn_few.cu's: one pass with a running maximum m and sum per row, m moved only
+// The mathematics is attn_few.cuh's: one pass with a running maximum m and sum per row, m moved only
 // when a score passes it by 8 (in log 2).  Work comes in tiles of 256 rows (attn_rows.cuh), two
 // halves of 128 with their own accumulators, and units of 128 positions; one block of 16 warps per SM
 // takes an equal share of the line of units.
@@ -31,7 +31,7 @@
 // order of the 16-bit results' own rounding, and summed in f32.  f16 weights are taken 2^7 times as large,
 // with the lag of m up to 2^15: they keep their 11 bits down to 2^-21 of the row's maximum, and below it are
 // off by up to 2^-32 of it (O stands in TMEM for the whole tile, so a unit cannot have a factor of its own as
-// in attn_few.cu).  8-bit codes are exact in f16; a K scale multiplies its column of S, a V scale its column
+// in attn_few.cuh).  8-bit codes are exact in f16; a K scale multiplies its column of S, a V scale its column
 // of P, and m follows the largest score + log2 of its V scale, so that P times scale stays under 2^15
 // whatever the scales are.  Where a unit's scales lie within 2^6 of each other the largest stands for all,
 // which may take that much of the room; elsewhere each position counts with its own, as a large one may have

@@ -208,6 +208,7 @@ constexpr size_t kAttnPartBytes = kFewPartBytes > kManyPartBytes ? kFewPartBytes
 
 // Sequences with few rows of a kv head, on mma.sync; any types.
 cudaError_t launch_attn_few(int cache_type, int dtype, int head_dim, const AttnArgs& a, int blocks, cudaStream_t s);
+cudaError_t launch_attn_few_shared(int cache_type, int dtype, int head_dim, const AttnArgs& a, int blocks, cudaStream_t s);
 // Sequences with many rows of a kv head, on tcgen05; 16-bit rows.
 bool attn_many_supported(int cache_type, int dtype);
 cudaError_t launch_attn_many(int cache_type, int dtype, int head_dim, const AttnArgs& a, int blocks, cudaStream_t s);
