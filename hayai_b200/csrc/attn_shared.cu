@@ -39,6 +39,11 @@ __device__ __noinline__ int tile_places(int tiles, int rows, int group, int from
     }
     return w;
 }
+// The new tokens of sequences [s0, s1), cut as kv_seq cuts them.
+__device__ __forceinline__ void group_tokens(const KvBatchDev& b, int s0, int s1, int& q0, int& q1) {
+    q0 = min(max(__ldg(b.q_start + s0), 0), b.n_tok);
+    q1 = min(max(__ldg(b.q_start + s1), q0), b.n_tok);
+}
 __device__ __noinline__ long long scan_1024(long long x, long long* scratch, long long& total) { return block_scan(x, scratch, total); }
 
 // A warp per group: how many tokens its sequences share for this step.  All new tokens have to see them all, so that
@@ -67,10 +72,15 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
         int most = min(max(given, 0), cap), seqs = 0, lead = b.n_seq - 1;
         if (s0 != a0 || s1 != a1 || most != given)
             if (ln == 0) atomicOr(b.err, kErrKvRange);
+        int q0, q1;
+        group_tokens(b, s0, s1, q0, q1);
 #pragma unroll 1
         for (int s = s0 + ln; s < s1; s += 32) {
             const KvSeq q = kv_seq(b, cap, s);
             if (q.q1 == q.q0) continue;
+            // Offsets that do not ascend (kv_seq reports them): the joining counts a sequence's rows from the group's
+            // first, so that a group with others shares nothing.
+            if (q.q0 < q0 || q.q1 > q1) most = 0;
             if (seqs++ == 0) lead = s;
             most = min(most, q.len - (q.q1 - q.q0));
         }
@@ -99,8 +109,8 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
 #pragma unroll 1
             for (int s = s0 + ln; s < s1; s += 32) of_s[s] = i;
         if (ln == 0) {
-            // its new tokens' rows, cut as kv_seq cuts them
-            const int q0 = min(max(__ldg(b.q_start + s0), 0), b.n_tok), q1 = min(max(__ldg(b.q_start + s1), q0), b.n_tok);
+            int q0, q1;
+            group_tokens(b, s0, s1, q0, q1);
             tok_s[i] = most ? q1 - q0 : 0;
             from_s[i] = 0;
             q0_s[i] = q0;

@@ -467,3 +467,23 @@ def test_shared_refusals(engine):
     empty = hb.KvBatch(s.table[:0], s.q_start[:1], s.kv_len[:0], 0)
     engine.attn_shared_dev(s.cache, empty, hb.KvShared(ints([0]), ints([])), q[:0], out[:0])
     engine.sync()
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16"), ("f16", "i8")])
+@pytest.mark.parametrize("new", [[2, 0, 2, 1], [100, 0, 100, 3], [7, 0, 1, 60]])
+def test_offsets_that_do_not_ascend_are_reported(engine, dtype, cache, new):
+    """A group whose sequences have rows before its first one's shares nothing: rows are those of the sequences by
+    themselves, and no others are written."""
+    s = Groups([(300, [(n, n + 5) for n in new])], 2, 64, 16, cache)
+    q = s.q(8, dtype)
+    first = sum(new) - new[0] - new[3]
+    starts = [first, first + new[0], 0, new[2], new[2]]  # the first sequence's rows lie behind the third's; the last has none
+    batch = hb.KvBatch(s.table, ints(starts), s.kv_len, s.rows, max(new))
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=DEV)
+    engine.attn_shared_dev(s.cache, batch, s.shared, q, out, lse=lse)
+    with pytest.raises(hb.CudaError, match="out of range"):
+        engine.sync()
+    order = torch.cat([torch.arange(first, first + new[0]), torch.arange(new[2])]).to(DEV)
+    s.new = [new[0], 0, new[2], 0]
+    close(s, dtype, out[order], lse[order], s.attention(q[order]))
+    assert (out[first + new[0]:] == 7).all() and (lse[first + new[0]:] == 7).all()
