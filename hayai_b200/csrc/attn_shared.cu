@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
 #pragma unroll 1
     for (int i = e0; i < e1; ++i) {  // a kv head's tiles and places
         const int rows = tok_s[i] * group, n = (rows + kTileRows - 1) / kTileRows;
-        tile_s[i] = elsewhere(i) ? i >= g.n && rows : n * g.kv_heads;
+        tile_s[i] = !elsewhere(i) ? n * g.kv_heads : i < g.n ? 0 : (int)(((unsigned)(tok_s[i] * g.heads) + kTileRows - 1) / kTileRows);
         place_s[i] = w_s[i] = elsewhere(i) ? 0 : tile_places(n, rows, group, from_s[i], len_s[i], pos_of(i));
         tiles += tile_s[i];
         places += (long long)w_s[i] * g.kv_heads;
@@ -175,14 +175,14 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
             }
             const int r = tok_s[lo] * group, per = (r + kTileRows - 1) / kTileRows, local = t - tile_s[lo], s = lo - g.n;
             const int pos = pos_of(lo);
-            const bool all = elsewhere(lo);  // all rows of a sequence, for the joining
+            const bool all = elsewhere(lo);  // rows of all query heads, for the joining
             x.hk = all ? -1 : local / per;
-            const int k = all ? 0 : local - x.hk * per;
+            const int k = all ? local : local - x.hk * per;
             x.r0 = k * kTileRows;
-            x.nr = all ? tok_s[lo] * g.heads : min(kTileRows, r - x.r0);
+            x.nr = min(kTileRows, (all ? tok_s[lo] * g.heads : r) - x.r0);
             x.q0 = q0_s[lo];
             x.from = from_s[lo];
-            x.len = tile_end(k, r, group, len_s[lo], pos);
+            x.len = all ? len_s[lo] : tile_end(k, r, group, len_s[lo], pos);
             x.row = lo < g.n ? g.row[lo] : s;
             x.pos0 = pos;
             x.pre = -1;
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
             if (!all) x.cost = tile_narrow(k, r) ? 1 : 2;
             x.units = all ? 0 : tile_units(x.from, x.len);
             if (s >= 0) runs = max(runs, (x.nr + 7) / 8);
-            x.place = place_s[lo] + (all ? 0 : x.hk * w_s[lo]) + (k ? tile_places(k, r, group, x.from, len_s[lo], pos) : 0);
+            x.place = place_s[lo];
+            if (!all) x.place += x.hk * w_s[lo] + (k ? tile_places(k, r, group, x.from, len_s[lo], pos) : 0);
             if (x.units) {
                 x.c0 = share.owner(x.place);
                 x.pieces = (share.owner(x.place + x.cost * (x.units - 1)) - x.c0 + 1) * (x.cost == 1 ? 2 : 1);
@@ -239,16 +240,20 @@ __global__ void __launch_bounds__(256, 4) attn_join_kernel(const __grid_constant
     const int n_tiles = __ldcg(p.line + kLineTiles), own = __ldcg(p.line + kLineOwn), runs = __ldcg(p.line + kLineRuns),
               ln = lane_id();
     const bool mine = ln < D / 4;
-    for (int w = blockIdx.x; w < (n_tiles - own) * runs; w += gridDim.x) {
+    if (n_tiles <= own) return;
+    // tile and run (eight rows of the tile), which are a block's distance apart: their product may not fit 32 bits
+    const int step = gridDim.x / runs, step_run = gridDim.x - step * runs;
+    for (int tile = own + blockIdx.x / runs, run = blockIdx.x % runs; tile < n_tiles;
+         run += step_run, tile += step + (run >= runs), run -= run >= runs ? runs : 0) {
         PrefixTile x;
-        const int4* const xs = reinterpret_cast<const int4*>(p.tiles + own + w / runs);
+        const int4* const xs = reinterpret_cast<const int4*>(p.tiles + tile);
 #pragma unroll
         for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(&x)[i] = __ldcg(xs + i);
-        const int r = w % runs * 8 + (threadIdx.x >> 5);
+        const int r = run * 8 + (threadIdx.x >> 5);
         if (r >= x.nr) continue;
         int row = x.r0 + r, hk = x.hk;
-        if (hk < 0) {  // the r-th of all (token, query head)
-            const int t = r / a.heads, h = r - t * a.heads;
+        if (hk < 0) {  // the sequence's row-th of all (token, query head)
+            const int t = row / a.heads, h = row - t * a.heads;
             hk = a.by_group(h);
             row = t * a.group + h - hk * a.group;
         }

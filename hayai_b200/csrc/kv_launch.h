@@ -174,8 +174,8 @@ struct alignas(16) PrefixTile {
     int place, units;    // the first of its places on the line (attn_prefix.cu); units of 128 positions
     int cost;            // places of a unit: 2, or 1 for up to 128 rows
     int q0;              // the first token of the group, or of the sequence
-    int hk, r0, nr;      // the kv head; the tile's first row and number of rows.  hk = -1: rows of all query heads, only for
-                         // the joining (what is behind the prefix has a result from elsewhere); nr may be any number then
+    int hk, r0, nr;      // the kv head; the tile's first row and number of rows.  hk = -1: (token, query head) rows, only for
+                         // the joining (what is behind the prefix has a result from elsewhere)
     int from, len;       // positions [from, len)
     int row;             // of the page table
     int piece, pieces;   // its first row in the pieces, and how many there are

@@ -487,3 +487,27 @@ def test_offsets_that_do_not_ascend_are_reported(engine, dtype, cache, new):
     s.new = [new[0], 0, new[2], 0]
     close(s, dtype, out[order], lse[order], s.attention(q[order]))
     assert (out[first + new[0]:] == 7).all() and (lse[first + new[0]:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,hint", [("f32", 0), ("bf16", 1)])
+def test_a_long_chunk_beside_single_tokens(engine, dtype, hint):
+    """Rows behind the prefixes that go to the kernel for few rows, of a long sequence and of short ones (16-bit rows
+    where the hint says single tokens): all of them are joined."""
+    s = Groups([(70, ONE * 3 + [(700, 720)] + [(1, 30)] * 5), (40, [(333, 333), (1, 1)]), (0, [(90, 90)])], 2, 64, 16, "f16")
+    s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
+    check(engine, s, 8, dtype, shared=hb.KvShared(s.starts, s.length, least=1))
+
+
+def test_a_chunk_of_millions_of_rows_beside_as_many_sequences_as_there_can_be(engine):
+    """2048 sequences, one of them of 8192 tokens: 1024 heads make 2^23 rows of that one alone.  Every row is written, and
+    as the paged attention has it: both are within 2^-13 (A + |out|) of the definition, and |out| <= A <= the largest value."""
+    s = Groups([(20, ONE * 2047 + [(8192, 8192)])], 1, 64, 64, "f16")
+    q = s.q(1024, "f32", scale=0.5)
+    out, plain = torch.full_like(q, math.nan), torch.empty_like(q)
+    lse, plain_lse = (torch.full(q.shape[:2], math.nan, device=DEV) for _ in range(2))
+    engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out, lse=lse)
+    engine.attn_paged_dev(s.cache, s.batch, q, plain, lse=plain_lse)
+    engine.sync()
+    most = s.pool[1].nan_to_num().abs().max().item()
+    assert ((out - plain).abs() <= 4 * 2.0 ** -13 * most).all()
+    assert ((lse - plain_lse).abs() <= 2 * (2.0 ** -12 + plain_lse.abs() * 2.0 ** -20)).all()
