@@ -72,12 +72,8 @@ struct Claims {
 
 __device__ __forceinline__ int pages_of(const PagesDev& p, int len) { return p.by_page(len + p.page_size - 1); }
 
-// A slot's length, held to what its table can have.
-__device__ __forceinline__ int slot_len(const PagesDev& p, int slot) {
-    const int n = p.len[slot], cap = p.max_pages * p.page_size, held = min(max(n, 0), cap);
-    if (n != held) atomicOr(p.err, kErrKvRange);
-    return held;
-}
+// Can a slot's table have so many tokens?
+__device__ __forceinline__ bool len_fits(const PagesDev& p, int n) { return n >= 0 && n <= p.max_pages * p.page_size; }
 __device__ __forceinline__ int* slot_table(const PagesDev& p, int slot) { return p.table + slot * p.stride; }
 
 // An item as the first kernel leaves it to the second (PagesDev::item): the slots and pages it is about.
@@ -104,7 +100,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagesDev p, const in
         if (i >= n) continue;
         const int a = first[i], b = second[i], slot = FORK ? b : a;
         const bool ok = (unsigned)slot < (unsigned)p.n_slots &&
-                        (FORK ? (unsigned)a < (unsigned)p.n_slots : b >= 0 && b <= p.max_pages * p.page_size);
+                        (FORK ? (unsigned)a < (unsigned)p.n_slots : len_fits(p, b));
         if (!ok) {
             atomicOr(p.err, kErrKvRange);
             continue;
@@ -121,25 +117,26 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagesDev p, const in
         const int i = 2 * threadIdx.x + e;
         if (x.slot < 0) continue;
         bool ok = claims.mine(x.slot, i);
+        int whole = 0;
         if (ok) {
-            x.old = slot_len(p, x.slot);
-            x.len = FORK ? slot_len(p, x.from) : second[i];
-            if (FORK) ok = x.old == 0;  // a child holds nothing
+            x.old = p.len[x.slot];
+            x.len = FORK ? p.len[x.from] : second[i];
+            ok = len_fits(p, x.old) && len_fits(p, x.len) && !(FORK && x.old);  // a child holds nothing
+        }
+        if (ok) {
+            // the tokens kept, and the page that the last of them share with the next ones
+            x.keep = FORK ? x.len : min(x.old, x.len);
+            whole = p.by_page(x.keep);
+            if (x.keep - whole * p.page_size) {
+                const int page = slot_table(p, x.from)[whole];
+                ok = (unsigned)page < (unsigned)p.n_pages;
+                if (ok && (FORK || p.refs[page] > 1)) x.part = page;
+            }
         }
         if (!ok) {
             atomicOr(p.err, kErrKvRange);
             x.slot = -1;
             continue;
-        }
-        // the tokens kept, and the page that the last of them share with the next ones
-        x.keep = FORK ? x.len : min(x.old, x.len);
-        const int whole = p.by_page(x.keep), rest = x.keep - whole * p.page_size;
-        if (rest) {
-            const int page = slot_table(p, x.from)[whole];
-            if ((unsigned)page >= (unsigned)p.n_pages)
-                atomicOr(p.err, kErrKvRange);
-            else if (FORK || p.refs[page] > 1)
-                x.part = page;
         }
         x.had = FORK ? 0 : pages_of(p, x.old);
         x.get = FORK ? whole : pages_of(p, x.len);
@@ -244,7 +241,10 @@ __global__ void __launch_bounds__(kWorkThreads) work_kernel(PagesDev p, const __
             const int i = (int)(w / runs), j = (int)(w - (long long)i * runs) * kWorkThreads + threadIdx.x;
             if constexpr (WORK == kCompactWork) {
                 int* const t = slot_table(p, i);
-                if (j >= pages_of(p, slot_len(p, i))) continue;
+                // of a length that does not fit, what the table can have: entries in use are not to name what has moved
+                const int len = p.len[i], held = min(max(len, 0), p.max_pages * p.page_size);
+                if (held != len) atomicOr(p.err, kErrKvRange);
+                if (j >= pages_of(p, held)) continue;
                 const int page = t[j];
                 if ((unsigned)page < (unsigned)p.n_pages) {
                     const int to = moved[page];

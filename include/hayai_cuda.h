@@ -382,9 +382,11 @@ int hc_kv_append_rope_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_
  * filled, belongs to the slot alone, so that appending never writes what another slot reads; whole pages may be
  * shared.  An array of slots, kv_len and the page table serve as a hc_kv_batch's with n_seq = n_slots.
  * Calls on one hc_kv_pages are made on one stream, or in an order that the caller sees to; they keep their plan in
- * `scratch`.  What is out of range on the device (slots, lengths, page numbers), a slot twice in a call, and a fork
- * into a slot that holds tokens are left out, and hc_sync reports HC_ERR_INVALID; so are items for which no free
- * page is left, with all later ones that take pages. */
+ * `scratch`.  Left out, and reported by hc_sync as HC_ERR_INVALID, are items whose slots or lengths (those that the slots
+ * have, as well) are out of range, or the number of the partly filled page that they keep; a slot's second time in a
+ * call; forks into slots that hold tokens; and items for which no free page is left, with all later ones that take
+ * pages.  Whole pages' numbers that are out of range are reported and otherwise left as they are: a child gets its
+ * parent's, and they are neither counted nor given back. */
 typedef struct hc_kv_pages {
     int n_slots, max_pages, n_layers;
     int32_t* page_table; /* [n_slots][table_stride] */

@@ -363,3 +363,61 @@ def test_pools_past_32_bits(engine):
     engine.kv_compact_dev(pages)
     engine.sync()
     assert table[:, :2].tolist() == [[2, 1], [2, 0]] and torch.equal(big[2], big[n - 1]) and (big[1, :, :5] == 2).all()
+
+
+@pytest.mark.parametrize("page", [-1, 40, 2**31 - 1, -2**31])
+@pytest.mark.parametrize("grow", [0, 1, 30])
+def test_a_partly_filled_page_out_of_range(engine, page, grow):
+    """Items that would keep it are left out, whatever an earlier use left in the child's table; others are done."""
+    p = Pool(page=16, max_pages=5)
+    p.do(engine, "resize", [0, 1, 5], [40, 50, 48], ok=True)
+    p.do(engine, "resize", [5], [0], ok=True)
+    p.do(engine, "resize", [2], [48], ok=True)  # slot 5's table still names pages that slot 2 has now
+    assert p.m_table[5][2] in p.m_table[2][:3]
+    mine = p.m_table[0][2]
+    p.table[0, 2] = p.m_table[0][2] = page
+    engine.kv_fork_dev(p.pages, ints([0, 1]), ints([5, 6]))
+    with pytest.raises(hb.CudaError, match="out of range"):
+        engine.sync()
+    p.fork([1], [6])
+    p.same()
+    engine.kv_resize_dev(p.pages, ints([0, 1]), ints([40 + grow, 33]))  # keeps its bad page
+    with pytest.raises(hb.CudaError, match="out of range"):
+        engine.sync()
+    p.resize([1], [33])
+    p.same()
+    p.table[0, 2] = p.m_table[0][2] = mine
+    p.do(engine, "resize", [0, 1, 2, 6], [0] * 4, ok=True)
+
+
+@pytest.mark.parametrize("page", [-1, 40])
+def test_a_whole_page_out_of_range_goes_to_the_child(engine, page):
+    """Reported, counted for nobody, and named by nobody else than parent and child."""
+    p = Pool(page=16, max_pages=5)
+    p.do(engine, "resize", [0], [40], ok=True)
+    lost = p.m_table[0][1]
+    p.table[0, 1] = page
+    engine.kv_fork_dev(p.pages, ints([0]), ints([5]))
+    with pytest.raises(hb.CudaError, match="out of range"):
+        engine.sync()
+    assert p.kv_len.tolist()[5] == 40 and p.table[5, :2].tolist() == [p.m_table[0][0], page]
+    assert p.refs[p.m_table[0][0]] == 2 and p.refs[lost] == 1
+    engine.kv_resize_dev(p.pages, ints([0, 5]), ints([0, 0]))
+    with pytest.raises(hb.CudaError, match="out of range"):
+        engine.sync()
+    assert p.refs.sum() == 1 and p.refs[lost] == 1 and not p.kv_len.any()
+
+
+@pytest.mark.parametrize("bad", [-5, 81, 2**31 - 1, -2**31])
+def test_slots_with_lengths_out_of_range(engine, bad):
+    """They are not forked, forked into or resized; items beside them are done."""
+    p = Pool(page=16, max_pages=5)
+    p.do(engine, "resize", [0, 1], [40, 50], ok=True)
+    p.kv_len[0] = p.m_len[0] = bad
+    for call, a, b, done in (("fork", [0, 1], [5, 6], ([1], [6])), ("fork", [1, 1], [0, 7], ([1], [7])),
+                             ("resize", [0, 1], [16, 70], ([1], [70])), ("resize", [0, 6], [0, 3], ([6], [3]))):
+        getattr(engine, f"kv_{call}_dev")(p.pages, ints(a), ints(b))
+        with pytest.raises(hb.CudaError, match="out of range"):
+            engine.sync()
+        getattr(p, call)(*done)
+        p.same()
