@@ -134,7 +134,8 @@ static int attn_make_workspace(const hc_engine* e, AttnWs* w) {
     return HC_OK;
 }
 
-// The workspace of the engine's stream, or of the captures on it, with `base` bytes for a shared prefix.
+// The workspace of the engine's stream, or of the captures on it, with `base` bytes for a shared prefix; *base_at is null
+// where there is no room for those.
 static int attn_workspace(hc_engine* e, AttnArgs* a, size_t base, void** base_at) {
     cudaStreamCaptureStatus status;
     HC_CUDA(cudaStreamIsCapturing(e->stream, &status));
@@ -142,12 +143,21 @@ static int attn_workspace(hc_engine* e, AttnArgs* a, size_t base, void** base_at
     AttnWs* w = e->attn_ws;
     while (w && (w->stream != e->stream || w->captured != captured || (captured && w->base.cap < base))) w = w->next;
     if (!w || w->base.cap < base) {
-        size_t size = base ? (size_t)1 << 20 : 0;  // a power of two: it grows few times
+        // a power of two, past 256 MB in quarters: it grows few times, and takes little more than it needs where that is much
+        size_t size = base ? (size_t)1 << 20 : 0;
         while (size < base) size *= 2;
+        if (const size_t step = size / 8; size > (size_t)256 << 20)
+            while (size - step >= base) size -= step;
         // a capture forbids its thread to allocate unless it says that it means to, outside the graph
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         HC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
         const bool fresh = !w;
+        size_t left = SIZE_MAX, all;
+        // an allocation that fails ends a capture: not to be tried where there is no room for it
+        if (captured && base && cudaMemGetInfo(&left, &all) == cudaSuccess && left < size + 2 * kAttnPartBytes * e->num_sms) {
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            return attn_workspace(e, a, 0, base_at);
+        }
         if (fresh) w = new (std::nothrow) AttnWs;
         int rc = !w ? hc_set_error(HC_ERR_CUDA, "attn_paged: out of host memory") : fresh ? attn_make_workspace(e, w) : HC_OK;
         if (!rc && size) rc = w->base.ensure(size);  // (freeing what was there waits for the calls that use it)
@@ -159,7 +169,7 @@ static int attn_workspace(hc_engine* e, AttnArgs* a, size_t base, void** base_at
         }
         if (rc) {
             cudaGetLastError();  // reported here: the next launch's check is not to find it
-            return rc;
+            return base ? attn_workspace(e, a, 0, base_at) : rc;
         }
         if (fresh) {
             w->stream = e->stream;
@@ -170,7 +180,7 @@ static int attn_workspace(hc_engine* e, AttnArgs* a, size_t base, void** base_at
     }
     a->part = (float*)w->part.p;
     a->count = (int*)w->count.p;
-    if (base_at) *base_at = w->base.p;
+    if (base_at) *base_at = base ? w->base.p : nullptr;
     return HC_OK;
 }
 
@@ -275,12 +285,7 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     // tables do not reach so far, else by the groups' lengths, on the device.
     const size_t token = 2 * (size_t)c->n_heads * (c->head_dim * (c->type == T_I8 ? 1 : 2) + (c->type == T_I8 ? 4 : 0));
     const long long least = g->least ? g->least : kShareBytes / (long long)token;  // tokens whose reading has to be saved
-    if (g->n_groups == 0 || b->n_tok < 2 || (b->n_seq - 1ll) * b->max_pages * c->page_size < least) {
-        rc = attn_workspace(e, &a, 0, nullptr);
-        if (rc) return rc;
-        const cudaError_t ce = attn_run(e, c, dtype, a, b->max_new);
-        return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
-    }
+    const bool may = g->n_groups && b->n_tok >= 2 && (b->n_seq - 1ll) * b->max_pages * c->page_size >= least;
     // f32 rows go to the kernel for few rows, whose terms attn_prefix.cu's operands do not hold, in two calls.
     const int sms = e->num_sms;
     const long long rows = (long long)b->n_tok * (long long)n_heads, kv = c->n_heads;
@@ -293,11 +298,12 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     if (shared > b->n_tok / 2) shared = b->n_tok / 2;
     if (shared > g->n_groups) shared = g->n_groups;
     const long long seqs = b->n_seq < b->n_tok ? b->n_seq : b->n_tok;  // with new tokens
-    const long long tiles = 2 * (rows / 256) + (shared + seqs) * kv;
-    // a row's result in a piece (of narrow tiles two) of its prefix and one behind it, and where a block's share ends
-    // in a tile, its rows once more
+    const long long tiles = 2 * (rows / 256) + (few ? 0 : shared * kv) + (behind ? seqs : seqs * kv);
+    // a row's result in a piece (of narrow tiles two) of its prefix, and one behind it unless it comes from the kernel
+    // for few rows; and where a block's share ends in a tile, its rows once more
     auto narrow = [&](long long n) { return n * kv * 128 < rows ? n * kv * 128 : rows; };
-    const long long pieces = few ? 0 : 2 * rows + narrow(shared) + narrow(seqs) + (long long)sms * 256;
+    const long long pieces =
+        few ? 0 : rows + narrow(shared) + (behind ? 0 : rows + narrow(seqs)) + (long long)sms * 256;
     size_t size = 0;
     auto room = [&](size_t n) {
         const size_t at = size;
@@ -310,8 +316,12 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
                  at_lse = room(r_behind), at_out = room(r_behind * c->head_dim), at_flse = room(r_few), at_few = room(r_few * c->head_dim),
                  at_ml = room((size_t)pieces * 2), at_part = room((size_t)pieces * c->head_dim);
     void* base = nullptr;
-    rc = attn_workspace(e, &a, size, &base);
+    rc = attn_workspace(e, &a, may ? size : 0, &base);
     if (rc) return rc;
+    if (!base) {  // nothing can be shared, or there is no room for it
+        const cudaError_t ce = attn_run(e, c, dtype, a, b->max_new);
+        return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
+    }
     auto place = [&](size_t at) { return (void*)((uint8_t*)base + at); };
     KvSharedDev d{};
     d.seq_start = g->seq_start;

@@ -511,3 +511,71 @@ def test_a_chunk_of_millions_of_rows_beside_as_many_sequences_as_there_can_be(en
     most = s.pool[1].nan_to_num().abs().max().item()
     assert ((out - plain).abs() <= 4 * 2.0 ** -13 * most).all()
     assert ((lse - plain_lse).abs() <= 2 * (2.0 ** -12 + plain_lse.abs() * 2.0 ** -20)).all()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_without_room_for_its_parts_nothing_is_shared(engine, captured):
+    """Where the workspace cannot be had the call is the paged attention's, bit for bit; once there is room it shares."""
+    s = Groups([(200, [(2, 30)] * 2048)], 4, 64, 16, "f16")
+    q = s.q(256, "f16")
+    assert q.shape[0] * 256 * 2 * 66 * 4 > 500 << 20  # two results and sums of a row, at least
+    out, plain = torch.empty_like(q), torch.empty_like(q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    engine.set_stream(stream)
+
+    def call():
+        if not captured:
+            engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out)
+            return None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out)
+        graph.replay()
+        return graph
+
+    engine.attn_paged_dev(s.cache, s.batch, q, plain)  # its code is there, and the part of the workspace that both have
+    small = Groups([(200, [(2, 30)] * 2)], 4, 64, 16, "f16")
+    x = small.q(4, "f16")
+    engine.attn_shared_dev(small.cache, small.batch, small.shared, x, torch.empty_like(x))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    filler = torch.empty(torch.cuda.mem_get_info()[0] - (400 << 20), dtype=torch.uint8, device=DEV)
+    graph = call()
+    torch.cuda.synchronize()
+    assert torch.equal(out, plain)
+    del filler, graph
+    torch.cuda.empty_cache()
+    graph = call()
+    torch.cuda.synchronize()
+    assert not torch.equal(out, plain)
+    most = s.pool[1].nan_to_num().abs().max().item()
+    assert ((out.double() - plain.double()).abs() <= 4 * 2.0 ** -10 * most).all()
+    del graph
+    engine.sync()
+    engine.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("dtype,cache,new", [("f16", "i8", 1), ("bf16", "bf16", 3), ("f32", "f16", 2)])
+@pytest.mark.parametrize("heads,dim", [(64, 64), (512, 128)])
+def test_the_workspace_is_as_large_as_it_is_said_to_be(engine, dtype, cache, new, heads, dim):
+    s = Groups([(500, [(new, 9)] * 700)], 2, dim, 16, cache)
+    q = s.q(heads, dtype)
+    out = torch.empty_like(q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    engine.set_stream(stream)
+    engine.attn_paged_dev(s.cache, s.batch, q, out)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out)
+    torch.cuda.synchronize()
+    took = before - torch.cuda.mem_get_info()[0]
+    most = (4.5 if dtype == "bf16" else 3.5) * s.rows * heads * (dim + 2) * 4 + (21 << 20)
+    least = 1 << 20
+    while least < most:
+        least *= 2
+    if least > 256 << 20:
+        least = min(n for n in range(4, 9) if n * least / 8 >= most) * least // 8
+    assert took <= least + (2 << 20)  # the driver's pages
+    engine.set_stream(torch.cuda.current_stream())
