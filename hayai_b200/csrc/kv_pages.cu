@@ -4,9 +4,10 @@
 //
 // Every call is two kernels.  The first, one block, decides: it reads the lengths and holders as they
 // stand, finds the lowest free pages, and writes new lengths, a list of page copies and what the tables
-// get.  The second, the whole GPU, rewrites the tables and copies the pages.  All results are those of
-// the items in order, one after the other, whatever the blocks' order: free pages are taken by a prefix
-// sum over the items, and counts of holders are whole numbers.
+// get.  The second, the whole GPU, rewrites the tables and copies the pages.  Lengths, holders and free
+// pages are read as they were before the call, for all items: one that cuts inside a page takes a copy where
+// others held it then, and what one item gives back serves no other of the call.  Only the free pages go round
+// in the items' order, by a prefix sum over them; holders are counted in whole numbers, in any order.
 //
 // Both are launched early (kv_launch.h): a call's second kernel, and the next call's first, wait for the one before
 // them on the GPU.

@@ -531,7 +531,8 @@ class CudaEngine:
 
     def kv_resize_dev(self, pages, slots, lens) -> None:
         """Slot slots[i] gets the length lens[i] (int32 tensors): pages are taken, the lowest free ones first, or
-        given back; a length of 0 lets the slot go."""
+        given back (free for the next call); a length of 0 lets the slot go.  A slot cut inside a page that others held
+        before the call gets a copy of it."""
         self._pages_here(pages)
         rc = self._kv_resize(self.handle, pages.ref, *pages.items(slots, lens, "slots and lens"))
         if rc:

@@ -404,8 +404,9 @@ int hc_kv_pages_scratch(int n_pages, size_t* out);
 int hc_kv_fork_dev(hc_engine* eng, const hc_kv_pages* pages, int n, const int32_t* parents, const int32_t* children);
 
 /* Slot slots[i] gets the length lens[i]: pages are taken (the lowest that were free before the call, in the order
- * of i and of the table) or given back; a length of 0 lets the slot go.  Where the last page kept is shared and
- * partly filled then, the slot gets a copy of it. */
+ * of i and of the table) or given back; a length of 0 lets the slot go.  Where the last page kept is partly filled then,
+ * and other table entries named it before the call, the slot gets a copy of it, whatever the call's other items do.
+ * Pages that the call gives back are free for the next one. */
 int hc_kv_resize_dev(hc_engine* eng, const hc_kv_pages* pages, int n, const int32_t* slots, const int32_t* lens);
 
 /* The pages in use move to the lowest numbers: of u of them, those numbered u and more go, in ascending order, to the

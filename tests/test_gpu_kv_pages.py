@@ -421,3 +421,21 @@ def test_slots_with_lengths_out_of_range(engine, bad):
             engine.sync()
         getattr(p, call)(*done)
         p.same()
+
+
+def test_holders_and_free_pages_are_those_before_the_call(engine):
+    """In a pool with one page left: of two that cut inside the page they share, the second finds none; one that cuts
+    inside a page whose other holder goes in the same call takes a copy, and what the other gives back is free after it."""
+    p = Pool(n_pages=4, slots=3, page=16, max_pages=4)
+    p.do(engine, "resize", [0], [48], ok=True)
+    p.do(engine, "fork", [0], [1], ok=True)
+    p.do(engine, "resize", [0, 1], [40, 40], ok=False)
+    assert p.m_len[:2] == [40, 48] and p.m_table[0][2] == 3
+    p.do(engine, "resize", [0], [0], ok=True)
+    assert p.m_refs == [1, 1, 1, 0]
+    p.do(engine, "fork", [1], [0], ok=True)
+    p.do(engine, "resize", [0, 1], [0, 20], ok=True)
+    assert p.m_table[1][1] == 3 and p.m_refs == [1, 0, 0, 1]
+    p.do(engine, "fork", [1], [0], ok=True)
+    p.do(engine, "resize", [0, 2], [0, 32], ok=False)
+    assert p.m_len == [0, 20, 0] and p.m_refs == [1, 0, 0, 1]
