@@ -556,6 +556,8 @@ static int check_pages(const char* what, hc_engine* e, const hc_kv_pages* p, Pag
         return hc_set_error(HC_ERR_INVALID, "%s: negative size n_slots=%d max_pages=%d", what, p->n_slots, p->max_pages);
     if ((long long)p->max_pages * c0->page_size > (1 << 30))
         return hc_set_error(HC_ERR_INVALID, "%s: %d pages of %d reach past 2^30 tokens", what, p->max_pages, c0->page_size);
+    if (c0->page_size > 1 << 26)  // a warp's copy counts a head's rows of a page, 16 bytes at a time, in 32 bits
+        return hc_set_error(HC_ERR_UNSUPPORTED, "%s: pages of %d tokens (at most 2^26)", what, c0->page_size);
     if (p->n_slots && (!p->page_table || !p->kv_len))
         return hc_set_error(HC_ERR_INVALID, "%s: null page table or kv_len", what);
     if (!p->refs || !p->scratch) return hc_set_error(HC_ERR_INVALID, "%s: null refs or scratch", what);

@@ -394,7 +394,7 @@ typedef struct hc_kv_pages {
     size_t table_stride;
     int32_t *kv_len, *refs;    /* [n_slots], [n_pages] */
     int32_t* scratch;          /* hc_kv_pages_scratch(n_pages) ints */
-    const hc_kv_cache* layers; /* host array, at most 256 */
+    const hc_kv_cache* layers; /* host array, at most 256; pages of at most 2^26 tokens */
 } hc_kv_pages;
 int hc_kv_pages_scratch(int n_pages, size_t* out);
 

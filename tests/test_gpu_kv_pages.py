@@ -439,3 +439,17 @@ def test_holders_and_free_pages_are_those_before_the_call(engine):
     p.do(engine, "fork", [1], [0], ok=True)
     p.do(engine, "resize", [0, 2], [0, 32], ok=False)
     assert p.m_len == [0, 20, 0] and p.m_refs == [1, 0, 0, 1]
+
+
+@pytest.mark.parametrize("page,fits", [(2**26, True), (2**26 + 1, False), (2**27, False)])
+def test_pages_of_more_tokens_than_a_copy_counts_are_refused(engine, page, fits):
+    """The description alone: no call gets as far as the pools."""
+    p = Pool(page=16, layers=1, max_pages=7)
+    p.pages._keep[-1][0].page_size = page
+    none = ints([])
+    for call in (lambda: engine.kv_resize_dev(p.pages, none, none), lambda: engine.kv_fork_dev(p.pages, none, none)):
+        if fits:
+            call()
+        else:
+            with pytest.raises(hb.CudaError, match="2\\^26"):
+                call()
