@@ -81,7 +81,8 @@ __device__ __forceinline__ KvPlace kv_find_seq(const KvBatchDev& b, int t) {
 }
 
 // ---------------------------------------------------------------- 8 elements of a row
-// (raw as loaded, so that many rows wait in few registers; as values)
+// (raw as loaded, so that many rows wait in few registers; as values.  load8 is for what no thread of the kernel writes,
+// load8_own for rows that it may write over, in place)
 template <class T>
 struct Elem;
 template <>
@@ -91,6 +92,9 @@ struct Elem<float> {
     };
     static __device__ __forceinline__ Raw load8(const float* p) {
         return {__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)};
+    }
+    static __device__ __forceinline__ Raw load8_own(const float* p) {
+        return {reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]};
     }
     static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
         x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w, x[4] = r.b.x, x[5] = r.b.y, x[6] = r.b.z, x[7] = r.b.w;
@@ -115,6 +119,7 @@ template <>
 struct Elem<__half> {
     using Raw = uint4;
     static __device__ __forceinline__ Raw load8(const __half* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+    static __device__ __forceinline__ Raw load8_own(const __half* p) { return *reinterpret_cast<const uint4*>(p); }
     static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -137,6 +142,7 @@ template <>
 struct Elem<__nv_bfloat16> {
     using Raw = uint4;
     static __device__ __forceinline__ Raw load8(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+    static __device__ __forceinline__ Raw load8_own(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
     static __device__ __forceinline__ void values(const Raw& r, float (&x)[8]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll

@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(kThreads) rope_rows_kernel(const __grid_consta
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long long o = (long long)min(u, heads - 1 - h0) * r.dim;
-            raw[u][0] = Elem<T>::load8(src + o + ln.c0);
-            raw[u][1] = Elem<T>::load8(src + o + ln.c1);
+            raw[u][0] = Elem<T>::load8_own(src + o + ln.c0);
+            raw[u][1] = Elem<T>::load8_own(src + o + ln.c1);
         }
         float2 cs[8];
         ln.angles(cs_s + t * half, cs);
@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_rope_kernel(const __grid_c
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int o = min(u, x.rows - 1) * D;
-            raw[u][0] = Elem<T>::load8(src + o + ln.c0);
-            raw[u][1] = Elem<T>::load8(src + o + ln.c1);
+            raw[u][0] = Elem<T>::load8_own(src + o + ln.c0);
+            raw[u][1] = Elem<T>::load8_own(src + o + ln.c1);
         }
     };
     Raw raw[U][2];
