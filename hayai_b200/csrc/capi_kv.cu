@@ -441,6 +441,8 @@ extern "C" int hc_rope_init(hc_rope* out, int layout, int head_dim, int rot_dim,
     return HC_OK;
 }
 
+// Are they the same rows?
+static bool rows_same(const void* x, size_t ldx, const void* out, size_t ldo, size_t n) { return x == out && (ldx == ldo || n == 1); }
 // May rows be written at `out` while rows are read at `x`?  Where both are the same rows, or no row of the one touches
 // a row of the other (slices of one array's rows, or apart altogether).
 static bool rows_apart(const void* x, size_t ldx, size_t wx, const void* out, size_t ldo, size_t wo, size_t n, size_t es) {
@@ -467,7 +469,7 @@ extern "C" int hc_rope_dev(hc_engine* e, const hc_rope* rope, int dtype, size_t 
     if (ldx < width || ldo < width || ldx > ((size_t)1 << 40) || ldo > ((size_t)1 << 40))
         return hc_set_error(HC_ERR_INVALID, "rope: leading dimension %zu out of range for rows of %zu", ldx < width ? ldx : ldo, width);
     if (((uintptr_t)x | (uintptr_t)out) % es) return hc_set_error(HC_ERR_INVALID, "rope: rows are not aligned to their type");
-    if (!(x == out && ldx == ldo) && !rows_apart(x, ldx, width, out, ldo, width, n_tok, es))
+    if (!rows_same(x, ldx, out, ldo, n_tok) && !rows_apart(x, ldx, width, out, ldo, width, n_tok, es))
         return hc_set_error(HC_ERR_INVALID, "rope: out must be x itself or not overlap it");
     const bool wide = rope_chunks(r) && (((uintptr_t)x | (uintptr_t)out) & 15) == 0 && ldx * es % 16 == 0 && ldo * es % 16 == 0;
     const RopeRows a{positions, x, out, (long long)ldx, (long long)ldo, (int)n_tok, (int)n_heads};
@@ -502,7 +504,7 @@ extern "C" int hc_kv_append_rope_dev(hc_engine* e, const hc_kv_cache* c, const h
     if (!rc) rc = check_rows(what, dtype, k, ldk, kw);
     if (!rc) rc = check_rows(what, dtype, v, ldv, kw);
     if (rc) return rc;
-    if ((!(q == q_out && ldq == ldqo) && !rows_apart(q, ldq, width, q_out, ldqo, width, n, es)) ||
+    if ((!rows_same(q, ldq, q_out, ldqo, n) && !rows_apart(q, ldq, width, q_out, ldqo, width, n, es)) ||
         !rows_apart(k, ldk, kw, q_out, ldqo, width, n, es) || !rows_apart(v, ldv, kw, q_out, ldqo, width, n, es))
         return hc_set_error(HC_ERR_INVALID, "%s: q_out must be q itself or overlap neither q, k nor v", what);
     const RopeAppend a{q, k, v, q_out, (long long)ldq, (long long)ldqo, (long long)ldk, (long long)ldv, (int)n_heads};

@@ -301,3 +301,26 @@ def test_append_refusals(engine):
     empty = hb.KvBatch(s.table[:0], s.q_start[:1], s.kv_len[:0], 0)
     engine.kv_append_rope_dev(cache, empty, rope, s.q[:0], s.k[:0], s.v[:0])
     engine.sync()
+
+
+def test_one_row_in_place_whatever_its_leading_dimensions(engine):
+    """A single row has no next one: in place is the same address."""
+    from hayai_b200 import _lib
+    x = torch.randn(1, 2, 64, device=DEV)
+    pos, rope = torch.tensor([7], dtype=torch.int32, device=DEV), hb.Rope(64)
+    want = torch.empty_like(x)
+    engine.rope_dev(rope, pos, x, want)
+    assert _lib.lib().hc_rope_dev(engine.handle, rope.ref, 0, 1, 2, pos.data_ptr(), x.data_ptr(), 128, x.data_ptr(), 256) == _lib.HC_OK
+    engine.sync()
+    assert torch.equal(x, want)
+    two = torch.randn(2, 2, 64, device=DEV)
+    assert _lib.lib().hc_rope_dev(engine.handle, rope.ref, 0, 2, 2, pos.data_ptr(), two.data_ptr(), 128, two.data_ptr(),
+                                  256) == _lib.HC_ERR_INVALID
+    s = Step([(1, 5)], 4, 2, 64, 16, "bf16", "f32")
+    q, q_want = s.q.clone(), torch.empty_like(s.q)
+    cache = hb.KvCache(*s.pools())
+    engine.kv_append_rope_dev(cache, s.batch, rope, s.q, s.k, s.v, q_want)
+    assert _lib.lib().hc_kv_append_rope_dev(engine.handle, cache.ref, s.batch.ref, rope.ref, 0, 4, q.data_ptr(), 256, q.data_ptr(), 512,
+                                            s.k.data_ptr(), 512, s.v.data_ptr(), 512) == _lib.HC_OK
+    engine.sync()
+    assert torch.equal(q, q_want)
