@@ -579,3 +579,44 @@ def test_the_workspace_is_as_large_as_it_is_said_to_be(engine, dtype, cache, new
         least = min(n for n in range(4, 9) if n * least / 8 >= most) * least // 8
     assert took <= least + (2 << 20)  # the driver's pages
     engine.set_stream(torch.cuda.current_stream())
+
+
+def laid_out(x, order, fill):
+    """The same pool [page][head][row][dim] in memory of another order or with room between its parts."""
+    n, h, r, d = x.shape
+    if order == "rows of all heads":  # [page][row][head]
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    if order == "heads apart":  # [head][page][row]
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+    shape, at = {"rows apart": ((n, h, r, 2 * d), (slice(None),) * 3 + (slice(d),)),
+                 "pages and heads apart": ((2 * n, h + 1, r, d), (slice(1, None, 2), slice(1, None)))}[order]
+    big = torch.full(shape, fill, dtype=x.dtype, device=DEV)
+    big[at] = x
+    return big[at]
+
+
+ORDERS = ["rows of all heads", "heads apart", "rows apart", "pages and heads apart"]
+
+
+@pytest.mark.parametrize("order", ORDERS)
+@pytest.mark.parametrize("cache,dtype", [("i8", "bf16"), ("i8", "f16"), ("i8", "f32"), ("bf16", "bf16"), ("f16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 24), (64, 1), (128, 300)])
+def test_pools_of_other_orders(engine, order, cache, dtype, dim, page):
+    """Bit for bit what the contiguous pool gives: chunks and single tokens, prefixes of several units and pages."""
+    s = Groups([(333, [(1, 1), (9, 40), (1, 150)]), (130, [(2, 2), (60, 70)])], 2, dim, page, cache)
+    q = s.q(8, dtype)
+    for hint in (0, 1):  # 1: what is behind the prefixes goes to the kernel for few rows
+        s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
+        plain = s.cache
+        want = check(engine, s, 8, dtype, q=q)
+        scale = []
+        for x in s.scale:
+            if x is not None:
+                wide = torch.full((x.shape[0], x[0].numel() + 5), math.nan, device=DEV)
+                wide[:, 3:-2] = x.flatten(1)
+                x = wide[:, 3:-2].unflatten(1, x.shape[1:])
+            scale.append(x)
+        s.cache = hb.KvCache(*(laid_out(x, order, 77 if cache == "i8" else math.nan) for x in s.pool), *scale)
+        got = check(engine, s, 8, dtype, q=q)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        s.cache = plain

@@ -324,3 +324,37 @@ def test_one_row_in_place_whatever_its_leading_dimensions(engine):
                                             s.k.data_ptr(), 512, s.v.data_ptr(), 512) == _lib.HC_OK
     engine.sync()
     assert torch.equal(q, q_want)
+
+
+@pytest.mark.parametrize("order", ["rows of all heads", "heads apart", "rows apart", "pages and heads apart"])
+@pytest.mark.parametrize("cache,dtype", [("i8", "bf16"), ("i8", "f32"), ("bf16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 1)])
+def test_append_to_pools_of_other_orders(engine, order, cache, dtype, dim, page):
+    """Bit for bit the rows that a contiguous pool gets, and nothing between them."""
+    s = Step(SHORT, 8, 2, dim, page, cache, dtype)
+    rope = hb.Rope(dim, base=1000.0)
+    plain = s.pools()
+    out, want = torch.empty_like(s.q), torch.empty_like(s.q)
+    engine.kv_append_rope_dev(hb.KvCache(*plain), s.batch, rope, s.q, s.k, s.v, want)
+    n, h, r, d = s.shape
+    whole, parts = [], []
+    for x in plain[:2]:
+        shape, perm, at = {"rows of all heads": ((n, r, h, d), (0, 2, 1, 3), ()), "heads apart": ((h, n, r, d), (1, 0, 2, 3), ()),
+                           "rows apart": ((n, h, r, 2 * d), (0, 1, 2, 3), (slice(None),) * 3 + (slice(d),)),
+                           "pages and heads apart": ((2 * n, h + 1, r, d), (0, 1, 2, 3), (slice(1, None, 2), slice(1, None)))}[order]
+        whole.append(torch.full(shape, 5, dtype=x.dtype, device=DEV))
+        parts.append(whole[-1].permute(perm)[at])
+    for x in plain[2:]:
+        if x is None:
+            parts.append(None)
+            continue
+        whole.append(torch.full((n, h * r + 5), 3.0, device=DEV))
+        parts.append(whole[-1][:, 2:-3].unflatten(1, (h, r)))
+    engine.kv_append_rope_dev(hb.KvCache(*parts), s.batch, rope, s.q, s.k, s.v, out)
+    engine.sync()
+    assert torch.equal(out, want)
+    assert all(a is None or torch.equal(a, b) for a, b in zip(parts, plain))
+    for x, fill in zip(parts, (5, 5, 3, 3)):
+        if x is not None:
+            x.fill_(fill)
+    assert all((w == f).all() for w, f in zip(whole, (5, 5, 3, 3)))
