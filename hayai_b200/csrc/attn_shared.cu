@@ -19,7 +19,13 @@ namespace hc {
 
 namespace {
 
-constexpr int kTileRows = 256, kUnit = 128, kOver = 2;
+// kOver: places of the line that stand for a tile's start and end (queries in, the first unit's way through the roles, O
+// out), some 12 us where a unit of a wide tile takes 2.  Tiles behind prefixes have few units, and lie together at the
+// line's end, so that too little for them leaves everything to a few blocks.  With 2, 6, 8, 10, 12, 14 of them (us in a
+// graph): 8 chunks of 256 bf16 tokens behind 16384, 32 heads on 8 of 128, 1177, 802, 677, 622, 577, 583 (the paged attention
+// 560); 6 groups of f16 chunks, 32 heads on 4, 206, 157, 157, 159, 159, 164; 8 chunks of 5 behind 4096 42.6, 37.8, 37.9, 39.8,
+// 39.7, 41.3; 64 single tokens behind 4100 8-bit ones, 64 heads on 8, 99, 90, 90, 93, 92, 92.
+constexpr int kTileRows = 256, kUnit = 128, kOver = 10;
 
 // Positions that tile k of `tok` tokens sees, at `pos` and following (kAllSeen: the whole of [from, len)).
 __device__ __forceinline__ int tile_end(int k, int rows, int group, int len, int pos) {
@@ -49,7 +55,7 @@ __device__ __noinline__ long long scan_1024(long long x, long long* scratch, lon
 // A warp per group: how many tokens its sequences share for this step.  All new tokens have to see them all, so that
 // they are at most the tokens that every sequence had before; a group of one sequence shares nothing.  Then the
 // tiles, in a line whose places the blocks of attn_prefix.cu share equally: a unit of a wide tile is two places, of a narrow
-// one one, and starting and finishing a tile counts as two more.
+// one one, and starting and finishing a tile counts as kOver more.
 __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvSharedDev g, int cap) {
     __shared__ long long scratch[33];
     __shared__ unsigned long long saved_s;
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
         pl += (long long)w * g.kv_heads;
     }
     const int n_tiles = fits ? (int)all_tiles : 0;
-    const int G = fits ? max(1, min(g.blocks, (int)U / 4)) : 1;  // shares of four places and more: every one has a unit
+    const int G = fits ? max(1, min(g.blocks, (int)U / 4)) : 1;  // shares of four places and more, so that those within a tile's units have one (others may have none)
     __syncthreads();
     const AttnShares share(max((int)(fits ? U : 0), 1), G);
     long long rows_before = 0;
