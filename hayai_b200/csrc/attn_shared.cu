@@ -59,23 +59,31 @@ __device__ __noinline__ long long scan_1024(long long x, long long* scratch, lon
 __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvSharedDev g, int cap) {
     __shared__ long long scratch[33];
     __shared__ unsigned long long saved_s;
-    __shared__ int runs_s;
+    __shared__ int runs_s, chunk_tiles_s;
     extern __shared__ int ent[];
     // entities: the groups' prefixes, then the sequences
     const int E = g.n + b.n_seq, tid = threadIdx.x, ln = lane_id(), group = g.heads / g.kv_heads;
     int *const tok_s = ent, *const from_s = tok_s + E, *const len_s = from_s + E, *const tile_s = len_s + E,
                *const place_s = tile_s + E, *const q0_s = place_s + E, *const w_s = q0_s + E, *const of_s = w_s + E;  // [n_seq] a sequence's group, or -1
     let_next_start();
-    if (tid == 0) saved_s = 0;
-#pragma unroll 1
-    for (int s = tid; s < b.n_seq; s += 1024) of_s[s] = -1;
+    if (tid == 0) saved_s = 0, chunk_tiles_s = 0;
     __syncthreads();
+#pragma unroll 1
+    for (int s = tid; s < b.n_seq; s += 1024) {
+        of_s[s] = -1;
+        if (!g.rule) continue;
+        const KvSeq q = kv_seq(b, cap, s);
+        const int rows = (q.q1 - q.q0) * group;
+        if (rows > kFewRows) atomicAdd(&chunk_tiles_s, (rows - 1) / kTileRows + 1);
+    }
+    __syncthreads();
+    const long long chunk_tiles = (long long)chunk_tiles_s * g.kv_heads;  // of the paged attention's kernel for many rows
     int *const s0_s = tile_s, *const s1_s = place_s, *const lead_s = w_s;  // the groups' sequences, until the tiles are counted
 #pragma unroll 1
     for (int i = tid >> 5; i < g.n; i += 32) {
         const int a0 = __ldg(g.seq_start + i), a1 = __ldg(g.seq_start + i + 1), given = __ldg(g.length + i);
         const int s0 = min(max(a0, 0), b.n_seq), s1 = min(max(a1, s0), b.n_seq);
-        int most = min(max(given, 0), cap), seqs = 0, lead = b.n_seq - 1;
+        int most = min(max(given, 0), cap), seqs = 0, lead = b.n_seq - 1, rows = 0, alone = 0;
         if (s0 != a0 || s1 != a1 || most != given)
             if (ln == 0) atomicOr(b.err, kErrKvRange);
         int q0, q1;
@@ -89,21 +97,39 @@ __global__ void __launch_bounds__(1024) attn_groups_kernel(KvBatchDev b, KvShare
             if (q.q0 < q0 || q.q1 > q1) most = 0;
             if (seqs++ == 0) lead = s;
             most = min(most, q.len - (q.q1 - q.q0));
+            rows += (q.q1 - q.q0) * group;
+            alone += ((q.q1 - q.q0) * group - 1) / g.tile + 1;
         }
         most = max(__reduce_min_sync(0xffffffffu, most), 0);
         seqs = __reduce_add_sync(0xffffffffu, seqs);
         lead = __reduce_min_sync(0xffffffffu, lead);
+        rows = __reduce_add_sync(0xffffffffu, rows);
+        alone = __reduce_add_sync(0xffffffffu, alone);
         if (seqs < 2) most = 0;
         if (ln == 0) {
             len_s[i] = most;
             s0_s[i] = s0;
             s1_s[i] = s1;
             lead_s[i] = lead;
-            if (most) atomicAdd(&saved_s, (unsigned long long)most * (seqs - 1));
+            if (most) {
+                // readings of the prefix that sharing saves
+                const int together = (rows - 1) / g.tile + 1;
+                long long saved = (long long)most * (seqs - 1);
+                if (g.rule && g.few)
+                    saved = (long long)most * (g.alone * alone - 8 * together) / 5;
+                else if (g.rule && chunk_tiles == 0)
+                    saved = (long long)most * (seqs - 1 - g.extra);
+                else if (g.rule && chunk_tiles >= g.blocks)
+                    saved = (long long)most * (25 * alone - 27 * together) / 25;
+                atomicAdd(&saved_s, (unsigned long long)saved);
+            }
         }
     }
     __syncthreads();
-    const bool worth = saved_s >= (unsigned long long)g.least;
+    long long least = g.least;
+    if (g.rule && !g.few && chunk_tiles) least = g.chunk;
+    if (g.rule && (g.few || chunk_tiles >= g.blocks)) least += g.moved;
+    const bool worth = (long long)saved_s >= least;
     if (!worth) {
         if (tid == 0) g.line[kLineTiles] = g.line[kLineOwn] = g.line[kLinePlaces] = 0;
         return;

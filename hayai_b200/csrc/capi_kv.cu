@@ -216,13 +216,33 @@ static int attn_args(const char* what, hc_engine* e, const hc_kv_cache* c, const
     return HC_OK;
 }
 
-constexpr int kFewRows = 16;
-
-// Bytes of keys and values that sharing prefixes has to save.  16 and 64 sequences of 32 heads on 8, as paged attention
-// and shared: behind 4096 bf16 tokens (252 MB saved) 37 and 47 us, 1024 (264 MB) 43 and 52; behind 16384 (1.0 GB) 103 and
-// 62, 4096 (1.1 GB) 109 and 57; behind 4096 8-bit tokens (134 MB) 34 and 42, 1024 (140 MB) 41 and 49, behind 16384 (535 MB)
-// 94 and 65, 4096 (561 MB) 100 and 62.
-constexpr long long kShareBytes = 384 << 20;
+// Whether sharing is worth it where the program gives no bound.  Readings of a prefix by tiles of rows are counted, alone
+// and together; the figures are us in a graph, paged and shared, of one group, 32 heads on 8 of 128, prefixes not in L2.
+// A bound has two sides: the host's, for what the page tables could hold at most, and the device's for what there is, which
+// is lower as the call has paid for the plan by then (9 to 12 us, where nothing is shared after all).
+struct ShareBound {
+    long long host, device;
+};
+// Single tokens (16-bit rows) pay for several kernels' starts, and for a prefix's units more than for a reading of it: as much
+// as for one more from 16-bit pages and three more from 8-bit ones.  bf16 pages: 16 sequences behind 4096 (240 MB saved)
+// 36 and 48, 8 behind 16384 (448 MB) 58 and 62, 40 behind 4096 (624 MB) 72 and 56, 16 behind 16384 (960 MB) 103 and 67, 4
+// behind 65536 (768 MB) 162 and 99.  8-bit: 16 behind 4096 (124 MB) 33 and 54, 8 behind 16384 (231 MB) 52 and 64, 40
+// behind 4096 (322 MB) 66 and 58, 16 behind 16384 (495 MB) 90 and 67; 4 behind 65536 (396 MB) 90 and 115, 8 (924) 165 and 115.
+constexpr ShareBound kShareBytes{300 << 20, 200 << 20}, kShareBytes8{190 << 20, 120 << 20};
+// Chunks have starts of the same cost either way.  Where they are fewer tiles than blocks, the paged attention splits tiles,
+// and whatever is read again can be saved: 8 of 5 tokens behind 1024 (28 MB) 37 and 36, 16 of 5 behind 1024 (60 MB) 44 and 44, 4
+// behind 4096 (48 MB) 44 and 36, 16 of 64 behind 4096 (240 MB) 140 and 135, 8 behind 16384 (448 MB) 214 and 177.  With more,
+// what counts is tiles that sharing fills, against its own tiles at 27/25 of the others' time and 16 bytes for each of
+// the rows' values in pieces: 16 of 256 tokens behind 16384 (960 MB, no tile saved) 1075 and 1281, 8 of 1000 (448 MB, 3 of 128)
+// 2342 and 2499, 16 of 100 (7 of 32) behind 16384 556 and 490, behind 1024 111 and 125; one of 3000 with 31 single tokens behind
+// 1024 265 and 337, behind 16384 1101 and 1044.
+constexpr ShareBound kShareChunkBytes{64 << 20, 32 << 20};
+// f32 rows read a prefix by up to 16 of them, which costs 8/5 of a reading by up to 8; in tokens of a kv head at the cheaper
+// one, less 48 of them for moving a row's parts (500 tokens and 63 single ones behind 1024: 249 and 308, behind 4096 679 and 619).
+// 8-bit pages: 16 sequences of 2 tokens behind 16384 (0.42 M saved) 120 and 136, 8 single tokens (0.63 M) 62 and 75, 40 behind
+// 4096 (0.79 M) 81 and 85, 8 of 5 behind 16384 (1.26 M) 178 and 155, 16 single ones (1.26 M) 114 and 94; bf16 pages, 8 (0.63 M) 85 and
+// 86, 40 behind 4096 (0.79 M) 107 and 93, 16 (1.26 M) 157 and 114.  16 tokens save nothing: 16 behind 16384 661 and 712.
+constexpr ShareBound kShareTokens{700000, 500000}, kShareTokens8{1000000, 750000};
 
 // Sequences with up to kFewRows rows per kv head go to the kernel for few rows (tiles of 8 or 16 rows), longer
 // ones to the other (tiles of 256): both are launched where the batch may have both.  At 16 rows, 16
@@ -281,19 +301,40 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         return hc_set_error(HC_ERR_INVALID, "attn_shared: %d groups (at most %d)", g->n_groups, HC_KV_MAX_SEQ);
     if (g->n_groups && (!g->seq_start || !g->length)) return hc_set_error(HC_ERR_INVALID, "attn_shared: null seq_start or length");
     if (none) return HC_OK;
-    // Sharing costs several kernels' starts, and is left where what it saves is not worth them: here where the page
-    // tables do not reach so far, else by the groups' lengths, on the device.
-    const size_t token = 2 * (size_t)c->n_heads * (c->head_dim * (c->type == T_I8 ? 1 : 2) + (c->type == T_I8 ? 4 : 0));
-    const long long least = g->least ? g->least : kShareBytes / (long long)token;  // tokens whose reading has to be saved
-    const bool may = g->n_groups && b->n_tok >= 2 && (b->n_seq - 1ll) * b->max_pages * c->page_size >= least;
     // f32 rows go to the kernel for few rows, whose terms attn_prefix.cu's operands do not hold, in two calls.
     const int sms = e->num_sms;
+    const bool few = !attn_many_supported(c->type, dtype), codes = c->type == T_I8;
     const long long rows = (long long)b->n_tok * (long long)n_heads, kv = c->n_heads;
+    const long long own_rows = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
+    // Sharing is left where what it saves is not worth its kernels: here where the page tables do not reach so far, else by
+    // the groups' lengths and rows, on the device.
+    const long long token = 2 * kv * (c->head_dim * (codes ? 1 : 2) + (codes ? 4 : 0));
+    KvSharedDev d{};
+    d.rule = g->least == 0;
+    d.tile = few ? 16 : 256;
+    d.extra = codes ? 3 : 1;
+    d.alone = own_rows > 8 ? 8 : 5;
+    d.chunk = kShareChunkBytes.device / token;
+    d.moved = few ? rows * 48 / kv : rows * c->head_dim * 16 / token;
+    const ShareBound bound = few ? (codes ? kShareTokens8 : kShareTokens) : codes ? kShareBytes8 : kShareBytes;
+    d.least = g->least ? g->least : bound.device / (few ? kv : token);
+    // the most that the sequences save, in fifths of readings of all that their tables hold
+    long long readings = 5 * (b->n_seq - 1ll), least = g->least;
+    const long long new_rows = (long long)b->n_tok * a.group;
+    if (d.rule && few) {
+        least = bound.host / kv;
+        readings = d.alone * (long long)b->n_seq - 8 * (d.alone == 8 ? 1 : (new_rows + 15) / 16);
+    } else if (d.rule && new_rows > (long long)kFewRows * b->n_seq) {  // one chunk at least
+        least = kShareChunkBytes.host / token;
+    } else if (d.rule) {
+        least = bound.host / token;
+        readings -= 5 * d.extra;
+    }
+    const bool may = g->n_groups && b->n_tok >= 2 && readings * b->max_pages * c->page_size / 5 >= least;
     // What a sequence has behind its prefix goes there too where it has few rows (single tokens): 64 of them with 30 to
     // 1500 8-bit tokens each take 43 us there, and 75 as tiles of attn_prefix.cu; 53 chunks of up to 60 tokens with up
     // to 300 before them 108 in the paged attention's kernels, and 75 as tiles.
-    const bool few = !attn_many_supported(c->type, dtype);
-    const bool behind = few || (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group <= kFewRows;
+    const bool behind = few || own_rows <= kFewRows;
     long long shared = b->n_seq / 2;  // groups that share anything: two sequences with new tokens each
     if (shared > b->n_tok / 2) shared = b->n_tok / 2;
     if (shared > g->n_groups) shared = g->n_groups;
@@ -323,7 +364,6 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "attn_shared launch");
     }
     auto place = [&](size_t at) { return (void*)((uint8_t*)base + at); };
-    KvSharedDev d{};
     d.seq_start = g->seq_start;
     d.length = g->length;
     d.n = g->n_groups;
@@ -331,7 +371,6 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
     d.q_start = (int*)place(at_q);
     d.len = (int*)place(at_len);
     d.row = (int*)place(at_row);
-    d.least = least;
     d.heads = a.heads;
     d.kv_heads = c->n_heads;
     d.few = few;
@@ -375,8 +414,7 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         x.base = a.base = (float*)place(at_out);
         x.base_lse = a.base_lse = (float*)place(at_lse);
         x.early = 1;
-        const long long most = (long long)(b->max_new && b->max_new < b->n_tok ? b->max_new : b->n_tok) * a.group;
-        x.max_rows = (int)(most < INT32_MAX ? most : INT32_MAX);
+        x.max_rows = (int)(own_rows < INT32_MAX ? own_rows : INT32_MAX);
         if (ce == cudaSuccess) ce = launch_attn_few(c->type, dtype, c->head_dim, x, sms, e->stream);
     }
     if (ce == cudaSuccess) ce = launch_attn_join(dtype, c->head_dim, a, p, sms, e->stream);

@@ -159,6 +159,13 @@ struct KvSharedDev {
     const int *seq_start, *length;
     int n;
     long long least;           // tokens that sharing has to save, or nothing is shared
+    // Without a bound of the program's (rule) what it saves is counted by what kernels take (capi_kv.cu):
+    int rule;
+    int tile;         // rows that read a prefix together: 256, or 16 of the kernel for few rows
+    int extra;        // single tokens: readings that the prefix's kernel costs more than it saves
+    int alone;        // f32 rows: what a sequence's reading by itself costs, in eighths of one by 16 rows
+    long long chunk;  // where sequences have more rows than the kernel for few takes, their bound
+    long long moved;  // and tokens whose reading takes as long as moving all rows' parts
     int heads, kv_heads;       // query heads, and those that the keys have
     int few, few_behind;       // the prefixes, or what is behind them, go to the kernel for few rows, else to attn_prefix.cu
     int *first;                // few_behind: [n_seq] shared tokens, where what is behind them starts
@@ -195,6 +202,8 @@ struct PrefixArgs {
     float *part, *part_ml;
     const float *few, *few_lse;
 };
+// Rows of a kv head up to which a sequence goes to the kernel for few rows.
+constexpr int kFewRows = 16;
 cudaError_t launch_attn_groups(const KvBatchDev& b, const KvSharedDev& g, int cap, cudaStream_t s);
 cudaError_t launch_attn_prefix(int cache_type, int dtype, int head_dim, const AttnArgs& a, const PrefixArgs& p, int blocks,
                                cudaStream_t s);

@@ -152,7 +152,7 @@ class KvShared:
     seq_start[g] to seq_start[g + 1] (int32 [n_groups + 1]), whose first length[g] positions (int32
     [n_groups]) are the same, and are read by the pages of the first one that has new tokens.  max_new: a bound
     on any group's new tokens, where the program knows one.  least: how many tokens of reading the sharing has
-    to save, over all groups, to be made (0: as many as its kernels' starts are worth)."""
+    to save, over all groups, to be made (0: by the library's rule, which leaves it where it would be slower)."""
 
     def __init__(self, seq_start, length, max_new: int = 0, least: int = 0):
         torch = _torch()

@@ -325,8 +325,8 @@ int hc_attn_paged_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batc
  * pages of the group's first sequence that has new tokens; those without may have gone.  Of a length past the tokens
  * that every such sequence had before its new ones, that much is shared.  max_new is the host's bound on any group's
  * new tokens (0: n_tok); a group with more is still computed, at lower speed.  least: how many tokens of reading the
- * call's sharing has to save, over all groups, to be made (0: as many as its kernels' starts are worth); the results
- * differ by roundings only. */
+ * call's sharing has to save, over all groups, to be made (0: by a rule of the library's, on the prefixes' lengths, the
+ * sequences' rows and the types, which leaves it where it would be slower). */
 typedef struct hc_kv_shared {
     int n_groups, max_new;
     int64_t least;

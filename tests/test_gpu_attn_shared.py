@@ -620,3 +620,29 @@ def test_pools_of_other_orders(engine, order, cache, dtype, dim, page):
         got = check(engine, s, 8, dtype, q=q)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         s.cache = plain
+
+
+@pytest.mark.parametrize("dtype,cache,groups,hint,made", [
+    ("bf16", "bf16", [(16384, [(256, 356)] * 8)], 0, False),  # full tiles: nothing but reading from L2 to save
+    ("bf16", "bf16", [(16384, [(17, 117)] * 8)], 0, True),
+    ("bf16", "bf16", [(2048, [(17, 117)] * 4)], 0, False),
+    ("bf16", "i8", [(65536, [(1, 101)] * 4)], 1, False),  # the prefix's units cost more than three readings
+    ("bf16", "i8", [(65536, [(1, 101)] * 8)], 1, True),
+    ("f16", "f16", [(16384, [(1, 101)] * 4)], 1, False),
+    ("f16", "f16", [(16384, [(1, 101)] * 16)], 1, True),
+    ("f32", "bf16", [(16384, [(16, 116)] * 16)], 16, False),  # 64 rows each: as many tiles of 16 together
+    ("f32", "bf16", [(16384, [(1, 101)] * 16)], 1, True),
+    ("f32", "i8", [(16384, [(5, 105)] * 8)], 5, True)])
+def test_the_rule_on_what_is_shared(engine, dtype, cache, groups, hint, made):
+    """Sharing is left where it would be slower, and made on the other side of the rule: the paged attention's bits tell."""
+    s = Groups(groups, 8, 128, 64, cache)
+    s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
+    q = s.q(32, dtype)
+    out, plain = torch.empty_like(q), torch.empty_like(q)
+    engine.attn_shared_dev(s.cache, s.batch, hb.KvShared(s.starts, s.length), q, out)
+    engine.attn_paged_dev(s.cache, s.batch, q, plain)
+    engine.sync()
+    assert torch.equal(out, plain) != made
+    c = 2.0 ** -13 if dtype == "f32" else 2.0 ** -10 if dtype == cache == "f16" else 2.0 ** -8
+    v = s.pool[1].float() if cache != "i8" else s.pool[1].float() * s.scale[1][..., None]
+    assert ((out.double() - plain.double()).abs() <= 4 * c * v.nan_to_num().abs().max().item()).all()
