@@ -646,3 +646,59 @@ def test_the_rule_on_what_is_shared(engine, dtype, cache, groups, hint, made):
     c = 2.0 ** -13 if dtype == "f32" else 2.0 ** -10 if dtype == cache == "f16" else 2.0 ** -8
     v = s.pool[1].float() if cache != "i8" else s.pool[1].float() * s.scale[1][..., None]
     assert ((out.double() - plain.double()).abs() <= 4 * c * v.nan_to_num().abs().max().item()).all()
+
+
+@pytest.mark.parametrize("dtype,cache,hint", [("f32", "i8", 0), ("f32", "bf16", 1), ("bf16", "i8", 1), ("f16", "f16", 1), ("bf16", "bf16", 0)])
+@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (4, 4)])
+def test_scale_and_strided_rows_of_the_other_kernels(engine, dtype, cache, hint, heads, kv_heads):
+    """f32 rows, and single tokens behind prefixes: rows apart, any scale, with a log-sum-exp and without."""
+    s = Groups([(90, ONE * 4 + [(1, 33), (3, 20)]), (0, [(2, 9)]), (160, [(1, 1), (1, 70)])], kv_heads, 64, 16, cache)
+    s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
+    buf = torch.randn(s.rows, 3, heads, 64, generator=s.g, device=DEV).to(T[dtype])
+    q = buf[:, 1]
+    for scale in (0.3, -0.2, 0.0, None):
+        out, lse = torch.full((s.rows, 2, heads, 64), 7.0, device=DEV).to(T[dtype]), torch.empty(s.rows, heads, device=DEV)
+        engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out[:, 1], scale=scale, lse=lse)
+        engine.sync()
+        close(s, dtype, out[:, 1], lse, s.attention(q, scale))
+        again = torch.empty_like(out)
+        engine.attn_shared_dev(s.cache, s.batch, s.shared, q, again[:, 1], scale=scale)
+        engine.sync()
+        assert (out[:, 0] == 7).all() and torch.equal(again[:, 1], out[:, 1])
+
+
+@pytest.mark.parametrize("dtype,cache,hint", [("f32", "i8", 0), ("bf16", "i8", 1), ("f16", "f16", 0)])
+def test_one_graph_through_sharing_and_none(engine, dtype, cache, hint):
+    """A captured call whose lengths change between replays: groups that share, that share nothing any more, sequences that
+    go; two streams' direct calls between them."""
+    s = Groups([(300, [(1, 40)] * 9), (64, [(1, 8), (1, 30)])], 2, 64, 16, cache)
+    s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
+    shared = hb.KvShared(s.starts, s.length, least=500)
+    q = s.q(8, dtype)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        engine.set_stream(torch.cuda.current_stream())
+        engine.attn_shared_dev(s.cache, s.batch, shared, q, out, lse=lse)
+    kv = list(s.kv)
+    for lengths, cut in (([300, 64], 0), ([50, 0], 0), ([300, 64], 30), ([0, 0], 0), ([300, 64], 0)):
+        s.length.copy_(ints(lengths))
+        s.kv = [k - cut if i else k for i, k in enumerate(kv)]
+        s.kv = [max(k, 1) for k in s.kv]
+        s.kv_len.copy_(ints(s.kv))
+        out.fill_(math.nan), lse.fill_(math.nan)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        close(s, dtype, out, lse, s.attention(q))
+        first = out.clone()
+        for st in (torch.cuda.Stream(), torch.cuda.Stream()):
+            engine.set_stream(st)
+            direct = torch.empty_like(q)
+            torch.cuda.synchronize()
+            engine.attn_shared_dev(s.cache, s.batch, shared, q, direct)
+            torch.cuda.synchronize()
+            assert torch.equal(direct, first)
+    engine.set_stream(torch.cuda.current_stream())
