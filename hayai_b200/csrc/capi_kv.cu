@@ -511,7 +511,7 @@ extern "C" int hc_rope_dev(hc_engine* e, const hc_rope* rope, int dtype, size_t 
         return hc_set_error(HC_ERR_INVALID, "rope: out must be x itself or not overlap it");
     const bool wide = rope_chunks(r) && (((uintptr_t)x | (uintptr_t)out) & 15) == 0 && ldx * es % 16 == 0 && ldo * es % 16 == 0;
     const RopeRows a{positions, x, out, (long long)ldx, (long long)ldo, (int)n_tok, (int)n_heads};
-    const cudaError_t ce = launch_rope(dtype, r, a, wide, e->stream);
+    const cudaError_t ce = launch_rope(dtype, r, a, wide, e->num_sms, e->stream);
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "rope launch");
 }
 
@@ -546,7 +546,7 @@ extern "C" int hc_kv_append_rope_dev(hc_engine* e, const hc_kv_cache* c, const h
         !rows_apart(k, ldk, kw, q_out, ldqo, width, n, es) || !rows_apart(v, ldv, kw, q_out, ldqo, width, n, es))
         return hc_set_error(HC_ERR_INVALID, "%s: q_out must be q itself or overlap neither q, k nor v", what);
     const RopeAppend a{q, k, v, q_out, (long long)ldq, (long long)ldqo, (long long)ldk, (long long)ldv, (int)n_heads};
-    const cudaError_t ce = launch_kv_append_rope(c->type, dtype, c->head_dim, r, cd, bd, a, e->stream);
+    const cudaError_t ce = launch_kv_append_rope(c->type, dtype, c->head_dim, r, cd, bd, a, e->num_sms, e->stream);
     return ce == cudaSuccess ? HC_OK : hc_cuda_error(ce, "kv_append_rope launch");
 }
 

@@ -41,9 +41,9 @@ struct RopeAppend {
     int heads;
 };
 // wide: sizes, strides and addresses in whole 16 bytes and chunks of 8 values.
-cudaError_t launch_rope(int dtype, const RopeDev& r, const RopeRows& a, bool wide, cudaStream_t s);
+cudaError_t launch_rope(int dtype, const RopeDev& r, const RopeRows& a, bool wide, int sms, cudaStream_t s);
 cudaError_t launch_kv_append_rope(int cache_type, int dtype, int head_dim, const RopeDev& r, const KvDev& c,
-                                  const KvBatchDev& b, const RopeAppend& a, cudaStream_t s);
+                                  const KvBatchDev& b, const RopeAppend& a, int sms, cudaStream_t s);
 
 // Division of 0 <= n < 2^31 by d >= 1 as a multiplication: with 2^k >= d and m = ceil(2^(31+k) / d),
 // floor(n m / 2^(31+k)) = floor(n / d), as m d - 2^(31+k) < d <= 2^k.

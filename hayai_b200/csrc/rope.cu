@@ -7,14 +7,18 @@
 // Angles.  A position times a frequency in f32 is off by whole radians far out (2^20 * 2^-24).  The
 // frequencies are kept in turns as 64-bit fixed point fractions instead, whose product with a whole
 // position wraps at whole turns by itself: three integer instructions leave the angle to 2^-32 of a
-// turn for every position of 32 bits, and sincospi takes it from there, to f32's own rounding.  A
-// position's angles are made once per block and token, and serve all heads.
+// turn for every position of 32 bits, and sincospi takes it from there, rounded to 24 bits: off by 2^-25 of
+// half a turn at most, as much as cos and sin are rounded by themselves.  A position's angles are made once
+// per block and token, and serve all heads.
 //
 // Bound by memory: a row is read once and written once.  A lane holds two chunks of 8 values, in the half layout
 // the two partners, so that nothing is exchanged between lanes but an 8-bit row's largest value.
 //
 // Measured: 9000 tokens of 32 bf16 heads of 128 26 us (5.6 TB/s, 86 % of the copy rate); 15947 tokens of prompts, 32
 // query heads turned and 8 kv heads turned and stored in 8 bits, 82 us (4.4 TB/s), one token 3.6 us in a graph.
+// The same prompts into bf16 pages 72 us (5.5 TB/s), f32 rows into f16 pages 119 (6.0); 64 and 256 single tokens 4.0 and 4.4
+// us, into 8-bit pages 4.3 and 4.8.  Rows at odd addresses, and heads turned in part that is no whole number of chunks, go a
+// value at a time (rope_any_kernel): 9000 tokens of 32 bf16 heads of 128 61 us, of 80 with 20 turned 51, one token 3.9.
 // In blocks of one round, each of which finds its tokens' places for itself, the prompts took 139 us; in 8 rounds 82, in 32
 // 92.  Queries, keys and values in loops of their own (a row's quantising for queries as well: 151 us).
 #include <type_traits>
@@ -295,7 +299,7 @@ cudaError_t rows(const RopeDev& r, const RopeRows& a, cudaStream_t s) {
 }
 
 template <class T>
-cudaError_t rows_by_size(const RopeDev& r, const RopeRows& a, bool wide, cudaStream_t s) {
+cudaError_t rows_by_size(const RopeDev& r, const RopeRows& a, bool wide, int sms, cudaStream_t s) {
     if (!wide) {
         const long long n = (long long)a.n_tok * ((a.heads + 7) / 8) * (r.dim - r.rot / 2);
         rope_any_kernel<T><<<(unsigned)((n + kThreads - 1) / kThreads), kThreads, 0, s>>>(r, a.pos, (const T*)a.x, a.ldx,
@@ -303,15 +307,15 @@ cudaError_t rows_by_size(const RopeDev& r, const RopeRows& a, bool wide, cudaStr
         return cudaGetLastError();
     }
     // one row a lane where all fit the GPU's threads at once, else more rows on their way and angles read once for them
-    if ((long long)a.n_tok * a.heads * (r.dim / 16) <= 148 * 2048) return rows<T, 1>(r, a, s);
+    if ((long long)a.n_tok * a.heads * (r.dim / 16) <= sms * 2048) return rows<T, 1>(r, a, s);
     return rows<T, sizeof(T) == 4 ? 2 : 4>(r, a, s);
 }
 
 template <class T, class C, int D, int U>
-cudaError_t append(const RopeDev& r, const KvDev& c, const KvBatchDev& b, const RopeAppend& a, cudaStream_t s) {
+cudaError_t append(const RopeDev& r, const KvDev& c, const KvBatchDev& b, const RopeAppend& a, int sms, cudaStream_t s) {
     const int per = ((a.heads + U - 1) / U + 2 * ((c.n_heads + U - 1) / U)) * (D / 16);
     // of many tokens a block takes several rounds: finding their places is a chain of loads that all of them share
-    const int tokens = min(32, max(max(1, kThreads / per), min(kRounds, b.n_tok / (148 * 4))));
+    const int tokens = min(32, max(max(1, kThreads / per), min(kRounds, b.n_tok / (sms * 4))));
     kv_append_rope_kernel<T, C, D, U><<<(unsigned)((b.n_tok + tokens - 1) / tokens + 1), kThreads, (size_t)tokens * r.rot * 4,
                                         s>>>(r, c, b, a, FastDiv((uint32_t)c.page_size), tokens);
     return cudaGetLastError();
@@ -319,34 +323,34 @@ cudaError_t append(const RopeDev& r, const KvDev& c, const KvBatchDev& b, const 
 
 template <class T, class C>
 cudaError_t append_by_size(int dim, const RopeDev& r, const KvDev& c, const KvBatchDev& b, const RopeAppend& a,
-                           cudaStream_t s) {
-    const bool few = (long long)b.n_tok * (a.heads + 2 * c.n_heads) * (dim / 16) <= 148 * 2048;
+                           int sms, cudaStream_t s) {
+    const bool few = (long long)b.n_tok * (a.heads + 2 * c.n_heads) * (dim / 16) <= sms * 2048;
     constexpr int U = sizeof(T) == 4 ? 2 : 4;
-    if (dim == 64) return few ? append<T, C, 64, 1>(r, c, b, a, s) : append<T, C, 64, U>(r, c, b, a, s);
-    return few ? append<T, C, 128, 1>(r, c, b, a, s) : append<T, C, 128, U>(r, c, b, a, s);
+    if (dim == 64) return few ? append<T, C, 64, 1>(r, c, b, a, sms, s) : append<T, C, 64, U>(r, c, b, a, sms, s);
+    return few ? append<T, C, 128, 1>(r, c, b, a, sms, s) : append<T, C, 128, U>(r, c, b, a, sms, s);
 }
 
 template <class T>
 cudaError_t append_by_cache(int ct, int dim, const RopeDev& r, const KvDev& c, const KvBatchDev& b, const RopeAppend& a,
-                            cudaStream_t s) {
-    if (ct == T_F16) return append_by_size<T, __half>(dim, r, c, b, a, s);
-    if (ct == T_BF16) return append_by_size<T, __nv_bfloat16>(dim, r, c, b, a, s);
-    return append_by_size<T, int8_t>(dim, r, c, b, a, s);
+                            int sms, cudaStream_t s) {
+    if (ct == T_F16) return append_by_size<T, __half>(dim, r, c, b, a, sms, s);
+    if (ct == T_BF16) return append_by_size<T, __nv_bfloat16>(dim, r, c, b, a, sms, s);
+    return append_by_size<T, int8_t>(dim, r, c, b, a, sms, s);
 }
 
 }  // namespace
 
-cudaError_t launch_rope(int dtype, const RopeDev& r, const RopeRows& a, bool wide, cudaStream_t s) {
-    if (dtype == T_F32) return rows_by_size<float>(r, a, wide, s);
-    if (dtype == T_F16) return rows_by_size<__half>(r, a, wide, s);
-    return rows_by_size<__nv_bfloat16>(r, a, wide, s);
+cudaError_t launch_rope(int dtype, const RopeDev& r, const RopeRows& a, bool wide, int sms, cudaStream_t s) {
+    if (dtype == T_F32) return rows_by_size<float>(r, a, wide, sms, s);
+    if (dtype == T_F16) return rows_by_size<__half>(r, a, wide, sms, s);
+    return rows_by_size<__nv_bfloat16>(r, a, wide, sms, s);
 }
 
 cudaError_t launch_kv_append_rope(int cache_type, int dtype, int head_dim, const RopeDev& r, const KvDev& c,
-                                  const KvBatchDev& b, const RopeAppend& a, cudaStream_t s) {
-    if (dtype == T_F32) return append_by_cache<float>(cache_type, head_dim, r, c, b, a, s);
-    if (dtype == T_F16) return append_by_cache<__half>(cache_type, head_dim, r, c, b, a, s);
-    return append_by_cache<__nv_bfloat16>(cache_type, head_dim, r, c, b, a, s);
+                                  const KvBatchDev& b, const RopeAppend& a, int sms, cudaStream_t s) {
+    if (dtype == T_F32) return append_by_cache<float>(cache_type, head_dim, r, c, b, a, sms, s);
+    if (dtype == T_F16) return append_by_cache<__half>(cache_type, head_dim, r, c, b, a, sms, s);
+    return append_by_cache<__nv_bfloat16>(cache_type, head_dim, r, c, b, a, sms, s);
 }
 
 }  // namespace hc
