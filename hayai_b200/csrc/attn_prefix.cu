@@ -28,9 +28,11 @@
 // times the keys' and values' time at the copy rate from 16-bit pages, and 3 times from 8-bit ones.  A
 // unit of a wide tile takes 3500 to 4000 cycles, where its products take 2048 and its exponentials as many: each
 // half's chain (scores in, weights 1800, products 800, and the waits between) is the time, not either pipe.  Two threads per row,
-// exponentials by polynomials, and scores read twice from a shorter loop took the same time or more.  A start takes
-// 12 us and more (45 us in all for 64 sequences behind 4100 8-bit tokens, whose units are 8 us): code that is run for the
-// first time, fetched line by line.
+// exponentials by polynomials, and scores read twice from a shorter loop took the same time or more.  Chunks that fill
+// their tiles run at 470 to 500 TFLOP/s (8 of 256 tokens behind 16384, 577 us at its best; attn_many.cu 560).  A tile's start
+// and end take some 12 us (attn_shared.cu, kOver), the block's later tiles' as well as its first: 31 us in all for 64
+// sequences behind 4100 8-bit tokens, whose units are 8.  Queries in, the first keys' way, a unit through all roles and O out
+// follow one another; which of them it is has not been measured apart.
 //
 // Formats as in attn_many.cu: products of f16 (f16 and 8-bit caches) or bf16, weights rounded to that type and
 // summed in f32; f16 weights are taken 2^7 times as large.  8-bit codes are exact in f16; a K scale multiplies its column of

@@ -9,9 +9,10 @@
 //     attn_few       of single tokens, what is behind the prefixes (AttnArgs::first), which has no tiles then
 //     attn_join      out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's pieces
 // or, of f32 rows, attn_few over the prefixes and again over what is behind them, and the joining.
-// attn_groups is one block whose time is its chain of dependent loads and scans (9 to 11 us); attn_join moves the pieces
+// attn_groups is one block whose time is its chain of dependent loads and scans (10 to 13 us); attn_join moves the pieces
 // once, 10 us for 4096 rows of 128 columns in f32 and 30 us for 28000.
-// Where nothing is shared after all, the two others find no tiles, and the paged attention's kernels behind them do the work.
+// Where nothing is shared after all, the two others find no tiles, and the paged attention's kernels behind them do the work:
+// 16 sequences behind 300 tokens, tables of 32768, 26 us (15 by themselves); 64 behind 1000 60 (43).
 #include "attn_rows.cuh"
 #include "block_scan.cuh"
 
