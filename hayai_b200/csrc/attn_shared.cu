@@ -6,7 +6,7 @@
 //     attn_groups    what every group shares for this step, and the tiles: of the prefixes, then of what every sequence
 //                    has behind its own
 //     attn_prefix    the tiles (attn_prefix.cu), in pieces
-//     attn_few       of single tokens, what is behind the prefixes (AttnArgs::first), which has no tiles then
+//     attn_few       of many single tokens, what is behind the prefixes (AttnArgs::first), which has no tiles then
 //     attn_join      out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's pieces
 // or, of f32 rows, attn_few over the prefixes and again over what is behind them, and the joining.
 // attn_groups is one block whose time is its chain of dependent loads and scans (10 to 13 us); attn_join moves the pieces

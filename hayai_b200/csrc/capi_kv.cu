@@ -224,14 +224,14 @@ struct ShareBound {
     long long host, device;
 };
 // Single tokens (16-bit rows) pay for several kernels' starts, and for a prefix's units more than for a reading of it: as much
-// as for one more from 16-bit pages and three more from 8-bit ones.  bf16 pages: 16 sequences behind 4096 (240 MB saved)
-// 36 and 48, 8 behind 16384 (448 MB) 58 and 62, 40 behind 4096 (624 MB) 72 and 56, 16 behind 16384 (960 MB) 103 and 67, 4
-// behind 65536 (768 MB) 162 and 99.  8-bit: 16 behind 4096 (124 MB) 33 and 54, 8 behind 16384 (231 MB) 52 and 64, 40
-// behind 4096 (322 MB) 66 and 58, 16 behind 16384 (495 MB) 90 and 67; 4 behind 65536 (396 MB) 90 and 115, 8 (924) 165 and 115.
+// as for one more from 16-bit pages and three more from 8-bit ones.  bf16 pages: 4 sequences behind 16384 (192 MB saved) 36 and
+// 45, 16 behind 4096 (240) 36 and 42, 8 behind 16384 (448) 59 and 48, 40 behind 4096 (624) 72 and 56, 16 behind 16384 (960) 102
+// and 53, 4 behind 65536 (768) 160 and 79.  8-bit: 16 behind 4096 (124 MB) 33 and 47, 8 behind 16384 (231) 52 and 53, 40 behind
+// 4096 (322) 66 and 59, 16 behind 16384 (495) 90 and 62; 4 behind 65536 (396) 90 and 94, 8 (924) 165 and 102.
 constexpr ShareBound kShareBytes{300 << 20, 200 << 20}, kShareBytes8{190 << 20, 120 << 20};
 // Chunks have starts of the same cost either way.  Where they are fewer tiles than blocks, the paged attention splits tiles,
-// and whatever is read again can be saved: 8 of 5 tokens behind 1024 (28 MB) 37 and 36, 16 of 5 behind 1024 (60 MB) 44 and 44, 4
-// behind 4096 (48 MB) 44 and 36, 16 of 64 behind 4096 (240 MB) 140 and 135, 8 behind 16384 (448 MB) 214 and 177.  With more,
+// and whatever is read again can be saved: 8 of 5 tokens behind 1024 (28 MB) 37 and 36, 16 of 5 behind 1024 (60 MB) 44 and 45, 4
+// behind 4096 (48 MB) 45 and 37, 16 of 64 behind 4096 (240 MB) 141 and 136, 8 behind 16384 (448 MB) 215 and 178.  With more,
 // what counts is tiles that sharing fills, against its own tiles at 27/25 of the others' time and 16 bytes for each of
 // the rows' values in pieces: 16 of 256 tokens behind 16384 (960 MB, no tile saved) 1075 and 1281, 8 of 1000 (448 MB, 3 of 128)
 // 2342 and 2499, 16 of 100 (7 of 32) behind 16384 556 and 490, behind 1024 111 and 125; one of 3000 with 31 single tokens behind
@@ -331,14 +331,16 @@ extern "C" int hc_attn_shared_dev(hc_engine* e, const hc_kv_cache* c, const hc_k
         readings -= 5 * d.extra;
     }
     const bool may = g->n_groups && b->n_tok >= 2 && readings * b->max_pages * c->page_size / 5 >= least;
-    // What a sequence has behind its prefix goes there too where it has few rows (single tokens): 64 of them with 30 to
-    // 1500 8-bit tokens each take 43 us there, and 75 as tiles of attn_prefix.cu; 53 chunks of up to 60 tokens with up
-    // to 300 before them 108 in the paged attention's kernels, and 75 as tiles.
-    const bool behind = few || own_rows <= kFewRows;
+    // What a sequence has behind its prefix goes there too where it has few rows (single tokens) and makes more than a block's
+    // tile, or two of 16-bit pages: us of calls behind 16384 tokens, 32 heads on 8 of 128, as tiles of attn_prefix.cu and
+    // there, 16 sequences with 50 tokens of their own each (128 tiles), 8-bit 62 and 66, bf16 54 and 63; with 1000 75 and 78, 66 and
+    // 78; 24 with 1000 89 and 86, 76 and 91; 36 with 50 (288) 85 and 76, 69 and 68; 64 with 50 116 and 82, 91 and 77, with
+    // 3000 260 and 163, 172 and 206; 128 with 50 199 and 107, 153 and 96.
+    const long long seqs = b->n_seq < b->n_tok ? b->n_seq : b->n_tok;  // with new tokens
+    const bool behind = few || (own_rows <= kFewRows && seqs * kv > (codes ? 1 : 2) * sms);
     long long shared = b->n_seq / 2;  // groups that share anything: two sequences with new tokens each
     if (shared > b->n_tok / 2) shared = b->n_tok / 2;
     if (shared > g->n_groups) shared = g->n_groups;
-    const long long seqs = b->n_seq < b->n_tok ? b->n_seq : b->n_tok;  // with new tokens
     const long long tiles = 2 * (rows / 256) + (few ? 0 : shared * kv) + (behind ? seqs : seqs * kv);
     // a row's result in a piece (of narrow tiles two) of its prefix, and one behind it unless it comes from the kernel
     // for few rows; and where a block's share ends in a tile, its rows once more

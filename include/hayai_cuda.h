@@ -339,7 +339,7 @@ typedef struct hc_kv_shared {
  * part by part (bf16; or f16, in which weights below 2^-21 of a part's largest have fewer bits), single tokens' too,
  * whose weights hc_attn_paged_dev rounds at a size of their own for every few positions.  Between the call's kernels
  * partial results lie in the engine, in a workspace of up to 4.5 * n_tok * n_heads * (head_dim + 2) floats and 21 MB (for
- * single tokens, and f32 rows, up to 3.5), which grows with the calls in powers of two, past 256 MB in quarters of
+ * many single tokens, and f32 rows, up to 3.5), which grows with the calls in powers of two, past 256 MB in quarters of
  * them.  It is made before the device knows whether sharing is worth it; where there is no room for it, nothing is shared. */
 int hc_attn_shared_dev(hc_engine* eng, const hc_kv_cache* cache, const hc_kv_batch* batch, const hc_kv_shared* shared,
                        int dtype, size_t n_heads, const void* q, size_t ldq, void* out, size_t ldo, float* lse, float scale);

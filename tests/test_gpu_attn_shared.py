@@ -493,9 +493,10 @@ def test_offsets_that_do_not_ascend_are_reported(engine, dtype, cache, new):
 def test_a_long_chunk_beside_single_tokens(engine, dtype, hint):
     """Rows behind the prefixes that go to the kernel for few rows, of a long sequence and of short ones (16-bit rows
     where the hint says single tokens): all of them are joined."""
-    s = Groups([(70, ONE * 3 + [(700, 720)] + [(1, 30)] * 5), (40, [(333, 333), (1, 1)]), (0, [(90, 90)])], 2, 64, 16, "f16")
-    s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
-    check(engine, s, 8, dtype, shared=hb.KvShared(s.starts, s.length, least=1))
+    for kv_heads, heads in ((2, 8), (32, 32)):
+        s = Groups([(70, ONE * 3 + [(700, 720)] + [(1, 30)] * 5), (40, [(333, 333), (1, 1)]), (0, [(90, 90)])], kv_heads, 64, 16, "f16")
+        s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
+        check(engine, s, heads, dtype, shared=hb.KvShared(s.starts, s.length, least=1))
 
 
 def test_a_chunk_of_millions_of_rows_beside_as_many_sequences_as_there_can_be(engine):
@@ -600,15 +601,16 @@ ORDERS = ["rows of all heads", "heads apart", "rows apart", "pages and heads apa
 
 @pytest.mark.parametrize("order", ORDERS)
 @pytest.mark.parametrize("cache,dtype", [("i8", "bf16"), ("i8", "f16"), ("i8", "f32"), ("bf16", "bf16"), ("f16", "bf16"), ("f16", "f32")])
-@pytest.mark.parametrize("dim,page", [(64, 16), (128, 24), (64, 1), (128, 300)])
-def test_pools_of_other_orders(engine, order, cache, dtype, dim, page):
+@pytest.mark.parametrize("dim,page,kv_heads", [(64, 16, 2), (128, 24, 2), (64, 1, 64), (128, 300, 2), (128, 20, 64)])
+def test_pools_of_other_orders(engine, order, cache, dtype, dim, page, kv_heads):
     """Bit for bit what the contiguous pool gives: chunks and single tokens, prefixes of several units and pages."""
-    s = Groups([(333, [(1, 1), (9, 40), (1, 150)]), (130, [(2, 2), (60, 70)])], 2, dim, page, cache)
-    q = s.q(8, dtype)
+    heads = max(kv_heads, 8)
+    s = Groups([(333, [(1, 1), (9, 40), (1, 150)]), (130, [(2, 2), (60, 70)])], kv_heads, dim, page, cache)
+    q = s.q(heads, dtype)
     for hint in (0, 1):  # 1: what is behind the prefixes goes to the kernel for few rows
         s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, hint)
         plain = s.cache
-        want = check(engine, s, 8, dtype, q=q)
+        want = check(engine, s, heads, dtype, q=q)
         scale = []
         for x in s.scale:
             if x is not None:
@@ -617,7 +619,7 @@ def test_pools_of_other_orders(engine, order, cache, dtype, dim, page):
                 x = wide[:, 3:-2].unflatten(1, x.shape[1:])
             scale.append(x)
         s.cache = hb.KvCache(*(laid_out(x, order, 77 if cache == "i8" else math.nan) for x in s.pool), *scale)
-        got = check(engine, s, 8, dtype, q=q)
+        got = check(engine, s, heads, dtype, q=q)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         s.cache = plain
 
@@ -649,7 +651,7 @@ def test_the_rule_on_what_is_shared(engine, dtype, cache, groups, hint, made):
 
 
 @pytest.mark.parametrize("dtype,cache,hint", [("f32", "i8", 0), ("f32", "bf16", 1), ("bf16", "i8", 1), ("f16", "f16", 1), ("bf16", "bf16", 0)])
-@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (4, 4)])
+@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (4, 4), (64, 64), (96, 48)])
 def test_scale_and_strided_rows_of_the_other_kernels(engine, dtype, cache, hint, heads, kv_heads):
     """f32 rows, and single tokens behind prefixes: rows apart, any scale, with a log-sum-exp and without."""
     s = Groups([(90, ONE * 4 + [(1, 33), (3, 20)]), (0, [(2, 9)]), (160, [(1, 1), (1, 70)])], kv_heads, 64, 16, cache)
@@ -702,3 +704,31 @@ def test_one_graph_through_sharing_and_none(engine, dtype, cache, hint):
             torch.cuda.synchronize()
             assert torch.equal(direct, first)
     engine.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("case", list(CASES))
+@pytest.mark.parametrize("cache,dtype", [("i8", "bf16"), ("i8", "f16"), ("f16", "f16"), ("f16", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(96, 96, 64, 16), (180, 60, 64, 24), (64, 64, 128, 100)])
+def test_groups_of_more_tiles_than_blocks(engine, case, cache, dtype, heads, kv_heads, dim, page):
+    """So many kv heads that what is behind the prefixes goes to the kernel for few rows, whatever sequences have more."""
+    s = Groups(CASES[case], kv_heads, dim, page, cache)
+    s.batch = hb.KvBatch(s.table, s.q_start, s.kv_len, s.rows, 1)
+    check(engine, s, heads, dtype)
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "i8"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("at", ["prefix", "own"])
+def test_not_finite_behind_many_tiles(engine, dtype, cache, at):
+    s = Groups([(40, [(1, 20)] * 3), (50, [(1, 9)] * 2)], 64, 64, 16, cache)
+    page = s.table[0, 1] if at == "prefix" else s.table[1, 3]
+    if cache == "i8":
+        s.scale[1][page.long(), 0, 2] = math.inf
+    else:
+        s.pool[1][page.long(), 0, 2, :] = math.inf
+    q = s.q(64, dtype)
+    out = torch.zeros_like(q)
+    engine.attn_shared_dev(s.cache, s.batch, s.shared, q, out)
+    engine.sync()
+    bad = ~out.isfinite().all(-1)
+    assert bad[:, 0].tolist() == ([True] * 3 if at == "prefix" else [False, True, False]) + [False, False]
+    assert not bad[:, 1:].any()
